@@ -34,6 +34,8 @@ extern "C" {
 #define B200_BF16 1
 #define B200_F16 2 /* the reference's kernels accept it: backends/triton_linear.py:100-105. Projections and prompt
                       attention on the tensor cores where rows allow 16-byte loads, the rest on the CUDA cores */
+#define B200_I8 3   /* codes of 8-bit operands (with scales): signed integers */
+#define B200_E4M3 4 /* or 8-bit floats, four exponent and three mantissa bits, 448 the largest */
 
 /* numerical modes: lowering.py:24-37 (_NUMERICAL_LOWERINGS) */
 #define B200_MODE_FAST 0
@@ -54,6 +56,7 @@ extern "C" {
 #define B200_STATUS_BAD_TOKEN_ID 4      /* embedding id outside [0, vocab): row zeroed    */
 #define B200_STATUS_BAD_POSITION 8      /* negative KV position: write skipped            */
 #define B200_STATUS_WAIT_TIMEOUT 16     /* a bounded in-kernel wait gave up: result invalid */
+#define B200_STATUS_NOT_FINITE 32       /* an infinity or NaN met an 8-bit format: saturated */
 
 /* launch-mode flags (b200_set_launch_mode) */
 #define B200_LAUNCH_PROGRAMMATIC 1      /* decode-chain kernels use programmatic dependent launch */
@@ -723,6 +726,80 @@ int b200_sequence_positions(const int64_t* lengths, const int32_t* slots, int32_
                             void* stream);
 int b200_advance_slots(int64_t* lengths, const int32_t* slots, const int32_t* starts, int64_t rows,
                        int64_t capacity, int32_t* status, void* stream);
+
+/* ---- Serving in 8 bits -------------------------------------------------------------
+ * No counterpart in the reference, which serves the types its models come in: a paged KV cache whose entries are 8-bit
+ * codes with a scale for each block of tokens and KV head, and projections in 8-bit integers. Same conventions as above.
+ *
+ * Cache. Pools are [num_blocks, kv_heads, block_size, head_dim] codes (cache_dtype B200_I8 or B200_E4M3), scales fp32
+ * [num_blocks, kv_heads], one pool and one vector of scales for K and for V; an entry stands for code * scale. The block
+ * table is that of the 16-bit paged layout.
+ *
+ * b200_paged_kv_store_8bit: writes the new rows x of key / value (B x H x T x D, any strides, B200_BF16 or B200_F16) at
+ * positions[b] .. positions[b] + T - 1. With T = 127 (B200_I8) or 448 (B200_E4M3) the largest code and s a block's scale
+ * so far (0 if its first row is among the new ones), every operation in fp32:
+ *   s' = max(s, amax|x| * (1 / T)), at least the smallest normal number where x is not all zero;
+ *   rows of the block in front: c' = round(c * (s / s')), only where s' > s;   new rows: c = round(x * (1 / s')),
+ * to the nearest code, ties to even. Rows behind the new ones are left as they are (and stand for code * s'). Infinities
+ * and NaN do not count in amax; they saturate, NaN becomes 0 (B200_I8) or stays NaN, and B200_STATUS_NOT_FINITE is set.
+ * A negative position or a table entry outside [0, num_blocks) sets B200_STATUS_BAD_POSITION, rows beyond the table
+ * B200_STATUS_KV_OVERFLOW; those rows are skipped. No block may belong to two sequences of one call. head_dim % 16 == 0.
+ *
+ * b200_paged_decode_attention_8bit: one query token per sequence, B x Hq x 1 x D in B200_BF16 or B200_F16 (last dim
+ * contiguous), over the first lengths[b] entries: softmax(scale * q . K + mask) V with fp32 scores, statistics and sums.
+ * The mask is additive, B x 1 x 1 x mask_len, or NULL. head_dim 64, 128 or 256, block_size a multiple of 32. A length
+ * above mask_len is clamped and sets B200_STATUS_LENGTH_OVER_MASK; tokens of a block outside [0, num_blocks) are left out
+ * and set B200_STATUS_BAD_POSITION. A sequence without tokens, or with every token masked by -inf, gives NaN as
+ * b200_decode_attention does. split_tokens: tokens a CTA serves (0: the library's choice); max_length_hint: the longest
+ * length the host expects (0: mask_len), which sizes the split and bounds nothing. Workspace (zero-filled once):
+ * b200_paged_decode_attention_8bit_workspace_bytes.
+ *
+ * b200_copy_kv_blocks: pool[layer, destinations[i]] = pool[layer, sources[i]] for every pool, layer and i in one launch:
+ * blocks of paged caches of any type (fork, compaction). A pool's block `j` of layer `l` is the block_bytes bytes at
+ * base + l * layer_stride + j * block_bytes. destinations[] are distinct and none of them is among sources[]; an index
+ * outside [0, num_blocks) is skipped and sets B200_STATUS_BAD_POSITION.
+ *
+ * b200_quantize_rows_int8: codes [rows, hidden] and one fp32 scale per row, code = round(y / scale), scale = amax|y| / 127
+ * (0 for a row of zeros, whose codes are 0), with
+ *   y = input                                                 norm_weight NULL (weights, or rows without a norm);
+ *   y = r * rsqrt(mean(r^2) + epsilon) * norm_weight          r = input, or round(input + residual), written to `sum`
+ * (which may be input or residual itself). A row whose y is not finite gets scale NaN and codes 0. dtype of input,
+ * residual, sum and norm_weight: any.
+ *
+ * b200_linear_int8: y[m, n] = (sum_k x[m, k] weight[n, k]) x_scales[m] weight_scales[n] + bias[n], sums in 32-bit integers
+ * (exact), then the epilogue in fp32 and one rounding to dtype: B200_EPILOGUE_RESIDUAL adds residual[m, n];
+ * B200_EPILOGUE_SWIGLU takes columns 2j and 2j + 1 as gate_j and up_j and gives silu(gate_j) up_j. x and weight are
+ * contiguous codes, K a multiple of 16 and at most 131056; bias, residual and output are of dtype. `status` receives
+ * B200_STATUS_WAIT_TIMEOUT if a bounded in-kernel wait gives up. */
+#define B200_MAX_COPY_POOLS 8
+typedef struct b200_block_pool {
+  void* base;
+  int64_t layer_stride; /* bytes */
+  int64_t block_bytes;
+} b200_block_pool;
+int b200_paged_kv_store_8bit(void* key_pool, void* value_pool, float* key_scales, float* value_scales,
+                             const int32_t* block_table, const void* key, const void* value, const int64_t* positions,
+                             int64_t batch, int64_t heads, int64_t tokens, int64_t head_dim, int64_t num_blocks,
+                             int64_t block_size, int64_t max_blocks_per_sequence, const int64_t key_strides[4],
+                             const int64_t value_strides[4], int dtype, int cache_dtype, int32_t* status, void* stream);
+int64_t b200_paged_decode_attention_8bit_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                                         int64_t head_dim, int64_t max_length, int64_t split_tokens);
+int b200_paged_decode_attention_8bit(
+    const void* query, const void* key_pool, const void* value_pool, const float* key_scales, const float* value_scales,
+    const int32_t* block_table, const int64_t* lengths, const void* mask, void* output, int64_t batch, int64_t q_heads,
+    int64_t kv_heads, int64_t head_dim, int64_t num_blocks, int64_t block_size, int64_t max_blocks_per_sequence,
+    int64_t mask_len, int64_t q_batch_stride, int64_t q_head_stride, int64_t mask_batch_stride, int mask_dtype, double scale,
+    int dtype, int cache_dtype, int64_t split_tokens, int64_t max_length_hint, void* workspace, int64_t workspace_bytes,
+    int32_t* status, void* stream);
+int b200_copy_kv_blocks(const b200_block_pool* pools, int64_t pool_count, const int32_t* sources,
+                        const int32_t* destinations, int64_t count, int64_t layers, int64_t num_blocks, int32_t* status,
+                        void* stream);
+int b200_quantize_rows_int8(const void* input, const void* residual, const void* norm_weight, void* sum, void* codes,
+                            float* scales, int64_t rows, int64_t hidden, int64_t input_row_stride,
+                            int64_t residual_row_stride, double epsilon, int dtype, void* stream);
+int b200_linear_int8(const void* x, const float* x_scales, const void* weight, const float* weight_scales, const void* bias,
+                     const void* residual, void* output, int64_t m, int64_t k, int64_t n, int dtype, int epilogue,
+                     int32_t* status, void* stream);
 
 #ifdef __cplusplus
 }

@@ -15,7 +15,7 @@ PACKAGE_DIR = Path(__file__).resolve().parent
 # B200_LIBRARY_PATH: another build of the same library (for instance the -DB200_TRACE one)
 LIBRARY_PATH = Path(os.environ.get("B200_LIBRARY_PATH", PACKAGE_DIR / "libb200serve.so"))
 
-F32, BF16, F16 = 0, 1, 2
+F32, BF16, F16, I8, E4M3 = 0, 1, 2, 3, 4
 MODE_FAST, MODE_PYTORCH_COMPATIBLE = 0, 1
 EPILOGUE_NONE, EPILOGUE_RESIDUAL, EPILOGUE_SWIGLU = 0, 1, 2
 
@@ -24,6 +24,7 @@ STATUS_LENGTH_OVER_MASK = 2
 STATUS_BAD_TOKEN_ID = 4
 STATUS_BAD_POSITION = 8
 STATUS_WAIT_TIMEOUT = 16
+STATUS_NOT_FINITE = 32
 
 LAUNCH_PROGRAMMATIC = 1
 LAUNCH_CONSTANT_WEIGHTS = 2
@@ -114,6 +115,14 @@ class PromptCall(ctypes.Structure):
                  "capacity", "num_blocks", "block_size", "max_blocks")] + \
                [("epsilon", c_double), ("scale", c_double), ("dtype", c_int), ("mode", c_int)]
 
+
+class BlockPool(ctypes.Structure):
+    """b200_block_pool of include/b200_serve.h."""
+
+    _fields_ = [("base", c_void_p), ("layer_stride", c_int64), ("block_bytes", c_int64)]
+
+
+MAX_COPY_POOLS = 8
 
 _DELTA, _RETENTION, _STEP = POINTER(DeltaInputs), POINTER(RetentionInputs), POINTER(StepOutput)
 
@@ -223,6 +232,14 @@ SIGNATURES = {
                                                                      c_void_p, c_void_p]),
     "b200_sequence_positions": (c_int, [c_void_p] * 3 + [c_int64, c_void_p]),
     "b200_advance_slots": (c_int, [c_void_p] * 3 + [c_int64, c_int64, c_void_p, c_void_p]),
+    "b200_paged_kv_store_8bit": (c_int, [c_void_p] * 8 + [c_int64] * 7 + [_I64P, _I64P, c_int, c_int, c_void_p, c_void_p]),
+    "b200_paged_decode_attention_8bit_workspace_bytes": (c_int64, [c_int64] * 6),
+    "b200_paged_decode_attention_8bit": (c_int, [c_void_p] * 9 + [c_int64] * 11 + [c_int, c_double, c_int, c_int, c_int64,
+                                                                                c_int64, c_void_p, c_int64, c_void_p,
+                                                                                c_void_p]),
+    "b200_copy_kv_blocks": (c_int, [POINTER(BlockPool), c_int64, c_void_p, c_void_p] + [c_int64] * 3 + [c_void_p, c_void_p]),
+    "b200_quantize_rows_int8": (c_int, [c_void_p] * 6 + [c_int64] * 4 + [c_double, c_int, c_void_p]),
+    "b200_linear_int8": (c_int, [c_void_p] * 7 + [c_int64] * 3 + [c_int, c_int, c_void_p, c_void_p]),
 }
 
 _library: ctypes.CDLL | None = None

@@ -1,0 +1,32 @@
+// Shared pieces of the operators in 8 bits: code types, their largest values, conversions.
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace b200 {
+
+// Codes of a cache: signed integers or e4m3. Both formats stand for code * scale.
+struct Int8Code {
+  static constexpr float kTop = 127.0f;
+  // Nearest integer, ties to even, of a value that the scale brings to [-127, 127]; infinities saturate, NaN gives 0.
+  __device__ static uint32_t encode(float v) {
+    return static_cast<uint32_t>(__float2int_rn(fminf(fmaxf(v == v ? v : 0.0f, -kTop), kTop))) & 0xffu;
+  }
+  __device__ static float decode(uint32_t code) { return static_cast<float>(static_cast<int8_t>(code)); }
+};
+struct E4m3Code {
+  static constexpr float kTop = 448.0f;
+  // Nearest e4m3 number, ties to even; what is beyond 448 saturates, NaN stays NaN.
+  __device__ static uint32_t encode(float v) { return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3); }
+  __device__ static float decode(uint32_t code) {
+    return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(code), __NV_E4M3)));
+  }
+};
+
+constexpr float kSmallestScale = 1.17549435e-38f;  // the smallest normal number: 1 / scale stays finite
+
+__device__ __forceinline__ bool is_finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
+
+}  // namespace b200

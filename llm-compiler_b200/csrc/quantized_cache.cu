@@ -1,0 +1,319 @@
+// A paged KV cache in 8 bits: the store that quantises new tokens into it, and copies of its blocks (of any paged cache's).
+//
+// Pools are [num_blocks, kv_heads, block_size, head_dim] codes with one fp32 scale per (block, KV head) for K and one for V.
+// A (block, head) is the unit of everything here: it is contiguous (the attention's tile copies read it as one run, and
+// need no stride over the heads of a token), and it is what a scale belongs to.
+#include <string.h>
+
+#include <algorithm>
+
+#include "quantized.cuh"
+
+namespace b200 {
+namespace {
+
+// ---------------------------------------------------------------------------------------------------------- store ----
+// One CTA per (block that receives rows, KV head, sequence, K or V). With x the new rows, T the code's largest value and s
+// the block's scale so far (0 where the block is entered at its first row):
+//     s' = max(s, amax|x| * fp32(1/T)),  rows held: c' = round(c * (s / s')),  new rows: c = round(x * (1 / s')).
+// s' only grows while a block fills, so a row is rounded anew only when a later token is larger than all before it.
+// Every step is one IEEE operation in fp32, so the codes do not depend on how the work is split.
+constexpr int kStoreThreads = 256;
+constexpr int kStoreVectors = 8;  // 16-byte loads a thread keeps: a 128 x 128 block is read once
+
+struct StoreParams {
+  const void* x[2];        // new keys, new values
+  int64_t strides[2][4];   // batch, head, token, element
+  uint8_t* pool[2];
+  float* scales[2];
+  const int32_t* table;
+  const int64_t* positions;
+  int32_t* status;
+  int64_t tokens, max_blocks, num_blocks;
+  int heads, dim, block_size;
+};
+
+template <typename T, typename Code, bool kVector>
+__global__ void __launch_bounds__(kStoreThreads)
+quantized_store_kernel(const StoreParams p) {
+  constexpr int per = kVector ? 8 : 1;  // elements a load takes
+  grid_launch_dependents();
+  __shared__ uint32_t most_bits[kStoreThreads / 32];
+  __shared__ int bad[kStoreThreads / 32];
+  const int h = blockIdx.y % p.heads, which = blockIdx.y / p.heads;
+  const int64_t b = blockIdx.z;
+  grid_dependency_wait();
+  const int64_t position = p.positions[b];
+  if (position < 0) {
+    if (threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0) atomicOr(p.status, B200_STATUS_BAD_POSITION);
+    return;
+  }
+  const int64_t column = position / p.block_size + blockIdx.x;
+  const int64_t first = position > column * p.block_size ? position : column * p.block_size;
+  const int64_t end = min(position + p.tokens, (column + 1) * p.block_size);
+  if (first >= end) return;
+  if (column >= p.max_blocks) {
+    if (threadIdx.x == 0) atomicOr(p.status, B200_STATUS_KV_OVERFLOW);
+    return;
+  }
+  const int64_t block = p.table[b * p.max_blocks + column];
+  if (block < 0 || block >= p.num_blocks) {
+    if (threadIdx.x == 0) atomicOr(p.status, B200_STATUS_BAD_POSITION);
+    return;
+  }
+  const int held = static_cast<int>(first - column * p.block_size), rows = static_cast<int>(end - first);
+  const int64_t* st = p.strides[which];
+  const T* x = static_cast<const T*>(p.x[which]) + b * st[0] + h * st[1] + (first - position) * st[2];
+  const int64_t slab = block * p.heads + h;
+  uint8_t* codes = p.pool[which] + slab * p.block_size * p.dim;
+  const int per_row = p.dim / per, items = rows * per_row;
+
+  // the largest finite magnitude of the new rows (as bits: magnitudes compare as integers)
+  uint4 kept[kStoreVectors];
+  uint32_t most = 0;
+  bool not_finite = false;
+  auto look = [&](float v) {
+    const uint32_t bits = __float_as_uint(v) & 0x7fffffffu;
+    if (bits < 0x7f800000u) most = max(most, bits);
+    else not_finite = true;
+  };
+  auto address = [&](int i) { return x + (i / per_row) * st[2] + (i % per_row) * per * st[3]; };
+  auto look_at = [&](const uint4& raw) {
+    Vec16<T> v;
+    v.load(reinterpret_cast<const T*>(&raw));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) look(v.v[e]);
+  };
+  if constexpr (kVector) {
+#pragma unroll
+    for (int j = 0; j < kStoreVectors; ++j) {
+      const int i = threadIdx.x + j * kStoreThreads;
+      kept[j] = make_uint4(0u, 0u, 0u, 0u);
+      if (i < items) kept[j] = *reinterpret_cast<const uint4*>(address(i));
+    }
+#pragma unroll
+    for (int j = 0; j < kStoreVectors; ++j) look_at(kept[j]);
+    for (int i = threadIdx.x + kStoreVectors * kStoreThreads; i < items; i += kStoreThreads)
+      look_at(*reinterpret_cast<const uint4*>(address(i)));
+  } else {
+    for (int i = threadIdx.x; i < items; i += kStoreThreads) look(Elem<T>::load(address(i)));
+  }
+  most = __reduce_max_sync(0xffffffffu, most);
+  const bool any_bad = __any_sync(0xffffffffu, not_finite);
+  if ((threadIdx.x & 31) == 0) {
+    most_bits[threadIdx.x >> 5] = most;
+    bad[threadIdx.x >> 5] = any_bad;
+  }
+  __syncthreads();
+  bool all_bad = false;
+#pragma unroll
+  for (int w = 0; w < kStoreThreads / 32; ++w) {
+    most = max(most, most_bits[w]);
+    all_bad = all_bad || bad[w] != 0;
+  }
+  const float before = held > 0 ? p.scales[which][slab] : 0.0f;
+  float scale = most > 0 ? fmaxf(__fmul_rn(__uint_as_float(most), 1.0f / Code::kTop), kSmallestScale) : 0.0f;
+  scale = fmaxf(scale, before);
+  const float inverse = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
+  __syncthreads();  // every thread has read the scale
+  if (threadIdx.x == 0) {
+    p.scales[which][slab] = scale;
+    if (all_bad) atomicOr(p.status, B200_STATUS_NOT_FINITE);
+  }
+  if (held > 0 && scale != before) {  // the rows in front, on the larger scale (dim is a multiple of 16)
+    const float ratio = __fdiv_rn(before, scale);
+    uint4* words = reinterpret_cast<uint4*>(codes);
+    for (int i = threadIdx.x; i < held * p.dim / 16; i += kStoreThreads) {
+      uint4 raw = words[i];
+      uint32_t* w = reinterpret_cast<uint32_t*>(&raw);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t packed = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          packed |= Code::encode(__fmul_rn(Code::decode((w[j] >> (8 * e)) & 0xffu), ratio)) << (8 * e);
+        w[j] = packed;
+      }
+      words[i] = raw;
+    }
+  }
+  uint8_t* out = codes + held * p.dim;
+  auto put = [&](const uint4& raw, int i) {
+    Vec16<T> v;
+    v.load(reinterpret_cast<const T*>(&raw));
+    uint2 packed = make_uint2(0u, 0u);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      packed.x |= Code::encode(__fmul_rn(v.v[e], inverse)) << (8 * e);
+      packed.y |= Code::encode(__fmul_rn(v.v[e + 4], inverse)) << (8 * e);
+    }
+    *reinterpret_cast<uint2*>(out + i * 8) = packed;
+  };
+  if constexpr (kVector) {
+#pragma unroll
+    for (int j = 0; j < kStoreVectors; ++j) {
+      const int i = threadIdx.x + j * kStoreThreads;
+      if (i < items) put(kept[j], i);
+    }
+    for (int i = threadIdx.x + kStoreVectors * kStoreThreads; i < items; i += kStoreThreads)
+      put(*reinterpret_cast<const uint4*>(address(i)), i);
+  } else {
+    for (int i = threadIdx.x; i < items; i += kStoreThreads)
+      out[i] = static_cast<uint8_t>(Code::encode(__fmul_rn(Elem<T>::load(address(i)), inverse)));
+  }
+}
+
+// ----------------------------------------------------------------------------------------------------------- copy ----
+// pool[layer, destinations[i]] = pool[layer, sources[i]] of every pool and layer in one launch. Nothing but bytes move:
+// each is read once and written once.
+constexpr int kCopyThreads = 256;
+constexpr int kCopyChunk = 16384;  // bytes of a block that one CTA moves
+constexpr int kMaxPools = B200_MAX_COPY_POOLS;
+
+struct CopyParams {
+  uint8_t* base[kMaxPools];
+  int64_t layer_stride[kMaxPools];  // bytes
+  int64_t block_bytes[kMaxPools];
+  int64_t first_unit[kMaxPools + 1];  // CTAs of the pools before
+  const int32_t* sources;
+  const int32_t* destinations;
+  int32_t* status;
+  int64_t num_blocks, layers, count;
+  int pools;
+};
+
+template <typename V>
+__device__ __forceinline__ void copy_run(uint8_t* to, const uint8_t* from, int64_t bytes) {
+  const int64_t n = bytes / static_cast<int64_t>(sizeof(V));
+  const V* src = reinterpret_cast<const V*>(from);
+  V* dst = reinterpret_cast<V*>(to);
+  for (int64_t i = threadIdx.x; i < n; i += kCopyThreads * 4) {
+    V held[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i + j * kCopyThreads < n) held[j] = src[i + j * kCopyThreads];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i + j * kCopyThreads < n) dst[i + j * kCopyThreads] = held[j];
+  }
+}
+
+__global__ void __launch_bounds__(kCopyThreads) copy_blocks_kernel(const CopyParams p) {
+  grid_launch_dependents();
+  grid_dependency_wait();
+  int pool = 0;
+  while (pool + 1 < p.pools && static_cast<int64_t>(blockIdx.x) >= p.first_unit[pool + 1]) ++pool;
+  const int64_t unit = blockIdx.x - p.first_unit[pool], bytes = p.block_bytes[pool];
+  auto place = [&](int64_t pair, int64_t layer, uint8_t** to, const uint8_t** from) {
+    const int64_t source = p.sources[pair], destination = p.destinations[pair];
+    if (source < 0 || source >= p.num_blocks || destination < 0 || destination >= p.num_blocks) {
+      atomicOr(p.status, B200_STATUS_BAD_POSITION);
+      return false;
+    }
+    uint8_t* base = p.base[pool] + layer * p.layer_stride[pool];
+    *to = base + destination * bytes;
+    *from = base + source * bytes;
+    return source != destination;
+  };
+  uint8_t* to;
+  const uint8_t* from;
+  if (bytes >= kCopyChunk / 16) {  // a CTA moves a piece of one block
+    const int64_t pieces = (bytes + kCopyChunk - 1) / kCopyChunk, piece = unit % pieces, pair = unit / pieces % p.count;
+    if (!place(pair, unit / pieces / p.count, &to, &from)) return;
+    const int64_t offset = piece * kCopyChunk, size = min(bytes - offset, static_cast<int64_t>(kCopyChunk));
+    if ((bytes & 15) == 0 && ((reinterpret_cast<uintptr_t>(p.base[pool]) | p.layer_stride[pool]) & 15) == 0)
+      copy_run<uint4>(to + offset, from + offset, size);
+    else
+      copy_run<uint8_t>(to + offset, from + offset, size);
+    return;
+  }
+  // small blocks (scales): a thread moves whole blocks
+  const int64_t i = unit * kCopyThreads + threadIdx.x;
+  if (i >= p.count * p.layers || !place(i % p.count, i / p.count, &to, &from)) return;
+  if ((bytes & 3) == 0 && ((reinterpret_cast<uintptr_t>(p.base[pool]) | p.layer_stride[pool]) & 3) == 0) {
+    for (int64_t e = 0; e < bytes; e += 4) *reinterpret_cast<uint32_t*>(to + e) = *reinterpret_cast<const uint32_t*>(from + e);
+  } else {
+    for (int64_t e = 0; e < bytes; ++e) to[e] = from[e];
+  }
+}
+
+template <typename T, typename Code>
+cudaError_t launch_store(const StoreParams& p, bool vector, int64_t batch, cudaStream_t stream) {
+  // a portion of T tokens touches at most this many blocks, wherever it starts
+  const int64_t columns = std::min<int64_t>((p.tokens + p.block_size - 2) / p.block_size + 1, p.max_blocks + 1);
+  const dim3 grid(static_cast<unsigned>(columns), static_cast<unsigned>(2 * p.heads), static_cast<unsigned>(batch));
+  return vector ? launch_chained(quantized_store_kernel<T, Code, true>, grid, dim3(kStoreThreads), 0, stream, p)
+                : launch_chained(quantized_store_kernel<T, Code, false>, grid, dim3(kStoreThreads), 0, stream, p);
+}
+
+}  // namespace
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" int b200_paged_kv_store_8bit(void* key_pool, void* value_pool, float* key_scales, float* value_scales,
+                                        const int32_t* block_table, const void* key, const void* value,
+                                        const int64_t* positions, int64_t batch, int64_t heads, int64_t tokens,
+                                        int64_t head_dim, int64_t num_blocks, int64_t block_size,
+                                        int64_t max_blocks_per_sequence, const int64_t key_strides[4],
+                                        const int64_t value_strides[4], int dtype, int cache_dtype, int32_t* status,
+                                        void* stream) {
+  if (!key_pool || !value_pool || !key_scales || !value_scales || !block_table || !key || !value || !positions || !status ||
+      batch < 0 || heads <= 0 || tokens < 0 || head_dim <= 0 || num_blocks <= 0 || block_size <= 0 ||
+      max_blocks_per_sequence <= 0)
+    return B200_ERR_BAD_ARGUMENT;
+  if ((dtype != B200_BF16 && dtype != B200_F16) || (cache_dtype != B200_I8 && cache_dtype != B200_E4M3) || head_dim % 16 != 0)
+    return B200_ERR_UNSUPPORTED;
+  if (!aligned16(key_pool) || !aligned16(value_pool)) return B200_ERR_ALIGNMENT;
+  if (batch > 65535 || heads > 32767 || head_dim * block_size > (int64_t(1) << 30)) return B200_ERR_TOO_LARGE;
+  if (batch == 0 || tokens == 0) return B200_OK;
+  StoreParams p = {};
+  p.x[0] = key; p.x[1] = value;
+  for (int i = 0; i < 4; ++i) { p.strides[0][i] = key_strides[i]; p.strides[1][i] = value_strides[i]; }
+  p.pool[0] = static_cast<uint8_t*>(key_pool); p.pool[1] = static_cast<uint8_t*>(value_pool);
+  p.scales[0] = key_scales; p.scales[1] = value_scales;
+  p.table = block_table; p.positions = positions; p.status = status;
+  p.tokens = tokens; p.max_blocks = max_blocks_per_sequence; p.num_blocks = num_blocks;
+  p.heads = static_cast<int>(heads); p.dim = static_cast<int>(head_dim); p.block_size = static_cast<int>(block_size);
+  bool vector = aligned16(key) && aligned16(value);
+  for (int i = 0; i < 2; ++i) {
+    vector = vector && p.strides[i][3] == 1;
+    for (int j = 0; j < 3; ++j) vector = vector && p.strides[i][j] % 8 == 0;
+  }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t error;
+  if (dtype == B200_BF16)
+    error = cache_dtype == B200_I8 ? launch_store<__nv_bfloat16, Int8Code>(p, vector, batch, s)
+                                   : launch_store<__nv_bfloat16, E4m3Code>(p, vector, batch, s);
+  else
+    error = cache_dtype == B200_I8 ? launch_store<__half, Int8Code>(p, vector, batch, s)
+                                   : launch_store<__half, E4m3Code>(p, vector, batch, s);
+  return error == cudaSuccess ? launch_status() : B200_ERR_LAUNCH;
+}
+
+extern "C" int b200_copy_kv_blocks(const b200_block_pool* pools, int64_t pool_count, const int32_t* sources,
+                                   const int32_t* destinations, int64_t count, int64_t layers, int64_t num_blocks,
+                                   int32_t* status, void* stream) {
+  if (!pools || !sources || !destinations || !status || pool_count <= 0 || count < 0 || layers <= 0 || num_blocks <= 0)
+    return B200_ERR_BAD_ARGUMENT;
+  if (pool_count > kMaxPools) return B200_ERR_TOO_LARGE;
+  CopyParams p = {};
+  p.sources = sources; p.destinations = destinations; p.status = status;
+  p.num_blocks = num_blocks; p.layers = layers; p.count = count;
+  p.pools = static_cast<int>(pool_count);
+  for (int i = 0; i < p.pools; ++i) {
+    if (!pools[i].base || pools[i].block_bytes <= 0 || (layers > 1 && pools[i].layer_stride < num_blocks * pools[i].block_bytes))
+      return B200_ERR_BAD_ARGUMENT;
+    p.base[i] = static_cast<uint8_t*>(pools[i].base);
+    p.layer_stride[i] = pools[i].layer_stride;
+    p.block_bytes[i] = pools[i].block_bytes;
+    const int64_t units = p.block_bytes[i] >= kCopyChunk / 16 ? ceil_div(p.block_bytes[i], kCopyChunk) * count * layers
+                                                              : ceil_div(count * layers, kCopyThreads);
+    p.first_unit[i + 1] = p.first_unit[i] + units;
+  }
+  if (count == 0) return B200_OK;
+  if (p.first_unit[p.pools] > 0x7fffffff) return B200_ERR_TOO_LARGE;
+  const cudaError_t error = launch_chained(copy_blocks_kernel, dim3(static_cast<unsigned>(p.first_unit[p.pools])),
+                                           dim3(kCopyThreads), 0, static_cast<cudaStream_t>(stream), p);
+  return error == cudaSuccess ? launch_status() : B200_ERR_LAUNCH;
+}

@@ -108,6 +108,8 @@ class DeviceRuntime:
             reasons.append("negative KV position (write skipped)")
         if value & _lib.STATUS_WAIT_TIMEOUT:
             reasons.append("a bounded in-kernel wait gave up (result invalid)")
+        if value & _lib.STATUS_NOT_FINITE:
+            reasons.append("an infinity or NaN met an 8-bit format (saturated)")
         raise KernelStatusError("; ".join(reasons) or f"status word {value}")
 
 

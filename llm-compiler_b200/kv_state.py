@@ -22,7 +22,7 @@ from typing import Callable, Optional, Sequence, Tuple
 
 import torch
 
-from . import kernels
+from . import kernels, quantized_kernels
 
 
 class ExecutionError(RuntimeError):
@@ -261,11 +261,15 @@ class PagedKVCacheState(PreallocatedKVCacheState):
                            torch.full((batch, max_blocks), -1, dtype=torch.int32, device=device))
         object.__setattr__(state, "_host_table", [[] for _ in range(batch)])
         object.__setattr__(state, "_free", list(range(num_blocks - 1, -1, -1)))
+        object.__setattr__(state, "_sharers", {})  # block -> sequences that hold it, where there are several
+        object.__setattr__(state, "_pools", (key_pool, value_pool))  # [layers, blocks, ...]
         return state
 
+    _kept = ("_length_arena", "block_size", "block_table", "_host_table", "_free", "_sharers", "_pools")
+
     def _derive(self, generation: int) -> "PagedKVCacheState":
-        state = PagedKVCacheState(self.keys, self.values, self.lengths, self.capacity, generation)
-        for name in ("_length_arena", "block_size", "block_table", "_host_table", "_free"):
+        state = type(self)(self.keys, self.values, self.lengths, self.capacity, generation)
+        for name in self._kept:
             object.__setattr__(state, name, getattr(self, name))
         return state
 
@@ -289,21 +293,82 @@ class PagedKVCacheState(PreallocatedKVCacheState):
                 self._host_table[b].append(self._free.pop())
                 changed = True
         if changed:
-            host = torch.full(tuple(self.block_table.shape), -1, dtype=torch.int32)
-            for b, row in enumerate(self._host_table):
-                host[b, :len(row)] = torch.tensor(row, dtype=torch.int32)
-            self.block_table.copy_(host)
+            self._write_table()
+
+    def _write_table(self) -> None:
+        host = torch.full(tuple(self.block_table.shape), -1, dtype=torch.int32)
+        for b, row in enumerate(self._host_table):
+            host[b, :len(row)] = torch.tensor(row, dtype=torch.int32)
+        self.block_table.copy_(host)
 
     def release(self, sequence: int) -> None:
-        """Returns a finished sequence's blocks to the pool and empties its lengths."""
+        """Returns a finished sequence's blocks to the pool (those it shares stay with the others) and empties its
+        lengths."""
 
-        self._free.extend(reversed(self._host_table[sequence]))
+        self._free.extend(block for block in reversed(self._host_table[sequence]) if self._let_go(block))
         self._host_table[sequence] = []
         self.block_table[sequence].fill_(-1)
         self._length_arena[:, sequence].zero_()
 
+    def _let_go(self, block: int) -> bool:
+        """One holder of a block less; True if it was the last."""
+
+        sharers = self._sharers.pop(block, 1) - 1
+        if sharers > 1:
+            self._sharers[block] = sharers
+        return sharers == 0
+
+    def fork(self, source: int, target: int, *, tokens: Optional[int] = None) -> None:
+        """Makes the empty sequence `target` a continuation of the first `tokens` cached tokens of `source` (default: all
+        of its lengths, read from the device, which synchronises). Whole blocks are shared; a last block that is only partly
+        full is copied in every layer, one launch, so that either sequence may append to its own. Host-side, between
+        steps; every layer slot's length of `target` becomes `tokens`."""
+
+        sequences = len(self._host_table)
+        if not (0 <= source < sequences and 0 <= target < sequences) or source == target:
+            raise ExecutionError("fork needs two different sequences of this state")
+        if self._host_table[target]:
+            raise ExecutionError(f"sequence {target} still holds blocks: release it first")
+        if tokens is None:
+            tokens = int(self.lengths[0][source].item())
+        held = self._host_table[source]
+        if tokens < 0 or tokens > len(held) * self.block_size:
+            raise ExecutionError(f"sequence {source} does not hold {tokens} tokens")
+        whole, partial = divmod(tokens, self.block_size)
+        if partial and not self._free:
+            raise ExecutionError("the KV block pool is exhausted")
+        row = held[:whole]
+        for block in row:
+            self._sharers[block] = self._sharers.get(block, 1) + 1
+        if partial:
+            row = row + [self._free.pop()]
+            quantized_kernels.b200_copy_kv_blocks(self._pools, [held[whole]], [row[-1]])
+        self._host_table[target] = row
+        self._write_table()
+        self._length_arena[:len(self.keys), target] = tokens
+
+    def compact(self) -> int:
+        """Moves blocks so that those in use are the lowest of the pool, one launch, and returns their number: what is
+        behind may be given to another use. Shared blocks stay shared. Host-side, between steps."""
+
+        used = sorted({block for row in self._host_table for block in row})
+        count = len(used)
+        sources = [block for block in used if block >= count]
+        targets = sorted(set(range(count)) - set(used))
+        if sources:
+            quantized_kernels.b200_copy_kv_blocks(self._pools, sources, targets)
+            moved = dict(zip(sources, targets))
+            for row in self._host_table:
+                row[:] = [moved.get(block, block) for block in row]
+            shared = {moved.get(block, block): n for block, n in self._sharers.items()}
+            self._sharers.clear()
+            self._sharers.update(shared)
+            self._write_table()
+        self._free[:] = range(self.keys[0].shape[0] - 1, count - 1, -1)
+        return count
+
     def blocks_in_use(self) -> int:
-        return sum(len(row) for row in self._host_table)
+        return len({block for row in self._host_table for block in row})
 
     def read(self, slot: int) -> Tuple[torch.Tensor, torch.Tensor]:
         raise ExecutionError("a paged KV state has no contiguous logical view; gather through block_table")
@@ -352,6 +417,78 @@ class PagedKVCacheState(PreallocatedKVCacheState):
         run = runner or kernels.b200_paged_decode_attention
         return run(query, pool_key, pool_value, self.block_table, lengths, attention_mask, scale=scale,
                    **options)
+
+
+class QuantizedPagedKVCacheState(PagedKVCacheState):
+    """The paged state with its entries in 8 bits: pools [blocks, Hkv, block_size, D] of int8 or float8_e4m3fn codes, and
+    per layer slot `key_scales[i]` / `value_scales[i]`, float32 [blocks, Hkv], one scale for each block of tokens and KV
+    head. `store` quantises 16-bit keys and values on their way in, `decode_attention` reads codes and scales; block table,
+    lengths, `reserve`, `release`, `fork` and `compact` are the paged state's."""
+
+    @classmethod
+    def allocate_paged(cls, *, num_layers: int, batch: int, max_tokens: int, block_size: int,
+                       num_blocks: int, kv_heads: int, head_dim: int, dtype: torch.dtype,
+                       device: torch.device | str, extra_length_rows: int = 0) -> "QuantizedPagedKVCacheState":
+        if dtype not in quantized_kernels.CACHE_CODES:
+            raise ExecutionError(f"a KV state in 8 bits holds int8 or float8_e4m3fn, not {dtype}")
+        # (a pool is addressed in blocks of H x block_size x D)
+        state = super().allocate_paged(num_layers=num_layers, batch=batch, max_tokens=max_tokens, block_size=block_size,
+                                       num_blocks=num_blocks, kv_heads=kv_heads, head_dim=head_dim, dtype=dtype,
+                                       device=device, extra_length_rows=extra_length_rows)
+        pools = tuple(pool.view(num_layers, num_blocks, kv_heads, block_size, head_dim) for pool in state._pools)
+        scales = tuple(torch.zeros(num_layers, num_blocks, kv_heads, dtype=torch.float32, device=device) for _ in range(2))
+        for name, value in (("keys", tuple(pools[0])), ("values", tuple(pools[1])), ("key_scales", tuple(scales[0])),
+                            ("value_scales", tuple(scales[1])), ("_pools", (*pools, *scales))):
+            object.__setattr__(state, name, value)
+        return state
+
+    _kept = PagedKVCacheState._kept + ("key_scales", "value_scales")
+
+    def gather(self, slot: int, sequence: int, tokens: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The values that the first `tokens` K and V entries of one sequence stand for, float32 T x H x D (a host-driven
+        debugging / test helper)."""
+
+        blocks = torch.tensor(self._host_table[sequence], dtype=torch.int64, device=self.keys[slot].device)
+
+        def rows(pool: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+            entries = pool[blocks].float() * scales[blocks][:, :, None, None]
+            return entries.transpose(1, 2).flatten(0, 1)[:tokens]
+
+        return rows(self.keys[slot], self.key_scales[slot]), rows(self.values[slot], self.value_scales[slot])
+
+    def store(self, slot: int, key: torch.Tensor, value: torch.Tensor, positions: torch.Tensor, *,
+              writer: Optional[Callable] = None) -> "QuantizedPagedKVCacheState":
+        pool_key, pool_value, _ = self._slot(slot)
+        if key.shape != value.shape or key.ndim != 4:
+            raise ExecutionError("KV store needs K and V of one B x H x T x D shape")
+        if key.shape[0] != self.block_table.shape[0] or key.shape[1] != pool_key.shape[1] or \
+                key.shape[3] != pool_key.shape[3]:
+            raise ExecutionError("KV store batch, heads or head_dim mismatch")
+        if positions.shape != (key.shape[0],) or positions.dtype != torch.int64:
+            raise ExecutionError("KV store positions must be a one-dimensional int64 batch tensor")
+        if key.shape[2] > self.capacity:
+            raise ExecutionError(f"KV store exceeds capacity {self.capacity}")
+        (writer or quantized_kernels.b200_paged_kv_store_8bit)(
+            pool_key, pool_value, self.key_scales[slot], self.value_scales[slot], self.block_table, key, value, positions)
+        return self
+
+    def decode_attention(self, slot: int, query: torch.Tensor, attention_mask: torch.Tensor, *,
+                         groups: int, scale: float, runner: Optional[Callable] = None,
+                         **options) -> torch.Tensor:
+        pool_key, pool_value, lengths = self._slot(slot)
+        if query.ndim != 4 or query.shape[2] != 1:
+            raise ExecutionError("decode attention query must be B x H x 1 x D")
+        if attention_mask is not None and (attention_mask.ndim != 4 or attention_mask.shape[2] != 1 or
+                                           attention_mask.shape[-1] > self.capacity):
+            raise ExecutionError("decode attention mask must be B x 1 x 1 x S with S <= capacity")
+        if groups <= 0 or query.shape[1] != pool_key.shape[1] * groups or \
+                query.shape[3] != pool_key.shape[3]:
+            raise ExecutionError("decode attention GQA groups or head_dim mismatch")
+        if options.get("split_tokens") is None:
+            options.pop("split_tokens", None)
+        run = runner or quantized_kernels.b200_paged_decode_attention_8bit
+        return run(query, pool_key, pool_value, self.key_scales[slot], self.value_scales[slot], self.block_table, lengths,
+                   attention_mask, scale=scale, **options)
 
 
 class SlotState:
