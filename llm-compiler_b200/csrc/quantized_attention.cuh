@@ -1,0 +1,594 @@
+// Decode attention over a paged cache in 8 bits: the kernel and its launch, instantiated per code type in a .cu of its own.
+//
+//     out = sum_t softmax_t(scale * ks * (q . ck_t) + mask_t) vs cv_t,   t < length,
+// with ck, cv the codes of token t and ks, vs the scales of its block. The G query heads of a KV head share one read of its
+// codes. What bounds it is that read: 2 * length * D bytes per KV head; per byte there are 2 G operations, which the tensor
+// cores take, and one conversion, which the CUDA cores do.
+//
+// Products. Codes become fp16, which holds every int8 and e4m3 value exactly, and are multiplied on mma m16n8k16 with the
+// TOKENS (or the elements of D) along M and the heads along N = 8: S^T = K Q^T, O^T = V^T P^T. Up to eight heads of a group
+// then cost one n-tile, where heads along M would pad them to sixteen. No element is shuffled:
+//  - the sum over D may run in any order, so a lane reads 16 consecutive bytes of a token as its part of four k-steps, and q
+//    is laid out once to match;
+//  - V comes through ldmatrix.trans in units of two bytes: a lane gets d and d + 1 of two tokens, and splits them into the
+//    two tokens' even and odd element, which are rows of two halves of an A operand;
+//  - P^T is transposed 8 x 8 by movmatrix.
+// q is brought to [1, 2) per head by a power of two (exact; fp16 alone would overflow), which goes back into the scores.
+//
+// Scales. ks multiplies the scores. vs is folded into the probabilities relative to a running reference `vref`, which the
+// accumulators are carried in; it follows vs (accumulators rescaled) only when they are more than 16 apart, so P stays well
+// inside fp16. P itself is fp16 (2^-11; it is at most e^5, below), its sum fp32. The running maximum moves only when a score passes
+// it by more than 5: the softmax is the same, and most tiles need no reduction across lanes.
+//
+// Work. A CTA serves `split_tokens` tokens of one (sequence, KV head, up to 8 NT heads). Its four warps take the 32-token
+// tiles in turn, each through a ring of its own that TMA fills: a tile never spans two blocks (block sizes are multiples of
+// 32), is contiguous in the pool, and is one box for K and one for V. Warps merge through shared memory; with several
+// splits the CTA that arrives last adds the partials in split order, so results do not depend on timing.
+#pragma once
+
+#include <algorithm>
+#include <type_traits>
+
+#include "quantized.cuh"
+#include "tensor_map.cuh"
+
+namespace b200 {
+namespace cache_attention {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kTile = 32;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kSlack = 5.0f;  // how far a score may pass the running maximum before it moves
+constexpr int64_t kCounterBytes = 65536;
+constexpr int64_t kMaxCounters = kCounterBytes / 4;
+
+struct Params {
+  const void* q;
+  const float* key_scales;
+  const float* value_scales;
+  const int32_t* table;
+  const int64_t* lengths;
+  const void* mask;
+  void* out;
+  float* ws_o;     // [items, splits, heads of a block, D]
+  float* ws_ml;    // [items, splits, heads of a block, 2]
+  int* counters;   // [items], zero between calls
+  int32_t* status;
+  int64_t q_batch_stride, q_head_stride, mask_batch_stride, num_blocks, max_blocks, mask_len, split_tokens;
+  int q_heads, kv_heads, group, head_blocks, block_heads, block_size, mask_dtype, num_splits;
+  int half;        // q and out are fp16, else bf16
+  int q_vector;    // rows of q may be read 16 bytes at a time
+  float scale;
+  uint32_t wait_limit;
+  int drop_loads;
+};
+
+// Four codes of a word as fp16: neighbours (bytes 0, 1 and 2, 3) for K, and every other (0, 2 and 1, 3) for V.
+template <typename Code>
+struct Convert;
+template <>
+struct Convert<Int8Code> {
+  // 0x64xx is 1024 + xx: a code with its sign bit turned, 0 .. 255, lands there by a byte permutation; 1152 comes off.
+  __device__ static uint32_t back(uint32_t pair) {
+    const uint32_t bias = 0x64806480u;
+    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&pair), *reinterpret_cast<const __half2*>(&bias));
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  __device__ static void neighbours(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    w ^= 0x80808080u;
+    lo = back(__byte_perm(w, 0x64646464u, 0x4140));
+    hi = back(__byte_perm(w, 0x64646464u, 0x4342));
+  }
+  __device__ static void every_other(uint32_t w, uint32_t& even, uint32_t& odd) {
+    w ^= 0x80808080u;
+    even = back(__byte_perm(w, 0x64646464u, 0x4240));
+    odd = back(__byte_perm(w, 0x64646464u, 0x4341));
+  }
+};
+template <>
+struct Convert<E4m3Code> {
+  __device__ static uint32_t two(uint16_t codes) {
+    uint32_t pair;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(pair) : "h"(codes));
+    return pair;
+  }
+  __device__ static void neighbours(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    lo = two(static_cast<uint16_t>(w));
+    hi = two(static_cast<uint16_t>(w >> 16));
+  }
+  __device__ static void every_other(uint32_t w, uint32_t& even, uint32_t& odd) {
+    neighbours(__byte_perm(w, 0u, 0x3120), even, odd);
+  }
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ float load_mask(const Params& p, int64_t i) {
+  if (p.mask_dtype == B200_F32) return static_cast<const float*>(p.mask)[i];
+  if (p.mask_dtype == B200_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p.mask)[i]);
+  return __half2float(static_cast<const __half*>(p.mask)[i]);
+}
+
+template <int D>
+struct Shape {
+  static constexpr int kRowBytes = D < 128 ? D : 128;         // a box is one swizzle span wide
+  static constexpr int kBoxes = D / kRowBytes;
+  static constexpr int kBoxBytes = kTile * kRowBytes;
+  static constexpr int kTileBytes = kTile * D;                 // K or V
+  static constexpr int kStages = D == 64 ? 4 : 3;
+  static constexpr int kRingBytes = kWarps * kStages * 2 * kTileBytes;
+  // byte offset of 16-byte chunk `chunk` of row `row` in a tile
+  __device__ static uint32_t at(int row, int chunk) {
+    if (D == 64) return row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
+    return (chunk >> 3) * kBoxBytes + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
+  }
+  // Which of eight tokens is row r of a fragment: rows that one 128-byte phase of a read takes together differ in bit 2,
+  // so that their swizzled chunks lie in different halves of the banks (64-byte rows: two rows make 128 bytes anyway).
+  __device__ static int token(int r) { return D == 64 ? r : (r >> 1) | ((r & 1) << 2); }
+};
+
+template <typename Code, int D, int NT, bool kMask>
+__global__ void __launch_bounds__(kThreads)
+cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_map,
+                       const __grid_constant__ CUtensorMap value_map) {
+  using S = Shape<D>;
+  constexpr int kStages = S::kStages, kSteps = D / 16, kHeads = 8 * NT;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  __shared__ __align__(8) uint64_t full[kWarps * kStages];
+  __shared__ float merge_m[kWarps][kHeads], merge_l[kWarps][kHeads];
+  __shared__ int last_flag;
+
+  grid_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
+  const int split = blockIdx.x, item_head = blockIdx.y, kv = item_head / p.head_blocks, hb = item_head % p.head_blocks;
+  const int64_t b = blockIdx.z;
+  const int head0 = kv * p.group + hb * p.block_heads;
+  const int heads = min(p.block_heads, p.group - hb * p.block_heads);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kWarps * kStages; ++s) mbarrier_init(smem_u32(&full[s]), 1);
+    fence_mbarrier_init();
+  }
+  grid_dependency_wait_cta();
+
+  int64_t length = max(p.lengths[b], static_cast<int64_t>(0));
+  if (length > p.mask_len) {
+    length = p.mask_len;
+    if (threadIdx.x == 0 && split == 0 && item_head == 0) atomicOr(p.status, B200_STATUS_LENGTH_OVER_MASK);
+  }
+  // splits that have tokens; the last one of the grid takes whatever is behind it
+  const int64_t wanted = (length + p.split_tokens - 1) / p.split_tokens;
+  const int splits = static_cast<int>(min(max(wanted, static_cast<int64_t>(1)), static_cast<int64_t>(p.num_splits)));
+  if (split >= splits) return;
+  const int64_t start = split * p.split_tokens, end = split == splits - 1 ? length : start + p.split_tokens;
+  const int64_t first_tile = start / kTile;  // (split_tokens is a multiple of kTile)
+  const int tiles = static_cast<int>((end - start + kTile - 1) / kTile);
+  const int mine = tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0;  // tiles warp, warp + kWarps, ...
+
+  const uint32_t ring = smem_u32(smem) + warp * kStages * 2 * S::kTileBytes;
+  const uint32_t bars = smem_u32(&full[warp * kStages]);
+  const int tiles_per_block = p.block_size / kTile;
+
+  // Block and scales of this warp's tiles, 32 tiles ahead in the lanes: lane i of window w holds tile 32 w + i.
+  struct Window { int block; float ks, vs; };
+  bool bad = false;
+  auto look_up = [&](int it) {
+    Window w = {-1, 0.0f, 0.0f};
+    if (it < mine) {
+      const int64_t column = (first_tile + warp + static_cast<int64_t>(it) * kWarps) / tiles_per_block;
+      w.block = p.table[b * p.max_blocks + column];
+      if (w.block < 0 || w.block >= p.num_blocks) {
+        w.block = -1;
+        bad = true;
+      } else {
+        const int64_t slab = static_cast<int64_t>(w.block) * p.kv_heads + kv;
+        w.ks = p.key_scales[slab];
+        w.vs = p.value_scales[slab];
+      }
+    }
+    return w;
+  };
+  Window now = look_up(lane), next = look_up(32 + lane);
+  int base = 0;  // of `now`
+  int issued = 0;
+  auto issue = [&](int it) {  // whole warp; a tile without a block has no copy
+    const int block = __shfl_sync(0xffffffffu, it - base < 32 ? now.block : next.block, it & 31);
+    if (block >= 0 && lane == 0 && !p.drop_loads) {
+      const int stage = it % kStages;
+      const uint32_t bar = bars + stage * 8, dst = ring + stage * 2 * S::kTileBytes;
+      const int row = static_cast<int>((first_tile + warp + static_cast<int64_t>(it) * kWarps) % tiles_per_block) * kTile;
+      const int slab = block * p.kv_heads + kv;
+      mbarrier_arrive_expect_tx(bar, 2 * S::kTileBytes);
+#pragma unroll
+      for (int x = 0; x < S::kBoxes; ++x) {
+        tma_load_3d(dst + x * S::kBoxBytes, &key_map, bar, x * S::kRowBytes, row, slab);
+        tma_load_3d(dst + S::kTileBytes + x * S::kBoxBytes, &value_map, bar, x * S::kRowBytes, row, slab);
+      }
+    }
+    issued = it + 1;
+  };
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s)
+    if (s < mine) issue(s);
+
+  // ---- q as B operands: lane (g, j) holds head g, elements 64 c + 16 j .. + 15 of every 64 ----
+  uint32_t qb[NT][kSteps][2];
+  float factor[NT][2];  // score of one product, for this lane's columns (heads 2 j, 2 j + 1)
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int head = 8 * t + g;
+    float v[D / 4];
+    if (head < heads) {
+      const int64_t offset = b * p.q_batch_stride + (head0 + head) * p.q_head_stride + 16 * j;
+      const uint16_t* q = static_cast<const uint16_t*>(p.q) + offset;
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) {
+        uint32_t raw[8];
+        if (p.q_vector) {
+          const uint4 a = *reinterpret_cast<const uint4*>(q + 64 * c), d = *reinterpret_cast<const uint4*>(q + 64 * c + 8);
+          raw[0] = a.x; raw[1] = a.y; raw[2] = a.z; raw[3] = a.w;
+          raw[4] = d.x; raw[5] = d.y; raw[6] = d.z; raw[7] = d.w;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            raw[e] = q[64 * c + 2 * e] | (static_cast<uint32_t>(q[64 * c + 2 * e + 1]) << 16);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          v[16 * c + 2 * e] = p.half ? Elem<__half>::lo(raw[e]) : bf16_lo(raw[e]);
+          v[16 * c + 2 * e + 1] = p.half ? Elem<__half>::hi(raw[e]) : bf16_hi(raw[e]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < D / 4; ++e) v[e] = 0.0f;
+    }
+    float most = 0.0f;
+#pragma unroll
+    for (int e = 0; e < D / 4; ++e) most = fmaxf(most, fabsf(v[e]));
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    const uint32_t exponent = min(max(__float_as_uint(most) >> 23, 1u), 253u);
+    const float down = __uint_as_float((254u - exponent) << 23), up = __uint_as_float(exponent << 23);
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {  // k-step i: bytes 4 (i % 4) .. + 3 of the lane's 16 in 64-element group i / 4
+      const int e = 16 * (i / 4) + 4 * (i % 4);
+      qb[t][i][0] = pack_half2(v[e] * down, v[e + 1] * down);
+      qb[t][i][1] = pack_half2(v[e + 2] * down, v[e + 3] * down);
+    }
+    factor[t][0] = p.scale * __shfl_sync(0xffffffffu, up, 8 * j);
+    factor[t][1] = p.scale * __shfl_sync(0xffffffffu, up, 8 * j + 4);
+  }
+
+  float m[NT][2], l[NT][2], o[NT][kSteps][4];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    m[t][0] = m[t][1] = -INFINITY;
+    l[t][0] = l[t][1] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.0f;
+  }
+  float vref = 0.0f;
+  bool timed_out = false;
+  const int my_token = S::token(g);
+  float mask_next[4];
+  auto fetch_mask = [&](int it) {
+    if constexpr (kMask) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int64_t token = (first_tile + warp + static_cast<int64_t>(it) * kWarps) * kTile + 8 * r + my_token;
+        mask_next[r] = it < mine && token < end ? load_mask(p, b * p.mask_batch_stride + token) : 0.0f;
+      }
+    }
+  };
+  fetch_mask(0);
+  // phases: a stage completes only where a copy was issued, so a tile without a block does not turn its parity
+  uint32_t phase = 0;
+
+  int it = 0;
+  for (; it < mine; ++it) {
+    if (it - base == 32) {
+      now = next;
+      base = it;
+      next = look_up(base + 32 + lane);
+    }
+    const int stage = it % kStages, at_lane = it & 31;
+    const int block = __shfl_sync(0xffffffffu, now.block, at_lane);
+    const float ks = __shfl_sync(0xffffffffu, now.ks, at_lane), vs = __shfl_sync(0xffffffffu, now.vs, at_lane);
+    if (block >= 0) {
+      if (!__all_sync(0xffffffffu, mbarrier_wait_bounded(bars + stage * 8, (phase >> stage) & 1, p.wait_limit))) {
+        timed_out = true;
+        break;
+      }
+      phase ^= 1u << stage;
+    }
+    __syncwarp();  // every lane is done with the stage that is filled next
+    if (it + kStages - 1 < mine) issue(it + kStages - 1);
+    float extra[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) extra[r] = kMask ? mask_next[r] : 0.0f;
+    fetch_mask(it + 1);
+    if (block < 0) continue;
+    const uint32_t keys = ring + stage * 2 * S::kTileBytes, values = keys + S::kTileBytes;
+    const int64_t token0 = (first_tile + warp + static_cast<int64_t>(it) * kWarps) * kTile;
+    const int valid = static_cast<int>(min(end - token0, static_cast<int64_t>(kTile)));
+
+    // ---- scores of 32 tokens ----
+    float s[NT][2][4];
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) s[t][mt][0] = s[t][mt][1] = s[t][mt][2] = s[t][mt][3] = 0.0f;
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) {
+        uint32_t w0[4], w1[4];
+        const int row = 16 * mt + my_token;
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w0[0]), "=r"(w0[1]), "=r"(w0[2]), "=r"(w0[3])
+                     : "r"(keys + S::at(row, 4 * c + j)));
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w1[0]), "=r"(w1[1]), "=r"(w1[2]), "=r"(w1[3])
+                     : "r"(keys + S::at(row + 8, 4 * c + j)));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t a[4];
+          Convert<Code>::neighbours(w0[i], a[0], a[2]);
+          Convert<Code>::neighbours(w1[i], a[1], a[3]);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) mma_f16_16816(s[t][mt], a, qb[t][4 * c + i][0], qb[t][4 * c + i][1]);
+        }
+      }
+    }
+    bool over = false;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float f = ks * factor[t][h], line = m[t][h] + kSlack;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {  // token 8 r + my_token
+          float& x = s[t][r >> 1][2 * (r & 1) + h];
+          x = kMask ? fmaf(x, f, extra[r]) : x * f;
+          if (valid < kTile && 8 * r + my_token >= valid) x = -INFINITY;
+          over = over || x > line;
+        }
+      }
+    if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float top = fmaxf(fmaxf(s[t][0][h], s[t][0][2 + h]), fmaxf(s[t][1][h], s[t][1][2 + h]));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+          top = fmaxf(top, m[t][h]);
+          const float keep = top == -INFINITY ? 1.0f : exp2_fast((m[t][h] - top) * kLog2e);
+          m[t][h] = top;
+          l[t][h] *= keep;
+#pragma unroll
+          for (int i = 0; i < kSteps; ++i) {
+            o[t][i][h] *= keep;
+            o[t][i][2 + h] *= keep;
+          }
+        }
+    }
+    if (vs > 0.0f && !(vs <= 16.0f * vref && vref <= 16.0f * vs)) {
+      // (2^60: far enough that nothing of the smaller side is seen in the larger one)
+      const float unit = vref > 0.0f ? fminf(fmaxf(vs, vref * 0x1p-60f), vref * 0x1p60f) : vs;
+      const float keep = vref > 0.0f ? vref / unit : 1.0f;
+      vref = unit;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+          o[t][i][0] *= keep; o[t][i][1] *= keep; o[t][i][2] *= keep; o[t][i][3] *= keep;
+        }
+    }
+    float weight = vref > 0.0f ? vs / vref : vs;
+    if (weight > 16.0f) weight = 16.0f;  // (a NaN stays)
+
+    // ---- probabilities, transposed into B operands ----
+    uint32_t pb[NT][2][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const float m0 = m[t][0] == -INFINITY ? 0.0f : m[t][0], m1 = m[t][1] == -INFINITY ? 0.0f : m[t][1];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float p0 = exp2_fast((s[t][r >> 1][2 * (r & 1)] - m0) * kLog2e);
+        const float p1 = exp2_fast((s[t][r >> 1][2 * (r & 1) + 1] - m1) * kLog2e);
+        l[t][0] += p0;
+        l[t][1] += p1;
+        pb[t][r >> 1][r & 1] = transpose_8x8(pack_half2(p0 * weight, p1 * weight));
+      }
+    }
+    if constexpr (std::is_same<Code, E4m3Code>::value) {
+      if (valid < kTile) {  // codes behind the end may be NaN, which a weight of zero does not silence
+        constexpr int kChunks = D / 16;
+        for (int i = lane; i < (kTile - valid) * kChunks; i += 32)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(values + S::at(valid + i / kChunks, i % kChunks)),
+                       "r"(0u) : "memory");
+        __syncwarp();
+      }
+    }
+    // ---- O^T += V^T P^T ----
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t r[4];
+        ldmatrix_x4_trans(r, values + S::at(16 * mt + ((lane >> 3) & 1) * 8 + S::token(lane & 7), 2 * c + (lane >> 4)));
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t a[4];
+          Convert<Code>::every_other(r[2 * half], a[0], a[1]);
+          Convert<Code>::every_other(r[2 * half + 1], a[2], a[3]);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) mma_f16_16816(o[t][2 * c + half], a, pb[t][mt][0], pb[t][mt][1]);
+        }
+      }
+  }
+  if (bad) atomicOr(p.status, B200_STATUS_BAD_POSITION);
+  if (timed_out) {  // copies in flight still write to this CTA's memory: wait for them, with the same limit
+    for (; it < issued; ++it) mbarrier_wait_bounded(bars + it % kStages * 8, (phase >> it % kStages) & 1, p.wait_limit);
+    if (lane == 0) atomicOr(p.status, B200_STATUS_WAIT_TIMEOUT);
+  }
+
+  // ---- the four warps' parts: O in units of 1, through the ring's memory ----
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float sum = l[t][h];
+      sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+      if (g == 0) {
+        merge_m[warp][8 * t + 2 * j + h] = m[t][h];
+        merge_l[warp][8 * t + 2 * j + h] = sum;
+      }
+    }
+  __syncthreads();  // every ring is done with
+  float* parts = reinterpret_cast<float*>(smem);  // [warp][head][D]
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int head = 8 * t + 2 * j + h;
+        *reinterpret_cast<float2*>(parts + (warp * kHeads + head) * D + 16 * i + 2 * g) =
+            make_float2(o[t][i][h] * vref, o[t][i][2 + h] * vref);
+      }
+  __syncthreads();
+  const int64_t item = b * gridDim.y + item_head;
+  for (int e = threadIdx.x; e < heads * D; e += kThreads) {
+    const int head = e / D, d = e % D;
+    float top = -INFINITY, sum = 0.0f, value = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, merge_m[w][head]);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float mw = merge_m[w][head], weight = mw == -INFINITY ? 0.0f : exp2_fast((mw - top) * kLog2e);
+      sum = fmaf(weight, merge_l[w][head], sum);
+      value = fmaf(weight, parts[(w * kHeads + head) * D + d], value);
+    }
+    if (splits == 1) {
+      const int64_t at = (b * p.q_heads + head0 + head) * D + d;
+      const float y = value / sum;  // (0 / 0 = NaN for a sequence without tokens)
+      if (p.half) static_cast<__half*>(p.out)[at] = __float2half_rn(y);
+      else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(y);
+    } else {
+      const int64_t part = (item * p.num_splits + split) * p.block_heads + head;
+      p.ws_o[part * D + d] = value;
+      if (d == 0) {
+        p.ws_ml[2 * part] = top;
+        p.ws_ml[2 * part + 1] = sum;
+      }
+    }
+  }
+  if (splits == 1) return;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) last_flag = atomicAdd(p.counters + item, 1) == splits - 1;
+  __syncthreads();
+  if (!last_flag) return;
+  __threadfence();
+  for (int e = threadIdx.x; e < heads * D / 4; e += kThreads) {
+    const int head = e / (D / 4), d = (e % (D / 4)) * 4;
+    const int64_t first = item * p.num_splits * p.block_heads + head;
+    float top = -INFINITY, sum = 0.0f;
+    float4 value = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int s0 = 0; s0 < splits; s0 += 8) {  // eight loads in flight
+      float2 ml[8];
+      float4 part[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool there = s0 + i < splits;
+        const int64_t at = first + static_cast<int64_t>(there ? s0 + i : s0) * p.block_heads;
+        ml[i] = __ldcg(reinterpret_cast<const float2*>(p.ws_ml) + at);
+        part[i] = __ldcg(reinterpret_cast<const float4*>(p.ws_o + at * D + d));
+        if (!there) ml[i] = make_float2(-INFINITY, 0.0f);
+      }
+      float over_all = top;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) over_all = fmaxf(over_all, ml[i].x);
+      const float keep = top == -INFINITY ? 0.0f : exp2_fast((top - over_all) * kLog2e);
+      top = over_all;
+      sum *= keep;
+      value.x *= keep; value.y *= keep; value.z *= keep; value.w *= keep;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (s0 + i >= splits) break;
+        const float weight = ml[i].x == -INFINITY ? 0.0f : exp2_fast((ml[i].x - top) * kLog2e);
+        sum = fmaf(weight, ml[i].y, sum);
+        value.x = fmaf(weight, part[i].x, value.x); value.y = fmaf(weight, part[i].y, value.y);
+        value.z = fmaf(weight, part[i].z, value.z); value.w = fmaf(weight, part[i].w, value.w);
+      }
+    }
+    const int64_t at = (b * p.q_heads + head0 + head) * D + d;
+    const uint32_t lo = p.half ? pack_half2(value.x / sum, value.y / sum) : pack_bf16x2(value.x / sum, value.y / sum);
+    const uint32_t hi = p.half ? pack_half2(value.z / sum, value.w / sum) : pack_bf16x2(value.z / sum, value.w / sum);
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = make_uint2(lo, hi);
+  }
+  if (threadIdx.x == 0) p.counters[item] = 0;
+}
+
+// [slabs, block_size, D] codes of one (block, head) after another, in boxes of 32 tokens x one swizzle span.
+template <int D>
+bool make_pool_map(CUtensorMap* map, const void* base, int64_t slabs, int64_t block_size) {
+  EncodeTiledFn encode = tensor_map_encoder();
+  if (encode == nullptr) return false;
+  const cuuint64_t dims[3] = {D, static_cast<cuuint64_t>(block_size), static_cast<cuuint64_t>(slabs)};
+  const cuuint64_t strides[2] = {D, static_cast<cuuint64_t>(D * block_size)};
+  const cuuint32_t box[3] = {Shape<D>::kRowBytes, kTile, 1}, element_strides[3] = {1, 1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, element_strides,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename Code, int D, int NT, bool kMask>
+int launch_shape(const Params& p, const void* keys, const void* values, int64_t batch, cudaStream_t stream) {
+  CUtensorMap key_map, value_map;
+  if (!make_pool_map<D>(&key_map, keys, p.num_blocks * p.kv_heads, p.block_size) ||
+      !make_pool_map<D>(&value_map, values, p.num_blocks * p.kv_heads, p.block_size))
+    return B200_ERR_UNSUPPORTED;
+  constexpr int smem = std::max(Shape<D>::kRingBytes, kWarps * 8 * NT * D * 4);
+  auto kernel = cache_attention_kernel<Code, D, NT, kMask>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return B200_ERR_LAUNCH;
+  const dim3 grid(static_cast<unsigned>(p.num_splits), static_cast<unsigned>(p.kv_heads * p.head_blocks),
+                  static_cast<unsigned>(batch));
+  return launch_chained(kernel, grid, dim3(kThreads), smem, stream, p, key_map, value_map) == cudaSuccess ? launch_status()
+                                                                                                   : B200_ERR_LAUNCH;
+}
+template <typename Code, int D, int NT>
+int launch_mask(const Params& p, const void* keys, const void* values, int64_t batch, cudaStream_t stream) {
+  return p.mask != nullptr ? launch_shape<Code, D, NT, true>(p, keys, values, batch, stream)
+                           : launch_shape<Code, D, NT, false>(p, keys, values, batch, stream);
+}
+// n-tiles of heads: one up to eight heads of a block, else two (head_dim 256: one, its accumulators fill the registers)
+template <typename Code>
+int launch_code(const Params& p, const void* keys, const void* values, int64_t batch, int64_t dim, cudaStream_t stream) {
+  const bool one = p.block_heads <= 8;
+  if (dim == 64)
+    return one ? launch_mask<Code, 64, 1>(p, keys, values, batch, stream) : launch_mask<Code, 64, 2>(p, keys, values, batch, stream);
+  if (dim == 128)
+    return one ? launch_mask<Code, 128, 1>(p, keys, values, batch, stream) : launch_mask<Code, 128, 2>(p, keys, values, batch, stream);
+  return launch_mask<Code, 256, 1>(p, keys, values, batch, stream);
+}
+
+int launch_int8(const Params& p, const void* keys, const void* values, int64_t batch, int64_t dim, cudaStream_t stream);
+int launch_e4m3(const Params& p, const void* keys, const void* values, int64_t batch, int64_t dim, cudaStream_t stream);
+
+}  // namespace cache_attention
+}  // namespace b200
