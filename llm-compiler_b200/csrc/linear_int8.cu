@@ -1,82 +1,601 @@
-// Projections in 8-bit integers: y = (c_x . c_w) s_x s_w + bias, then SwiGLU or a residual, rounded once.
+// Projections in 8-bit integers on the tensor cores: y = (c_x . c_w) s_x s_w + bias, then SwiGLU or a residual, rounded once.
 //
-// c_x [M, K] and c_w [N, K] are codes with a scale per row (token) and per output column; their products are summed in
-// 32-bit integers, which is exact, so a result does not depend on the order or the split of the sum. K is at most
-// 131056: 131056 * 128 * 128 is below 2^31.
+// c_x [M, K] and c_w [N, K] are codes with a scale per row (token) and per output column. tcgen05.mma kind::i8 multiplies
+// 32 of them along K in the time of 16 bf16 and sums in 32-bit integers, which is exact (K is at most 131056: 131056 * 128 *
+// 128 is below 2^31): the result does not depend on the order or on the split of a sum, and a projection may be cut
+// anywhere along K. Both operands are K-major; a stage of the rings holds 128 codes of K, one 128-byte swizzled row each,
+// copied by TMA with zeros beyond M, N and K. Two kernels:
+//
+// linear_int8_stream_kernel, up to 256 rows (decode, short prompts): bound by the read of the weight. The WEIGHT's columns
+//   lie along the product's M (128 of them a tile) and all rows of x along its N, so every weight byte is read once and no
+//   row of x is padded beyond the next multiple of 16. The k-blocks of all tiles are one list, of which every CTA (one
+//   per SM) takes an equal run: any N and K fill the GPU alike. A tile that several CTAs share is summed in the workspace
+//   by integer additions, whose order does not matter, and finished by the CTA that arrives last.
+// linear_int8_pair_kernel, beyond: bound by the tensor cores. Two SMs work on one tile of 256 rows x up to 256 columns
+//   (cta_group::2): each holds half of both operands, which halves the bytes that shared memory and L2 deliver per product
+//   (at 128 x 256 a CTA they are what limits it: 96 of 128 bytes a cycle in, as many out). Two accumulators alternate, so
+//   the epilogue of a tile runs under the products of the next.
+#include <algorithm>
+
 #include "quantized.cuh"
+#include "tcgen05.cuh"
+#include "tensor_map.cuh"
 
 namespace b200 {
 namespace {
 
 constexpr int kMaxK = 131056;
+constexpr int kBK = 128;          // codes of a k-block: one 128-byte row
+constexpr int kEpilogueWarps = 4;
+constexpr int kThreads = (kEpilogueWarps + 2) * 32;  // and a producer and a product warp
+constexpr int kRowsAtMost = 256;  // of the stream kernel
+constexpr int kRingBytes = 192 * 1024;
+constexpr int64_t kCounterBytes = 4096;
 
 struct Int8LinearParams {
-  const int8_t* x;
   const float* x_scales;
-  const int8_t* w;
   const float* w_scales;
   const void* bias;
   const void* residual;
   void* out;
+  int32_t* sums;      // stream: [CTAs][rows][128] of tiles that are shared, zero between calls
+  int32_t* counters;  // stream: one per CTA, zero between calls
   int32_t* status;
   int m, k, n, epilogue;
+  int cols;     // stream: rows of x, rounded up to 16, the product's N. pair: columns of a tile
+  int stages;   // stream
+  int n_fastest;  // pair: order of the tiles
+  uint32_t wait_limit;
+  int drop_loads;
 };
 
-// 64 x 64 outputs a CTA of 256 threads, 4 x 4 each, K in steps of 64 codes through shared memory.
+// Instruction descriptor of kind::i8: 32-bit integer accumulator, both operands signed, K-major.
+__host__ __device__ constexpr uint32_t instruction_descriptor_i8(int m, int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+template <int CTAS>
+__device__ __forceinline__ void umma_i8_if(uint32_t leader, uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                           uint32_t accumulate) {
+  if constexpr (CTAS == 1)
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(leader) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(leader) : "memory");
+}
+// The products so far arrive on the barrier at this offset in both CTAs of the pair.
+__device__ __forceinline__ void umma_commit_pair_if(uint32_t leader, uint32_t bar) {
+  asm volatile("{\n\t.reg .pred q;\n\t.reg .b16 both;\n\tsetp.ne.b32 q, %1, 0;\n\tmov.b16 both, 3;\n\t"
+               "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], both;\n\t}"
+               ::"r"(bar), "r"(leader) : "memory");
+}
+// A box into this CTA's memory whose bytes count on a barrier of the pair's first CTA.
+__device__ __forceinline__ void tma_load_pair_if(uint32_t leader, uint32_t dst, const void* tensor_map, uint32_t bar, int c0, int c1) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t}"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tensor_map)), "r"(bar), "r"(c0), "r"(c1), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, int rank) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+  return remote;
+}
+
+// A producer that gives up at stage s of turn `turn`: the copies that it has asked for still write to shared memory.
+__device__ __forceinline__ void wait_for_copies(uint64_t* full, int stages, int s, int turn, uint32_t limit) {
+  for (int i = 0; i < stages; ++i) {
+    const int last = i < s ? turn : turn - 1;
+    if (last >= 0) mbarrier_wait_warp(smem_u32(&full[i]), last & 1, limit);
+  }
+}
+
+// gate / (1 + e^-gate) * up on the special-function unit: the exponential and the quotient are good to a few units of 2^-23.
+// (1 + e^-gate is infinite below -88, where the quotient, -0, is the right answer; a gate of -infinity gives NaN as 0 * infinity does.)
+__device__ __forceinline__ float silu_times(float gate, float up) {
+  return __fdividef(gate, 1.0f + __expf(-gate)) * up;
+}
+
+// ------------------------------------------------------------------------------------------------------------ stream ----
+__device__ __forceinline__ bool all_of_epilogue(bool mine) {
+  uint32_t all;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.and.pred q, 1, 128, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+               : "=r"(all) : "r"(static_cast<uint32_t>(mine)) : "memory");
+  return all != 0;
+}
+
 template <typename T>
-__global__ void __launch_bounds__(256) linear_int8_kernel(const Int8LinearParams p) {
-  __shared__ uint32_t xs[64][17], ws[64][17];
+__global__ void __launch_bounds__(kThreads, 1)
+linear_int8_stream_kernel(const Int8LinearParams p, const __grid_constant__ CUtensorMap w_map,
+                          const __grid_constant__ CUtensorMap x_map) {
+  constexpr int kMaxStages = 10;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2];
+  __shared__ float scales[kRowsAtMost];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int failed, last_flag;
+
   grid_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int stages = p.stages, stage_bytes = (128 + p.cols) * 128;
+  int acc_columns = 16;  // of an accumulator, a power of two
+  while (acc_columns < p.cols) acc_columns *= 2;
+  const int tmem_columns = 2 * acc_columns;
+  const uint32_t smem_base = smem_u32(smem);
+  const int nkb = (p.k + kBK - 1) / kBK, tiles = (p.n + 127) / 128, total = tiles * nkb, ctas = gridDim.x;
+  const int share = total / ctas, more_by_one = total - share * ctas;
+  auto run_start = [&](int c) { return c * share + min(c, more_by_one); };
+  const int run_first = run_start(blockIdx.x), run_end = run_start(blockIdx.x + 1);
+
+  if (threadIdx.x == 0) {
+    failed = 0;
+    for (int s = 0; s < stages; ++s) {
+      mbarrier_init(smem_u32(&full[s]), 1);
+      mbarrier_init(smem_u32(&empty[s]), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbarrier_init(smem_u32(&acc_full[a]), 1);
+      mbarrier_init(smem_u32(&acc_empty[a]), kEpilogueWarps);
+    }
+    fence_mbarrier_init();
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&w_map)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&x_map)) : "memory");
+  }
+  if (warp == kEpilogueWarps + 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                 ::"r"(smem_u32(&tmem_slot)), "r"(static_cast<uint32_t>(tmem_columns)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem_base = tmem_slot;
   grid_dependency_wait();
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int n0 = blockIdx.x * 64, m0 = blockIdx.y * 64;
-  int acc[4][4] = {};
-  for (int k0 = 0; k0 < p.k; k0 += 64) {
-    const int r = threadIdx.x >> 2, c = (threadIdx.x & 3) * 16;  // K is a multiple of 16
-    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-    const uint4 a = m0 + r < p.m && k0 + c < p.k
-        ? *reinterpret_cast<const uint4*>(p.x + static_cast<int64_t>(m0 + r) * p.k + k0 + c) : zero;
-    const uint4 b = n0 + r < p.n && k0 + c < p.k
-        ? *reinterpret_cast<const uint4*>(p.w + static_cast<int64_t>(n0 + r) * p.k + k0 + c) : zero;
-    __syncthreads();
-    xs[r][c / 4] = a.x; xs[r][c / 4 + 1] = a.y; xs[r][c / 4 + 2] = a.z; xs[r][c / 4 + 3] = a.w;
-    ws[r][c / 4] = b.x; ws[r][c / 4 + 1] = b.y; ws[r][c / 4 + 2] = b.z; ws[r][c / 4 + 3] = b.w;
-    __syncthreads();
+
+  if (warp == kEpilogueWarps && !p.drop_loads) {
+    // ---- producer: the run's k-blocks, across tile ends ----
+    const uint32_t leader = elect_one();
+    int tile = run_first / nkb, kb = run_first % nkb;
+    for (int i = 0, s = 0, turn = 0; i < run_end - run_first; ++i) {
+      if (turn > 0 && !mbarrier_wait_warp(smem_u32(&empty[s]), (turn - 1) & 1, p.wait_limit)) {
+        failed = 1;
+        wait_for_copies(full, stages, s, turn, p.wait_limit);
+        break;
+      }
+      const uint32_t bar = smem_u32(&full[s]), dst = smem_base + s * stage_bytes;
+      mbarrier_arrive_expect_tx_if(leader, bar, stage_bytes);
+      tma_load_2d_if(leader, dst, &w_map, bar, kb * kBK, tile * 128);
+      tma_load_2d_if(leader, dst + 128 * 128, &x_map, bar, kb * kBK, 0);
+      if (++kb == nkb) { kb = 0; ++tile; }
+      if (++s == stages) { s = 0; ++turn; }
+    }
+  } else if (warp == kEpilogueWarps + 1) {
+    // ---- products ----
+    const uint32_t leader = elect_one();
+    const uint32_t idesc = instruction_descriptor_i8(128, p.cols);
+    int kb = run_first % nkb, done = 0;
+    bool ok = true;
+    for (int i = 0, s = 0, turn = 0; i < run_end - run_first; ++done) {
+      const int count = min(nkb - kb, run_end - run_first - i), acc = done & 1;
+      if (done >= 2 && !mbarrier_wait_warp(smem_u32(&acc_empty[acc]), ((done >> 1) - 1) & 1, p.wait_limit)) ok = false;
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t d = tmem_base + acc * acc_columns;
+      for (int j = 0; j < count; ++j, ++i) {
+        if (!mbarrier_wait_warp(smem_u32(&full[s]), turn & 1, p.wait_limit)) { ok = false; break; }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint64_t a_desc = smem_descriptor(smem_base + s * stage_bytes), b_desc = descriptor_advance(a_desc, 128 * 128);
 #pragma unroll
-    for (int kk = 0; kk < 16; ++kk) {
+        for (int q = 0; q < kBK / 32; ++q)
+          umma_i8_if<1>(leader, d, descriptor_advance(a_desc, q * 32), descriptor_advance(b_desc, q * 32), idesc,
+                        (j > 0 || q > 0) ? 1u : 0u);
+        umma_commit_if(leader, smem_u32(&empty[s]));
+        if (++s == stages) { s = 0; ++turn; }
+      }
+      if (!ok) break;
+      umma_commit_if(leader, smem_u32(&acc_full[acc]));
+      kb = 0;
+    }
+    if (!ok) failed = 1;
+  } else if (warp < kEpilogueWarps) {
+    // ---- epilogue: a thread owns one column of y, the accumulator's columns are the rows ----
+    for (int r = threadIdx.x; r < p.m; r += kEpilogueWarps * 32) scales[r] = p.x_scales[r];
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    const bool swiglu = p.epilogue == B200_EPILOGUE_SWIGLU;
+    const int64_t out_cols = swiglu ? p.n / 2 : p.n;
+    T* out = static_cast<T*>(p.out);
+    const T* residual = static_cast<const T*>(p.residual);
+    int tile = run_first / nkb, kb = run_first % nkb;
+    bool ok = true;
+    for (int i = 0, done = 0; i < run_end - run_first; ++done, ++tile) {
+      const int count = min(nkb - kb, run_end - run_first - i), acc = done & 1;
+      const bool whole = count == nkb;
+      const int tile_first = run_first + i - kb;  // of the list
+      i += count;
+      kb = 0;
+      const int col = tile * 128 + warp * 32 + lane;
+      const bool there = col < p.n;
+      const float w_scale = there ? p.w_scales[col] : 0.0f;
+      const float bias = there && p.bias != nullptr ? Elem<T>::load(static_cast<const T*>(p.bias) + col) : 0.0f;
+      auto finish = [&](int row, int sum) {  // all lanes: SwiGLU's pairs are neighbours
+        float y = static_cast<float>(sum) * scales[row] * w_scale + bias;
+        if (swiglu) {
+          const float other = __shfl_xor_sync(0xffffffffu, y, 1);
+          if (there && (lane & 1) == 0) Elem<T>::store(out + row * out_cols + col / 2, silu_times(y, other));
+        } else if (there) {
+          const int64_t at = row * out_cols + col;
+          if (residual != nullptr) y += Elem<T>::load(residual + at);
+          Elem<T>::store(out + at, y);
+        }
+      };
+      // (the four warps leave together: they meet at barriers below)
+      ok = all_of_epilogue(mbarrier_wait_bounded(smem_u32(&acc_full[acc]), (done >> 1) & 1, p.wait_limit));
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t t_addr = tmem_base + acc * acc_columns + (static_cast<uint32_t>(warp * 32) << 16);
+      auto each_row = [&](auto&& use) {
+#pragma unroll 1
+        for (int r0 = 0; r0 < p.m; r0 += 16) {
+          float v[16];
+          tmem_load_32x32(t_addr + r0, v);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+          for (int r = 0; r < 16; ++r)
+            if (r0 + r < p.m) use(r0 + r, __float_as_int(v[r]));
+        }
+      };
+      if (whole) {
+        each_row(finish);
+      } else {
+        const auto run_of = [&](int x) {
+          const int longer = more_by_one * (share + 1);
+          return x < longer ? x / (share + 1) : more_by_one + (x - longer) / share;
+        };
+        const int c_first = run_of(tile_first), parts = run_of(tile_first + nkb - 1) - c_first + 1;
+        int32_t* sums = p.sums + (static_cast<int64_t>(c_first) * p.cols) * 128 + warp * 32 + lane;
+        each_row([&](int row, int sum) {
+          asm volatile("red.relaxed.gpu.global.add.s32 [%0], %1;" ::"l"(sums + row * 128), "r"(sum) : "memory");
+        });
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        if (threadIdx.x == 0) {
+          __threadfence();
+          last_flag = atomicAdd(p.counters + c_first, 1) == parts - 1;
+          __threadfence();
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        if (last_flag) {
+          for (int r0 = 0; r0 < p.m; r0 += 16) {
+            int v[16];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          acc[i][j] = __dp4a(static_cast<int>(xs[ty * 4 + i][kk]), static_cast<int>(ws[tx * 4 + j][kk]), acc[i][j]);
+            for (int r = 0; r < 16; ++r) v[r] = r0 + r < p.m ? __ldcg(sums + (r0 + r) * 128) : 0;
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (r0 + r < p.m) {
+                sums[(r0 + r) * 128] = 0;
+                finish(r0 + r, v[r]);
+              }
+          }
+          if (threadIdx.x == 0) p.counters[c_first] = 0;
+        }
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&acc_empty[acc])) : "memory");
+    }
+    if (!ok) failed = 1;
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0 && failed) atomicOr(p.status, B200_STATUS_WAIT_TIMEOUT);
+  if (warp == kEpilogueWarps + 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;"
+                 ::"r"(tmem_base), "r"(static_cast<uint32_t>(tmem_columns)) : "memory");
+}
+
+// -------------------------------------------------------------------------------------------------------------- pair ----
+constexpr int kPairStages = 6;
+constexpr int kPairStageBytes = 2 * 128 * 128;  // half of 256 rows of x, half of up to 256 of the weight
+constexpr int kPairSmem = kPairStages * kPairStageBytes + kEpilogueWarps * 4096;
+
+// 32 accumulator columns of one row: scaled, with the bias. Columns beyond n are not used.
+template <typename T>
+__device__ __forceinline__ void scale_chunk(const Int8LinearParams& p, float row_scale, int col0, float (&v)[32]) {
+  if (col0 + 32 <= p.n) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float* w = p.w_scales + col0 + 4 * i;  // (uniform over the warp; the vector starts anywhere)
+      float4 s;
+      if ((reinterpret_cast<uintptr_t>(p.w_scales) & 15u) == 0) s = *reinterpret_cast<const float4*>(w);
+      else s = make_float4(w[0], w[1], w[2], w[3]);
+      v[4 * i] = static_cast<float>(__float_as_int(v[4 * i])) * row_scale * s.x;
+      v[4 * i + 1] = static_cast<float>(__float_as_int(v[4 * i + 1])) * row_scale * s.y;
+      v[4 * i + 2] = static_cast<float>(__float_as_int(v[4 * i + 2])) * row_scale * s.z;
+      v[4 * i + 3] = static_cast<float>(__float_as_int(v[4 * i + 3])) * row_scale * s.w;
+    }
+    if (p.bias != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] += Elem<T>::load(static_cast<const T*>(p.bias) + col0 + i);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const bool there = col0 + i < p.n;
+      v[i] = there ? static_cast<float>(__float_as_int(v[i])) * row_scale * p.w_scales[col0 + i] : 0.0f;
+      if (there && p.bias != nullptr) v[i] += Elem<T>::load(static_cast<const T*>(p.bias) + col0 + i);
     }
   }
-  const bool swiglu = p.epilogue == B200_EPILOGUE_SWIGLU;
-  const int out_cols = swiglu ? p.n / 2 : p.n;
-  for (int i = 0; i < 4; ++i) {
-    const int row = m0 + ty * 4 + i;
-    if (row >= p.m) break;
-    float y[4];
-    for (int j = 0; j < 4; ++j) {
-      const int col = n0 + tx * 4 + j;
-      y[j] = 0.0f;
-      if (col >= p.n) continue;
-      y[j] = static_cast<float>(acc[i][j]) * p.x_scales[row] * p.w_scales[col];
-      if (p.bias) y[j] += Elem<T>::load(static_cast<const T*>(p.bias) + col);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtensorMap x_map,
+                        const __grid_constant__ CUtensorMap w_map) {
+  extern __shared__ __align__(1024) unsigned char smem[];
+  __shared__ __align__(8) uint64_t full[kPairStages], empty[kPairStages], acc_full[2], acc_empty[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int failed;
+
+  grid_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = cluster_cta_rank();
+  const int bn = p.cols, half = bn / 2;
+  const uint32_t smem_base = smem_u32(smem);
+  const int nkb = (p.k + kBK - 1) / kBK;
+  const int tiles_n = (p.n + bn - 1) / bn, tiles_m = (p.m + 255) / 256, tiles = tiles_n * tiles_m;
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  auto place = [&](int tile, int& tile_m, int& tile_n) {
+    if (p.n_fastest) { tile_m = tile / tiles_n; tile_n = tile - tile_m * tiles_n; }
+    else { tile_n = tile / tiles_m; tile_m = tile - tile_n * tiles_m; }
+  };
+
+  if (threadIdx.x == 0) {
+    failed = 0;
+    for (int s = 0; s < kPairStages; ++s) {
+      mbarrier_init(smem_u32(&full[s]), 1);
+      mbarrier_init(smem_u32(&empty[s]), 1);
     }
-    for (int j = 0; j < 4; ++j) {
-      const int col = n0 + tx * 4 + j;
-      if (col >= p.n) continue;
-      T* out = static_cast<T*>(p.out) + static_cast<int64_t>(row) * out_cols;
-      if (swiglu) {
-        if (j % 2 == 0) Elem<T>::store(out + col / 2, y[j] / (1.0f + expf(-y[j])) * y[j + 1]);
-      } else {
-        const float more = p.epilogue == B200_EPILOGUE_RESIDUAL
-            ? Elem<T>::load(static_cast<const T*>(p.residual) + static_cast<int64_t>(row) * p.n + col) : 0.0f;
-        Elem<T>::store(out + col, y[j] + more);
+    for (int a = 0; a < 2; ++a) {
+      mbarrier_init(smem_u32(&acc_full[a]), 1);
+      mbarrier_init(smem_u32(&acc_empty[a]), 2 * kEpilogueWarps);  // (the first CTA's counts: both CTAs' warps)
+    }
+    fence_mbarrier_init();
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&x_map)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&w_map)) : "memory");
+  }
+  if (warp == kEpilogueWarps + 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                 ::"r"(smem_u32(&tmem_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  cluster_sync();  // the other CTA's barriers are ready
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem_base = tmem_slot;
+  grid_dependency_wait();
+
+  if (warp == kEpilogueWarps && !p.drop_loads) {
+    // ---- producer: this CTA's halves; all bytes of a stage count on the first CTA's barrier ----
+    const uint32_t leader = elect_one();
+    bool ok = true;
+    int s = 0, turn = 0;
+    for (int tile = pair; ok && tile < tiles; tile += pairs) {
+      int tile_m, tile_n;
+      place(tile, tile_m, tile_n);
+      for (int kb = 0; kb < nkb; ++kb) {
+        if (turn > 0 && !mbarrier_wait_warp(smem_u32(&empty[s]), (turn - 1) & 1, p.wait_limit)) {
+          ok = false;
+          if (rank == 0) wait_for_copies(full, kPairStages, s, turn, p.wait_limit);
+          break;
+        }
+        const uint32_t dst = smem_base + s * kPairStageBytes;
+        if (rank == 0) mbarrier_arrive_expect_tx_if(leader, smem_u32(&full[s]), 2 * (128 + half) * 128);
+        const uint32_t bar = map_to_rank(smem_u32(&full[s]), 0);
+        tma_load_pair_if(leader, dst, &x_map, bar, kb * kBK, tile_m * 256 + rank * 128);
+        tma_load_pair_if(leader, dst + 128 * 128, &w_map, bar, kb * kBK, tile_n * bn + rank * half);
+        if (++s == kPairStages) { s = 0; ++turn; }
       }
     }
+    if (!ok) failed = 1;
+  } else if (warp == kEpilogueWarps + 1 && rank == 0) {
+    // ---- products of both CTAs, issued by the first ----
+    const uint32_t leader = elect_one();
+    const uint32_t idesc = instruction_descriptor_i8(256, bn);
+    bool ok = true;
+    int s = 0, turn = 0, done = 0;
+    for (int tile = pair; ok && tile < tiles; tile += pairs, ++done) {
+      const int acc = done & 1;
+      if (done >= 2 && !mbarrier_wait_warp(smem_u32(&acc_empty[acc]), ((done >> 1) - 1) & 1, p.wait_limit)) { ok = false; break; }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t d = tmem_base + acc * 256;
+      for (int kb = 0; kb < nkb; ++kb) {
+        if (!mbarrier_wait_warp(smem_u32(&full[s]), turn & 1, p.wait_limit)) { ok = false; break; }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint64_t a_desc = smem_descriptor(smem_base + s * kPairStageBytes), b_desc = descriptor_advance(a_desc, 128 * 128);
+#pragma unroll
+        for (int q = 0; q < kBK / 32; ++q)
+          umma_i8_if<2>(leader, d, descriptor_advance(a_desc, q * 32), descriptor_advance(b_desc, q * 32), idesc,
+                        (kb > 0 || q > 0) ? 1u : 0u);
+        umma_commit_pair_if(leader, smem_u32(&empty[s]));
+        if (++s == kPairStages) { s = 0; ++turn; }
+      }
+      if (ok) umma_commit_pair_if(leader, smem_u32(&acc_full[acc]));
+    }
+    if (!ok) failed = 1;
+  } else if (warp < kEpilogueWarps) {
+    // ---- epilogue: this CTA's 128 rows; warp w reads lanes 32 w .. of the accumulator ----
+    const bool swiglu = p.epilogue == B200_EPILOGUE_SWIGLU;
+    const int out_cols = swiglu ? p.n / 2 : p.n;
+    T* out = static_cast<T*>(p.out);
+    const T* residual = static_cast<const T*>(p.residual);
+    constexpr int kVec = 16 / static_cast<int>(sizeof(T)), kSegment = 8 * kVec;  // output columns of 128 bytes
+    const bool staged = (out_cols * static_cast<int>(sizeof(T))) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0 &&
+                        (residual == nullptr || (reinterpret_cast<uintptr_t>(residual) & 15u) == 0);
+    const int span = swiglu ? 2 * kSegment : kSegment;  // accumulator columns of a segment
+    const uint32_t stage_tile = smem_base + kPairStages * kPairStageBytes + warp * 4096;
+    const uint32_t acc_empty_first = map_to_rank(smem_u32(&acc_empty[0]), 0);
+    bool ok = true;
+    int done = 0;
+    for (int tile = pair; tile < tiles; tile += pairs, ++done) {
+      int tile_m, tile_n;
+      place(tile, tile_m, tile_n);
+      const int acc = done & 1, row0 = tile_m * 256 + rank * 128 + warp * 32, row = row0 + lane;
+      const float row_scale = row < p.m ? p.x_scales[row] : 0.0f;
+      ok = ok && __all_sync(0xffffffffu, mbarrier_wait_bounded(smem_u32(&acc_full[acc]), (done >> 1) & 1, p.wait_limit));
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t t_addr = tmem_base + acc * 256 + (static_cast<uint32_t>(warp * 32) << 16);
+      const int n_end = min(p.n, (tile_n + 1) * bn);
+#pragma unroll 1
+      for (int c0 = 0; c0 < bn;) {
+        const int col0 = tile_n * bn + c0;
+        if (col0 >= n_end) break;  // (warp-uniform)
+        if (staged && c0 + span <= bn && col0 + span <= n_end) {
+          uint4 packed[8];
+#pragma unroll
+          for (int part = 0; part < kSegment / 16; ++part) {  // 16 output columns at a time
+            float y[16];
+            if (swiglu) {
+              float v[32];
+              tmem_load_32x32(t_addr + c0 + part * 32, v);
+              scale_chunk<T>(p, row_scale, col0 + part * 32, v);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) y[i] = silu_times(v[2 * i], v[2 * i + 1]);
+            } else {
+              if (part % 2 == 1) continue;  // (32 columns at a time)
+              float v[32];
+              tmem_load_32x32(t_addr + c0 + part * 16, v);
+              scale_chunk<T>(p, row_scale, col0 + part * 16, v);
+              if (residual != nullptr && row < p.m) {
+                const T* r = residual + static_cast<int64_t>(row) * p.n + col0 + part * 16;
+#pragma unroll
+                for (int i = 0; i < 32 / kVec; ++i) {
+                  Vec16<T> other;
+                  other.load(r + i * kVec);
+#pragma unroll
+                  for (int e = 0; e < kVec; ++e) v[i * kVec + e] += other.v[e];
+                }
+              }
+#pragma unroll
+              for (int i = 0; i < 32 / kVec; ++i) {
+                Vec16<T> t;
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) t.v[e] = v[i * kVec + e];
+                t.store(reinterpret_cast<T*>(&packed[(part * 16) / kVec + i]));
+              }
+              continue;
+            }
+#pragma unroll
+            for (int i = 0; i < 16 / kVec; ++i) {
+              Vec16<T> t;
+#pragma unroll
+              for (int e = 0; e < kVec; ++e) t.v[e] = y[i * kVec + e];
+              t.store(reinterpret_cast<T*>(&packed[(part * 16) / kVec + i]));
+            }
+          }
+          __syncwarp();  // the round before has been read
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage_tile + lane * 128 + ((u ^ (lane & 7)) << 4)),
+                         "r"(packed[u].x), "r"(packed[u].y), "r"(packed[u].z), "r"(packed[u].w) : "memory");
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {  // four whole 128-byte row segments an instruction
+            const int r = i * 4 + (lane >> 3), u = lane & 7;
+            uint4 value;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(value.x), "=r"(value.y), "=r"(value.z), "=r"(value.w)
+                         : "r"(stage_tile + r * 128 + ((u ^ (r & 7)) << 4)));
+            if (row0 + r < p.m)
+              *reinterpret_cast<uint4*>(out + static_cast<int64_t>(row0 + r) * out_cols + (swiglu ? col0 / 2 : col0) + u * kVec) = value;
+          }
+          c0 += span;
+        } else {
+          float v[32];
+          tmem_load_32x32(t_addr + c0, v);
+          scale_chunk<T>(p, row_scale, col0, v);
+          if (row < p.m) {
+            if (swiglu) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                if (col0 + 2 * i < n_end)
+                  Elem<T>::store(out + static_cast<int64_t>(row) * out_cols + col0 / 2 + i, silu_times(v[2 * i], v[2 * i + 1]));
+            } else {
+              const int64_t at = static_cast<int64_t>(row) * p.n + col0;
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (col0 + i < n_end)
+                  Elem<T>::store(out + at + i, v[i] + (residual != nullptr ? Elem<T>::load(residual + at + i) : 0.0f));
+            }
+          }
+          c0 += 32;
+        }
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0)
+        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(acc_empty_first + acc * 8) : "memory");
+    }
+    if (!ok) failed = 1;
   }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0 && failed) atomicOr(p.status, B200_STATUS_WAIT_TIMEOUT);
+  cluster_sync();  // neither CTA leaves while the other may still signal it
+  if (warp == kEpilogueWarps + 1)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+}
+
+// [rows, K] codes in boxes of box_rows x 128 (128-byte rows, 128B swizzle); zeros beyond both.
+bool make_code_map(CUtensorMap* map, const void* base, int64_t rows, int64_t k, int box_rows) {
+  EncodeTiledFn encode = tensor_map_encoder();
+  if (encode == nullptr) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(k)};
+  const cuuint32_t box[2] = {kBK, static_cast<cuuint32_t>(box_rows)}, element_strides[2] = {1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, element_strides,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int stream_rows(int64_t m) { return static_cast<int>(ceil_div(m, 16) * 16); }
+
+template <typename T>
+int launch_stream(Int8LinearParams p, const void* x, const void* w, cudaStream_t stream) {
+  p.cols = stream_rows(p.m);
+  p.stages = std::min(10, kRingBytes / ((128 + p.cols) * 128));
+  CUtensorMap w_map, x_map;
+  if (!make_code_map(&w_map, w, p.n, p.k, 128) || !make_code_map(&x_map, x, p.m, p.k, p.cols)) return B200_ERR_UNSUPPORTED;
+  const int64_t blocks = ceil_div(p.n, 128) * ceil_div(p.k, kBK);
+  const int ctas = static_cast<int>(std::min<int64_t>(kNumSMs, ceil_div(blocks, 4)));
+  auto kernel = linear_int8_stream_kernel<T>;
+  static_assert(tensor_memory_fits(512, kRingBytes), "tensor memory under programmatic launches");
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes) != cudaSuccess) return B200_ERR_LAUNCH;
+  return launch_chained(kernel, dim3(ctas), dim3(kThreads), kRingBytes, stream, p, w_map, x_map) == cudaSuccess
+             ? launch_status() : B200_ERR_LAUNCH;
+}
+
+template <typename T>
+int launch_pair(Int8LinearParams p, const void* x, const void* w, cudaStream_t stream) {
+  // columns of a tile: the fewest column-steps over all rounds of the GPU's pairs
+  const int64_t tiles_m = ceil_div(p.m, 256);
+  constexpr int kPairs = kNumSMs / 2;
+  int64_t best = INT64_MAX;
+  for (int bn = 256; bn >= 128; bn -= 32) {
+    const int64_t cost = ceil_div(tiles_m * ceil_div(p.n, bn), kPairs) * bn;
+    if (cost < best) { best = cost; p.cols = bn; }
+  }
+  p.n_fastest = p.n <= p.m;
+  CUtensorMap x_map, w_map;
+  if (!make_code_map(&x_map, x, p.m, p.k, 128) || !make_code_map(&w_map, w, p.n, p.k, p.cols / 2)) return B200_ERR_UNSUPPORTED;
+  const int64_t tiles = tiles_m * ceil_div(p.n, p.cols);
+  const unsigned pairs = static_cast<unsigned>(std::min<int64_t>(kPairs, tiles));
+  auto kernel = linear_int8_pair_kernel<T>;
+  static_assert(tensor_memory_fits(512, kPairSmem), "tensor memory under programmatic launches");
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem) != cudaSuccess) return B200_ERR_LAUNCH;
+  return launch_chained_cluster(kernel, dim3(2 * pairs), dim3(kThreads), kPairSmem, stream, 2u, p, x_map, w_map) == cudaSuccess
+             ? launch_status() : B200_ERR_LAUNCH;
 }
 
 }  // namespace
@@ -84,9 +603,15 @@ __global__ void __launch_bounds__(256) linear_int8_kernel(const Int8LinearParams
 
 using namespace b200;
 
+extern "C" int64_t b200_linear_int8_workspace_bytes(int64_t m, int64_t k, int64_t n) {
+  if (m <= 0 || k <= 0 || n <= 0 || m > kRowsAtMost) return 0;
+  return kCounterBytes + static_cast<int64_t>(kNumSMs) * stream_rows(m) * 128 * 4;
+}
+
 extern "C" int b200_linear_int8(const void* x, const float* x_scales, const void* weight, const float* weight_scales,
                                 const void* bias, const void* residual, void* output, int64_t m, int64_t k, int64_t n,
-                                int dtype, int epilogue, int32_t* status, void* stream) {
+                                int dtype, int epilogue, void* workspace, int64_t workspace_bytes, int32_t* status,
+                                void* stream) {
   if (!x || !x_scales || !weight || !weight_scales || !output || !status || m < 0 || k <= 0 || n <= 0 || !known_dtype(dtype) ||
       epilogue < B200_EPILOGUE_NONE || epilogue > B200_EPILOGUE_SWIGLU ||
       (epilogue == B200_EPILOGUE_RESIDUAL) != (residual != nullptr))
@@ -96,16 +621,20 @@ extern "C" int b200_linear_int8(const void* x, const float* x_scales, const void
   if (k > kMaxK || m > (1 << 22) || n > (1 << 22)) return B200_ERR_TOO_LARGE;
   if (m == 0) return B200_OK;
   Int8LinearParams p = {};
-  p.x = static_cast<const int8_t*>(x); p.x_scales = x_scales;
-  p.w = static_cast<const int8_t*>(weight); p.w_scales = weight_scales;
+  p.x_scales = x_scales; p.w_scales = weight_scales;
   p.bias = bias; p.residual = residual; p.out = output; p.status = status;
   p.m = static_cast<int>(m); p.k = static_cast<int>(k); p.n = static_cast<int>(n); p.epilogue = epilogue;
-  if (ceil_div(m, 64) > 65535) return B200_ERR_TOO_LARGE;
-  const dim3 grid(static_cast<unsigned>(ceil_div(n, 64)), static_cast<unsigned>(ceil_div(m, 64)));
-  cudaError_t error = cudaSuccess;
+  p.wait_limit = wait_limit(); p.drop_loads = drop_loads();
+  if (m <= kRowsAtMost) {
+    if (!workspace || workspace_bytes < b200_linear_int8_workspace_bytes(m, k, n)) return B200_ERR_WORKSPACE;
+    p.counters = static_cast<int32_t*>(workspace);
+    p.sums = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + kCounterBytes);
+  }
+  int code = B200_ERR_UNSUPPORTED;
   with_element_type(dtype, [&](auto tag) {
-    error = launch_chained(linear_int8_kernel<typename decltype(tag)::type>, grid, dim3(256), 0,
-                           static_cast<cudaStream_t>(stream), p);
+    using T = typename decltype(tag)::type;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    code = m <= kRowsAtMost ? launch_stream<T>(p, x, weight, s) : launch_pair<T>(p, x, weight, s);
   });
-  return error == cudaSuccess ? launch_status() : B200_ERR_LAUNCH;
+  return code;
 }
