@@ -769,8 +769,7 @@ int b200_advance_slots(int64_t* lengths, const int32_t* slots, const int32_t* st
  * b200_linear_int8: y[m, n] = (sum_k x[m, k] weight[n, k]) x_scales[m] weight_scales[n] + bias[n], sums in 32-bit integers
  * (exact), then the epilogue in fp32 and one rounding to dtype: B200_EPILOGUE_RESIDUAL adds residual[m, n];
  * B200_EPILOGUE_SWIGLU takes columns 2j and 2j + 1 as gate_j and up_j and gives silu(gate_j) up_j. x and weight are
- * contiguous codes, K a multiple of 16 and at most 131056; bias, residual and output are of dtype. Workspace
- * (zero-filled once, left so; none beyond 256 rows): b200_linear_int8_workspace_bytes. `status` receives
+ * contiguous codes, K a multiple of 16 and at most 131056; bias, residual and output are of dtype. `status` receives
  * B200_STATUS_WAIT_TIMEOUT if a bounded in-kernel wait gives up. */
 #define B200_MAX_COPY_POOLS 8
 typedef struct b200_block_pool {
@@ -798,10 +797,9 @@ int b200_copy_kv_blocks(const b200_block_pool* pools, int64_t pool_count, const 
 int b200_quantize_rows_int8(const void* input, const void* residual, const void* norm_weight, void* sum, void* codes,
                             float* scales, int64_t rows, int64_t hidden, int64_t input_row_stride,
                             int64_t residual_row_stride, double epsilon, int dtype, void* stream);
-int64_t b200_linear_int8_workspace_bytes(int64_t m, int64_t k, int64_t n);
 int b200_linear_int8(const void* x, const float* x_scales, const void* weight, const float* weight_scales, const void* bias,
                      const void* residual, void* output, int64_t m, int64_t k, int64_t n, int dtype, int epilogue,
-                     void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+                     int32_t* status, void* stream);
 
 #ifdef __cplusplus
 }

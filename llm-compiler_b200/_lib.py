@@ -239,8 +239,7 @@ SIGNATURES = {
                                                                                 c_void_p]),
     "b200_copy_kv_blocks": (c_int, [POINTER(BlockPool), c_int64, c_void_p, c_void_p] + [c_int64] * 3 + [c_void_p, c_void_p]),
     "b200_quantize_rows_int8": (c_int, [c_void_p] * 6 + [c_int64] * 4 + [c_double, c_int, c_void_p]),
-    "b200_linear_int8_workspace_bytes": (c_int64, [c_int64] * 3),
-    "b200_linear_int8": (c_int, [c_void_p] * 7 + [c_int64] * 3 + [c_int, c_int, c_void_p, c_int64, c_void_p, c_void_p]),
+    "b200_linear_int8": (c_int, [c_void_p] * 7 + [c_int64] * 3 + [c_int, c_int, c_void_p, c_void_p]),
 }
 
 _library: ctypes.CDLL | None = None

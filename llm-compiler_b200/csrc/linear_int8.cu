@@ -8,9 +8,9 @@
 //
 // linear_int8_stream_kernel, up to 256 rows (decode, short prompts): bound by the read of the weight. The WEIGHT's columns
 //   lie along the product's M (128 of them a tile) and all rows of x along its N, so every weight byte is read once and no
-//   row of x is padded beyond the next multiple of 16. The k-blocks of all tiles are one list, of which every CTA (one
-//   per SM) takes an equal run: any N and K fill the GPU alike. A tile that several CTAs share is summed in the workspace
-//   by integer additions, whose order does not matter, and finished by the CTA that arrives last.
+//   row of x is padded beyond the next multiple of 16. A CTA per SM takes whole tiles in turn; where there are fewer tiles
+//   than SMs, the K slices of a tile are the CTAs of a cluster, which add their sums through distributed shared memory
+//   (4.0 us less than integer additions in global memory at 64 x 384 x 512, where the slices then wait for one another there).
 // linear_int8_pair_kernel, beyond: bound by the tensor cores. Two SMs work on one tile of 256 rows x up to 256 columns
 //   (cta_group::2): each holds half of both operands, which halves the bytes that shared memory and L2 deliver per product
 //   (at 128 x 256 a CTA they are what limits it: 96 of 128 bytes a cycle in, as many out). Two accumulators alternate, so
@@ -30,7 +30,6 @@ constexpr int kEpilogueWarps = 4;
 constexpr int kThreads = (kEpilogueWarps + 2) * 32;  // and a producer and a product warp
 constexpr int kRowsAtMost = 256;  // of the stream kernel
 constexpr int kRingBytes = 192 * 1024;
-constexpr int64_t kCounterBytes = 4096;
 
 struct Int8LinearParams {
   const float* x_scales;
@@ -38,12 +37,11 @@ struct Int8LinearParams {
   const void* bias;
   const void* residual;
   void* out;
-  int32_t* sums;      // stream: [CTAs][rows][128] of tiles that are shared, zero between calls
-  int32_t* counters;  // stream: one per CTA, zero between calls
   int32_t* status;
   int m, k, n, epilogue;
   int cols;     // stream: rows of x, rounded up to 16, the product's N. pair: columns of a tile
   int stages;   // stream
+  int slices;   // stream: of K, the CTAs of a cluster
   int n_fastest;  // pair: order of the tiles
   uint32_t wait_limit;
   int drop_loads;
@@ -100,11 +98,11 @@ __device__ __forceinline__ float silu_times(float gate, float up) {
 }
 
 // ------------------------------------------------------------------------------------------------------------ stream ----
-__device__ __forceinline__ bool all_of_epilogue(bool mine) {
-  uint32_t all;
-  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.and.pred q, 1, 128, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
-               : "=r"(all) : "r"(static_cast<uint32_t>(mine)) : "memory");
-  return all != 0;
+__device__ __forceinline__ int4 load_cluster_i32x4(uint32_t remote) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(remote)
+               : "memory");
+  return v;
 }
 
 template <typename T>
@@ -116,7 +114,7 @@ linear_int8_stream_kernel(const Int8LinearParams p, const __grid_constant__ CUte
   __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2];
   __shared__ float scales[kRowsAtMost];
   __shared__ uint32_t tmem_slot;
-  __shared__ int failed, last_flag;
+  __shared__ int failed;
 
   grid_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -125,10 +123,10 @@ linear_int8_stream_kernel(const Int8LinearParams p, const __grid_constant__ CUte
   while (acc_columns < p.cols) acc_columns *= 2;
   const int tmem_columns = 2 * acc_columns;
   const uint32_t smem_base = smem_u32(smem);
-  const int nkb = (p.k + kBK - 1) / kBK, tiles = (p.n + 127) / 128, total = tiles * nkb, ctas = gridDim.x;
-  const int share = total / ctas, more_by_one = total - share * ctas;
-  auto run_start = [&](int c) { return c * share + min(c, more_by_one); };
-  const int run_first = run_start(blockIdx.x), run_end = run_start(blockIdx.x + 1);
+  const int all_kb = (p.k + kBK - 1) / kBK, tiles = (p.n + 127) / 128;
+  const int rank = p.slices > 1 ? cluster_cta_rank() : 0;
+  const int kb_first = all_kb * rank / p.slices, nkb = all_kb * (rank + 1) / p.slices - kb_first;  // this slice: two at least
+  const int tile_first = blockIdx.x / p.slices, tile_step = gridDim.x / p.slices;
 
   if (threadIdx.x == 0) {
     failed = 0;
@@ -154,130 +152,112 @@ linear_int8_stream_kernel(const Int8LinearParams p, const __grid_constant__ CUte
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_base = tmem_slot;
   grid_dependency_wait();
+  const bool swiglu = p.epilogue == B200_EPILOGUE_SWIGLU;
+  const int64_t out_cols = swiglu ? p.n / 2 : p.n;
+  T* out = static_cast<T*>(p.out);
+  const T* residual = static_cast<const T*>(p.residual);
 
   if (warp == kEpilogueWarps && !p.drop_loads) {
-    // ---- producer: the run's k-blocks, across tile ends ----
+    // ---- producer: the ring runs on across tile ends ----
     const uint32_t leader = elect_one();
-    int tile = run_first / nkb, kb = run_first % nkb;
-    for (int i = 0, s = 0, turn = 0; i < run_end - run_first; ++i) {
-      if (turn > 0 && !mbarrier_wait_warp(smem_u32(&empty[s]), (turn - 1) & 1, p.wait_limit)) {
-        failed = 1;
-        wait_for_copies(full, stages, s, turn, p.wait_limit);
-        break;
+    int s = 0, turn = 0;
+    bool ok = true;
+    for (int tile = tile_first; ok && tile < tiles; tile += tile_step)
+      for (int kb = 0; kb < nkb; ++kb) {
+        if (turn > 0 && !mbarrier_wait_warp(smem_u32(&empty[s]), (turn - 1) & 1, p.wait_limit)) {
+          failed = 1;
+          wait_for_copies(full, stages, s, turn, p.wait_limit);
+          ok = false;
+          break;
+        }
+        const uint32_t bar = smem_u32(&full[s]), dst = smem_base + s * stage_bytes;
+        mbarrier_arrive_expect_tx_if(leader, bar, stage_bytes);
+        tma_load_2d_if(leader, dst, &w_map, bar, (kb_first + kb) * kBK, tile * 128);
+        tma_load_2d_if(leader, dst + 128 * 128, &x_map, bar, (kb_first + kb) * kBK, 0);
+        if (++s == stages) { s = 0; ++turn; }
       }
-      const uint32_t bar = smem_u32(&full[s]), dst = smem_base + s * stage_bytes;
-      mbarrier_arrive_expect_tx_if(leader, bar, stage_bytes);
-      tma_load_2d_if(leader, dst, &w_map, bar, kb * kBK, tile * 128);
-      tma_load_2d_if(leader, dst + 128 * 128, &x_map, bar, kb * kBK, 0);
-      if (++kb == nkb) { kb = 0; ++tile; }
-      if (++s == stages) { s = 0; ++turn; }
-    }
   } else if (warp == kEpilogueWarps + 1) {
     // ---- products ----
     const uint32_t leader = elect_one();
     const uint32_t idesc = instruction_descriptor_i8(128, p.cols);
-    int kb = run_first % nkb, done = 0;
+    int s = 0, turn = 0, done = 0;
     bool ok = true;
-    for (int i = 0, s = 0, turn = 0; i < run_end - run_first; ++done) {
-      const int count = min(nkb - kb, run_end - run_first - i), acc = done & 1;
-      if (done >= 2 && !mbarrier_wait_warp(smem_u32(&acc_empty[acc]), ((done >> 1) - 1) & 1, p.wait_limit)) ok = false;
-      if (!ok) break;
+    for (int tile = tile_first; ok && tile < tiles; tile += tile_step, ++done) {
+      const int acc = done & 1;
+      if (done >= 2 && !mbarrier_wait_warp(smem_u32(&acc_empty[acc]), ((done >> 1) - 1) & 1, p.wait_limit)) { ok = false; break; }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t d = tmem_base + acc * acc_columns;
-      for (int j = 0; j < count; ++j, ++i) {
+      for (int kb = 0; kb < nkb; ++kb) {
         if (!mbarrier_wait_warp(smem_u32(&full[s]), turn & 1, p.wait_limit)) { ok = false; break; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint64_t a_desc = smem_descriptor(smem_base + s * stage_bytes), b_desc = descriptor_advance(a_desc, 128 * 128);
 #pragma unroll
         for (int q = 0; q < kBK / 32; ++q)
           umma_i8_if<1>(leader, d, descriptor_advance(a_desc, q * 32), descriptor_advance(b_desc, q * 32), idesc,
-                        (j > 0 || q > 0) ? 1u : 0u);
+                        (kb > 0 || q > 0) ? 1u : 0u);
         umma_commit_if(leader, smem_u32(&empty[s]));
         if (++s == stages) { s = 0; ++turn; }
       }
-      if (!ok) break;
-      umma_commit_if(leader, smem_u32(&acc_full[acc]));
-      kb = 0;
+      if (ok) umma_commit_if(leader, smem_u32(&acc_full[acc]));
     }
     if (!ok) failed = 1;
   } else if (warp < kEpilogueWarps) {
-    // ---- epilogue: a thread owns one column of y, the accumulator's columns are the rows ----
-    for (int r = threadIdx.x; r < p.m; r += kEpilogueWarps * 32) scales[r] = p.x_scales[r];
+    // ---- epilogue: lanes of the accumulator are columns of y, its columns are rows ----
+    for (int r = threadIdx.x; r < p.cols; r += kEpilogueWarps * 32) scales[r] = r < p.m ? p.x_scales[r] : 0.0f;
     asm volatile("bar.sync 1, 128;" ::: "memory");
-    const bool swiglu = p.epilogue == B200_EPILOGUE_SWIGLU;
-    const int64_t out_cols = swiglu ? p.n / 2 : p.n;
-    T* out = static_cast<T*>(p.out);
-    const T* residual = static_cast<const T*>(p.residual);
-    int tile = run_first / nkb, kb = run_first % nkb;
     bool ok = true;
-    for (int i = 0, done = 0; i < run_end - run_first; ++done, ++tile) {
-      const int count = min(nkb - kb, run_end - run_first - i), acc = done & 1;
-      const bool whole = count == nkb;
-      const int tile_first = run_first + i - kb;  // of the list
-      i += count;
-      kb = 0;
-      const int col = tile * 128 + warp * 32 + lane;
-      const bool there = col < p.n;
-      const float w_scale = there ? p.w_scales[col] : 0.0f;
-      const float bias = there && p.bias != nullptr ? Elem<T>::load(static_cast<const T*>(p.bias) + col) : 0.0f;
-      auto finish = [&](int row, int sum) {  // all lanes: SwiGLU's pairs are neighbours
-        float y = static_cast<float>(sum) * scales[row] * w_scale + bias;
-        if (swiglu) {
-          const float other = __shfl_xor_sync(0xffffffffu, y, 1);
-          if (there && (lane & 1) == 0) Elem<T>::store(out + row * out_cols + col / 2, silu_times(y, other));
-        } else if (there) {
-          const int64_t at = row * out_cols + col;
-          if (residual != nullptr) y += Elem<T>::load(residual + at);
-          Elem<T>::store(out + at, y);
-        }
-      };
-      // (the four warps leave together: they meet at barriers below)
-      ok = all_of_epilogue(mbarrier_wait_bounded(smem_u32(&acc_full[acc]), (done >> 1) & 1, p.wait_limit));
+    int done = 0;
+    for (int tile = tile_first; tile < tiles; tile += tile_step, ++done) {
+      const int acc = done & 1;
+      ok = __all_sync(0xffffffffu, mbarrier_wait_bounded(smem_u32(&acc_full[acc]), (done >> 1) & 1, p.wait_limit));
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t t_addr = tmem_base + acc * acc_columns + (static_cast<uint32_t>(warp * 32) << 16);
-      auto each_row = [&](auto&& use) {
+      if (p.slices > 1) {
+        // (one tile a CTA: every stage has been read, the sums take the ring's place: [row][128])
 #pragma unroll 1
         for (int r0 = 0; r0 < p.m; r0 += 16) {
           float v[16];
           tmem_load_32x32(t_addr + r0, v);
+          const uint32_t to = smem_base + r0 * 512 + (warp * 32 + lane) * 4;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + r * 512), "f"(v[r]) : "memory");
+        }
+        break;
+      }
+      // a thread owns a column; 16 rows at a time: all operands before all stores, which the compiler may not swap
+      const int col = tile * 128 + warp * 32 + lane;
+      const bool there = col < p.n;
+      const float w_scale = there ? p.w_scales[col] : 0.0f;
+      const float bias = there && p.bias != nullptr ? Elem<T>::load(static_cast<const T*>(p.bias) + col) : 0.0f;
+      const bool writes = there && !(swiglu && (lane & 1) != 0);
+      T* to = out + (swiglu ? col / 2 : col);
+#pragma unroll 1
+      for (int r0 = 0; r0 < p.m; r0 += 16) {
+        float v[16];
+        if (residual != nullptr) {
+          float other[16];
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            if (r0 + r < p.m) use(r0 + r, __float_as_int(v[r]));
-        }
-      };
-      if (whole) {
-        each_row(finish);
-      } else {
-        const auto run_of = [&](int x) {
-          const int longer = more_by_one * (share + 1);
-          return x < longer ? x / (share + 1) : more_by_one + (x - longer) / share;
-        };
-        const int c_first = run_of(tile_first), parts = run_of(tile_first + nkb - 1) - c_first + 1;
-        int32_t* sums = p.sums + (static_cast<int64_t>(c_first) * p.cols) * 128 + warp * 32 + lane;
-        each_row([&](int row, int sum) {
-          asm volatile("red.relaxed.gpu.global.add.s32 [%0], %1;" ::"l"(sums + row * 128), "r"(sum) : "memory");
-        });
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        if (threadIdx.x == 0) {
-          __threadfence();
-          last_flag = atomicAdd(p.counters + c_first, 1) == parts - 1;
-          __threadfence();
-        }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        if (last_flag) {
-          for (int r0 = 0; r0 < p.m; r0 += 16) {
-            int v[16];
+            other[r] = there && r0 + r < p.m ? Elem<T>::load(residual + (r0 + r) * out_cols + col) : 0.0f;
+          tmem_load_32x32(t_addr + r0, v);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) v[r] = r0 + r < p.m ? __ldcg(sums + (r0 + r) * 128) : 0;
+          for (int r = 0; r < 16; ++r)
+            v[r] = static_cast<float>(__float_as_int(v[r])) * scales[r0 + r] * w_scale + bias + other[r];
+        } else {
+          tmem_load_32x32(t_addr + r0, v);
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-              if (r0 + r < p.m) {
-                sums[(r0 + r) * 128] = 0;
-                finish(r0 + r, v[r]);
-              }
+          for (int r = 0; r < 16; ++r) v[r] = static_cast<float>(__float_as_int(v[r])) * scales[r0 + r] * w_scale + bias;
+          if (swiglu) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) v[r] = silu_times(v[r], __shfl_xor_sync(0xffffffffu, v[r], 1));
           }
-          if (threadIdx.x == 0) p.counters[c_first] = 0;
+        }
+        if (writes) {
+          T* at = to + r0 * out_cols;
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (r0 + r < p.m) Elem<T>::store(at + r * out_cols, v[r]);
         }
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -285,6 +265,47 @@ linear_int8_stream_kernel(const Int8LinearParams p, const __grid_constant__ CUte
       if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&acc_empty[acc])) : "memory");
     }
     if (!ok) failed = 1;
+  }
+  __syncwarp();
+  if (p.slices > 1) {
+    // ---- the slices' sums: this CTA finishes rows rank, rank + slices, ...; a lane takes four columns ----
+    cluster_sync();
+    const int col = tile_first * 128 + 4 * lane;
+    float w_scale[4], bias[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      w_scale[c] = col + c < p.n ? p.w_scales[col + c] : 0.0f;
+      bias[c] = col + c < p.n && p.bias != nullptr ? Elem<T>::load(static_cast<const T*>(p.bias) + col + c) : 0.0f;
+    }
+    for (int row = rank + warp * p.slices; row < p.m; row += kThreads / 32 * p.slices) {
+      int4 part[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        part[i] = i < p.slices ? load_cluster_i32x4(map_to_rank(smem_base + row * 512 + lane * 16, i)) : make_int4(0, 0, 0, 0);
+      float y[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        y[c] = residual != nullptr && col + c < p.n ? Elem<T>::load(residual + row * out_cols + col + c) : 0.0f;
+#pragma unroll
+      for (int i = 1; i < 8; ++i) {
+        part[0].x += part[i].x; part[0].y += part[i].y; part[0].z += part[i].z; part[0].w += part[i].w;
+      }
+      const float scale = scales[row];
+      y[0] += static_cast<float>(part[0].x) * scale * w_scale[0] + bias[0];
+      y[1] += static_cast<float>(part[0].y) * scale * w_scale[1] + bias[1];
+      y[2] += static_cast<float>(part[0].z) * scale * w_scale[2] + bias[2];
+      y[3] += static_cast<float>(part[0].w) * scale * w_scale[3] + bias[3];
+      if (swiglu) {
+        if (col < p.n) Elem<T>::store(out + row * out_cols + col / 2, silu_times(y[0], y[1]));
+        if (col + 2 < p.n) Elem<T>::store(out + row * out_cols + col / 2 + 1, silu_times(y[2], y[3]));
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (col + c < p.n) Elem<T>::store(out + row * out_cols + col + c, y[c]);
+      }
+    }
+    __syncwarp();
+    cluster_sync();  // (the others may still read this CTA's sums)
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
@@ -567,13 +588,16 @@ int launch_stream(Int8LinearParams p, const void* x, const void* w, cudaStream_t
   p.stages = std::min(10, kRingBytes / ((128 + p.cols) * 128));
   CUtensorMap w_map, x_map;
   if (!make_code_map(&w_map, w, p.n, p.k, 128) || !make_code_map(&x_map, x, p.m, p.k, p.cols)) return B200_ERR_UNSUPPORTED;
-  const int64_t blocks = ceil_div(p.n, 128) * ceil_div(p.k, kBK);
-  const int ctas = static_cast<int>(std::min<int64_t>(kNumSMs, ceil_div(blocks, 4)));
+  // slices of K that fill the GPU where the tiles do not: clusters of 2, 4 or 8, two k-blocks a slice at least
+  const int64_t tiles = ceil_div(p.n, 128), blocks = ceil_div(p.k, kBK);
+  p.slices = 1;
+  while (p.slices < 8 && tiles * p.slices * 2 <= kNumSMs && blocks >= p.slices * 4) p.slices *= 2;
+  const unsigned ctas = static_cast<unsigned>(p.slices > 1 ? tiles * p.slices : std::min<int64_t>(kNumSMs, tiles));
   auto kernel = linear_int8_stream_kernel<T>;
   static_assert(tensor_memory_fits(512, kRingBytes), "tensor memory under programmatic launches");
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes) != cudaSuccess) return B200_ERR_LAUNCH;
-  return launch_chained(kernel, dim3(ctas), dim3(kThreads), kRingBytes, stream, p, w_map, x_map) == cudaSuccess
-             ? launch_status() : B200_ERR_LAUNCH;
+  return launch_chained_cluster(kernel, dim3(ctas), dim3(kThreads), kRingBytes, stream, static_cast<unsigned>(p.slices), p,
+                                w_map, x_map) == cudaSuccess ? launch_status() : B200_ERR_LAUNCH;
 }
 
 template <typename T>
@@ -603,15 +627,9 @@ int launch_pair(Int8LinearParams p, const void* x, const void* w, cudaStream_t s
 
 using namespace b200;
 
-extern "C" int64_t b200_linear_int8_workspace_bytes(int64_t m, int64_t k, int64_t n) {
-  if (m <= 0 || k <= 0 || n <= 0 || m > kRowsAtMost) return 0;
-  return kCounterBytes + static_cast<int64_t>(kNumSMs) * stream_rows(m) * 128 * 4;
-}
-
 extern "C" int b200_linear_int8(const void* x, const float* x_scales, const void* weight, const float* weight_scales,
                                 const void* bias, const void* residual, void* output, int64_t m, int64_t k, int64_t n,
-                                int dtype, int epilogue, void* workspace, int64_t workspace_bytes, int32_t* status,
-                                void* stream) {
+                                int dtype, int epilogue, int32_t* status, void* stream) {
   if (!x || !x_scales || !weight || !weight_scales || !output || !status || m < 0 || k <= 0 || n <= 0 || !known_dtype(dtype) ||
       epilogue < B200_EPILOGUE_NONE || epilogue > B200_EPILOGUE_SWIGLU ||
       (epilogue == B200_EPILOGUE_RESIDUAL) != (residual != nullptr))
@@ -625,11 +643,6 @@ extern "C" int b200_linear_int8(const void* x, const float* x_scales, const void
   p.bias = bias; p.residual = residual; p.out = output; p.status = status;
   p.m = static_cast<int>(m); p.k = static_cast<int>(k); p.n = static_cast<int>(n); p.epilogue = epilogue;
   p.wait_limit = wait_limit(); p.drop_loads = drop_loads();
-  if (m <= kRowsAtMost) {
-    if (!workspace || workspace_bytes < b200_linear_int8_workspace_bytes(m, k, n)) return B200_ERR_WORKSPACE;
-    p.counters = static_cast<int32_t*>(workspace);
-    p.sums = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + kCounterBytes);
-  }
   int code = B200_ERR_UNSUPPORTED;
   with_element_type(dtype, [&](auto tag) {
     using T = typename decltype(tag)::type;

@@ -279,13 +279,9 @@ def b200_linear_int8(values: torch.Tensor, scales: torch.Tensor, weight: torch.T
     if output.numel() == 0:
         return output
     rt = runtime(device)
-    library, m = _lib.load(), scales.numel()
-    need = library.b200_linear_int8_workspace_bytes(m, k, n)
-    workspace = rt.own_workspace("linear_int8", need) if need else None
-    code = library.b200_linear_int8(
+    code = _lib.load().b200_linear_int8(
         values.data_ptr(), scales.data_ptr(), weight.data_ptr(), weight_scales.data_ptr(), _ptr(bias), _ptr(residual),
-        output.data_ptr(), m, k, n, _code(out_dtype), _EPILOGUES[epilogue], _ptr(workspace), need, rt.status.data_ptr(),
-        _stream())
+        output.data_ptr(), scales.numel(), k, n, _code(out_dtype), _EPILOGUES[epilogue], rt.status.data_ptr(), _stream())
     _check(code, "b200_linear_int8")
     _count(rt)
     return output

@@ -70,18 +70,14 @@ def test_quantised_rows_and_linear_refusals():
         _lib.ERR_BAD_ARGUMENT
     assert rows(n=0) == 0
 
-    def linear(x=FAKE, weight=FAKE, residual=None, m=4, k=64, n=8, dtype=_lib.BF16, epilogue=0, workspace=None, nbytes=0):
-        return library.b200_linear_int8(x, FAKE, weight, FAKE, None, residual, FAKE, m, k, n, dtype, epilogue, workspace, nbytes,
-                                        FAKE, None)
+    def linear(x=FAKE, weight=FAKE, residual=None, m=4, k=64, n=8, dtype=_lib.BF16, epilogue=0):
+        return library.b200_linear_int8(x, FAKE, weight, FAKE, None, residual, FAKE, m, k, n, dtype, epilogue, FAKE, None)
 
     assert linear(x=None) == linear(k=0) == linear(epilogue=3) == linear(epilogue=1) == linear(residual=FAKE) == \
         linear(dtype=_lib.I8) == _lib.ERR_BAD_ARGUMENT
     assert linear(k=72) == linear(n=7, epilogue=2) == _lib.ERR_UNSUPPORTED
     assert linear(weight=ODD) == _lib.ERR_ALIGNMENT
     assert linear(k=131072) == _lib.ERR_TOO_LARGE
-    need = library.b200_linear_int8_workspace_bytes(4, 64, 8)
-    assert linear() == linear(workspace=FAKE, nbytes=need - 1) == _lib.ERR_WORKSPACE
-    assert library.b200_linear_int8_workspace_bytes(257, 64, 8) == 0
     assert linear(m=0) == 0
 
 
