@@ -316,43 +316,22 @@ linear_int8_stream_kernel(const Int8LinearParams p, const __grid_constant__ CUte
 }
 
 // -------------------------------------------------------------------------------------------------------------- pair ----
-constexpr int kPairStages = 6;
-constexpr int kPairStageBytes = 2 * 128 * 128;  // half of 256 rows of x, half of up to 256 of the weight
-constexpr int kPairSmem = kPairStages * kPairStageBytes + kEpilogueWarps * 4096;
-
-// 32 accumulator columns of one row: scaled, with the bias. Columns beyond n are not used.
 template <typename T>
-__device__ __forceinline__ void scale_chunk(const Int8LinearParams& p, float row_scale, int col0, float (&v)[32]) {
-  if (col0 + 32 <= p.n) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float* w = p.w_scales + col0 + 4 * i;  // (uniform over the warp; the vector starts anywhere)
-      float4 s;
-      if ((reinterpret_cast<uintptr_t>(p.w_scales) & 15u) == 0) s = *reinterpret_cast<const float4*>(w);
-      else s = make_float4(w[0], w[1], w[2], w[3]);
-      v[4 * i] = static_cast<float>(__float_as_int(v[4 * i])) * row_scale * s.x;
-      v[4 * i + 1] = static_cast<float>(__float_as_int(v[4 * i + 1])) * row_scale * s.y;
-      v[4 * i + 2] = static_cast<float>(__float_as_int(v[4 * i + 2])) * row_scale * s.z;
-      v[4 * i + 3] = static_cast<float>(__float_as_int(v[4 * i + 3])) * row_scale * s.w;
-    }
-    if (p.bias != nullptr) {
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] += Elem<T>::load(static_cast<const T*>(p.bias) + col0 + i);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const bool there = col0 + i < p.n;
-      v[i] = there ? static_cast<float>(__float_as_int(v[i])) * row_scale * p.w_scales[col0 + i] : 0.0f;
-      if (there && p.bias != nullptr) v[i] += Elem<T>::load(static_cast<const T*>(p.bias) + col0 + i);
-    }
-  }
+__host__ __device__ constexpr int pair_stages() { return sizeof(T) == 4 ? 5 : 6; }  // (staging tiles of fp32 take the sixth one's place)
+constexpr int kPairStageBytes = 2 * 128 * 128;  // half of 256 rows of x, half of up to 256 of the weight
+constexpr int kPairWarps = 8;      // of the epilogue: two for each quarter of the accumulator's lanes
+constexpr int kPairThreads = (kPairWarps + 2) * 32;
+
+template <typename T>
+constexpr int pair_smem() {
+  return pair_stages<T>() * kPairStageBytes + kPairWarps * (32 * 32 * static_cast<int>(sizeof(T)) + 4 * 32 * 8);
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kPairThreads, 1)
 linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtensorMap x_map,
                         const __grid_constant__ CUtensorMap w_map) {
+  constexpr int kPairStages = pair_stages<T>();
   extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ __align__(8) uint64_t full[kPairStages], empty[kPairStages], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_slot;
@@ -378,13 +357,13 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
     }
     for (int a = 0; a < 2; ++a) {
       mbarrier_init(smem_u32(&acc_full[a]), 1);
-      mbarrier_init(smem_u32(&acc_empty[a]), 2 * kEpilogueWarps);  // (the first CTA's counts: both CTAs' warps)
+      mbarrier_init(smem_u32(&acc_empty[a]), 2 * kPairWarps);  // (the first CTA's counts: both CTAs' warps)
     }
     fence_mbarrier_init();
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&x_map)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&w_map)) : "memory");
   }
-  if (warp == kEpilogueWarps + 1) {
+  if (warp == kPairWarps + 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
                  ::"r"(smem_u32(&tmem_slot)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
@@ -396,7 +375,7 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
   const uint32_t tmem_base = tmem_slot;
   grid_dependency_wait();
 
-  if (warp == kEpilogueWarps && !p.drop_loads) {
+  if (warp == kPairWarps && !p.drop_loads) {
     // ---- producer: this CTA's halves; all bytes of a stage count on the first CTA's barrier ----
     const uint32_t leader = elect_one();
     bool ok = true;
@@ -419,7 +398,7 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
       }
     }
     if (!ok) failed = 1;
-  } else if (warp == kEpilogueWarps + 1 && rank == 0) {
+  } else if (warp == kPairWarps + 1 && rank == 0) {
     // ---- products of both CTAs, issued by the first ----
     const uint32_t leader = elect_one();
     const uint32_t idesc = instruction_descriptor_i8(256, bn);
@@ -444,113 +423,145 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
       if (ok) umma_commit_pair_if(leader, smem_u32(&acc_full[acc]));
     }
     if (!ok) failed = 1;
-  } else if (warp < kEpilogueWarps) {
-    // ---- epilogue: this CTA's 128 rows; warp w reads lanes 32 w .. of the accumulator ----
+  } else if (warp < kPairWarps) {
+    // ---- epilogue: this CTA's 128 rows; lanes 32 (warp % 4) .., every other chunk of 32 columns ----
+    // Everything that comes from memory (scales, bias, the first residual chunk) is asked for before the wait for the
+    // products. A chunk leaves through a staging tile, so that a store writes whole rows of it and a residual is read so.
     const bool swiglu = p.epilogue == B200_EPILOGUE_SWIGLU;
     const int out_cols = swiglu ? p.n / 2 : p.n;
     T* out = static_cast<T*>(p.out);
     const T* residual = static_cast<const T*>(p.residual);
-    constexpr int kVec = 16 / static_cast<int>(sizeof(T)), kSegment = 8 * kVec;  // output columns of 128 bytes
+    constexpr int kVec = 16 / static_cast<int>(sizeof(T)), kUnits = 32 / kVec;  // of 16 bytes: a row of a chunk
     const bool staged = (out_cols * static_cast<int>(sizeof(T))) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0 &&
                         (residual == nullptr || (reinterpret_cast<uintptr_t>(residual) & 15u) == 0);
-    const int span = swiglu ? 2 * kSegment : kSegment;  // accumulator columns of a segment
-    const uint32_t stage_tile = smem_base + kPairStages * kPairStageBytes + warp * 4096;
+    const int quarter = warp & 3, turn0 = warp >> 2;
+    constexpr int kStageTile = 32 * 32 * static_cast<int>(sizeof(T));
+    const uint32_t stage_tile = smem_base + kPairStages * kPairStageBytes + warp * kStageTile;
+    float2* column_terms = reinterpret_cast<float2*>(smem + kPairStages * kPairStageBytes + kPairWarps * kStageTile) + warp * 128;
     const uint32_t acc_empty_first = map_to_rank(smem_u32(&acc_empty[0]), 0);
+    // 16-byte unit `unit` of row r of a chunk with `units` of them: 128 bytes of rows side by side never share a bank
+    auto unit_at = [&](int r, int unit, int units) {
+      return stage_tile + r * units * 16 + ((unit ^ ((r * units >> 3) & (units - 1))) << 4);
+    };
     bool ok = true;
     int done = 0;
     for (int tile = pair; tile < tiles; tile += pairs, ++done) {
       int tile_m, tile_n;
       place(tile, tile_m, tile_n);
-      const int acc = done & 1, row0 = tile_m * 256 + rank * 128 + warp * 32, row = row0 + lane;
+      const int acc = done & 1, row0 = tile_m * 256 + rank * 128 + quarter * 32, row = row0 + lane;
+      const int n_end = min(p.n, (tile_n + 1) * bn);
       const float row_scale = row < p.m ? p.x_scales[row] : 0.0f;
+      __syncwarp();  // (the tile before is done with the terms)
+      for (int c0 = turn0 * 32, q = 0; c0 < bn; c0 += 64, ++q) {
+        const int col = tile_n * bn + c0 + lane;
+        column_terms[q * 32 + lane] = make_float2(
+            col < n_end ? p.w_scales[col] : 0.0f,
+            col < n_end && p.bias != nullptr ? Elem<T>::load(static_cast<const T*>(p.bias) + col) : 0.0f);
+      }
+      uint4 ahead[kUnits];  // the next chunk's residual: rows side by side over the lanes
+      auto fetch = [&](int c0) {
+        if (residual == nullptr || !staged || tile_n * bn + c0 + 32 > n_end) return;
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+          const int r = (i * 32 + lane) / kUnits, unit = (i * 32 + lane) % kUnits;
+          ahead[i] = row0 + r < p.m ? *reinterpret_cast<const uint4*>(residual + static_cast<int64_t>(row0 + r) * p.n +
+                                                                      tile_n * bn + c0 + unit * kVec)
+                                    : make_uint4(0u, 0u, 0u, 0u);
+        }
+      };
+      fetch(turn0 * 32);
       ok = ok && __all_sync(0xffffffffu, mbarrier_wait_bounded(smem_u32(&acc_full[acc]), (done >> 1) & 1, p.wait_limit));
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint32_t t_addr = tmem_base + acc * 256 + (static_cast<uint32_t>(warp * 32) << 16);
-      const int n_end = min(p.n, (tile_n + 1) * bn);
+      const uint32_t t_addr = tmem_base + acc * 256 + (static_cast<uint32_t>(quarter * 32) << 16);
 #pragma unroll 1
-      for (int c0 = 0; c0 < bn;) {
+      for (int c0 = turn0 * 32, q = 0; c0 < bn; c0 += 64, ++q) {
         const int col0 = tile_n * bn + c0;
         if (col0 >= n_end) break;  // (warp-uniform)
-        if (staged && c0 + span <= bn && col0 + span <= n_end) {
-          uint4 packed[8];
+        float v[32];
+        tmem_load_32x32(t_addr + c0, v);
+        const float4* terms = reinterpret_cast<const float4*>(column_terms + q * 32);  // scale, bias of two columns
 #pragma unroll
-          for (int part = 0; part < kSegment / 16; ++part) {  // 16 output columns at a time
-            float y[16];
-            if (swiglu) {
-              float v[32];
-              tmem_load_32x32(t_addr + c0 + part * 32, v);
-              scale_chunk<T>(p, row_scale, col0 + part * 32, v);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) y[i] = silu_times(v[2 * i], v[2 * i + 1]);
-            } else {
-              if (part % 2 == 1) continue;  // (32 columns at a time)
-              float v[32];
-              tmem_load_32x32(t_addr + c0 + part * 16, v);
-              scale_chunk<T>(p, row_scale, col0 + part * 16, v);
-              if (residual != nullptr && row < p.m) {
-                const T* r = residual + static_cast<int64_t>(row) * p.n + col0 + part * 16;
-#pragma unroll
-                for (int i = 0; i < 32 / kVec; ++i) {
-                  Vec16<T> other;
-                  other.load(r + i * kVec);
-#pragma unroll
-                  for (int e = 0; e < kVec; ++e) v[i * kVec + e] += other.v[e];
-                }
-              }
-#pragma unroll
-              for (int i = 0; i < 32 / kVec; ++i) {
-                Vec16<T> t;
-#pragma unroll
-                for (int e = 0; e < kVec; ++e) t.v[e] = v[i * kVec + e];
-                t.store(reinterpret_cast<T*>(&packed[(part * 16) / kVec + i]));
-              }
-              continue;
-            }
-#pragma unroll
-            for (int i = 0; i < 16 / kVec; ++i) {
-              Vec16<T> t;
-#pragma unroll
-              for (int e = 0; e < kVec; ++e) t.v[e] = y[i * kVec + e];
-              t.store(reinterpret_cast<T*>(&packed[(part * 16) / kVec + i]));
-            }
-          }
-          __syncwarp();  // the round before has been read
-#pragma unroll
-          for (int u = 0; u < 8; ++u)
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage_tile + lane * 128 + ((u ^ (lane & 7)) << 4)),
-                         "r"(packed[u].x), "r"(packed[u].y), "r"(packed[u].z), "r"(packed[u].w) : "memory");
-          __syncwarp();
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {  // four whole 128-byte row segments an instruction
-            const int r = i * 4 + (lane >> 3), u = lane & 7;
-            uint4 value;
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(value.x), "=r"(value.y), "=r"(value.z), "=r"(value.w)
-                         : "r"(stage_tile + r * 128 + ((u ^ (r & 7)) << 4)));
-            if (row0 + r < p.m)
-              *reinterpret_cast<uint4*>(out + static_cast<int64_t>(row0 + r) * out_cols + (swiglu ? col0 / 2 : col0) + u * kVec) = value;
-          }
-          c0 += span;
-        } else {
-          float v[32];
-          tmem_load_32x32(t_addr + c0, v);
-          scale_chunk<T>(p, row_scale, col0, v);
+        for (int i = 0; i < 16; ++i) {
+          const float4 t = terms[i];
+          v[2 * i] = fmaf(static_cast<float>(__float_as_int(v[2 * i])) * row_scale, t.x, t.y);
+          v[2 * i + 1] = fmaf(static_cast<float>(__float_as_int(v[2 * i + 1])) * row_scale, t.z, t.w);
+        }
+        if (!staged || col0 + 32 > n_end) {
           if (row < p.m) {
+            const int64_t at = static_cast<int64_t>(row) * out_cols + (swiglu ? col0 / 2 : col0);
             if (swiglu) {
 #pragma unroll
               for (int i = 0; i < 16; ++i)
-                if (col0 + 2 * i < n_end)
-                  Elem<T>::store(out + static_cast<int64_t>(row) * out_cols + col0 / 2 + i, silu_times(v[2 * i], v[2 * i + 1]));
+                if (col0 + 2 * i < n_end) Elem<T>::store(out + at + i, silu_times(v[2 * i], v[2 * i + 1]));
             } else {
-              const int64_t at = static_cast<int64_t>(row) * p.n + col0;
 #pragma unroll
               for (int i = 0; i < 32; ++i)
-                if (col0 + i < n_end)
-                  Elem<T>::store(out + at + i, v[i] + (residual != nullptr ? Elem<T>::load(residual + at + i) : 0.0f));
+                if (col0 + i < n_end) Elem<T>::store(out + at + i, v[i] + (residual ? Elem<T>::load(residual + at + i) : 0.0f));
             }
           }
-          c0 += 32;
+          continue;
+        }
+        __syncwarp();  // the chunk before has been read
+        if (swiglu) {
+          constexpr int kHalf = kUnits / 2;
+#pragma unroll
+          for (int unit = 0; unit < kHalf; ++unit) {
+            Vec16<T> t;
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) t.v[e] = silu_times(v[2 * (unit * kVec + e)], v[2 * (unit * kVec + e) + 1]);
+            uint4 packed;
+            t.store(reinterpret_cast<T*>(&packed));
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(unit_at(lane, unit, kHalf)), "r"(packed.x), "r"(packed.y),
+                         "r"(packed.z), "r"(packed.w) : "memory");
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < kHalf; ++i) {
+            const int r = (i * 32 + lane) / kHalf, unit = (i * 32 + lane) % kHalf;
+            uint4 value;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(value.x), "=r"(value.y), "=r"(value.z), "=r"(value.w)
+                         : "r"(unit_at(r, unit, kHalf)));
+            if (row0 + r < p.m)
+              *reinterpret_cast<uint4*>(out + static_cast<int64_t>(row0 + r) * out_cols + col0 / 2 + unit * kVec) = value;
+          }
+          continue;
+        }
+        if (residual != nullptr) {
+#pragma unroll
+          for (int i = 0; i < kUnits; ++i)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(unit_at((i * 32 + lane) / kUnits, (i * 32 + lane) % kUnits, kUnits)),
+                         "r"(ahead[i].x), "r"(ahead[i].y), "r"(ahead[i].z), "r"(ahead[i].w) : "memory");
+          if (c0 + 64 < bn) fetch(c0 + 64);
+          __syncwarp();
+        }
+#pragma unroll
+        for (int unit = 0; unit < kUnits; ++unit) {
+          Vec16<T> t;
+          uint4 packed;
+          if (residual != nullptr) {
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(packed.x), "=r"(packed.y), "=r"(packed.z), "=r"(packed.w)
+                         : "r"(unit_at(lane, unit, kUnits)));
+            t.load(reinterpret_cast<const T*>(&packed));
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) t.v[e] += v[unit * kVec + e];
+          } else {
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) t.v[e] = v[unit * kVec + e];
+          }
+          t.store(reinterpret_cast<T*>(&packed));
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(unit_at(lane, unit, kUnits)), "r"(packed.x), "r"(packed.y),
+                       "r"(packed.z), "r"(packed.w) : "memory");
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+          const int r = (i * 32 + lane) / kUnits, unit = (i * 32 + lane) % kUnits;
+          uint4 value;
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(value.x), "=r"(value.y), "=r"(value.z), "=r"(value.w)
+                       : "r"(unit_at(r, unit, kUnits)));
+          if (row0 + r < p.m)
+            *reinterpret_cast<uint4*>(out + static_cast<int64_t>(row0 + r) * out_cols + col0 + unit * kVec) = value;
         }
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -564,7 +575,7 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
   __syncthreads();
   if (threadIdx.x == 0 && failed) atomicOr(p.status, B200_STATUS_WAIT_TIMEOUT);
   cluster_sync();  // neither CTA leaves while the other may still signal it
-  if (warp == kEpilogueWarps + 1)
+  if (warp == kPairWarps + 1)
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
 }
 
@@ -616,9 +627,9 @@ int launch_pair(Int8LinearParams p, const void* x, const void* w, cudaStream_t s
   const int64_t tiles = tiles_m * ceil_div(p.n, p.cols);
   const unsigned pairs = static_cast<unsigned>(std::min<int64_t>(kPairs, tiles));
   auto kernel = linear_int8_pair_kernel<T>;
-  static_assert(tensor_memory_fits(512, kPairSmem), "tensor memory under programmatic launches");
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem) != cudaSuccess) return B200_ERR_LAUNCH;
-  return launch_chained_cluster(kernel, dim3(2 * pairs), dim3(kThreads), kPairSmem, stream, 2u, p, x_map, w_map) == cudaSuccess
+  static_assert(tensor_memory_fits(512, pair_smem<T>()) && pair_smem<T>() + 1024 <= 227 * 1024, "tensor memory under programmatic launches");
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, pair_smem<T>()) != cudaSuccess) return B200_ERR_LAUNCH;
+  return launch_chained_cluster(kernel, dim3(2 * pairs), dim3(kPairThreads), pair_smem<T>(), stream, 2u, p, x_map, w_map) == cudaSuccess
              ? launch_status() : B200_ERR_LAUNCH;
 }
 
