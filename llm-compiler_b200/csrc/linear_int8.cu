@@ -91,10 +91,13 @@ __device__ __forceinline__ void wait_for_copies(uint64_t* full, int stages, int 
   }
 }
 
-// gate / (1 + e^-gate) * up on the special-function unit: the exponential and the quotient are good to a few units of 2^-23.
-// (1 + e^-gate is infinite below -88, where the quotient, -0, is the right answer; a gate of -infinity gives NaN as 0 * infinity does.)
+// gate / (1 + e^-gate) * up on the special-function unit: 2^x and 1 / x there are good to two units of 2^-23, and the
+// exponent's rounding adds |gate| of them. (Below -88 the sum is infinite and its reciprocal 0: the right answer.)
 __device__ __forceinline__ float silu_times(float gate, float up) {
-  return __fdividef(gate, 1.0f + __expf(-gate)) * up;
+  float power, inverse;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(power) : "f"(-1.4426950408889634f * gate));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(1.0f + power));
+  return gate * inverse * up;
 }
 
 // ------------------------------------------------------------------------------------------------------------ stream ----
@@ -474,12 +477,17 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t t_addr = tmem_base + acc * 256 + (static_cast<uint32_t>(quarter * 32) << 16);
+      uint32_t raw[32];  // the next chunk's sums, on their way while a chunk is worked on
+      tmem_load_32x32_issue(t_addr + turn0 * 32, raw);
 #pragma unroll 1
       for (int c0 = turn0 * 32, q = 0; c0 < bn; c0 += 64, ++q) {
         const int col0 = tile_n * bn + c0;
         if (col0 >= n_end) break;  // (warp-uniform)
+        tmem_load_wait(raw);
         float v[32];
-        tmem_load_32x32(t_addr + c0, v);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(raw[i]);
+        if (c0 + 64 < bn) tmem_load_32x32_issue(t_addr + c0 + 64, raw);
         const float4* terms = reinterpret_cast<const float4*>(column_terms + q * 32);  // scale, bias of two columns
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -564,6 +572,7 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
             *reinterpret_cast<uint4*>(out + static_cast<int64_t>(row0 + r) * out_cols + col0 + unit * kVec) = value;
         }
       }
+      tmem_load_wait(raw);  // (of a chunk beyond n, if there is one)
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0)
