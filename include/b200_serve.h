@@ -772,34 +772,62 @@ int b200_advance_slots(int64_t* lengths, const int32_t* slots, const int32_t* st
  * contiguous codes, K a multiple of 16 and at most 131056; bias, residual and output are of dtype. `status` receives
  * B200_STATUS_WAIT_TIMEOUT if a bounded in-kernel wait gives up. */
 #define B200_MAX_COPY_POOLS 8
+/* (arguments in structs of 8-byte fields: a host that launches from an interpreter packs them in one step) */
+typedef struct b200_cache_store_call {
+  void *key_pool, *value_pool;
+  float *key_scales, *value_scales;
+  const int32_t* block_table;
+  const void *key, *value;
+  const int64_t* positions;
+  int32_t* status;
+  int64_t batch, heads, tokens, head_dim, num_blocks, block_size, max_blocks_per_sequence;
+  int64_t key_strides[4], value_strides[4];
+  int64_t dtype, cache_dtype;
+} b200_cache_store_call;
+typedef struct b200_cache_attention_call {
+  const void *query, *key_pool, *value_pool;
+  const float *key_scales, *value_scales;
+  const int32_t* block_table;
+  const int64_t* lengths;
+  const void* mask;
+  void *output, *workspace;
+  int32_t* status;
+  int64_t batch, q_heads, kv_heads, head_dim, num_blocks, block_size, max_blocks_per_sequence, mask_len;
+  int64_t q_batch_stride, q_head_stride, mask_batch_stride;
+  int64_t mask_dtype, dtype, cache_dtype, split_tokens, max_length_hint, workspace_bytes;
+  double scale;
+} b200_cache_attention_call;
 typedef struct b200_block_pool {
   void* base;
   int64_t layer_stride; /* bytes */
   int64_t block_bytes;
 } b200_block_pool;
-int b200_paged_kv_store_8bit(void* key_pool, void* value_pool, float* key_scales, float* value_scales,
-                             const int32_t* block_table, const void* key, const void* value, const int64_t* positions,
-                             int64_t batch, int64_t heads, int64_t tokens, int64_t head_dim, int64_t num_blocks,
-                             int64_t block_size, int64_t max_blocks_per_sequence, const int64_t key_strides[4],
-                             const int64_t value_strides[4], int dtype, int cache_dtype, int32_t* status, void* stream);
+typedef struct b200_quantize_rows_call {
+  const void *input, *residual, *norm_weight;
+  void *sum, *codes;
+  float* scales;
+  int64_t rows, hidden, input_row_stride, residual_row_stride, dtype;
+  double epsilon;
+} b200_quantize_rows_call;
+typedef struct b200_linear_int8_call {
+  const void* x;
+  const float* x_scales;
+  const void* weight;
+  const float* weight_scales;
+  const void *bias, *residual;
+  void* output;
+  int32_t* status;
+  int64_t m, k, n, dtype, epilogue;
+} b200_linear_int8_call;
+int b200_paged_kv_store_8bit(const b200_cache_store_call* call, void* stream);
 int64_t b200_paged_decode_attention_8bit_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads,
                                                          int64_t head_dim, int64_t max_length, int64_t split_tokens);
-int b200_paged_decode_attention_8bit(
-    const void* query, const void* key_pool, const void* value_pool, const float* key_scales, const float* value_scales,
-    const int32_t* block_table, const int64_t* lengths, const void* mask, void* output, int64_t batch, int64_t q_heads,
-    int64_t kv_heads, int64_t head_dim, int64_t num_blocks, int64_t block_size, int64_t max_blocks_per_sequence,
-    int64_t mask_len, int64_t q_batch_stride, int64_t q_head_stride, int64_t mask_batch_stride, int mask_dtype, double scale,
-    int dtype, int cache_dtype, int64_t split_tokens, int64_t max_length_hint, void* workspace, int64_t workspace_bytes,
-    int32_t* status, void* stream);
+int b200_paged_decode_attention_8bit(const b200_cache_attention_call* call, void* stream);
 int b200_copy_kv_blocks(const b200_block_pool* pools, int64_t pool_count, const int32_t* sources,
                         const int32_t* destinations, int64_t count, int64_t layers, int64_t num_blocks, int32_t* status,
                         void* stream);
-int b200_quantize_rows_int8(const void* input, const void* residual, const void* norm_weight, void* sum, void* codes,
-                            float* scales, int64_t rows, int64_t hidden, int64_t input_row_stride,
-                            int64_t residual_row_stride, double epsilon, int dtype, void* stream);
-int b200_linear_int8(const void* x, const float* x_scales, const void* weight, const float* weight_scales, const void* bias,
-                     const void* residual, void* output, int64_t m, int64_t k, int64_t n, int dtype, int epilogue,
-                     int32_t* status, void* stream);
+int b200_quantize_rows_int8(const b200_quantize_rows_call* call, void* stream);
+int b200_linear_int8(const b200_linear_int8_call* call, void* stream);
 
 #ifdef __cplusplus
 }

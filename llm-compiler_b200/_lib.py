@@ -116,12 +116,6 @@ class PromptCall(ctypes.Structure):
                [("epsilon", c_double), ("scale", c_double), ("dtype", c_int), ("mode", c_int)]
 
 
-class BlockPool(ctypes.Structure):
-    """b200_block_pool of include/b200_serve.h."""
-
-    _fields_ = [("base", c_void_p), ("layer_stride", c_int64), ("block_bytes", c_int64)]
-
-
 MAX_COPY_POOLS = 8
 
 _DELTA, _RETENTION, _STEP = POINTER(DeltaInputs), POINTER(RetentionInputs), POINTER(StepOutput)
@@ -232,14 +226,13 @@ SIGNATURES = {
                                                                      c_void_p, c_void_p]),
     "b200_sequence_positions": (c_int, [c_void_p] * 3 + [c_int64, c_void_p]),
     "b200_advance_slots": (c_int, [c_void_p] * 3 + [c_int64, c_int64, c_void_p, c_void_p]),
-    "b200_paged_kv_store_8bit": (c_int, [c_void_p] * 8 + [c_int64] * 7 + [_I64P, _I64P, c_int, c_int, c_void_p, c_void_p]),
+    # (structs of 8-byte fields, packed by the caller: quantized_kernels.py)
+    "b200_paged_kv_store_8bit": (c_int, [c_char_p, c_void_p]),
     "b200_paged_decode_attention_8bit_workspace_bytes": (c_int64, [c_int64] * 6),
-    "b200_paged_decode_attention_8bit": (c_int, [c_void_p] * 9 + [c_int64] * 11 + [c_int, c_double, c_int, c_int, c_int64,
-                                                                                c_int64, c_void_p, c_int64, c_void_p,
-                                                                                c_void_p]),
-    "b200_copy_kv_blocks": (c_int, [POINTER(BlockPool), c_int64, c_void_p, c_void_p] + [c_int64] * 3 + [c_void_p, c_void_p]),
-    "b200_quantize_rows_int8": (c_int, [c_void_p] * 6 + [c_int64] * 4 + [c_double, c_int, c_void_p]),
-    "b200_linear_int8": (c_int, [c_void_p] * 7 + [c_int64] * 3 + [c_int, c_int, c_void_p, c_void_p]),
+    "b200_paged_decode_attention_8bit": (c_int, [c_char_p, c_void_p]),
+    "b200_copy_kv_blocks": (c_int, [c_char_p, c_int64, c_void_p, c_void_p] + [c_int64] * 3 + [c_void_p, c_void_p]),
+    "b200_quantize_rows_int8": (c_int, [c_char_p, c_void_p]),
+    "b200_linear_int8": (c_int, [c_char_p, c_void_p]),
 }
 
 _library: ctypes.CDLL | None = None

@@ -617,7 +617,8 @@ int launch_stream(Int8LinearParams p, const void* x, const void* w, cudaStream_t
   const unsigned ctas = static_cast<unsigned>(p.slices > 1 ? tiles * p.slices : std::min<int64_t>(kNumSMs, tiles));
   auto kernel = linear_int8_stream_kernel<T>;
   static_assert(tensor_memory_fits(512, kRingBytes), "tensor memory under programmatic launches");
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes) != cudaSuccess) return B200_ERR_LAUNCH;
+  static std::atomic<uint64_t> allowed{0};
+  if (!allow_shared_memory(kernel, kRingBytes, allowed)) return B200_ERR_LAUNCH;
   return launch_chained_cluster(kernel, dim3(ctas), dim3(kThreads), kRingBytes, stream, static_cast<unsigned>(p.slices), p,
                                 w_map, x_map) == cudaSuccess ? launch_status() : B200_ERR_LAUNCH;
 }
@@ -639,7 +640,8 @@ int launch_pair(Int8LinearParams p, const void* x, const void* w, cudaStream_t s
   const unsigned pairs = static_cast<unsigned>(std::min<int64_t>(kPairs, tiles));
   auto kernel = linear_int8_pair_kernel<T>;
   static_assert(tensor_memory_fits(512, pair_smem<T>()) && pair_smem<T>() + 1024 <= 227 * 1024, "tensor memory under programmatic launches");
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, pair_smem<T>()) != cudaSuccess) return B200_ERR_LAUNCH;
+  static std::atomic<uint64_t> allowed{0};
+  if (!allow_shared_memory(kernel, pair_smem<T>(), allowed)) return B200_ERR_LAUNCH;
   return launch_chained_cluster(kernel, dim3(2 * pairs), dim3(kPairThreads), pair_smem<T>(), stream, 2u, p, x_map, w_map) == cudaSuccess
              ? launch_status() : B200_ERR_LAUNCH;
 }
@@ -649,27 +651,29 @@ int launch_pair(Int8LinearParams p, const void* x, const void* w, cudaStream_t s
 
 using namespace b200;
 
-extern "C" int b200_linear_int8(const void* x, const float* x_scales, const void* weight, const float* weight_scales,
-                                const void* bias, const void* residual, void* output, int64_t m, int64_t k, int64_t n,
-                                int dtype, int epilogue, int32_t* status, void* stream) {
-  if (!x || !x_scales || !weight || !weight_scales || !output || !status || m < 0 || k <= 0 || n <= 0 || !known_dtype(dtype) ||
-      epilogue < B200_EPILOGUE_NONE || epilogue > B200_EPILOGUE_SWIGLU ||
-      (epilogue == B200_EPILOGUE_RESIDUAL) != (residual != nullptr))
+extern "C" int b200_linear_int8(const b200_linear_int8_call* call, void* stream) {
+  if (!call) return B200_ERR_BAD_ARGUMENT;
+  const b200_linear_int8_call& c = *call;
+  const int dtype = static_cast<int>(c.dtype);
+  const int64_t m = c.m, k = c.k, n = c.n;
+  if (!c.x || !c.x_scales || !c.weight || !c.weight_scales || !c.output || !c.status || m < 0 || k <= 0 || n <= 0 ||
+      c.dtype != dtype || !known_dtype(dtype) || c.epilogue < B200_EPILOGUE_NONE || c.epilogue > B200_EPILOGUE_SWIGLU ||
+      (c.epilogue == B200_EPILOGUE_RESIDUAL) != (c.residual != nullptr))
     return B200_ERR_BAD_ARGUMENT;
-  if (k % 16 != 0 || (epilogue == B200_EPILOGUE_SWIGLU && n % 2 != 0)) return B200_ERR_UNSUPPORTED;
-  if (!aligned16(x) || !aligned16(weight)) return B200_ERR_ALIGNMENT;
+  if (k % 16 != 0 || (c.epilogue == B200_EPILOGUE_SWIGLU && n % 2 != 0)) return B200_ERR_UNSUPPORTED;
+  if (!aligned16(c.x) || !aligned16(c.weight)) return B200_ERR_ALIGNMENT;
   if (k > kMaxK || m > (1 << 22) || n > (1 << 22)) return B200_ERR_TOO_LARGE;
   if (m == 0) return B200_OK;
   Int8LinearParams p = {};
-  p.x_scales = x_scales; p.w_scales = weight_scales;
-  p.bias = bias; p.residual = residual; p.out = output; p.status = status;
-  p.m = static_cast<int>(m); p.k = static_cast<int>(k); p.n = static_cast<int>(n); p.epilogue = epilogue;
+  p.x_scales = c.x_scales; p.w_scales = c.weight_scales;
+  p.bias = c.bias; p.residual = c.residual; p.out = c.output; p.status = c.status;
+  p.m = static_cast<int>(m); p.k = static_cast<int>(k); p.n = static_cast<int>(n); p.epilogue = static_cast<int>(c.epilogue);
   p.wait_limit = wait_limit(); p.drop_loads = drop_loads();
   int code = B200_ERR_UNSUPPORTED;
   with_element_type(dtype, [&](auto tag) {
     using T = typename decltype(tag)::type;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    code = m <= kRowsAtMost ? launch_stream<T>(p, x, weight, s) : launch_pair<T>(p, x, weight, s);
+    code = m <= kRowsAtMost ? launch_stream<T>(p, c.x, c.weight, s) : launch_pair<T>(p, c.x, c.weight, s);
   });
   return code;
 }

@@ -3,6 +3,8 @@
 
 #include <cuda_fp8.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace b200 {
@@ -28,5 +30,18 @@ struct E4m3Code {
 constexpr float kSmallestScale = 1.17549435e-38f;  // the smallest normal number: 1 / scale stays finite
 
 __device__ __forceinline__ bool is_finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
+
+// Opt-in to `bytes` of dynamic shared memory of a kernel, asked of the runtime once per device (a third of a microsecond a
+// call otherwise). `done`: a bit per device, of this kernel and size.
+template <typename Kernel>
+inline bool allow_shared_memory(Kernel kernel, int bytes, std::atomic<uint64_t>& done) {
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return false;
+  const uint64_t bit = device < 64 ? uint64_t(1) << device : 0;
+  if ((done.load(std::memory_order_relaxed) & bit) != 0) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return true;
+}
 
 }  // namespace b200

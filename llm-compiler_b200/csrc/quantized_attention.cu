@@ -49,50 +49,47 @@ extern "C" int64_t b200_paged_decode_attention_8bit_workspace_bytes(int64_t batc
   return parts > 0 ? kCounterBytes + parts * (head_dim + 2) * 4 : 0;
 }
 
-extern "C" int b200_paged_decode_attention_8bit(
-    const void* query, const void* key_pool, const void* value_pool, const float* key_scales, const float* value_scales,
-    const int32_t* block_table, const int64_t* lengths, const void* mask, void* output, int64_t batch, int64_t q_heads,
-    int64_t kv_heads, int64_t head_dim, int64_t num_blocks, int64_t block_size, int64_t max_blocks_per_sequence,
-    int64_t mask_len, int64_t q_batch_stride, int64_t q_head_stride, int64_t mask_batch_stride, int mask_dtype, double scale,
-    int dtype, int cache_dtype, int64_t split_tokens, int64_t max_length_hint, void* workspace, int64_t workspace_bytes,
-    int32_t* status, void* stream) {
-  if (!query || !key_pool || !value_pool || !key_scales || !value_scales || !block_table || !lengths || !output || !status ||
-      batch < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || num_blocks <= 0 || block_size <= 0 ||
-      max_blocks_per_sequence <= 0 || mask_len <= 0 || mask_len > max_blocks_per_sequence * block_size || split_tokens < 0)
+extern "C" int b200_paged_decode_attention_8bit(const b200_cache_attention_call* call, void* stream) {
+  if (!call) return B200_ERR_BAD_ARGUMENT;
+  const b200_cache_attention_call& c = *call;
+  if (!c.query || !c.key_pool || !c.value_pool || !c.key_scales || !c.value_scales || !c.block_table || !c.lengths ||
+      !c.output || !c.status || c.batch < 0 || c.q_heads <= 0 || c.kv_heads <= 0 || c.q_heads % c.kv_heads != 0 ||
+      c.num_blocks <= 0 || c.block_size <= 0 || c.max_blocks_per_sequence <= 0 || c.mask_len <= 0 ||
+      c.mask_len > c.max_blocks_per_sequence * c.block_size || c.split_tokens < 0 ||
+      (c.mask && (c.mask_dtype < 0 || c.mask_dtype > B200_F16)))
     return B200_ERR_BAD_ARGUMENT;
-  if (mask && !known_dtype(mask_dtype)) return B200_ERR_BAD_ARGUMENT;
-  if ((dtype != B200_BF16 && dtype != B200_F16) || (cache_dtype != B200_I8 && cache_dtype != B200_E4M3) ||
-      (head_dim != 64 && head_dim != 128 && head_dim != 256) || block_size % kTile != 0)
+  if ((c.dtype != B200_BF16 && c.dtype != B200_F16) || (c.cache_dtype != B200_I8 && c.cache_dtype != B200_E4M3) ||
+      (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256) || c.block_size % kTile != 0)
     return B200_ERR_UNSUPPORTED;
-  if (!aligned16(key_pool) || !aligned16(value_pool) || (reinterpret_cast<uintptr_t>(output) & 7u) != 0)
+  if (!aligned16(c.key_pool) || !aligned16(c.value_pool) || (reinterpret_cast<uintptr_t>(c.output) & 7u) != 0)
     return B200_ERR_ALIGNMENT;
-  if (batch > 65535 || q_heads > 65535 || num_blocks * kv_heads > INT32_MAX || num_blocks > INT32_MAX ||
-      block_size > (1 << 20) || mask_len > (int64_t(1) << 40))
+  if (c.batch > 65535 || c.q_heads > 65535 || c.num_blocks > INT32_MAX || c.num_blocks * c.kv_heads > INT32_MAX ||
+      c.block_size > (1 << 20) || c.mask_len > (int64_t(1) << 40))
     return B200_ERR_TOO_LARGE;
-  if (batch == 0) return B200_OK;
-  const int64_t longest = max_length_hint > 0 && max_length_hint < mask_len ? max_length_hint : mask_len;
-  const Plan plan = plan_of(batch, q_heads, kv_heads, head_dim, longest, split_tokens);
+  if (c.batch == 0) return B200_OK;
+  const int64_t longest = c.max_length_hint > 0 && c.max_length_hint < c.mask_len ? c.max_length_hint : c.mask_len;
+  const Plan plan = plan_of(c.batch, c.q_heads, c.kv_heads, c.head_dim, longest, c.split_tokens);
   if (plan.splits > 65535) return B200_ERR_TOO_LARGE;
   Params p = {};
-  const int64_t parts = plan.parts(batch, kv_heads);
+  const int64_t parts = plan.parts(c.batch, c.kv_heads);
   if (parts > 0) {
-    if (!workspace || workspace_bytes < kCounterBytes + parts * (head_dim + 2) * 4) return B200_ERR_WORKSPACE;
-    p.counters = static_cast<int*>(workspace);
-    p.ws_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes);
-    p.ws_ml = p.ws_o + parts * head_dim;
+    if (!c.workspace || c.workspace_bytes < kCounterBytes + parts * (c.head_dim + 2) * 4) return B200_ERR_WORKSPACE;
+    p.counters = static_cast<int*>(c.workspace);
+    p.ws_o = reinterpret_cast<float*>(static_cast<char*>(c.workspace) + kCounterBytes);
+    p.ws_ml = p.ws_o + parts * c.head_dim;
   }
-  p.q = query; p.key_scales = key_scales; p.value_scales = value_scales; p.table = block_table; p.lengths = lengths;
-  p.mask = mask; p.out = output; p.status = status;
-  p.q_batch_stride = q_batch_stride; p.q_head_stride = q_head_stride; p.mask_batch_stride = mask_batch_stride;
-  p.num_blocks = num_blocks; p.max_blocks = max_blocks_per_sequence; p.mask_len = mask_len;
+  p.q = c.query; p.key_scales = c.key_scales; p.value_scales = c.value_scales; p.table = c.block_table;
+  p.lengths = c.lengths; p.mask = c.mask; p.out = c.output; p.status = c.status;
+  p.q_batch_stride = c.q_batch_stride; p.q_head_stride = c.q_head_stride; p.mask_batch_stride = c.mask_batch_stride;
+  p.num_blocks = c.num_blocks; p.max_blocks = c.max_blocks_per_sequence; p.mask_len = c.mask_len;
   p.split_tokens = plan.split_tokens; p.num_splits = static_cast<int>(plan.splits);
-  p.q_heads = static_cast<int>(q_heads); p.kv_heads = static_cast<int>(kv_heads);
-  p.group = static_cast<int>(q_heads / kv_heads);
+  p.q_heads = static_cast<int>(c.q_heads); p.kv_heads = static_cast<int>(c.kv_heads);
+  p.group = static_cast<int>(c.q_heads / c.kv_heads);
   p.head_blocks = static_cast<int>(plan.head_blocks); p.block_heads = static_cast<int>(plan.block_heads);
-  p.block_size = static_cast<int>(block_size); p.mask_dtype = mask_dtype; p.half = dtype == B200_F16;
-  p.q_vector = aligned16(query) && q_batch_stride % 8 == 0 && q_head_stride % 8 == 0;
-  p.scale = static_cast<float>(scale); p.wait_limit = wait_limit(); p.drop_loads = drop_loads();
+  p.block_size = static_cast<int>(c.block_size); p.mask_dtype = static_cast<int>(c.mask_dtype); p.half = c.dtype == B200_F16;
+  p.q_vector = aligned16(c.query) && c.q_batch_stride % 8 == 0 && c.q_head_stride % 8 == 0;
+  p.scale = static_cast<float>(c.scale); p.wait_limit = wait_limit(); p.drop_loads = drop_loads();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return cache_dtype == B200_I8 ? launch_int8(p, key_pool, value_pool, batch, head_dim, s)
-                                : launch_e4m3(p, key_pool, value_pool, batch, head_dim, s);
+  return c.cache_dtype == B200_I8 ? launch_int8(p, c.key_pool, c.value_pool, c.batch, c.head_dim, s)
+                                  : launch_e4m3(p, c.key_pool, c.value_pool, c.batch, c.head_dim, s);
 }

@@ -565,7 +565,8 @@ int launch_shape(const Params& p, const void* keys, const void* values, int64_t 
     return B200_ERR_UNSUPPORTED;
   constexpr int smem = std::max(Shape<D>::kRingBytes, kWarps * 8 * NT * D * 4);
   auto kernel = cache_attention_kernel<Code, D, NT, kMask>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return B200_ERR_LAUNCH;
+  static std::atomic<uint64_t> allowed{0};
+  if (!allow_shared_memory(kernel, smem, allowed)) return B200_ERR_LAUNCH;
   const dim3 grid(static_cast<unsigned>(p.num_splits), static_cast<unsigned>(p.kv_heads * p.head_blocks),
                   static_cast<unsigned>(batch));
   return launch_chained(kernel, grid, dim3(kThreads), smem, stream, p, key_map, value_map) == cudaSuccess ? launch_status()

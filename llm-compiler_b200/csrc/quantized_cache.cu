@@ -251,35 +251,33 @@ cudaError_t launch_store(const StoreParams& p, bool vector, int64_t batch, cudaS
 
 using namespace b200;
 
-extern "C" int b200_paged_kv_store_8bit(void* key_pool, void* value_pool, float* key_scales, float* value_scales,
-                                        const int32_t* block_table, const void* key, const void* value,
-                                        const int64_t* positions, int64_t batch, int64_t heads, int64_t tokens,
-                                        int64_t head_dim, int64_t num_blocks, int64_t block_size,
-                                        int64_t max_blocks_per_sequence, const int64_t key_strides[4],
-                                        const int64_t value_strides[4], int dtype, int cache_dtype, int32_t* status,
-                                        void* stream) {
-  if (!key_pool || !value_pool || !key_scales || !value_scales || !block_table || !key || !value || !positions || !status ||
-      batch < 0 || heads <= 0 || tokens < 0 || head_dim <= 0 || num_blocks <= 0 || block_size <= 0 ||
-      max_blocks_per_sequence <= 0)
+extern "C" int b200_paged_kv_store_8bit(const b200_cache_store_call* call, void* stream) {
+  if (!call) return B200_ERR_BAD_ARGUMENT;
+  const b200_cache_store_call& c = *call;
+  if (!c.key_pool || !c.value_pool || !c.key_scales || !c.value_scales || !c.block_table || !c.key || !c.value ||
+      !c.positions || !c.status || c.batch < 0 || c.heads <= 0 || c.tokens < 0 || c.head_dim <= 0 || c.num_blocks <= 0 ||
+      c.block_size <= 0 || c.max_blocks_per_sequence <= 0)
     return B200_ERR_BAD_ARGUMENT;
-  if ((dtype != B200_BF16 && dtype != B200_F16) || (cache_dtype != B200_I8 && cache_dtype != B200_E4M3) || head_dim % 16 != 0)
+  const int64_t dtype = c.dtype, cache_dtype = c.cache_dtype;
+  if ((dtype != B200_BF16 && dtype != B200_F16) || (cache_dtype != B200_I8 && cache_dtype != B200_E4M3) || c.head_dim % 16 != 0)
     return B200_ERR_UNSUPPORTED;
-  if (!aligned16(key_pool) || !aligned16(value_pool)) return B200_ERR_ALIGNMENT;
-  if (batch > 65535 || heads > 32767 || head_dim * block_size > (int64_t(1) << 30)) return B200_ERR_TOO_LARGE;
-  if (batch == 0 || tokens == 0) return B200_OK;
+  if (!aligned16(c.key_pool) || !aligned16(c.value_pool)) return B200_ERR_ALIGNMENT;
+  if (c.batch > 65535 || c.heads > 32767 || c.head_dim * c.block_size > (int64_t(1) << 30)) return B200_ERR_TOO_LARGE;
+  if (c.batch == 0 || c.tokens == 0) return B200_OK;
   StoreParams p = {};
-  p.x[0] = key; p.x[1] = value;
-  for (int i = 0; i < 4; ++i) { p.strides[0][i] = key_strides[i]; p.strides[1][i] = value_strides[i]; }
-  p.pool[0] = static_cast<uint8_t*>(key_pool); p.pool[1] = static_cast<uint8_t*>(value_pool);
-  p.scales[0] = key_scales; p.scales[1] = value_scales;
-  p.table = block_table; p.positions = positions; p.status = status;
-  p.tokens = tokens; p.max_blocks = max_blocks_per_sequence; p.num_blocks = num_blocks;
-  p.heads = static_cast<int>(heads); p.dim = static_cast<int>(head_dim); p.block_size = static_cast<int>(block_size);
-  bool vector = aligned16(key) && aligned16(value);
+  p.x[0] = c.key; p.x[1] = c.value;
+  for (int i = 0; i < 4; ++i) { p.strides[0][i] = c.key_strides[i]; p.strides[1][i] = c.value_strides[i]; }
+  p.pool[0] = static_cast<uint8_t*>(c.key_pool); p.pool[1] = static_cast<uint8_t*>(c.value_pool);
+  p.scales[0] = c.key_scales; p.scales[1] = c.value_scales;
+  p.table = c.block_table; p.positions = c.positions; p.status = c.status;
+  p.tokens = c.tokens; p.max_blocks = c.max_blocks_per_sequence; p.num_blocks = c.num_blocks;
+  p.heads = static_cast<int>(c.heads); p.dim = static_cast<int>(c.head_dim); p.block_size = static_cast<int>(c.block_size);
+  bool vector = aligned16(c.key) && aligned16(c.value);
   for (int i = 0; i < 2; ++i) {
     vector = vector && p.strides[i][3] == 1;
     for (int j = 0; j < 3; ++j) vector = vector && p.strides[i][j] % 8 == 0;
   }
+  const int64_t batch = c.batch;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t error;
   if (dtype == B200_BF16)

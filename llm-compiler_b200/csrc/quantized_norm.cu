@@ -164,19 +164,20 @@ cudaError_t quantize_typed(const QuantParams& p, cudaStream_t stream) {
 
 using namespace b200;
 
-extern "C" int b200_quantize_rows_int8(const void* input, const void* residual, const void* norm_weight, void* sum,
-                                       void* codes, float* scales, int64_t rows, int64_t hidden, int64_t input_row_stride,
-                                       int64_t residual_row_stride, double epsilon, int dtype, void* stream) {
-  if (!input || !codes || !scales || rows < 0 || hidden <= 0 || input_row_stride < hidden ||
-      (residual && (!sum || residual_row_stride < hidden)) || !known_dtype(dtype))
+extern "C" int b200_quantize_rows_int8(const b200_quantize_rows_call* call, void* stream) {
+  if (!call) return B200_ERR_BAD_ARGUMENT;
+  const b200_quantize_rows_call& c = *call;
+  const int dtype = static_cast<int>(c.dtype);
+  if (!c.input || !c.codes || !c.scales || c.rows < 0 || c.hidden <= 0 || c.input_row_stride < c.hidden ||
+      (c.residual && (!c.sum || c.residual_row_stride < c.hidden)) || c.dtype != dtype || !known_dtype(dtype))
     return B200_ERR_BAD_ARGUMENT;
-  if (rows > 0x7fffffff) return B200_ERR_TOO_LARGE;
-  if (rows == 0) return B200_OK;
+  if (c.rows > 0x7fffffff) return B200_ERR_TOO_LARGE;
+  if (c.rows == 0) return B200_OK;
   QuantParams p = {};
-  p.x = input; p.residual = residual; p.weight = norm_weight; p.sum = residual ? sum : nullptr;
-  p.codes = static_cast<int8_t*>(codes); p.scales = scales;
-  p.rows = rows; p.hidden = hidden; p.x_stride = input_row_stride; p.residual_stride = residual_row_stride;
-  p.epsilon = static_cast<float>(epsilon);
+  p.x = c.input; p.residual = c.residual; p.weight = c.norm_weight; p.sum = c.residual ? c.sum : nullptr;
+  p.codes = static_cast<int8_t*>(c.codes); p.scales = c.scales;
+  p.rows = c.rows; p.hidden = c.hidden; p.x_stride = c.input_row_stride; p.residual_stride = c.residual_row_stride;
+  p.epsilon = static_cast<float>(c.epsilon);
   cudaError_t error = cudaSuccess;
   with_element_type(dtype, [&](auto tag) {
     error = quantize_typed<typename decltype(tag)::type>(p, static_cast<cudaStream_t>(stream));

@@ -1,20 +1,49 @@
 """Python wrappers over the C ABI for serving in 8 bits (include/b200_serve.h, "Serving in 8 bits"): a paged KV cache of
 8-bit codes with a scale for each block of tokens and KV head, copies of cache blocks, rows quantised to 8-bit integers
 behind a norm, and projections in 8-bit integers. Same rules as kernels.py: preconditions raise before anything is
-launched, launches go to torch's current stream and never synchronise, and there is no fallback to PyTorch."""
+launched, launches go to torch's current stream and never synchronise, and there is no fallback to PyTorch.
+
+Short calls are bound by the host, so the wrappers count their steps: arguments are packed into the ABI's structs by one
+struct.pack (0.7 us; 27 ctypes arguments take 3.8), outputs are made like an input where they are."""
 
 from __future__ import annotations
 
+import functools
+import struct
 from typing import List, Optional, Sequence, Tuple, Union
 
 import torch
 
 from . import _lib
-from .kernels import (_EPILOGUES, _check, _code, _count, _dense, _ptr, _require_cuda, _stream, runtime)
+from .kernels import (_DTYPE_CODES, _EPILOGUES, _RUNTIMES, DeviceRuntime, _check, _code, _dense, _guard_current_device,
+                      _stream, runtime)
 
-# The formats of a cache in 8 bits: the code of the C ABI and the largest code.
+# The formats of a cache in 8 bits: the code of the C ABI.
 CACHE_CODES = {torch.int8: _lib.I8, torch.float8_e4m3fn: _lib.E4M3}
 MAX_K = 131056  # (a sum of that many products of two 8-bit integers stays below 2^31)
+
+# The ABI's structs: pointers, 64-bit integers, doubles.
+_STORE_CALL = struct.Struct("=9Q17q").pack
+_ATTENTION_CALL = struct.Struct("=11Q17qd").pack
+_ROWS_CALL = struct.Struct("=6Q5qd").pack
+_LINEAR_CALL = struct.Struct("=8Q5q").pack
+
+
+def _runtime_of(first: torch.Tensor, *others: Optional[torch.Tensor]) -> DeviceRuntime:
+    """The runtime of the operands' GPU, which is the current one; anything else is refused."""
+
+    try:
+        index = first.get_device()
+        for tensor in others:
+            if tensor is not None and tensor.get_device() != index:
+                raise ValueError("all operands must live on the same CUDA device")
+    except AttributeError as error:
+        raise ValueError("operands must be CUDA tensors") from error
+    if index < 0:
+        raise ValueError("the B200 backend only runs CUDA tensors (there is no CPU fallback)")
+    if index != torch._C._cuda_getDevice():
+        _guard_current_device(first.device)
+    return _RUNTIMES.get(index) or runtime(first.device)
 
 
 def _cache_code(dtype: torch.dtype) -> int:
@@ -32,8 +61,9 @@ def _check_cache(key_pool: torch.Tensor, value_pool: torch.Tensor, key_scales: t
     if len(shape) != 4 or value_pool.shape != shape or not key_pool.is_contiguous() or not value_pool.is_contiguous() or \
             key_pool.dtype != value_pool.dtype:
         raise ValueError("KV pools must be contiguous blocks x H x block_size x D tensors of one shape and dtype")
+    per_block = shape[:2]
     for scales in (key_scales, value_scales):
-        if scales.shape != shape[:2] or scales.dtype != torch.float32 or not scales.is_contiguous():
+        if scales.shape != per_block or scales.dtype != torch.float32 or not scales.is_contiguous():
             raise ValueError("scales must be contiguous float32 blocks x H tensors")
     if block_table.dtype != torch.int32 or block_table.ndim != 2 or block_table.shape[0] != batch or \
             not block_table.is_contiguous():
@@ -49,9 +79,10 @@ def b200_paged_kv_store_8bit(key_pool: torch.Tensor, value_pool: torch.Tensor, k
     magnitude it has been given / 127 (int8) or / 448 (float8_e4m3fn); where a new row raises it, the rows in front of it
     are rounded anew to the larger scale. A block that is entered at its first row forgets what it held.
 
-    Pools are blocks x H x block_size x D, scales float32 blocks x H, the table int32 B x max_blocks."""
+    Pools are blocks x H x block_size x D, scales float32 blocks x H, the table int32 B x max_blocks. No block may belong
+    to two sequences of one call."""
 
-    device = _require_cuda(key_pool, value_pool, key_scales, value_scales, block_table, key, value, positions)
+    rt = _runtime_of(key_pool, value_pool, key_scales, value_scales, block_table, key, value, positions)
     if key.ndim != 4 or key.shape != value.shape or key.dtype != value.dtype:
         raise ValueError("key/value must be B x H x T x D tensors of one shape and dtype")
     batch, heads, tokens, dim = key.shape
@@ -64,16 +95,22 @@ def b200_paged_kv_store_8bit(key_pool: torch.Tensor, value_pool: torch.Tensor, k
         raise ValueError("head_dim must be a multiple of 16")
     if positions.shape != (batch,) or positions.dtype != torch.int64 or not positions.is_contiguous():
         raise ValueError("positions must be a contiguous int64 batch vector")
+    cache = _cache_code(key_pool.dtype)
     if batch == 0 or tokens == 0:
         return
-    rt = runtime(device)
-    code = _lib.load().b200_paged_kv_store_8bit(
+    code = _lib.load().b200_paged_kv_store_8bit(_STORE_CALL(
         key_pool.data_ptr(), value_pool.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), block_table.data_ptr(),
-        key.data_ptr(), value.data_ptr(), positions.data_ptr(), batch, heads, tokens, dim, blocks, block_size,
-        block_table.shape[1], _lib.i64_array(key.stride()), _lib.i64_array(value.stride()), _code(key.dtype),
-        _cache_code(key_pool.dtype), rt.status.data_ptr(), _stream())
-    _check(code, "b200_paged_kv_store_8bit")
-    _count(rt)
+        key.data_ptr(), value.data_ptr(), positions.data_ptr(), rt.status.data_ptr(), batch, heads, tokens, dim, blocks,
+        block_size, block_table.shape[1], *key.stride(), *value.stride(), _DTYPE_CODES[key.dtype], cache), _stream())
+    if code:
+        _check(code, "b200_paged_kv_store_8bit")
+    rt.launches += 1
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention_need(batch: int, q_heads: int, kv_heads: int, dim: int, longest: int, split_tokens: int) -> int:
+    return int(_lib.load().b200_paged_decode_attention_8bit_workspace_bytes(batch, q_heads, kv_heads, dim, longest,
+                                                                            split_tokens))
 
 
 def b200_paged_decode_attention_8bit(query: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor,
@@ -82,9 +119,10 @@ def b200_paged_decode_attention_8bit(query: torch.Tensor, key_pool: torch.Tensor
                                      split_tokens: int = 0, max_length_hint: int = 0) -> torch.Tensor:
     """serve.decode_attention over a paged cache in 8 bits: query B x Hq x 1 x D (bf16 or fp16), the first lengths[b]
     entries of each sequence, an additive B x 1 x 1 x S mask or None. Returns B x Hq x 1 x D. Scores, softmax statistics
-    and sums are fp32; a sequence without tokens, or with every token masked by -inf, gives NaN."""
+    and sums are fp32; a sequence without tokens, or with every token masked by -inf, gives NaN. max_length_hint sizes the
+    split of the work and bounds nothing."""
 
-    device = _require_cuda(query, key_pool, value_pool, key_scales, value_scales, block_table, lengths, attention_mask)
+    rt = _runtime_of(query, key_pool, value_pool, key_scales, value_scales, block_table, lengths, attention_mask)
     if query.ndim != 4 or query.shape[2] != 1:
         raise ValueError("query must be B x H x 1 x D")
     batch, q_heads, _, dim = query.shape
@@ -99,36 +137,36 @@ def b200_paged_decode_attention_8bit(query: torch.Tensor, key_pool: torch.Tensor
         raise ValueError("the block size must be a multiple of 32 tokens")
     if lengths.shape != (batch,) or lengths.dtype != torch.int64 or not lengths.is_contiguous():
         raise ValueError("lengths must be a contiguous int64 batch vector")
-    if query.stride(3) != 1:
+    q_batch_stride, q_head_stride, _, q_stride = query.stride()
+    if q_stride != 1:
         query = _dense(query)
-    capacity = block_table.shape[1] * block_size
-    mask_len, mask_stride, mask_code = capacity, 0, _lib.F32
+        q_batch_stride, q_head_stride = q_heads * dim, dim
+    max_blocks = block_table.shape[1]
+    mask_pointer, mask_len, mask_stride, mask_code = 0, max_blocks * block_size, 0, _lib.F32
     if attention_mask is not None:
         if attention_mask.ndim != 4 or attention_mask.shape[:3] != (batch, 1, 1):
             raise ValueError("attention_mask must be B x 1 x 1 x S")
-        mask_len = attention_mask.shape[3]
-        if mask_len > capacity or mask_len <= 0:
+        if attention_mask.shape[3] > mask_len or attention_mask.shape[3] <= 0:
             raise ValueError("mask length must be in [1, capacity]")
+        mask_len = attention_mask.shape[3]
         if attention_mask.stride(3) != 1:
             attention_mask = _dense(attention_mask)
-        mask_stride = attention_mask.stride(0)
-        mask_code = _code(attention_mask.dtype)
-    output = query.new_empty((batch, q_heads, 1, dim))
+        mask_pointer, mask_stride, mask_code = attention_mask.data_ptr(), attention_mask.stride(0), _code(attention_mask.dtype)
+    cache = _cache_code(key_pool.dtype)
+    output = torch.empty_like(query) if query.is_contiguous() else query.new_empty((batch, q_heads, 1, dim))
     if batch == 0:
         return output
-    rt = runtime(device)
-    library = _lib.load()
-    longest = min(max_length_hint, mask_len) if max_length_hint > 0 else mask_len
-    need = library.b200_paged_decode_attention_8bit_workspace_bytes(batch, q_heads, kv_heads, dim, longest, split_tokens)
-    workspace = rt.own_workspace("decode_attention_8bit", need) if need else None
-    code = library.b200_paged_decode_attention_8bit(
+    need = _attention_need(batch, q_heads, kv_heads, dim, min(max_length_hint, mask_len) if max_length_hint > 0 else mask_len,
+                           split_tokens)
+    workspace = rt.own_workspace("decode_attention_8bit", need).data_ptr() if need else 0
+    code = _lib.load().b200_paged_decode_attention_8bit(_ATTENTION_CALL(
         query.data_ptr(), key_pool.data_ptr(), value_pool.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),
-        block_table.data_ptr(), lengths.data_ptr(), _ptr(attention_mask), output.data_ptr(), batch, q_heads, kv_heads, dim,
-        blocks, block_size, block_table.shape[1], mask_len, query.stride(0), query.stride(1), mask_stride, mask_code,
-        float(scale), _code(query.dtype), _cache_code(key_pool.dtype), int(split_tokens), int(max_length_hint),
-        _ptr(workspace), need, rt.status.data_ptr(), _stream())
-    _check(code, "b200_paged_decode_attention_8bit")
-    _count(rt)
+        block_table.data_ptr(), lengths.data_ptr(), mask_pointer, output.data_ptr(), workspace, rt.status.data_ptr(), batch,
+        q_heads, kv_heads, dim, blocks, block_size, max_blocks, mask_len, q_batch_stride, q_head_stride, mask_stride, mask_code,
+        _DTYPE_CODES[query.dtype], cache, split_tokens, max_length_hint, need, scale), _stream())
+    if code:
+        _check(code, "b200_paged_decode_attention_8bit")
+    rt.launches += 1
     return output
 
 
@@ -149,32 +187,37 @@ def b200_copy_kv_blocks(pools: Sequence[torch.Tensor], sources: Union[torch.Tens
 
     if not pools or len(pools) > _lib.MAX_COPY_POOLS:
         raise ValueError(f"between one and {_lib.MAX_COPY_POOLS} pools are copied at once")
-    device = _require_cuda(*pools)
+    rt = _runtime_of(*pools)
     layers, blocks = pools[0].shape[:2] if pools[0].ndim >= 2 else (0, 0)
-    table = (_lib.BlockPool * len(pools))()
-    for entry, pool in zip(table, pools):
-        if pool.ndim < 2 or pool.shape[:2] != (layers, blocks) or pool.numel() == 0 or not pool.is_contiguous():
+    places: List[int] = []
+    for pool in pools:
+        stride = pool.stride()
+        if len(stride) < 2 or pool.shape[0] != layers or pool.shape[1] != blocks or not pool.is_contiguous() or \
+                pool.numel() == 0:
             raise ValueError("pools must be contiguous layers x blocks x ... tensors that agree in layers and blocks")
         size = pool.element_size()
-        entry.base, entry.layer_stride, entry.block_bytes = pool.data_ptr(), pool.stride(0) * size, pool.stride(1) * size
+        places += (pool.data_ptr(), stride[0] * size, stride[1] * size)
     sources, destinations = _block_index(sources, "sources"), _block_index(destinations, "destinations")
-    if len(sources) != len(destinations):
+    count = len(sources)
+    if count != len(destinations):
         raise ValueError("sources and destinations must be of one length")
     if not isinstance(sources, torch.Tensor) and not isinstance(destinations, torch.Tensor):
         if any(not 0 <= i < blocks for i in (*sources, *destinations)):
             raise ValueError(f"block indices must be in [0, {blocks})")
-        if len(set(destinations)) != len(destinations) or set(destinations) & set(sources):
+        if len(set(destinations)) != count or set(destinations) & set(sources):
             raise ValueError("destinations must be distinct and none of them a source")
-    if len(sources) == 0:
+    if count == 0:
         return
-    sources, destinations = (i if isinstance(i, torch.Tensor) else torch.tensor(i, dtype=torch.int32, device=device)
-                             for i in (sources, destinations))
-    _require_cuda(pools[0], sources, destinations)
-    rt = runtime(device)
-    code = _lib.load().b200_copy_kv_blocks(table, len(pools), sources.data_ptr(), destinations.data_ptr(),
-                                           sources.numel(), layers, blocks, rt.status.data_ptr(), _stream())
-    _check(code, "b200_copy_kv_blocks")
-    _count(rt)
+    if not isinstance(sources, torch.Tensor):
+        sources = torch.tensor(sources, dtype=torch.int32, device=pools[0].device)
+    if not isinstance(destinations, torch.Tensor):
+        destinations = torch.tensor(destinations, dtype=torch.int32, device=pools[0].device)
+    _runtime_of(pools[0], sources, destinations)
+    code = _lib.load().b200_copy_kv_blocks(struct.pack(f"={len(places)}Q", *places), len(pools), sources.data_ptr(),
+                                           destinations.data_ptr(), count, layers, blocks, rt.status.data_ptr(), _stream())
+    if code:
+        _check(code, "b200_copy_kv_blocks")
+    rt.launches += 1
 
 
 def _row_stride(tensor: torch.Tensor) -> Optional[int]:
@@ -189,34 +232,40 @@ def _row_stride(tensor: torch.Tensor) -> Optional[int]:
 
 def _quantize(tensor: torch.Tensor, residual: Optional[torch.Tensor], weight: Optional[torch.Tensor], epsilon: float,
               what: str):
-    device = _require_cuda(tensor, residual, weight)
-    if tensor.ndim < 1 or tensor.shape[-1] <= 0:
+    rt = _runtime_of(tensor, residual, weight)
+    shape, dtype = tensor.shape, tensor.dtype
+    if not shape or shape[-1] <= 0:
         raise ValueError("the input must have rows of at least one element")
-    hidden = tensor.shape[-1]
-    if weight is not None and (weight.shape != (hidden,) or weight.dtype != tensor.dtype or not weight.is_contiguous()):
-        raise ValueError("weight must be a contiguous vector of the row length in the input dtype")
+    hidden, code_dtype = shape[-1], _code(dtype)
+    weight_pointer = residual_pointer = total_pointer = 0
+    if weight is not None:
+        if weight.shape != (hidden,) or weight.dtype != dtype or not weight.is_contiguous():
+            raise ValueError("weight must be a contiguous vector of the row length in the input dtype")
+        weight_pointer = weight.data_ptr()
     stride = _row_stride(tensor)
     if stride is None:
         tensor, stride = _dense(tensor), hidden
+    like = tensor if stride == hidden else None  # (contiguous: outputs may be made like it)
     residual_stride, total = hidden, None
     if residual is not None:
-        if residual.shape != tensor.shape or residual.dtype != tensor.dtype:
+        if residual.shape != shape or residual.dtype != dtype:
             raise ValueError("residual must match the input's shape and dtype")
         residual_stride = _row_stride(residual)
         if residual_stride is None:
             residual, residual_stride = _dense(residual), hidden
-        total = torch.empty(tensor.shape, dtype=tensor.dtype, device=device)
-    rows = tensor.numel() // hidden
-    codes = torch.empty(tensor.shape, dtype=torch.int8, device=device)
-    scales = torch.empty(tensor.shape[:-1], dtype=torch.float32, device=device)
+        total = torch.empty_like(tensor) if like is not None else tensor.new_empty(shape)
+        residual_pointer, total_pointer = residual.data_ptr(), total.data_ptr()
+    codes = torch.empty_like(tensor, dtype=torch.int8) if like is not None else tensor.new_empty(shape, dtype=torch.int8)
+    scales = tensor.new_empty(shape[:-1], dtype=torch.float32)
+    rows = scales.numel()
     if rows == 0:
         return codes, scales, total
-    rt = runtime(device)
-    code = _lib.load().b200_quantize_rows_int8(
-        tensor.data_ptr(), _ptr(residual), _ptr(weight), _ptr(total), codes.data_ptr(), scales.data_ptr(), rows, hidden,
-        stride, residual_stride, float(epsilon), _code(tensor.dtype), _stream())
-    _check(code, what)
-    _count(rt)
+    code = _lib.load().b200_quantize_rows_int8(_ROWS_CALL(
+        tensor.data_ptr(), residual_pointer, weight_pointer, total_pointer, codes.data_ptr(), scales.data_ptr(), rows, hidden,
+        stride, residual_stride, code_dtype, epsilon), _stream())
+    if code:
+        _check(code, what)
+    rt.launches += 1
     return codes, scales, total
 
 
@@ -227,6 +276,8 @@ def b200_rms_norm_int8(tensor: torch.Tensor, weight: torch.Tensor, *, epsilon: f
     scales float32 per row, sum). sum = round(tensor + residual) in the input dtype (None without a residual: the rows
     themselves are normalised); codes * scales stand for the normalised rows, the largest of each row being 127."""
 
+    if weight is None:
+        raise ValueError("a norm has a weight")
     return _quantize(tensor, residual, weight, epsilon, "b200_rms_norm_int8")
 
 
@@ -247,7 +298,7 @@ def b200_linear_int8(values: torch.Tensor, scales: torch.Tensor, weight: torch.T
     are of out_dtype. epilogue "residual": y + residual; "swiglu": weight holds gate_j and up_j alternating, the result is
     silu(gate) * up with N / 2 columns. One rounding, at the end. K must be a multiple of 16."""
 
-    device = _require_cuda(values, scales, weight, weight_scales, bias, residual)
+    rt = _runtime_of(values, scales, weight, weight_scales, bias, residual)
     if weight.ndim != 2:
         raise ValueError("weight must be N x K")
     n, k = weight.shape
@@ -256,7 +307,8 @@ def b200_linear_int8(values: torch.Tensor, scales: torch.Tensor, weight: torch.T
         raise ValueError("the last input dimension must equal the weight's K")
     if values.dtype != torch.int8 or weight.dtype != torch.int8:
         raise ValueError("values and weight must be int8")
-    if scales.shape != shape[:-1] or weight_scales.shape != (n,) or scales.dtype != torch.float32 or \
+    leading = shape[:-1]
+    if scales.shape != leading or weight_scales.shape != (n,) or scales.dtype != torch.float32 or \
             weight_scales.dtype != torch.float32:
         raise ValueError("scales must be float32, one per row of values and one per row of weight")
     if not (values.is_contiguous() and weight.is_contiguous() and scales.is_contiguous() and weight_scales.is_contiguous()):
@@ -267,21 +319,27 @@ def b200_linear_int8(values: torch.Tensor, scales: torch.Tensor, weight: torch.T
         raise ValueError(f"unknown epilogue {epilogue!r}")
     if epilogue == "swiglu" and n % 2:
         raise ValueError("swiglu needs an even number of weight rows")
-    if bias is not None and (bias.shape != (n,) or bias.dtype != out_dtype or not bias.is_contiguous()):
-        raise ValueError("bias must be a contiguous vector of N elements in out_dtype")
-    output = torch.empty((*shape[:-1], n // 2 if epilogue == "swiglu" else n), dtype=out_dtype, device=device)
+    code_dtype = _code(out_dtype)
+    bias_pointer = residual_pointer = 0
+    if bias is not None:
+        if bias.shape != (n,) or bias.dtype != out_dtype or not bias.is_contiguous():
+            raise ValueError("bias must be a contiguous vector of N elements in out_dtype")
+        bias_pointer = bias.data_ptr()
+    output = values.new_empty((*leading, n // 2 if epilogue == "swiglu" else n), dtype=out_dtype)
     if epilogue == "residual":
         if residual is None or residual.shape != output.shape or residual.dtype != out_dtype:
             raise ValueError("residual must match the output shape and dtype")
         residual = _dense(residual)
+        residual_pointer = residual.data_ptr()
     elif residual is not None:
         raise ValueError("residual given without the residual epilogue")
-    if output.numel() == 0:
+    m = scales.numel()
+    if m == 0 or n == 0:
         return output
-    rt = runtime(device)
-    code = _lib.load().b200_linear_int8(
-        values.data_ptr(), scales.data_ptr(), weight.data_ptr(), weight_scales.data_ptr(), _ptr(bias), _ptr(residual),
-        output.data_ptr(), scales.numel(), k, n, _code(out_dtype), _EPILOGUES[epilogue], rt.status.data_ptr(), _stream())
-    _check(code, "b200_linear_int8")
-    _count(rt)
+    code = _lib.load().b200_linear_int8(_LINEAR_CALL(
+        values.data_ptr(), scales.data_ptr(), weight.data_ptr(), weight_scales.data_ptr(), bias_pointer, residual_pointer,
+        output.data_ptr(), rt.status.data_ptr(), m, k, n, code_dtype, _EPILOGUES[epilogue]), _stream())
+    if code:
+        _check(code, "b200_linear_int8")
+    rt.launches += 1
     return output

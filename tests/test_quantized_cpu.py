@@ -1,7 +1,7 @@
 """Serving in 8 bits without a GPU: what the C ABI refuses before any launch, what the wrappers refuse, and the block
 bookkeeping of fork, release and compact with the copies written down instead of made."""
 
-import ctypes
+import struct
 
 import pytest
 import torch
@@ -10,15 +10,14 @@ import llm_compiler_b200 as b200
 from llm_compiler_b200 import _lib, quantized_kernels
 from llm_compiler_b200.kv_state import ExecutionError, PagedKVCacheState, QuantizedPagedKVCacheState
 
-FAKE = ctypes.c_void_p(256)      # never dereferenced: rejected on the host
-ODD = ctypes.c_void_p(264)
-STRIDES = _lib.i64_array([128, 64, 64, 1])
+FAKE, ODD = 256, 264  # never dereferenced: rejected on the host
 
 
 def store(pool=FAKE, batch=1, heads=2, tokens=1, dim=64, blocks=4, size=32, columns=2, dtype=_lib.BF16, cache=_lib.I8,
           status=FAKE):
-    return _lib.load().b200_paged_kv_store_8bit(pool, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, batch, heads, tokens, dim,
-                                                blocks, size, columns, STRIDES, STRIDES, dtype, cache, status, None)
+    call = struct.pack("=9Q17q", pool or 0, *[FAKE] * 7, status or 0, batch, heads, tokens, dim, blocks, size, columns,
+                       128, 64, 64, 1, 128, 64, 64, 1, dtype, cache)
+    return _lib.load().b200_paged_kv_store_8bit(call, None)
 
 
 def test_store_refusals():
@@ -30,11 +29,11 @@ def test_store_refusals():
     assert store(batch=0) == store(tokens=0) == 0
 
 
-def attention(query=FAKE, pool=FAKE, mask=None, batch=1, heads=4, kv_heads=2, dim=64, blocks=4, size=32, columns=2,
-              mask_len=64, mask_dtype=_lib.F32, dtype=_lib.BF16, cache=_lib.I8, split=0, workspace=None, nbytes=0):
-    return _lib.load().b200_paged_decode_attention_8bit(
-        query, pool, FAKE, FAKE, FAKE, FAKE, FAKE, mask, FAKE, batch, heads, kv_heads, dim, blocks, size, columns, mask_len,
-        256, 64, 0, mask_dtype, 0.125, dtype, cache, split, 0, workspace, nbytes, FAKE, None)
+def attention(query=FAKE, pool=FAKE, mask=0, batch=1, heads=4, kv_heads=2, dim=64, blocks=4, size=32, columns=2,
+              mask_len=64, mask_dtype=_lib.F32, dtype=_lib.BF16, cache=_lib.I8, split=0, workspace=0, nbytes=0):
+    call = struct.pack("=11Q17qd", query or 0, pool, *[FAKE] * 5, mask, FAKE, workspace, FAKE, batch, heads, kv_heads, dim,
+                       blocks, size, columns, mask_len, 256, 64, 0, mask_dtype, dtype, cache, split, 0, nbytes, 0.125)
+    return _lib.load().b200_paged_decode_attention_8bit(call, None)
 
 
 def test_attention_refusals():
@@ -43,19 +42,22 @@ def test_attention_refusals():
     assert attention(dim=96) == attention(size=48) == attention(dtype=_lib.F32) == attention(cache=_lib.F16) == \
         _lib.ERR_UNSUPPORTED
     assert attention(pool=ODD) == _lib.ERR_ALIGNMENT
+    assert attention(batch=70000) == attention(blocks=1 << 31) == _lib.ERR_TOO_LARGE
+    need = _lib.load().b200_paged_decode_attention_8bit_workspace_bytes(1, 4, 2, 64, 64, 32)
+    assert need > 0 and attention(split=32) == attention(split=32, workspace=FAKE, nbytes=need - 1) == _lib.ERR_WORKSPACE
     assert attention(batch=0) == 0
 
 
 def test_copy_refusals():
     library = _lib.load()
-    pools = (_lib.BlockPool * 9)(*[_lib.BlockPool(256, 4096, 1024) for _ in range(9)])
+    pools = struct.pack("=27Q", *[FAKE, 4096, 1024] * 9)
 
     def copy(count=1, n=2, layers=2, blocks=4, sources=FAKE, table=pools):
         return library.b200_copy_kv_blocks(table, count, sources, FAKE, n, layers, blocks, FAKE, None)
 
     assert copy(sources=None) == copy(count=0) == copy(n=-1) == copy(layers=0) == copy(blocks=0) == _lib.ERR_BAD_ARGUMENT
     assert copy(blocks=5) == _lib.ERR_BAD_ARGUMENT  # layers that overlap
-    assert copy(table=(_lib.BlockPool * 1)(_lib.BlockPool(None, 4096, 1024))) == _lib.ERR_BAD_ARGUMENT
+    assert copy(table=struct.pack("=3Q", 0, 4096, 1024)) == _lib.ERR_BAD_ARGUMENT
     assert copy(count=9) == _lib.ERR_TOO_LARGE
     assert copy(n=0) == 0
 
@@ -64,14 +66,16 @@ def test_quantised_rows_and_linear_refusals():
     library = _lib.load()
 
     def rows(x=FAKE, residual=None, total=None, n=2, hidden=64, stride=64, dtype=_lib.BF16):
-        return library.b200_quantize_rows_int8(x, residual, FAKE, total, FAKE, FAKE, n, hidden, stride, 64, 1e-6, dtype, None)
+        return library.b200_quantize_rows_int8(struct.pack("=6Q5qd", x or 0, residual or 0, FAKE, total or 0, FAKE, FAKE, n,
+                                                           hidden, stride, 64, dtype, 1e-6), None)
 
     assert rows(x=None) == rows(residual=FAKE) == rows(hidden=0) == rows(stride=63) == rows(dtype=_lib.I8) == \
         _lib.ERR_BAD_ARGUMENT
     assert rows(n=0) == 0
 
     def linear(x=FAKE, weight=FAKE, residual=None, m=4, k=64, n=8, dtype=_lib.BF16, epilogue=0):
-        return library.b200_linear_int8(x, FAKE, weight, FAKE, None, residual, FAKE, m, k, n, dtype, epilogue, FAKE, None)
+        return library.b200_linear_int8(struct.pack("=8Q5q", x or 0, FAKE, weight, FAKE, 0, residual or 0, FAKE, FAKE, m, k, n,
+                                                    dtype, epilogue), None)
 
     assert linear(x=None) == linear(k=0) == linear(epilogue=3) == linear(epilogue=1) == linear(residual=FAKE) == \
         linear(dtype=_lib.I8) == _lib.ERR_BAD_ARGUMENT
