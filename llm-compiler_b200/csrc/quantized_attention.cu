@@ -10,28 +10,30 @@ int launch_int8(const Params& p, const void* keys, const void* values, int64_t b
 
 namespace {
 struct Plan {
-  int64_t head_blocks, block_heads, split_tokens, splits;
+  int64_t head_blocks, block_heads, splits;
+  bool cluster;
   int64_t parts(int64_t batch, int64_t kv_heads) const {
-    return splits > 1 ? batch * kv_heads * head_blocks * splits * block_heads : 0;
+    return splits > 1 && !cluster ? batch * kv_heads * head_blocks * splits * block_heads : 0;
   }
 };
-Plan plan_of(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t max_length, int64_t split_tokens) {
+Plan plan_of(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t longest, int64_t split_tokens) {
   Plan plan;
   const int64_t group = q_heads / kv_heads;
   plan.head_blocks = ceil_div(group, dim == 256 ? 8 : 16);
   plan.block_heads = ceil_div(group, plan.head_blocks);
   const int64_t items = batch * kv_heads * plan.head_blocks;
-  if (split_tokens <= 0) {
-    const int64_t resident = static_cast<int64_t>(kNumSMs) * (dim == 64 ? 3 : dim == 128 ? 2 : 1);
-    const int64_t most = std::max<int64_t>(1, resident / items);
-    split_tokens = std::max<int64_t>(ceil_div(max_length, most), 128);
+  if (split_tokens > 0) {
+    plan.splits = ceil_div(longest, split_tokens);
+  } else {
+    const int64_t resident = static_cast<int64_t>(kNumSMs) * (dim == 64 ? 4 : dim == 128 ? 2 : 1);
+    plan.splits = std::min(std::max<int64_t>(resident / items, 1), ceil_div(longest, kTile * kWarps));
   }
-  plan.split_tokens = ceil_div(split_tokens, kTile) * kTile;
-  plan.splits = ceil_div(max_length, plan.split_tokens);
-  if (items > kMaxCounters) {  // (that many sequences fill the GPU by themselves)
-    plan.splits = 1;
-    plan.split_tokens = std::max(plan.split_tokens, ceil_div(max_length, kTile) * kTile);
-  }
+  // (a CTA has a tile for each of its warps; that many sequences fill the GPU by themselves)
+  plan.splits = std::max<int64_t>(1, std::min(plan.splits, ceil_div(longest, kTile * kWarps)));
+  if (items > kMaxCounters) plan.splits = std::min<int64_t>(plan.splits, 8);
+  plan.cluster = plan.splits > 1 && plan.splits <= 8;
+  if (plan.cluster)  // clusters of a power of two fit every GPC
+    while ((plan.splits & (plan.splits - 1)) != 0) ++plan.splits;
   return plan;
 }
 }  // namespace
@@ -64,7 +66,7 @@ extern "C" int b200_paged_decode_attention_8bit(const b200_cache_attention_call*
   if (!aligned16(c.key_pool) || !aligned16(c.value_pool) || (reinterpret_cast<uintptr_t>(c.output) & 7u) != 0)
     return B200_ERR_ALIGNMENT;
   if (c.batch > 65535 || c.q_heads > 65535 || c.num_blocks > INT32_MAX || c.num_blocks * c.kv_heads > INT32_MAX ||
-      c.block_size > (1 << 20) || c.mask_len > (int64_t(1) << 40))
+      c.block_size > (1 << 20) || c.max_blocks_per_sequence * c.block_size > INT32_MAX / 2)
     return B200_ERR_TOO_LARGE;
   if (c.batch == 0) return B200_OK;
   const int64_t longest = c.max_length_hint > 0 && c.max_length_hint < c.mask_len ? c.max_length_hint : c.mask_len;
@@ -82,7 +84,7 @@ extern "C" int b200_paged_decode_attention_8bit(const b200_cache_attention_call*
   p.lengths = c.lengths; p.mask = c.mask; p.out = c.output; p.status = c.status;
   p.q_batch_stride = c.q_batch_stride; p.q_head_stride = c.q_head_stride; p.mask_batch_stride = c.mask_batch_stride;
   p.num_blocks = c.num_blocks; p.max_blocks = c.max_blocks_per_sequence; p.mask_len = c.mask_len;
-  p.split_tokens = plan.split_tokens; p.num_splits = static_cast<int>(plan.splits);
+  p.num_splits = static_cast<int>(plan.splits); p.cluster = plan.cluster;
   p.q_heads = static_cast<int>(c.q_heads); p.kv_heads = static_cast<int>(c.kv_heads);
   p.group = static_cast<int>(c.q_heads / c.kv_heads);
   p.head_blocks = static_cast<int>(plan.head_blocks); p.block_heads = static_cast<int>(plan.block_heads);

@@ -20,10 +20,12 @@
 // inside fp16. P itself is fp16 (2^-11; it is at most e^5, below), its sum fp32. The running maximum moves only when a score passes
 // it by more than 5: the softmax is the same, and most tiles need no reduction across lanes.
 //
-// Work. A CTA serves `split_tokens` tokens of one (sequence, KV head, up to 8 NT heads). Its four warps take the 32-token
-// tiles in turn, each through a ring of its own that TMA fills: a tile never spans two blocks (block sizes are multiples of
-// 32), is contiguous in the pool, and is one box for K and one for V. Warps merge through shared memory; with several
-// splits the CTA that arrives last adds the partials in split order, so results do not depend on timing.
+// Work. The tiles (32 tokens) of one (sequence, KV head, up to 8 NT heads) are dealt to `splits` CTAs of four warps, a tile
+// to a warp in turn: which tiles a warp has does not depend on the length, so it asks for their blocks while the length is
+// on its way. Each warp has a ring of its own that TMA fills: a tile never spans two blocks (block sizes are multiples of
+// 32), is contiguous in the pool, and is one box for K and one for V. Warps merge through shared memory. Up to eight splits
+// are a cluster, whose CTAs merge through distributed shared memory; more leave partials in the workspace, which the CTA
+// that arrives last adds in split order. Either way results do not depend on timing.
 #pragma once
 
 #include <algorithm>
@@ -51,12 +53,13 @@ struct Params {
   const int64_t* lengths;
   const void* mask;
   void* out;
-  float* ws_o;     // [items, splits, heads of a block, D]
+  float* ws_o;     // more splits than a cluster holds: [items, splits, heads of a block, D]
   float* ws_ml;    // [items, splits, heads of a block, 2]
   int* counters;   // [items], zero between calls
   int32_t* status;
-  int64_t q_batch_stride, q_head_stride, mask_batch_stride, num_blocks, max_blocks, mask_len, split_tokens;
+  int64_t q_batch_stride, q_head_stride, mask_batch_stride, num_blocks, max_blocks, mask_len;
   int q_heads, kv_heads, group, head_blocks, block_heads, block_size, mask_dtype, num_splits;
+  int cluster;     // the splits are a cluster
   int half;        // q and out are fp16, else bf16
   int q_vector;    // rows of q may be read 16 bytes at a time
   float scale;
@@ -128,7 +131,7 @@ struct Shape {
   static constexpr int kBoxes = D / kRowBytes;
   static constexpr int kBoxBytes = kTile * kRowBytes;
   static constexpr int kTileBytes = kTile * D;                 // K or V
-  static constexpr int kStages = D == 64 ? 4 : 3;
+  static constexpr int kStages = 3;
   static constexpr int kRingBytes = kWarps * kStages * 2 * kTileBytes;
   // byte offset of 16-byte chunk `chunk` of row `row` in a tile
   __device__ static uint32_t at(int row, int chunk) {
@@ -149,6 +152,7 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
   extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ __align__(8) uint64_t full[kWarps * kStages];
   __shared__ float merge_m[kWarps][kHeads], merge_l[kWarps][kHeads];
+  __shared__ float joined[kHeads][2];  // this CTA's maximum and sum
   __shared__ int last_flag;
 
   grid_launch_dependents();
@@ -161,67 +165,69 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
     for (int s = 0; s < kWarps * kStages; ++s) mbarrier_init(smem_u32(&full[s]), 1);
     fence_mbarrier_init();
   }
+  const int tiles_per_block = p.block_size / kTile, stride = kWarps * p.num_splits, my_first = split * kWarps + warp;
+  const int32_t* table = p.table + b * p.max_blocks;
+  const int max_tiles = static_cast<int>(p.max_blocks) * tiles_per_block;
   grid_dependency_wait_cta();
 
-  int64_t length = max(p.lengths[b], static_cast<int64_t>(0));
-  if (length > p.mask_len) {
-    length = p.mask_len;
+  // Places of this warp's tiles, 32 tiles ahead in the lanes: lane i of a window that starts at `it` holds tile it + i.
+  struct Window { int slab, row; float ks, vs; };  // (block, head), row in the block
+  bool bad = false;
+  auto block_of = [&](int it, int& row) {
+    const int tile = my_first + it * stride;
+    if (tile >= max_tiles) return -1;
+    const int column = tile / tiles_per_block;
+    row = (tile - column * tiles_per_block) * kTile;
+    return table[column];
+  };
+  Window now = {}, next = {};
+  int block_now = block_of(lane, now.row), block_next = block_of(lane + 32, next.row);
+  int64_t length64 = max(p.lengths[b], static_cast<int64_t>(0));
+  if (length64 > p.mask_len) {
+    length64 = p.mask_len;
     if (threadIdx.x == 0 && split == 0 && item_head == 0) atomicOr(p.status, B200_STATUS_LENGTH_OVER_MASK);
   }
-  // splits that have tokens; the last one of the grid takes whatever is behind it
-  const int64_t wanted = (length + p.split_tokens - 1) / p.split_tokens;
-  const int splits = static_cast<int>(min(max(wanted, static_cast<int64_t>(1)), static_cast<int64_t>(p.num_splits)));
-  if (split >= splits) return;
-  const int64_t start = split * p.split_tokens, end = split == splits - 1 ? length : start + p.split_tokens;
-  const int64_t first_tile = start / kTile;  // (split_tokens is a multiple of kTile)
-  const int tiles = static_cast<int>((end - start + kTile - 1) / kTile);
-  const int mine = tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0;  // tiles warp, warp + kWarps, ...
+  const int length = static_cast<int>(length64), tiles = (length + kTile - 1) / kTile;
+  // CTAs that have tiles; without a cluster the others are not waited for
+  const int active = min(max((tiles + kWarps - 1) / kWarps, 1), p.num_splits);
+  if (!p.cluster && split >= active) return;
+  const int mine = tiles > my_first ? (tiles - my_first + stride - 1) / stride : 0;
 
   const uint32_t ring = smem_u32(smem) + warp * kStages * 2 * S::kTileBytes;
   const uint32_t bars = smem_u32(&full[warp * kStages]);
-  const int tiles_per_block = p.block_size / kTile;
-
-  // Block and scales of this warp's tiles, 32 tiles ahead in the lanes: lane i of window w holds tile 32 w + i.
-  struct Window { int block; float ks, vs; };
-  bool bad = false;
-  auto look_up = [&](int it) {
-    Window w = {-1, 0.0f, 0.0f};
-    if (it < mine) {
-      const int64_t column = (first_tile + warp + static_cast<int64_t>(it) * kWarps) / tiles_per_block;
-      w.block = p.table[b * p.max_blocks + column];
-      if (w.block < 0 || w.block >= p.num_blocks) {
-        w.block = -1;
-        bad = true;
-      } else {
-        const int64_t slab = static_cast<int64_t>(w.block) * p.kv_heads + kv;
-        w.ks = p.key_scales[slab];
-        w.vs = p.value_scales[slab];
-      }
+  auto settle = [&](int it, int block, Window& w) {
+    w.slab = -1;
+    if (it >= mine) return;
+    if (block < 0 || block >= p.num_blocks) {
+      bad = true;
+      return;
     }
-    return w;
+    w.slab = block * p.kv_heads + kv;
+    w.ks = p.key_scales[w.slab];
+    w.vs = p.value_scales[w.slab];
   };
-  Window now = look_up(lane), next = look_up(32 + lane);
-  int base = 0;  // of `now`
-  int issued = 0;
-  auto issue = [&](int it) {  // whole warp; a tile without a block has no copy
-    const int block = __shfl_sync(0xffffffffu, it - base < 32 ? now.block : next.block, it & 31);
-    if (block >= 0 && lane == 0 && !p.drop_loads) {
-      const int stage = it % kStages;
-      const uint32_t bar = bars + stage * 8, dst = ring + stage * 2 * S::kTileBytes;
-      const int row = static_cast<int>((first_tile + warp + static_cast<int64_t>(it) * kWarps) % tiles_per_block) * kTile;
-      const int slab = block * p.kv_heads + kv;
+  settle(lane, block_now, now);
+  settle(lane + 32, block_next, next);
+  int base = 0, issued = 0;  // of `now`; tiles asked for
+  int issue_stage = 0;
+  auto issue = [&]() {  // the lane that holds the tile's place asks for it; a tile without a block has no copy
+    const Window& w = issued - base < 32 ? now : next;
+    if (lane == (issued & 31) && w.slab >= 0 && !p.drop_loads) {
+      const uint32_t bar = bars + issue_stage * 8, dst = ring + issue_stage * 2 * S::kTileBytes;
       mbarrier_arrive_expect_tx(bar, 2 * S::kTileBytes);
 #pragma unroll
       for (int x = 0; x < S::kBoxes; ++x) {
-        tma_load_3d(dst + x * S::kBoxBytes, &key_map, bar, x * S::kRowBytes, row, slab);
-        tma_load_3d(dst + S::kTileBytes + x * S::kBoxBytes, &value_map, bar, x * S::kRowBytes, row, slab);
+        tma_load_3d(dst + x * S::kBoxBytes, &key_map, bar, x * S::kRowBytes, w.row, w.slab);
+        tma_load_3d(dst + S::kTileBytes + x * S::kBoxBytes, &value_map, bar, x * S::kRowBytes, w.row, w.slab);
       }
     }
-    issued = it + 1;
+    __syncwarp();
+    ++issued;
+    issue_stage = issue_stage + 1 == kStages ? 0 : issue_stage + 1;
   };
 #pragma unroll
   for (int s = 0; s < kStages - 1; ++s)
-    if (s < mine) issue(s);
+    if (s < mine) issue();
 
   // ---- q as B operands: lane (g, j) holds head g, elements 64 c + 16 j .. + 15 of every 64 ----
   uint32_t qb[NT][kSteps][2];
@@ -272,6 +278,9 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
     factor[t][1] = p.scale * __shfl_sync(0xffffffffu, up, 8 * j + 4);
   }
 
+  // Scores without a mask are in units of log 2; with one they stay natural, since a mask of the type's lowest value would
+  // leave its range.
+  constexpr float kUnit = kMask ? 1.0f : kLog2e, kToLog2 = kMask ? kLog2e : 1.0f;
   float m[NT][2], l[NT][2], o[NT][kSteps][4];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
@@ -288,8 +297,8 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
     if constexpr (kMask) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int64_t token = (first_tile + warp + static_cast<int64_t>(it) * kWarps) * kTile + 8 * r + my_token;
-        mask_next[r] = it < mine && token < end ? load_mask(p, b * p.mask_batch_stride + token) : 0.0f;
+        const int token = (my_first + it * stride) * kTile + 8 * r + my_token;
+        mask_next[r] = it < mine && token < length ? load_mask(p, b * p.mask_batch_stride + token) : 0.0f;
       }
     }
   };
@@ -297,33 +306,32 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
   // phases: a stage completes only where a copy was issued, so a tile without a block does not turn its parity
   uint32_t phase = 0;
 
-  int it = 0;
-  for (; it < mine; ++it) {
+  int it = 0, stage = 0;
+  for (; it < mine; ++it, stage = stage + 1 == kStages ? 0 : stage + 1) {
     if (it - base == 32) {
       now = next;
       base = it;
-      next = look_up(base + 32 + lane);
+      const int block = block_of(base + 32 + lane, next.row);
+      settle(base + 32 + lane, block, next);
     }
-    const int stage = it % kStages, at_lane = it & 31;
-    const int block = __shfl_sync(0xffffffffu, now.block, at_lane);
-    const float ks = __shfl_sync(0xffffffffu, now.ks, at_lane), vs = __shfl_sync(0xffffffffu, now.vs, at_lane);
-    if (block >= 0) {
-      if (!__all_sync(0xffffffffu, mbarrier_wait_bounded(bars + stage * 8, (phase >> stage) & 1, p.wait_limit))) {
+    const int slab = __shfl_sync(0xffffffffu, now.slab, it & 31);
+    const float ks = __shfl_sync(0xffffffffu, now.ks, it & 31), vs = __shfl_sync(0xffffffffu, now.vs, it & 31);
+    if (slab >= 0) {
+      if (!__all_sync(0xffffffffu, mbarrier_wait_ready_first(bars + stage * 8, (phase >> stage) & 1, p.wait_limit))) {
         timed_out = true;
         break;
       }
       phase ^= 1u << stage;
     }
     __syncwarp();  // every lane is done with the stage that is filled next
-    if (it + kStages - 1 < mine) issue(it + kStages - 1);
+    if (issued < mine) issue();
     float extra[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) extra[r] = kMask ? mask_next[r] : 0.0f;
     fetch_mask(it + 1);
-    if (block < 0) continue;
+    if (slab < 0) continue;
     const uint32_t keys = ring + stage * 2 * S::kTileBytes, values = keys + S::kTileBytes;
-    const int64_t token0 = (first_tile + warp + static_cast<int64_t>(it) * kWarps) * kTile;
-    const int valid = static_cast<int>(min(end - token0, static_cast<int64_t>(kTile)));
+    const int valid = min(length - (my_first + it * stride) * kTile, kTile);
 
     // ---- scores of 32 tokens ----
     float s[NT][2][4];
@@ -354,15 +362,26 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float f = ks * factor[t][h], line = m[t][h] + kSlack;
+        const float f = ks * factor[t][h] * kUnit;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {  // token 8 r + my_token
           float& x = s[t][r >> 1][2 * (r & 1) + h];
           x = kMask ? fmaf(x, f, extra[r]) : x * f;
-          if (valid < kTile && 8 * r + my_token >= valid) x = -INFINITY;
-          over = over || x > line;
         }
       }
+    if (valid < kTile) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (8 * r + my_token >= valid) {
+#pragma unroll
+          for (int t = 0; t < NT; ++t) s[t][r >> 1][2 * (r & 1)] = s[t][r >> 1][2 * (r & 1) + 1] = -INFINITY;
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        over = over || fmaxf(fmaxf(s[t][0][h], s[t][0][2 + h]), fmaxf(s[t][1][h], s[t][1][2 + h])) > m[t][h] + kSlack;
     if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
       for (int t = 0; t < NT; ++t)
@@ -373,7 +392,7 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
           top = fmaxf(top, m[t][h]);
-          const float keep = top == -INFINITY ? 1.0f : exp2_fast((m[t][h] - top) * kLog2e);
+          const float keep = top == -INFINITY ? 1.0f : exp2_fast((m[t][h] - top) * kToLog2);
           m[t][h] = top;
           l[t][h] *= keep;
 #pragma unroll
@@ -405,8 +424,8 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
       const float m0 = m[t][0] == -INFINITY ? 0.0f : m[t][0], m1 = m[t][1] == -INFINITY ? 0.0f : m[t][1];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float p0 = exp2_fast((s[t][r >> 1][2 * (r & 1)] - m0) * kLog2e);
-        const float p1 = exp2_fast((s[t][r >> 1][2 * (r & 1) + 1] - m1) * kLog2e);
+        const float p0 = exp2_fast((s[t][r >> 1][2 * (r & 1)] - m0) * kToLog2);
+        const float p1 = exp2_fast((s[t][r >> 1][2 * (r & 1) + 1] - m1) * kToLog2);
         l[t][0] += p0;
         l[t][1] += p1;
         pb[t][r >> 1][r & 1] = transpose_8x8(pack_half2(p0 * weight, p1 * weight));
@@ -472,74 +491,118 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
       }
   __syncthreads();
   const int64_t item = b * gridDim.y + item_head;
-  for (int e = threadIdx.x; e < heads * D; e += kThreads) {
-    const int head = e / D, d = e % D;
-    float top = -INFINITY, sum = 0.0f, value = 0.0f;
+  // merged by a thread for a whole row of four; NaN in a part stays (a weight of zero does not silence it)
+  auto put_out = [&](int head, int d, float4 value, float sum) {  // (0 / 0 = NaN for a sequence without tokens)
+    const int64_t at = (b * p.q_heads + head0 + head) * D + d;
+    const float scale = 1.0f / sum;
+    value.x *= scale; value.y *= scale; value.z *= scale; value.w *= scale;
+    const uint32_t lo = p.half ? pack_half2(value.x, value.y) : pack_bf16x2(value.x, value.y);
+    const uint32_t hi = p.half ? pack_half2(value.z, value.w) : pack_bf16x2(value.z, value.w);
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = make_uint2(lo, hi);
+  };
+  auto add_part = [](float weight, float l, const float4& part, float& sum, float4& value) {
+    sum = fmaf(weight, l, sum);
+    value.x = fmaf(weight, part.x, value.x); value.y = fmaf(weight, part.y, value.y);
+    value.z = fmaf(weight, part.z, value.z); value.w = fmaf(weight, part.w, value.w);
+  };
+  auto weight_of = [&](float one, float top) { return one == -INFINITY ? 0.0f : exp2_fast((one - top) * kToLog2); };
+  const bool alone = active == 1;
+  for (int e = threadIdx.x; e < heads * (D / 4); e += kThreads) {
+    const int head = e / (D / 4), d = e % (D / 4) * 4;
+    float top = -INFINITY, sum = 0.0f;
+    float4 value = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) top = fmaxf(top, merge_m[w][head]);
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float mw = merge_m[w][head], weight = mw == -INFINITY ? 0.0f : exp2_fast((mw - top) * kLog2e);
-      sum = fmaf(weight, merge_l[w][head], sum);
-      value = fmaf(weight, parts[(w * kHeads + head) * D + d], value);
-    }
-    if (splits == 1) {
-      const int64_t at = (b * p.q_heads + head0 + head) * D + d;
-      const float y = value / sum;  // (0 / 0 = NaN for a sequence without tokens)
-      if (p.half) static_cast<__half*>(p.out)[at] = __float2half_rn(y);
-      else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(y);
+    for (int w = 0; w < kWarps; ++w)
+      add_part(weight_of(merge_m[w][head], top), merge_l[w][head],
+               *reinterpret_cast<const float4*>(parts + (w * kHeads + head) * D + d), sum, value);
+    if (alone) {
+      if (split == 0) put_out(head, d, value, sum);
+    } else if (p.cluster) {  // (each place of the first warp's part is read by the thread that writes it)
+      *reinterpret_cast<float4*>(parts + head * D + d) = value;
+      if (d == 0) {
+        joined[head][0] = top;
+        joined[head][1] = sum;
+      }
     } else {
       const int64_t part = (item * p.num_splits + split) * p.block_heads + head;
-      p.ws_o[part * D + d] = value;
+      *reinterpret_cast<float4*>(p.ws_o + part * D + d) = value;
       if (d == 0) {
         p.ws_ml[2 * part] = top;
         p.ws_ml[2 * part + 1] = sum;
       }
     }
   }
-  if (splits == 1) return;
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0) last_flag = atomicAdd(p.counters + item, 1) == splits - 1;
-  __syncthreads();
-  if (!last_flag) return;
-  __threadfence();
-  for (int e = threadIdx.x; e < heads * D / 4; e += kThreads) {
-    const int head = e / (D / 4), d = (e % (D / 4)) * 4;
-    const int64_t first = item * p.num_splits * p.block_heads + head;
-    float top = -INFINITY, sum = 0.0f;
-    float4 value = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int s0 = 0; s0 < splits; s0 += 8) {  // eight loads in flight
+  if (p.cluster) {
+    if (alone) return;  // (all CTAs of the cluster: the length is theirs)
+    __syncwarp();
+    cluster_sync();
+    for (int e = threadIdx.x * p.num_splits + split; e < heads * (D / 4); e += kThreads * p.num_splits) {
+      const int head = e / (D / 4), d = e % (D / 4) * 4;
       float2 ml[8];
       float4 part[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const bool there = s0 + i < splits;
-        const int64_t at = first + static_cast<int64_t>(there ? s0 + i : s0) * p.block_heads;
+        if (i >= active) break;
+        const float4 both = load_cluster_f32x4(smem_u32(parts + head * D + d), i);
+        part[i] = both;
+        ml[i].x = load_cluster_f32(smem_u32(&joined[head][0]), i);
+        ml[i].y = load_cluster_f32(smem_u32(&joined[head][1]), i);
+      }
+      float top = -INFINITY, sum = 0.0f;
+      float4 value = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i >= active) break;
+        top = fmaxf(top, ml[i].x);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i >= active) break;
+        add_part(weight_of(ml[i].x, top), ml[i].y, part[i], sum, value);
+      }
+      put_out(head, d, value, sum);
+    }
+    __syncwarp();
+    cluster_sync();  // (the others may still read this CTA's part)
+    return;
+  }
+  if (alone) return;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __threadfence();  // (behind the barrier: the partials of all threads)
+    last_flag = atomicAdd(p.counters + item, 1) == active - 1;
+    __threadfence();
+  }
+  __syncthreads();
+  if (!last_flag) return;
+  for (int e = threadIdx.x; e < heads * (D / 4); e += kThreads) {
+    const int head = e / (D / 4), d = e % (D / 4) * 4;
+    const int64_t first = item * p.num_splits * p.block_heads + head;
+    float top = -INFINITY, sum = 0.0f;
+    float4 value = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int s0 = 0; s0 < active; s0 += 16) {  // sixteen loads in flight
+      float2 ml[16];
+      float4 part[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int64_t at = first + static_cast<int64_t>(min(s0 + i, active - 1)) * p.block_heads;
         ml[i] = __ldcg(reinterpret_cast<const float2*>(p.ws_ml) + at);
         part[i] = __ldcg(reinterpret_cast<const float4*>(p.ws_o + at * D + d));
-        if (!there) ml[i] = make_float2(-INFINITY, 0.0f);
       }
       float over_all = top;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) over_all = fmaxf(over_all, ml[i].x);
-      const float keep = top == -INFINITY ? 0.0f : exp2_fast((top - over_all) * kLog2e);
+      for (int i = 0; i < 16; ++i) over_all = fmaxf(over_all, ml[i].x);  // (the last one again does no harm)
+      const float keep = weight_of(top, over_all);
       top = over_all;
       sum *= keep;
       value.x *= keep; value.y *= keep; value.z *= keep; value.w *= keep;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (s0 + i >= splits) break;
-        const float weight = ml[i].x == -INFINITY ? 0.0f : exp2_fast((ml[i].x - top) * kLog2e);
-        sum = fmaf(weight, ml[i].y, sum);
-        value.x = fmaf(weight, part[i].x, value.x); value.y = fmaf(weight, part[i].y, value.y);
-        value.z = fmaf(weight, part[i].z, value.z); value.w = fmaf(weight, part[i].w, value.w);
-      }
+      for (int i = 0; i < 16; ++i)
+        if (s0 + i < active) add_part(weight_of(ml[i].x, top), ml[i].y, part[i], sum, value);
     }
-    const int64_t at = (b * p.q_heads + head0 + head) * D + d;
-    const uint32_t lo = p.half ? pack_half2(value.x / sum, value.y / sum) : pack_bf16x2(value.x / sum, value.y / sum);
-    const uint32_t hi = p.half ? pack_half2(value.z / sum, value.w / sum) : pack_bf16x2(value.z / sum, value.w / sum);
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = make_uint2(lo, hi);
+    put_out(head, d, value, sum);
   }
   if (threadIdx.x == 0) p.counters[item] = 0;
 }
@@ -569,8 +632,8 @@ int launch_shape(const Params& p, const void* keys, const void* values, int64_t 
   if (!allow_shared_memory(kernel, smem, allowed)) return B200_ERR_LAUNCH;
   const dim3 grid(static_cast<unsigned>(p.num_splits), static_cast<unsigned>(p.kv_heads * p.head_blocks),
                   static_cast<unsigned>(batch));
-  return launch_chained(kernel, grid, dim3(kThreads), smem, stream, p, key_map, value_map) == cudaSuccess ? launch_status()
-                                                                                                   : B200_ERR_LAUNCH;
+  return launch_chained_cluster(kernel, grid, dim3(kThreads), smem, stream, p.cluster ? static_cast<unsigned>(p.num_splits) : 1u,
+                                p, key_map, value_map) == cudaSuccess ? launch_status() : B200_ERR_LAUNCH;
 }
 template <typename Code, int D, int NT>
 int launch_mask(const Params& p, const void* keys, const void* values, int64_t batch, cudaStream_t stream) {
