@@ -25,10 +25,18 @@ Plan plan_of(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim, int6
   if (split_tokens > 0) {
     plan.splits = ceil_div(longest, split_tokens);
   } else {
-    const int64_t resident = static_cast<int64_t>(kNumSMs) * (dim == 64 ? 4 : dim == 128 ? 2 : 1);
-    plan.splits = std::min(std::max<int64_t>(resident / items, 1), ceil_div(longest, kTile * kWarps));
+    // One round of the CTAs that the GPU holds at once, if a power of two of splits fits: a CTA streams nothing for some 5 us
+    // at its start and end, and a second round waits for that (32 x 4096 tokens, 4 heads of 128: 28 us in 256 CTAs, 39 in
+    // 512; 64 x 4096, 2 heads of 64: 18 in 512, 24 in 1024). Beyond a cluster's eight only 1024 tokens and more a CTA (16 x
+    // 4096, 2 heads of 64: 9.5 in 8 splits, 11 in 16; 1 x 32768, 4 heads of 128: 36 in 8, 20 in 32, 22 in 64). Where one
+    // round cannot split at all, several of short CTAs even out lengths that differ (64 ragged to 8192, 4 heads of 128: 79
+    // in one split, 63 in two, 59 in four; 64 x 4096 of one length 47, 64 and 62).
+    const int64_t slots = static_cast<int64_t>(kNumSMs) * (dim == 64 ? 4 : dim == 128 ? 3 : 1), rounds = slots / items;
+    plan.splits = 1;
+    while (plan.splits * 2 <= rounds && (plan.splits < 8 || plan.splits * 2 * 1024 <= longest)) plan.splits *= 2;
+    if (rounds < 2) plan.splits = rounds == 1 ? 4 : 2 * slots >= items ? 2 : 1;
   }
-  // (a CTA has a tile for each of its warps; that many sequences fill the GPU by themselves)
+  // (a CTA has a tile for each of its warps)
   plan.splits = std::max<int64_t>(1, std::min(plan.splits, ceil_div(longest, kTile * kWarps)));
   if (items > kMaxCounters) plan.splits = std::min<int64_t>(plan.splits, 8);
   plan.cluster = plan.splits > 1 && plan.splits <= 8;

@@ -21,11 +21,10 @@
 // it by more than 5: the softmax is the same, and most tiles need no reduction across lanes.
 //
 // Work. The tiles (32 tokens) of one (sequence, KV head, up to 8 NT heads) are dealt to `splits` CTAs of four warps, a tile
-// to a warp in turn: which tiles a warp has does not depend on the length, so it asks for their blocks while the length is
-// on its way. Each warp has a ring of its own that TMA fills: a tile never spans two blocks (block sizes are multiples of
-// 32), is contiguous in the pool, and is one box for K and one for V. Warps merge through shared memory. Up to eight splits
-// are a cluster, whose CTAs merge through distributed shared memory; more leave partials in the workspace, which the CTA
-// that arrives last adds in split order. Either way results do not depend on timing.
+// to a warp in turn. Each warp has a ring of its own that TMA fills: a tile never spans two blocks (block sizes are multiples
+// of 32), is contiguous in the pool, and is one box for K and one for V. Warps merge through shared memory. Up to eight
+// splits are a cluster, whose CTAs merge through distributed shared memory; more leave partials in the workspace, which the
+// CTA that arrives last adds in split order. Either way results do not depend on timing.
 #pragma once
 
 #include <algorithm>
@@ -44,6 +43,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 5.0f;  // how far a score may pass the running maximum before it moves
 constexpr int64_t kCounterBytes = 65536;
 constexpr int64_t kMaxCounters = kCounterBytes / 4;
+constexpr int kTableCache = 512;  // entries of a sequence's row of the block table that wait in shared memory
 
 struct Params {
   const void* q;
@@ -131,7 +131,7 @@ struct Shape {
   static constexpr int kBoxes = D / kRowBytes;
   static constexpr int kBoxBytes = kTile * kRowBytes;
   static constexpr int kTileBytes = kTile * D;                 // K or V
-  static constexpr int kStages = 3;
+  static constexpr int kStages = D == 128 ? 2 : 3;  // (shorter rings, more CTAs: 61 us where 96 KB of rings take 72, ragged to 8192)
   static constexpr int kRingBytes = kWarps * kStages * 2 * kTileBytes;
   // byte offset of 16-byte chunk `chunk` of row `row` in a tile
   __device__ static uint32_t at(int row, int chunk) {
@@ -153,7 +153,7 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
   __shared__ __align__(8) uint64_t full[kWarps * kStages];
   __shared__ float merge_m[kWarps][kHeads], merge_l[kWarps][kHeads];
   __shared__ float joined[kHeads][2];  // this CTA's maximum and sum
-  __shared__ int last_flag;
+  __shared__ int last_flag, row_cache[kTableCache];
 
   grid_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
@@ -165,49 +165,53 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
     for (int s = 0; s < kWarps * kStages; ++s) mbarrier_init(smem_u32(&full[s]), 1);
     fence_mbarrier_init();
   }
-  const int tiles_per_block = p.block_size / kTile, stride = kWarps * p.num_splits, my_first = split * kWarps + warp;
+  const int tiles_per_block = p.block_size / kTile, my_first = split * kWarps + warp;
   const int32_t* table = p.table + b * p.max_blocks;
-  const int max_tiles = static_cast<int>(p.max_blocks) * tiles_per_block;
   grid_dependency_wait_cta();
 
-  // Places of this warp's tiles, 32 tiles ahead in the lanes: lane i of a window that starts at `it` holds tile it + i.
-  struct Window { int slab, row; float ks, vs; };  // (block, head), row in the block
-  bool bad = false;
-  auto block_of = [&](int it, int& row) {
-    const int tile = my_first + it * stride;
-    if (tile >= max_tiles) return -1;
-    const int column = tile / tiles_per_block;
-    row = (tile - column * tiles_per_block) * kTile;
-    return table[column];
-  };
-  Window now = {}, next = {};
-  int block_now = block_of(lane, now.row), block_next = block_of(lane + 32, next.row);
+  // The row of the block table is asked for beside the length.
+  const int cached = static_cast<int>(min(p.max_blocks, static_cast<int64_t>(kTableCache)));
+  int entries[kTableCache / kThreads];
+#pragma unroll
+  for (int i = 0; i < kTableCache / kThreads; ++i) {
+    const int column = threadIdx.x + i * kThreads;
+    entries[i] = column < cached ? table[column] : -1;
+  }
   int64_t length64 = max(p.lengths[b], static_cast<int64_t>(0));
   if (length64 > p.mask_len) {
     length64 = p.mask_len;
     if (threadIdx.x == 0 && split == 0 && item_head == 0) atomicOr(p.status, B200_STATUS_LENGTH_OVER_MASK);
   }
+#pragma unroll
+  for (int i = 0; i < kTableCache / kThreads; ++i) row_cache[threadIdx.x + i * kThreads] = entries[i];
+  __syncthreads();
   const int length = static_cast<int>(length64), tiles = (length + kTile - 1) / kTile;
-  // CTAs that have tiles; without a cluster the others are not waited for
-  const int active = min(max((tiles + kWarps - 1) / kWarps, 1), p.num_splits);
-  if (!p.cluster && split >= active) return;
+  const int active = max(min((tiles + kWarps - 1) / kWarps, p.num_splits), 1);  // splits with a tile for each warp
+  if (split >= active) return;  // (a cluster's barriers do not wait for CTAs that have left)
+  const int stride = kWarps * active;
   const int mine = tiles > my_first ? (tiles - my_first + stride - 1) / stride : 0;
 
-  const uint32_t ring = smem_u32(smem) + warp * kStages * 2 * S::kTileBytes;
-  const uint32_t bars = smem_u32(&full[warp * kStages]);
-  auto settle = [&](int it, int block, Window& w) {
-    w.slab = -1;
-    if (it >= mine) return;
+  // Places of this warp's tiles, 32 tiles ahead in the lanes: lane i of a window that starts at `it` holds tile it + i.
+  struct Window { int slab, row; float ks, vs; };  // (block, head), row in the block
+  bool bad = false;
+  auto look_up = [&](int it) {
+    Window w = {-1, 0, 0.0f, 0.0f};
+    if (it >= mine) return w;
+    const int tile = my_first + it * stride, column = tile / tiles_per_block;
+    const int block = column < kTableCache ? row_cache[column] : table[column];
     if (block < 0 || block >= p.num_blocks) {
       bad = true;
-      return;
+      return w;
     }
     w.slab = block * p.kv_heads + kv;
+    w.row = (tile - column * tiles_per_block) * kTile;
     w.ks = p.key_scales[w.slab];
     w.vs = p.value_scales[w.slab];
+    return w;
   };
-  settle(lane, block_now, now);
-  settle(lane + 32, block_next, next);
+  const uint32_t ring = smem_u32(smem) + warp * kStages * 2 * S::kTileBytes;
+  const uint32_t bars = smem_u32(&full[warp * kStages]);
+  Window now = look_up(lane), next = look_up(lane + 32);
   int base = 0, issued = 0;  // of `now`; tiles asked for
   int issue_stage = 0;
   auto issue = [&]() {  // the lane that holds the tile's place asks for it; a tile without a block has no copy
@@ -311,8 +315,7 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
     if (it - base == 32) {
       now = next;
       base = it;
-      const int block = block_of(base + 32 + lane, next.row);
-      settle(base + 32 + lane, block, next);
+      next = look_up(base + 32 + lane);
     }
     const int slab = __shfl_sync(0xffffffffu, now.slab, it & 31);
     const float ks = __shfl_sync(0xffffffffu, now.ks, it & 31), vs = __shfl_sync(0xffffffffu, now.vs, it & 31);
@@ -535,10 +538,10 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
     }
   }
   if (p.cluster) {
-    if (alone) return;  // (all CTAs of the cluster: the length is theirs)
+    if (alone) return;
     __syncwarp();
     cluster_sync();
-    for (int e = threadIdx.x * p.num_splits + split; e < heads * (D / 4); e += kThreads * p.num_splits) {
+    for (int e = threadIdx.x * active + split; e < heads * (D / 4); e += kThreads * active) {
       const int head = e / (D / 4), d = e % (D / 4) * 4;
       float2 ml[8];
       float4 part[8];
