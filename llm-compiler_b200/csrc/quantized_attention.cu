@@ -10,7 +10,7 @@ int launch_int8(const Params& p, const void* keys, const void* values, int64_t b
 
 namespace {
 struct Plan {
-  int64_t head_blocks, block_heads, splits;
+  int64_t head_blocks, block_heads, splits, rounds;  // rounds of the CTAs that the GPU holds at once
   bool cluster;
   int64_t parts(int64_t batch, int64_t kv_heads) const {
     return splits > 1 && !cluster ? batch * kv_heads * head_blocks * splits * block_heads : 0;
@@ -22,6 +22,7 @@ Plan plan_of(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim, int6
   plan.head_blocks = ceil_div(group, dim == 256 ? 8 : 16);
   plan.block_heads = ceil_div(group, plan.head_blocks);
   const int64_t items = batch * kv_heads * plan.head_blocks;
+  const int64_t slots = static_cast<int64_t>(kNumSMs) * (dim == 64 ? 4 : dim == 128 ? 3 : 1);
   if (split_tokens > 0) {
     plan.splits = ceil_div(longest, split_tokens);
   } else {
@@ -31,10 +32,10 @@ Plan plan_of(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim, int6
     // 4096, 2 heads of 64: 9.5 in 8 splits, 11 in 16; 1 x 32768, 4 heads of 128: 36 in 8, 20 in 32, 22 in 64). Where one
     // round cannot split at all, several of short CTAs even out lengths that differ (64 ragged to 8192, 4 heads of 128: 79
     // in one split, 63 in two, 59 in four; 64 x 4096 of one length 47, 64 and 62).
-    const int64_t slots = static_cast<int64_t>(kNumSMs) * (dim == 64 ? 4 : dim == 128 ? 3 : 1), rounds = slots / items;
+    const int64_t rounds = slots / items;
     plan.splits = 1;
     while (plan.splits * 2 <= rounds && (plan.splits < 8 || plan.splits * 2 * 1024 <= longest)) plan.splits *= 2;
-    if (rounds < 2) plan.splits = rounds == 1 ? 4 : 2 * slots >= items ? 2 : 1;
+    if (rounds == 1) plan.splits = 2;
   }
   // (a CTA has a tile for each of its warps)
   plan.splits = std::max<int64_t>(1, std::min(plan.splits, ceil_div(longest, kTile * kWarps)));
@@ -42,6 +43,7 @@ Plan plan_of(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim, int6
   plan.cluster = plan.splits > 1 && plan.splits <= 8;
   if (plan.cluster)  // clusters of a power of two fit every GPC
     while ((plan.splits & (plan.splits - 1)) != 0) ++plan.splits;
+  plan.rounds = ceil_div(items * plan.splits, slots);
   return plan;
 }
 }  // namespace
@@ -93,6 +95,8 @@ extern "C" int b200_paged_decode_attention_8bit(const b200_cache_attention_call*
   p.q_batch_stride = c.q_batch_stride; p.q_head_stride = c.q_head_stride; p.mask_batch_stride = c.mask_batch_stride;
   p.num_blocks = c.num_blocks; p.max_blocks = c.max_blocks_per_sequence; p.mask_len = c.mask_len;
   p.num_splits = static_cast<int>(plan.splits); p.cluster = plan.cluster;
+  p.batch = static_cast<int>(c.batch);
+  p.sorted = plan.rounds > 1 && c.batch > 1 && c.batch <= kTableCache;
   p.q_heads = static_cast<int>(c.q_heads); p.kv_heads = static_cast<int>(c.kv_heads);
   p.group = static_cast<int>(c.q_heads / c.kv_heads);
   p.head_blocks = static_cast<int>(plan.head_blocks); p.block_heads = static_cast<int>(plan.block_heads);

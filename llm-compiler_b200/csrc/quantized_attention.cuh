@@ -58,8 +58,9 @@ struct Params {
   int* counters;   // [items], zero between calls
   int32_t* status;
   int64_t q_batch_stride, q_head_stride, mask_batch_stride, num_blocks, max_blocks, mask_len;
-  int q_heads, kv_heads, group, head_blocks, block_heads, block_size, mask_dtype, num_splits;
+  int q_heads, kv_heads, group, head_blocks, block_heads, block_size, mask_dtype, num_splits, batch;
   int cluster;     // the splits are a cluster
+  int sorted;      // CTAs take the sequences from the longest to the shortest
   int half;        // q and out are fp16, else bf16
   int q_vector;    // rows of q may be read 16 bytes at a time
   float scale;
@@ -153,12 +154,13 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
   __shared__ __align__(8) uint64_t full[kWarps * kStages];
   __shared__ float merge_m[kWarps][kHeads], merge_l[kWarps][kHeads];
   __shared__ float joined[kHeads][2];  // this CTA's maximum and sum
-  __shared__ int last_flag, row_cache[kTableCache];
+  __shared__ int last_flag;
+  __shared__ __align__(16) int row_cache[kTableCache];
 
   grid_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, j = lane & 3;
   const int split = blockIdx.x, item_head = blockIdx.y, kv = item_head / p.head_blocks, hb = item_head % p.head_blocks;
-  const int64_t b = blockIdx.z;
+  int64_t b = blockIdx.z;
   const int head0 = kv * p.group + hb * p.block_heads;
   const int heads = min(p.block_heads, p.group - hb * p.block_heads);
   if (threadIdx.x == 0) {
@@ -166,8 +168,29 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
     fence_mbarrier_init();
   }
   const int tiles_per_block = p.block_size / kTile, my_first = split * kWarps + warp;
-  const int32_t* table = p.table + b * p.max_blocks;
   grid_dependency_wait_cta();
+  if (p.sorted) {
+    // Several rounds of CTAs: the longest sequences first, so that the last round is short (64 ragged to 8192, 4 heads of
+    // 128: 62 us in the order of the batch). The CTAs at z take the sequence that z others are longer than.
+    for (int i = threadIdx.x; i < kTableCache; i += kThreads) {
+      const int64_t n = i < p.batch ? min(p.lengths[i], p.mask_len) : -1;
+      row_cache[i] = i < p.batch ? static_cast<int>(max(n, static_cast<int64_t>(0))) : -1;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < p.batch; i += kThreads) {
+      const int mine = row_cache[i];
+      int longer = 0;
+      for (int other = 0; other < p.batch; other += 4) {
+        const int4 four = *reinterpret_cast<const int4*>(row_cache + other);  // (-1 beyond the batch)
+        longer += (four.x > mine || (four.x == mine && other < i)) + (four.y > mine || (four.y == mine && other + 1 < i)) +
+                  (four.z > mine || (four.z == mine && other + 2 < i)) + (four.w > mine || (four.w == mine && other + 3 < i));
+      }
+      if (longer == static_cast<int>(blockIdx.z)) last_flag = i;
+    }
+    __syncthreads();
+    b = last_flag;
+  }
+  const int32_t* table = p.table + b * p.max_blocks;
 
   // The row of the block table is asked for beside the length.
   const int cached = static_cast<int>(min(p.max_blocks, static_cast<int64_t>(kTableCache)));
@@ -211,7 +234,8 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
   };
   const uint32_t ring = smem_u32(smem) + warp * kStages * 2 * S::kTileBytes;
   const uint32_t bars = smem_u32(&full[warp * kStages]);
-  Window now = look_up(lane), next = look_up(lane + 32);
+  Window now = look_up(lane), next = {-1, 0, 0.0f, 0.0f};
+  if (mine > 32) next = look_up(lane + 32);
   int base = 0, issued = 0;  // of `now`; tiles asked for
   int issue_stage = 0;
   auto issue = [&]() {  // the lane that holds the tile's place asks for it; a tile without a block has no copy
