@@ -38,7 +38,7 @@ Plan plan_of(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim, int6
     if (rounds == 1) plan.splits = 2;
   }
   // (a CTA has a tile for each of its warps)
-  plan.splits = std::max<int64_t>(1, std::min(plan.splits, ceil_div(longest, kTile * kWarps)));
+  plan.splits = std::max<int64_t>(1, std::min(plan.splits, ceil_div(longest, 32 * kWarps)));
   if (items > kMaxCounters) plan.splits = std::min<int64_t>(plan.splits, 8);
   plan.cluster = plan.splits > 1 && plan.splits <= 8;
   if (plan.cluster)  // clusters of a power of two fit every GPC
@@ -71,7 +71,7 @@ extern "C" int b200_paged_decode_attention_8bit(const b200_cache_attention_call*
       (c.mask && (c.mask_dtype < 0 || c.mask_dtype > B200_F16)))
     return B200_ERR_BAD_ARGUMENT;
   if ((c.dtype != B200_BF16 && c.dtype != B200_F16) || (c.cache_dtype != B200_I8 && c.cache_dtype != B200_E4M3) ||
-      (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256) || c.block_size % kTile != 0)
+      (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256) || c.block_size % 32 != 0)
     return B200_ERR_UNSUPPORTED;
   if (!aligned16(c.key_pool) || !aligned16(c.value_pool) || (reinterpret_cast<uintptr_t>(c.output) & 7u) != 0)
     return B200_ERR_ALIGNMENT;

@@ -38,7 +38,6 @@ namespace cache_attention {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kTile = 32;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 5.0f;  // how far a score may pass the running maximum before it moves
 constexpr int64_t kCounterBytes = 65536;
@@ -128,11 +127,13 @@ __device__ __forceinline__ float load_mask(const Params& p, int64_t i) {
 
 template <int D>
 struct Shape {
+  static constexpr int kTile = 32;                             // tokens of a tile (D 128: 16 and a fourth CTA, 37 -> 41 us at 3 x 30001)
   static constexpr int kRowBytes = D < 128 ? D : 128;         // a box is one swizzle span wide
   static constexpr int kBoxes = D / kRowBytes;
   static constexpr int kBoxBytes = kTile * kRowBytes;
   static constexpr int kTileBytes = kTile * D;                 // K or V
   static constexpr int kStages = D == 128 ? 2 : 3;  // (shorter rings, more CTAs: 61 us where 96 KB of rings take 72, ragged to 8192)
+  static constexpr int kResident(int n_tiles) { return D == 256 ? 1 : D == 64 && n_tiles == 1 ? 4 : 3; }  // CTAs of an SM
   static constexpr int kRingBytes = kWarps * kStages * 2 * kTileBytes;
   // byte offset of 16-byte chunk `chunk` of row `row` in a tile
   __device__ static uint32_t at(int row, int chunk) {
@@ -145,10 +146,11 @@ struct Shape {
 };
 
 template <typename Code, int D, int NT, bool kMask>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, (Shape<D>::kResident(NT)))
 cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_map,
                        const __grid_constant__ CUtensorMap value_map) {
   using S = Shape<D>;
+  constexpr int kTile = S::kTile, kParts = kTile / 16, kEach = kTile / 8;  // m-tiles; a lane's tokens
   constexpr int kStages = S::kStages, kSteps = D / 16, kHeads = 8 * NT;
   extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ __align__(8) uint64_t full[kWarps * kStages];
@@ -257,6 +259,10 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
   for (int s = 0; s < kStages - 1; ++s)
     if (s < mine) issue();
 
+  // Scores without a mask are in units of log 2; with one they stay natural, since a mask of the type's lowest value would
+  // leave its range.
+  constexpr float kUnit = kMask ? 1.0f : kLog2e, kToLog2 = kMask ? kLog2e : 1.0f;
+
   // ---- q as B operands: lane (g, j) holds head g, elements 64 c + 16 j .. + 15 of every 64 ----
   uint32_t qb[NT][kSteps][2];
   float factor[NT][2];  // score of one product, for this lane's columns (heads 2 j, 2 j + 1)
@@ -302,13 +308,10 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
       qb[t][i][0] = pack_half2(v[e] * down, v[e + 1] * down);
       qb[t][i][1] = pack_half2(v[e + 2] * down, v[e + 3] * down);
     }
-    factor[t][0] = p.scale * __shfl_sync(0xffffffffu, up, 8 * j);
-    factor[t][1] = p.scale * __shfl_sync(0xffffffffu, up, 8 * j + 4);
+    factor[t][0] = p.scale * kUnit * __shfl_sync(0xffffffffu, up, 8 * j);
+    factor[t][1] = p.scale * kUnit * __shfl_sync(0xffffffffu, up, 8 * j + 4);
   }
 
-  // Scores without a mask are in units of log 2; with one they stay natural, since a mask of the type's lowest value would
-  // leave its range.
-  constexpr float kUnit = kMask ? 1.0f : kLog2e, kToLog2 = kMask ? kLog2e : 1.0f;
   float m[NT][2], l[NT][2], o[NT][kSteps][4];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
@@ -317,14 +320,14 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.0f;
   }
-  float vref = 0.0f;
+  float vref = 0.0f, inverse_vref = 1.0f;
   bool timed_out = false;
   const int my_token = S::token(g);
-  float mask_next[4];
+  float mask_next[kEach];
   auto fetch_mask = [&](int it) {
     if constexpr (kMask) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
+      for (int r = 0; r < kEach; ++r) {
         const int token = (my_first + it * stride) * kTile + 8 * r + my_token;
         mask_next[r] = it < mine && token < length ? load_mask(p, b * p.mask_batch_stride + token) : 0.0f;
       }
@@ -352,18 +355,18 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
     }
     __syncwarp();  // every lane is done with the stage that is filled next
     if (issued < mine) issue();
-    float extra[4];
+    float extra[kEach];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) extra[r] = kMask ? mask_next[r] : 0.0f;
+    for (int r = 0; r < kEach; ++r) extra[r] = kMask ? mask_next[r] : 0.0f;
     fetch_mask(it + 1);
     if (slab < 0) continue;
     const uint32_t keys = ring + stage * 2 * S::kTileBytes, values = keys + S::kTileBytes;
     const int valid = min(length - (my_first + it * stride) * kTile, kTile);
 
-    // ---- scores of 32 tokens ----
-    float s[NT][2][4];
+    // ---- scores of the tile ----
+    float s[NT][kParts][4];
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
+    for (int mt = 0; mt < kParts; ++mt) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) s[t][mt][0] = s[t][mt][1] = s[t][mt][2] = s[t][mt][3] = 0.0f;
 #pragma unroll
@@ -384,21 +387,27 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
         }
       }
     }
+    auto highest = [&](int t, int h) {
+      float top = fmaxf(s[t][0][h], s[t][0][2 + h]);
+#pragma unroll
+      for (int mt = 1; mt < kParts; ++mt) top = fmaxf(top, fmaxf(s[t][mt][h], s[t][mt][2 + h]));
+      return top;
+    };
     bool over = false;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float f = ks * factor[t][h] * kUnit;
+        const float f = ks * factor[t][h];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {  // token 8 r + my_token
+        for (int r = 0; r < kEach; ++r) {  // token 8 r + my_token
           float& x = s[t][r >> 1][2 * (r & 1) + h];
           x = kMask ? fmaf(x, f, extra[r]) : x * f;
         }
       }
     if (valid < kTile) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+      for (int r = 0; r < kEach; ++r)
         if (8 * r + my_token >= valid) {
 #pragma unroll
           for (int t = 0; t < NT; ++t) s[t][r >> 1][2 * (r & 1)] = s[t][r >> 1][2 * (r & 1) + 1] = -INFINITY;
@@ -408,13 +417,13 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        over = over || fmaxf(fmaxf(s[t][0][h], s[t][0][2 + h]), fmaxf(s[t][1][h], s[t][1][2 + h])) > m[t][h] + kSlack;
+        over = over || highest(t, h) > m[t][h] + kSlack;
     if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          float top = fmaxf(fmaxf(s[t][0][h], s[t][0][2 + h]), fmaxf(s[t][1][h], s[t][1][2 + h]));
+          float top = highest(t, h);
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
@@ -434,6 +443,7 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
       const float unit = vref > 0.0f ? fminf(fmaxf(vs, vref * 0x1p-60f), vref * 0x1p60f) : vs;
       const float keep = vref > 0.0f ? vref / unit : 1.0f;
       vref = unit;
+      inverse_vref = 1.0f / unit;
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -441,16 +451,16 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
           o[t][i][0] *= keep; o[t][i][1] *= keep; o[t][i][2] *= keep; o[t][i][3] *= keep;
         }
     }
-    float weight = vref > 0.0f ? vs / vref : vs;
+    float weight = vs * inverse_vref;
     if (weight > 16.0f) weight = 16.0f;  // (a NaN stays)
 
     // ---- probabilities, transposed into B operands ----
-    uint32_t pb[NT][2][2];
+    uint32_t pb[NT][kParts][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const float m0 = m[t][0] == -INFINITY ? 0.0f : m[t][0], m1 = m[t][1] == -INFINITY ? 0.0f : m[t][1];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
+      for (int r = 0; r < kEach; ++r) {
         const float p0 = exp2_fast((s[t][r >> 1][2 * (r & 1)] - m0) * kToLog2);
         const float p1 = exp2_fast((s[t][r >> 1][2 * (r & 1) + 1] - m1) * kToLog2);
         l[t][0] += p0;
@@ -469,7 +479,7 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
     }
     // ---- O^T += V^T P^T ----
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
+    for (int mt = 0; mt < kParts; ++mt)
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         uint32_t r[4];
@@ -641,7 +651,7 @@ bool make_pool_map(CUtensorMap* map, const void* base, int64_t slabs, int64_t bl
   if (encode == nullptr) return false;
   const cuuint64_t dims[3] = {D, static_cast<cuuint64_t>(block_size), static_cast<cuuint64_t>(slabs)};
   const cuuint64_t strides[2] = {D, static_cast<cuuint64_t>(D * block_size)};
-  const cuuint32_t box[3] = {Shape<D>::kRowBytes, kTile, 1}, element_strides[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {Shape<D>::kRowBytes, Shape<D>::kTile, 1}, element_strides[3] = {1, 1, 1};
   return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, element_strides,
                 CU_TENSOR_MAP_INTERLEAVE_NONE, D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
