@@ -17,6 +17,12 @@ struct Int8Code {
     return static_cast<uint32_t>(__float2int_rn(fminf(fmaxf(v == v ? v : 0.0f, -kTop), kTop))) & 0xffu;
   }
   __device__ static float decode(uint32_t code) { return static_cast<float>(static_cast<int8_t>(code)); }
+  // Four codes of finite values that the scale brings to [-127.4, 127.4]: v + 1.5 * 2^23 rounds to the nearest integer, ties
+  // to even, and leaves it in the low byte.
+  __device__ static uint32_t encode_four(float a, float b, float c, float d) {
+    const auto byte = [](float v) { return __float_as_uint(__fadd_rn(v, 12582912.0f)); };
+    return __byte_perm(__byte_perm(byte(a), byte(b), 0x0040), __byte_perm(byte(c), byte(d), 0x0040), 0x5410);
+  }
 };
 struct E4m3Code {
   static constexpr float kTop = 448.0f;
@@ -24,6 +30,10 @@ struct E4m3Code {
   __device__ static uint32_t encode(float v) { return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3); }
   __device__ static float decode(uint32_t code) {
     return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(code), __NV_E4M3)));
+  }
+  __device__ static uint32_t encode_four(float a, float b, float c, float d) {
+    return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3) |
+           (static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3)) << 16);
   }
 };
 

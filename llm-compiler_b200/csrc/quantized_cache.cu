@@ -34,12 +34,11 @@ struct StoreParams {
 };
 
 template <typename T, typename Code, bool kVector>
-__global__ void __launch_bounds__(kStoreThreads)
+__global__ void __launch_bounds__(kStoreThreads, 4)
 quantized_store_kernel(const StoreParams p) {
   constexpr int per = kVector ? 8 : 1;  // elements a load takes
   grid_launch_dependents();
-  __shared__ uint32_t most_bits[kStoreThreads / 32];
-  __shared__ int bad[kStoreThreads / 32];
+  __shared__ uint32_t parts[kStoreThreads / 32];
   const int h = blockIdx.y % p.heads, which = blockIdx.y / p.heads;
   const int64_t b = blockIdx.z;
   grid_dependency_wait();
@@ -57,62 +56,74 @@ quantized_store_kernel(const StoreParams p) {
     return;
   }
   const int64_t block = p.table[b * p.max_blocks + column];
+  const int held = static_cast<int>(first - column * p.block_size), rows = static_cast<int>(end - first);
+  const int64_t* st = p.strides[which];
+  const T* x = static_cast<const T*>(p.x[which]) + b * st[0] + h * st[1] + (first - position) * st[2];
+  const int per_row = p.dim / per, items = rows * per_row;
+  // item i is load i % per_row of row i / per_row; a thread stays in its column where a row divides the CTA's threads
+  const int my_row = threadIdx.x / per_row, my_column = threadIdx.x - my_row * per_row;
+  const int row_step = kStoreThreads % per_row == 0 ? kStoreThreads / per_row : 0;
+  auto address = [&](int j) {  // the thread's j-th
+    if (row_step > 0) return x + (my_row + j * row_step) * st[2] + my_column * per * st[3];
+    const int i = threadIdx.x + j * kStoreThreads, row = i / per_row;
+    return x + row * st[2] + (i - row * per_row) * per * st[3];
+  };
+
+  // The largest magnitude of the new rows: without their signs, 16-bit floats compare as integers, two in a word. The rows
+  // are asked for beside the block.
+  constexpr uint32_t kInfinity = IsHalf<T>::value ? 0x7c00u : 0x7f80u;
+  uint4 kept[kStoreVectors];
+  uint32_t pair = 0;
+  auto look_at = [&](const uint4& raw) {
+    pair = __vmaxu2(__vmaxu2(pair, raw.x & 0x7fff7fffu), raw.y & 0x7fff7fffu);
+    pair = __vmaxu2(__vmaxu2(pair, raw.z & 0x7fff7fffu), raw.w & 0x7fff7fffu);
+  };
+  auto bits_of = [&](int j) { return static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(address(j))) & 0x7fffu; };
+  auto largest_of_all = [&](uint32_t v) {
+    v = __reduce_max_sync(0xffffffffu, v);
+    __syncthreads();  // (what was there has been read)
+    if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = v;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kStoreThreads / 32; ++w) v = max(v, parts[w]);
+    return v;
+  };
+  const int mine = items > static_cast<int>(threadIdx.x) ? (items - threadIdx.x + kStoreThreads - 1) / kStoreThreads : 0;
+  if constexpr (kVector) {
+#pragma unroll
+    for (int j = 0; j < kStoreVectors; ++j) {
+      kept[j] = make_uint4(0u, 0u, 0u, 0u);
+      if (j < mine) kept[j] = *reinterpret_cast<const uint4*>(address(j));
+    }
+  }
   if (block < 0 || block >= p.num_blocks) {
     if (threadIdx.x == 0) atomicOr(p.status, B200_STATUS_BAD_POSITION);
     return;
   }
-  const int held = static_cast<int>(first - column * p.block_size), rows = static_cast<int>(end - first);
-  const int64_t* st = p.strides[which];
-  const T* x = static_cast<const T*>(p.x[which]) + b * st[0] + h * st[1] + (first - position) * st[2];
   const int64_t slab = block * p.heads + h;
   uint8_t* codes = p.pool[which] + slab * p.block_size * p.dim;
-  const int per_row = p.dim / per, items = rows * per_row;
-
-  // the largest finite magnitude of the new rows (as bits: magnitudes compare as integers)
-  uint4 kept[kStoreVectors];
-  uint32_t most = 0;
-  bool not_finite = false;
-  auto look = [&](float v) {
-    const uint32_t bits = __float_as_uint(v) & 0x7fffffffu;
-    if (bits < 0x7f800000u) most = max(most, bits);
-    else not_finite = true;
-  };
-  auto address = [&](int i) { return x + (i / per_row) * st[2] + (i % per_row) * per * st[3]; };
-  auto look_at = [&](const uint4& raw) {
-    Vec16<T> v;
-    v.load(reinterpret_cast<const T*>(&raw));
-#pragma unroll
-    for (int e = 0; e < 8; ++e) look(v.v[e]);
-  };
+  const float before = held > 0 ? p.scales[which][slab] : 0.0f;
   if constexpr (kVector) {
 #pragma unroll
-    for (int j = 0; j < kStoreVectors; ++j) {
-      const int i = threadIdx.x + j * kStoreThreads;
-      kept[j] = make_uint4(0u, 0u, 0u, 0u);
-      if (i < items) kept[j] = *reinterpret_cast<const uint4*>(address(i));
-    }
-#pragma unroll
     for (int j = 0; j < kStoreVectors; ++j) look_at(kept[j]);
-    for (int i = threadIdx.x + kStoreVectors * kStoreThreads; i < items; i += kStoreThreads)
-      look_at(*reinterpret_cast<const uint4*>(address(i)));
+    for (int j = kStoreVectors; j < mine; ++j) look_at(*reinterpret_cast<const uint4*>(address(j)));
   } else {
-    for (int i = threadIdx.x; i < items; i += kStoreThreads) look(Elem<T>::load(address(i)));
+    for (int j = 0; j < mine; ++j) pair = max(pair, bits_of(j));
   }
-  most = __reduce_max_sync(0xffffffffu, most);
-  const bool any_bad = __any_sync(0xffffffffu, not_finite);
-  if ((threadIdx.x & 31) == 0) {
-    most_bits[threadIdx.x >> 5] = most;
-    bad[threadIdx.x >> 5] = any_bad;
+  uint32_t most = largest_of_all(max(pair & 0xffffu, pair >> 16));
+  const bool all_bad = most >= kInfinity;
+  if (all_bad) {  // once more, of the finite ones
+    pair = 0;
+    for (int i = threadIdx.x; i < rows * p.dim; i += kStoreThreads) {
+      const int row = i / p.dim;
+      const uint32_t bits = *reinterpret_cast<const uint16_t*>(x + row * st[2] + (i - row * p.dim) * st[3]) & 0x7fffu;
+      if (bits < kInfinity) pair = max(pair, bits);
+    }
+    most = largest_of_all(pair);
   }
-  __syncthreads();
-  bool all_bad = false;
-#pragma unroll
-  for (int w = 0; w < kStoreThreads / 32; ++w) {
-    most = max(most, most_bits[w]);
-    all_bad = all_bad || bad[w] != 0;
-  }
-  const float before = held > 0 ? p.scales[which][slab] : 0.0f;
-  float scale = most > 0 ? fmaxf(__fmul_rn(__uint_as_float(most), 1.0f / Code::kTop), kSmallestScale) : 0.0f;
+  const uint16_t most_bits = static_cast<uint16_t>(most);
+  const float largest = Elem<T>::load(reinterpret_cast<const T*>(&most_bits));
+  float scale = most > 0 ? fmaxf(__fmul_rn(largest, 1.0f / Code::kTop), kSmallestScale) : 0.0f;
   scale = fmaxf(scale, before);
   const float inverse = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
   __syncthreads();  // every thread has read the scale
@@ -138,28 +149,31 @@ quantized_store_kernel(const StoreParams p) {
     }
   }
   uint8_t* out = codes + held * p.dim;
-  auto put = [&](const uint4& raw, int i) {
+  auto put = [&](const uint4& raw, int j) {
     Vec16<T> v;
     v.load(reinterpret_cast<const T*>(&raw));
     uint2 packed = make_uint2(0u, 0u);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      packed.x |= Code::encode(__fmul_rn(v.v[e], inverse)) << (8 * e);
-      packed.y |= Code::encode(__fmul_rn(v.v[e + 4], inverse)) << (8 * e);
+    for (int e = 0; e < 8; ++e) v.v[e] = __fmul_rn(v.v[e], inverse);
+    if (!all_bad) {
+      packed = make_uint2(Code::encode_four(v.v[0], v.v[1], v.v[2], v.v[3]), Code::encode_four(v.v[4], v.v[5], v.v[6], v.v[7]));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        packed.x |= Code::encode(v.v[e]) << (8 * e);
+        packed.y |= Code::encode(v.v[e + 4]) << (8 * e);
+      }
     }
-    *reinterpret_cast<uint2*>(out + i * 8) = packed;
+    *reinterpret_cast<uint2*>(out + (threadIdx.x + j * kStoreThreads) * 8) = packed;
   };
   if constexpr (kVector) {
 #pragma unroll
-    for (int j = 0; j < kStoreVectors; ++j) {
-      const int i = threadIdx.x + j * kStoreThreads;
-      if (i < items) put(kept[j], i);
-    }
-    for (int i = threadIdx.x + kStoreVectors * kStoreThreads; i < items; i += kStoreThreads)
-      put(*reinterpret_cast<const uint4*>(address(i)), i);
+    for (int j = 0; j < kStoreVectors; ++j)
+      if (j < mine) put(kept[j], j);
+    for (int j = kStoreVectors; j < mine; ++j) put(*reinterpret_cast<const uint4*>(address(j)), j);
   } else {
-    for (int i = threadIdx.x; i < items; i += kStoreThreads)
-      out[i] = static_cast<uint8_t>(Code::encode(__fmul_rn(Elem<T>::load(address(i)), inverse)));
+    for (int j = 0; j < mine; ++j)
+      out[threadIdx.x + j * kStoreThreads] = static_cast<uint8_t>(Code::encode(__fmul_rn(Elem<T>::load(address(j)), inverse)));
   }
 }
 
