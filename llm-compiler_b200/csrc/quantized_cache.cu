@@ -34,7 +34,7 @@ struct StoreParams {
 };
 
 template <typename T, typename Code, bool kVector>
-__global__ void __launch_bounds__(kStoreThreads, 4)
+__global__ void __launch_bounds__(kStoreThreads, 3)
 quantized_store_kernel(const StoreParams p) {
   constexpr int per = kVector ? 8 : 1;  // elements a load takes
   grid_launch_dependents();
