@@ -1,13 +1,8 @@
-// Decode attention over a paged cache in 8 bits: checks, the split of the work, and the instances for integer codes
-// (quantized_attention.cuh).
+// Decode attention over a paged cache in 8 bits: checks and the split of the work (quantized_attention.cuh has the kernel).
 #include "quantized_attention.cuh"
 
 namespace b200 {
 namespace cache_attention {
-int launch_int8(const Params& p, const void* keys, const void* values, int64_t batch, int64_t dim, cudaStream_t stream) {
-  return launch_code<Int8Code>(p, keys, values, batch, dim, stream);
-}
-
 namespace {
 struct Plan {
   int64_t head_blocks, block_heads, splits, rounds;  // rounds of the CTAs that the GPU holds at once
@@ -100,10 +95,11 @@ extern "C" int b200_paged_decode_attention_8bit(const b200_cache_attention_call*
   p.q_heads = static_cast<int>(c.q_heads); p.kv_heads = static_cast<int>(c.kv_heads);
   p.group = static_cast<int>(c.q_heads / c.kv_heads);
   p.head_blocks = static_cast<int>(plan.head_blocks); p.block_heads = static_cast<int>(plan.block_heads);
-  p.block_size = static_cast<int>(c.block_size); p.mask_dtype = static_cast<int>(c.mask_dtype); p.half = c.dtype == B200_F16;
+  p.block_size = static_cast<int>(c.block_size); p.mask_dtype = static_cast<int>(c.mask_dtype);
   p.q_vector = aligned16(c.query) && c.q_batch_stride % 8 == 0 && c.q_head_stride % 8 == 0;
   p.scale = static_cast<float>(c.scale); p.wait_limit = wait_limit(); p.drop_loads = drop_loads();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return c.cache_dtype == B200_I8 ? launch_int8(p, c.key_pool, c.value_pool, c.batch, c.head_dim, s)
-                                  : launch_e4m3(p, c.key_pool, c.value_pool, c.batch, c.head_dim, s);
+  const auto launch = c.cache_dtype == B200_I8 ? (c.dtype == B200_BF16 ? launch_int8_bf16 : launch_int8_f16)
+                                               : (c.dtype == B200_BF16 ? launch_e4m3_bf16 : launch_e4m3_f16);
+  return launch(p, c.key_pool, c.value_pool, c.batch, c.head_dim, s);
 }

@@ -1,4 +1,5 @@
-// Decode attention over a paged cache in 8 bits: the kernel and its launch, instantiated per code type in a .cu of its own.
+// Decode attention over a paged cache in 8 bits: the kernel and its launch, instantiated per code and query type in a .cu of
+// its own.
 //
 //     out = sum_t softmax_t(scale * ks * (q . ck_t) + mask_t) vs cv_t,   t < length,
 // with ck, cv the codes of token t and ks, vs the scales of its block. The G query heads of a KV head share one read of its
@@ -17,8 +18,10 @@
 //
 // Scales. ks multiplies the scores. vs is folded into the probabilities relative to a running reference `vref`, which the
 // accumulators are carried in; it follows vs (accumulators rescaled) only when they are more than 16 apart, so P stays well
-// inside fp16. P itself is fp16 (2^-11; it is at most e^5, below), its sum fp32. The running maximum moves only when a score passes
-// it by more than 5: the softmax is the same, and most tiles need no reduction across lanes.
+// inside fp16. The running maximum moves only when a score passes it by more than 5: the softmax is the same, and most tiles
+// need no reduction across lanes. P is rounded to fp16, half a step of which is 2^-11 of it, its sum stays fp32: an eighth of
+// the rounding of a bf16 result. An fp16 result's own rounding is no larger than P's, so there P is two fp16 numbers, what the
+// first leaves in the second (2^-22): one more product per V fragment.
 //
 // Work. The tiles (32 tokens) of one (sequence, KV head, up to 8 NT heads) are dealt to `splits` CTAs of four warps, a tile
 // to a warp in turn. Each warp has a ring of its own that TMA fills: a tile never spans two blocks (block sizes are multiples
@@ -60,7 +63,6 @@ struct Params {
   int q_heads, kv_heads, group, head_blocks, block_heads, block_size, mask_dtype, num_splits, batch;
   int cluster;     // the splits are a cluster
   int sorted;      // CTAs take the sequences from the longest to the shortest
-  int half;        // q and out are fp16, else bf16
   int q_vector;    // rows of q may be read 16 bytes at a time
   float scale;
   uint32_t wait_limit;
@@ -145,7 +147,7 @@ struct Shape {
   __device__ static int token(int r) { return D == 64 ? r : (r >> 1) | ((r & 1) << 2); }
 };
 
-template <typename Code, int D, int NT, bool kMask>
+template <typename T, typename Code, int D, int NT, bool kMask>
 __global__ void __launch_bounds__(kThreads, (Shape<D>::kResident(NT)))
 cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_map,
                        const __grid_constant__ CUtensorMap value_map) {
@@ -287,8 +289,8 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          v[16 * c + 2 * e] = p.half ? Elem<__half>::lo(raw[e]) : bf16_lo(raw[e]);
-          v[16 * c + 2 * e + 1] = p.half ? Elem<__half>::hi(raw[e]) : bf16_hi(raw[e]);
+          v[16 * c + 2 * e] = Elem<T>::lo(raw[e]);
+          v[16 * c + 2 * e + 1] = Elem<T>::hi(raw[e]);
         }
       }
     } else {
@@ -455,7 +457,7 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
     if (weight > 16.0f) weight = 16.0f;  // (a NaN stays)
 
     // ---- probabilities, transposed into B operands ----
-    uint32_t pb[NT][kParts][2];
+    uint32_t pb[NT][kParts][2], rest[NT][kParts][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const float m0 = m[t][0] == -INFINITY ? 0.0f : m[t][0], m1 = m[t][1] == -INFINITY ? 0.0f : m[t][1];
@@ -465,7 +467,11 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
         const float p1 = exp2_fast((s[t][r >> 1][2 * (r & 1) + 1] - m1) * kToLog2);
         l[t][0] += p0;
         l[t][1] += p1;
-        pb[t][r >> 1][r & 1] = transpose_8x8(pack_half2(p0 * weight, p1 * weight));
+        const float w0 = p0 * weight, w1 = p1 * weight;
+        const uint32_t both = pack_half2(w0, w1);
+        pb[t][r >> 1][r & 1] = transpose_8x8(both);
+        if constexpr (IsHalf<T>::value)
+          rest[t][r >> 1][r & 1] = transpose_8x8(pack_half2(w0 - Elem<__half>::lo(both), w1 - Elem<__half>::hi(both)));
       }
     }
     if constexpr (std::is_same<Code, E4m3Code>::value) {
@@ -490,7 +496,10 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
           Convert<Code>::every_other(r[2 * half], a[0], a[1]);
           Convert<Code>::every_other(r[2 * half + 1], a[2], a[3]);
 #pragma unroll
-          for (int t = 0; t < NT; ++t) mma_f16_16816(o[t][2 * c + half], a, pb[t][mt][0], pb[t][mt][1]);
+          for (int t = 0; t < NT; ++t) {
+            mma_f16_16816(o[t][2 * c + half], a, pb[t][mt][0], pb[t][mt][1]);
+            if constexpr (IsHalf<T>::value) mma_f16_16816(o[t][2 * c + half], a, rest[t][mt][0], rest[t][mt][1]);
+          }
         }
       }
   }
@@ -533,9 +542,7 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
     const int64_t at = (b * p.q_heads + head0 + head) * D + d;
     const float scale = 1.0f / sum;
     value.x *= scale; value.y *= scale; value.z *= scale; value.w *= scale;
-    const uint32_t lo = p.half ? pack_half2(value.x, value.y) : pack_bf16x2(value.x, value.y);
-    const uint32_t hi = p.half ? pack_half2(value.z, value.w) : pack_bf16x2(value.z, value.w);
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) = make_uint2(lo, hi);
+    *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at) = make_uint2(Elem<T>::pack(value.x, value.y), Elem<T>::pack(value.z, value.w));
   };
   auto add_part = [](float weight, float l, const float4& part, float& sum, float4& value) {
     sum = fmaf(weight, l, sum);
@@ -657,14 +664,14 @@ bool make_pool_map(CUtensorMap* map, const void* base, int64_t slabs, int64_t bl
                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename Code, int D, int NT, bool kMask>
+template <typename T, typename Code, int D, int NT, bool kMask>
 int launch_shape(const Params& p, const void* keys, const void* values, int64_t batch, cudaStream_t stream) {
   CUtensorMap key_map, value_map;
   if (!make_pool_map<D>(&key_map, keys, p.num_blocks * p.kv_heads, p.block_size) ||
       !make_pool_map<D>(&value_map, values, p.num_blocks * p.kv_heads, p.block_size))
     return B200_ERR_UNSUPPORTED;
   constexpr int smem = std::max(Shape<D>::kRingBytes, kWarps * 8 * NT * D * 4);
-  auto kernel = cache_attention_kernel<Code, D, NT, kMask>;
+  auto kernel = cache_attention_kernel<T, Code, D, NT, kMask>;
   static std::atomic<uint64_t> allowed{0};
   if (!allow_shared_memory(kernel, smem, allowed)) return B200_ERR_LAUNCH;
   const dim3 grid(static_cast<unsigned>(p.num_splits), static_cast<unsigned>(p.kv_heads * p.head_blocks),
@@ -672,24 +679,27 @@ int launch_shape(const Params& p, const void* keys, const void* values, int64_t 
   return launch_chained_cluster(kernel, grid, dim3(kThreads), smem, stream, p.cluster ? static_cast<unsigned>(p.num_splits) : 1u,
                                 p, key_map, value_map) == cudaSuccess ? launch_status() : B200_ERR_LAUNCH;
 }
-template <typename Code, int D, int NT>
+template <typename T, typename Code, int D, int NT>
 int launch_mask(const Params& p, const void* keys, const void* values, int64_t batch, cudaStream_t stream) {
-  return p.mask != nullptr ? launch_shape<Code, D, NT, true>(p, keys, values, batch, stream)
-                           : launch_shape<Code, D, NT, false>(p, keys, values, batch, stream);
+  return p.mask != nullptr ? launch_shape<T, Code, D, NT, true>(p, keys, values, batch, stream)
+                           : launch_shape<T, Code, D, NT, false>(p, keys, values, batch, stream);
 }
 // n-tiles of heads: one up to eight heads of a block, else two (head_dim 256: one, its accumulators fill the registers)
-template <typename Code>
+template <typename T, typename Code>
 int launch_code(const Params& p, const void* keys, const void* values, int64_t batch, int64_t dim, cudaStream_t stream) {
   const bool one = p.block_heads <= 8;
   if (dim == 64)
-    return one ? launch_mask<Code, 64, 1>(p, keys, values, batch, stream) : launch_mask<Code, 64, 2>(p, keys, values, batch, stream);
+    return one ? launch_mask<T, Code, 64, 1>(p, keys, values, batch, stream) : launch_mask<T, Code, 64, 2>(p, keys, values, batch, stream);
   if (dim == 128)
-    return one ? launch_mask<Code, 128, 1>(p, keys, values, batch, stream) : launch_mask<Code, 128, 2>(p, keys, values, batch, stream);
-  return launch_mask<Code, 256, 1>(p, keys, values, batch, stream);
+    return one ? launch_mask<T, Code, 128, 1>(p, keys, values, batch, stream) : launch_mask<T, Code, 128, 2>(p, keys, values, batch, stream);
+  return launch_mask<T, Code, 256, 1>(p, keys, values, batch, stream);
 }
 
-int launch_int8(const Params& p, const void* keys, const void* values, int64_t batch, int64_t dim, cudaStream_t stream);
-int launch_e4m3(const Params& p, const void* keys, const void* values, int64_t batch, int64_t dim, cudaStream_t stream);
+// instances, in a file each
+int launch_int8_bf16(const Params& p, const void* keys, const void* values, int64_t batch, int64_t dim, cudaStream_t stream);
+int launch_int8_f16(const Params& p, const void* keys, const void* values, int64_t batch, int64_t dim, cudaStream_t stream);
+int launch_e4m3_bf16(const Params& p, const void* keys, const void* values, int64_t batch, int64_t dim, cudaStream_t stream);
+int launch_e4m3_f16(const Params& p, const void* keys, const void* values, int64_t batch, int64_t dim, cudaStream_t stream);
 
 }  // namespace cache_attention
 }  // namespace b200

@@ -67,12 +67,15 @@ class Cache:
 def attention(query, keys, values, table, lengths, mask, scale):
     """(result, bound on the kernels' distance from it): B x Hq x 1 x D.
 
-    The bound, with A = sum p|v| / sum p and u = 2^-24: the result's own rounding; a probability rounded to 11 bits, or to
-    2^-25 of the largest where that is coarser (times 16: block scales up to 16 apart share an accumulator); scores from
-    products of D terms in 32 bits, each off by at most (D + 4) u of the sum of magnitudes, which moves a probability by
-    that much and its normalisation by as much again; sums of `length` terms; an exponential good to 2^-21."""
+    The bound, with A = sum p|v| / sum p and u = 2^-24: the result's own rounding; a probability rounded to fp16 (2^-11 of
+    it; 2^-22 for fp16 results, where two numbers hold it), or to 2^-25 of the largest where that is coarser (times 16: block
+    scales up to 16 apart share an accumulator); scores from products of D terms in 32 bits, each off by at most (D + 4) u of
+    the sum of magnitudes, and by 2^-25 of the query's largest times the keys' sum (its smallest elements in fp16), which
+    moves a probability by that much and its normalisation by as much again; sums of `length` terms; an exponential good to
+    2^-21."""
     query = query.cpu()
     half = HALF_STEP[query.dtype]
+    probability = 2.0 ** -11 if query.dtype == torch.bfloat16 else 2.0 ** -22
     q = query.double()
     batch, heads, _, dim = q.shape
     out, bound = torch.empty_like(q), torch.empty_like(q)
@@ -84,7 +87,7 @@ def attention(query, keys, values, table, lengths, mask, scale):
         for h in range(heads):
             kk, vv = k[h // group], v[h // group]
             scores = kk @ q[b, h, 0] * scale
-            slack = (dim + 4) * u * (kk.abs() @ q[b, h, 0].abs()) * scale
+            slack = ((dim + 4) * u * (kk.abs() @ q[b, h, 0].abs()) + 2.0 ** -25 * q[b, h, 0].abs().max() * kk.abs().sum(1)) * scale
             if mask is not None:
                 extra = mask[b, 0, 0, :length].double()
                 scores = scores + extra
@@ -95,7 +98,7 @@ def attention(query, keys, values, table, lengths, mask, scale):
             largest = vv.abs().max() if length else 0.0
             off = 2 * slack.nan_to_num(0.0, 0.0, 0.0).max() if length else 0.0
             peak = p.max() if length else 0.0
-            bound[b, h, 0] = half * out[b, h, 0].abs() + a * (2.0 ** -11 + 2.0 ** -21 + 2 * u * length + off) + \
+            bound[b, h, 0] = half * out[b, h, 0].abs() + a * (probability + 2.0 ** -21 + 2 * u * length + off) + \
                 16 * 2.0 ** -25 * length * largest * peak + 1e-30
     return out, bound
 

@@ -43,8 +43,11 @@ def test_attention_refusals():
         _lib.ERR_UNSUPPORTED
     assert attention(pool=ODD) == _lib.ERR_ALIGNMENT
     assert attention(batch=70000) == attention(blocks=1 << 31) == _lib.ERR_TOO_LARGE
-    need = _lib.load().b200_paged_decode_attention_8bit_workspace_bytes(1, 4, 2, 64, 64, 32)
-    assert need > 0 and attention(split=32) == attention(split=32, workspace=FAKE, nbytes=need - 1) == _lib.ERR_WORKSPACE
+    # sixteen splits of 128 tokens: more than a cluster, with partials in a workspace
+    need = _lib.load().b200_paged_decode_attention_8bit_workspace_bytes(1, 4, 2, 64, 2048, 128)
+    split = dict(columns=64, mask_len=2048, split=128)
+    assert need > 0 and attention(**split) == attention(**split, workspace=FAKE, nbytes=need - 1) == _lib.ERR_WORKSPACE
+    assert _lib.load().b200_paged_decode_attention_8bit_workspace_bytes(1, 4, 2, 64, 2048, 1024) == 0
     assert attention(batch=0) == 0
 
 

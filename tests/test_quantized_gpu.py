@@ -9,7 +9,7 @@ import torch
 
 import llm_compiler_b200 as b200
 import quantized_helpers as ref
-from llm_compiler_b200 import kernels
+from llm_compiler_b200 import _lib, kernels
 from llm_compiler_b200.kv_state import ExecutionError, PagedKVCacheState, QuantizedPagedKVCacheState
 
 pytestmark = pytest.mark.gpu
@@ -341,6 +341,77 @@ def test_attention_is_the_same_from_run_to_run_on_streams_and_in_replayed_graphs
                 graphs[i].replay()
     torch.cuda.synchronize()
     assert all(torch.equal(outputs[i], want[i]) for i in range(2))
+
+
+def test_wrappers_refuse_what_does_not_fit():
+    state = make_state(torch.int8)
+    cache = (state.keys[0], state.values[0], state.key_scales[0], state.value_scales[0], state.block_table)
+    rows = torch.zeros(4, 2, 1, 64, dtype=torch.bfloat16, device="cuda")
+    at = state.positions(0)
+    wrong = lambda i, t: tuple(t if j == i else c for j, c in enumerate(cache))
+    for arguments in ((*cache, rows.float(), rows.float(), at), (*cache, rows, rows[:, :1], at), (*cache, rows[:, :1], rows[:, :1], at),
+                      (*cache, rows, rows, at.int()), (*cache, rows, rows, at[:2]), (*cache, rows, rows.half(), at),
+                      (*wrong(0, cache[0].float()), rows, rows, at), (*wrong(2, cache[2].half()), rows, rows, at),
+                      (*wrong(2, cache[2][:, :1]), rows, rows, at), (*wrong(4, cache[4].long()), rows, rows, at),
+                      (*wrong(4, cache[4][:2]), rows, rows, at), (*cache, rows.cpu(), rows, at)):
+        with pytest.raises(ValueError):
+            b200.b200_paged_kv_store_8bit(*arguments)
+    query = torch.zeros(4, 4, 1, 64, dtype=torch.bfloat16, device="cuda")
+    lengths = state.lengths[0]
+    for arguments in ((query.float(), *cache, lengths, None), (query[:, :3], *cache, lengths, None), (query[:2], *cache, lengths, None),
+                      (query.expand(4, 4, 2, 64), *cache, lengths, None), (query, *cache, lengths.int(), None),
+                      (query, *cache, lengths, torch.zeros(4, 1, 1, 257, device="cuda")),
+                      (query, *cache, lengths, torch.zeros(4, 1, 2, 9, device="cuda"))):
+        with pytest.raises(ValueError):
+            b200.b200_paged_decode_attention_8bit(*arguments, scale=1.0)
+    for pools, sources, destinations in (([], [0], [1]), ([at], [0], [1]), (state._pools, [0], [24]), (state._pools, [0], [-1]),
+                                         (state._pools, [0, 1], [2, 2]), (state._pools, [0, 1], [1, 2]), (state._pools, [0], [1, 2]),
+                                         (state._pools, torch.tensor([0], device="cuda"), [1]),
+                                         ([state._pools[0], state._pools[1][:1]], [0], [1])):
+        with pytest.raises(ValueError):
+            b200.b200_copy_kv_blocks(pools, sources, destinations)
+    x, w = torch.zeros(2, 64, device="cuda"), torch.zeros(64, device="cuda")
+    for call in (lambda: b200.b200_rms_norm_int8(x, w.half(), epsilon=1e-6), lambda: b200.b200_rms_norm_int8(x, w[:5], epsilon=1e-6),
+                 lambda: b200.b200_rms_norm_int8(x, None, epsilon=1e-6), lambda: b200.b200_rms_norm_int8(x, w, epsilon=1e-6, residual=x[:1]),
+                 lambda: b200.b200_quantize_rows_int8(x.to(torch.int32))):
+        with pytest.raises(ValueError):
+            call()
+    v, vs = b200.b200_quantize_rows_int8(x)
+    for arguments, options in (((v, vs, v.float(), vs), {}), ((v, vs[:1], v, vs), {}), ((v[:, :40], vs, v[:, :40], vs), {}),
+                               ((v, vs, v, vs, w[:2].half()), {}), ((v, vs, v, vs), dict(epilogue="gelu")),
+                               ((v, vs, v, vs), dict(epilogue="residual")), ((v, vs, v, vs), dict(residual=x)),
+                               ((v, vs, v[:1], vs[:1]), dict(epilogue="swiglu")), ((v, vs, v, vs), dict(out_dtype=torch.int8)),
+                               ((v[:, :24].contiguous(), vs, v[:, :24].contiguous(), vs), {})):
+        with pytest.raises(ValueError):
+            b200.b200_linear_int8(*arguments, **options)
+
+
+def test_waits_that_run_out_set_the_status_and_leave_the_next_calls_right():
+    """Kernels whose copies never come: every wait gives up, the status says so, and the same calls are right afterwards."""
+    g = torch.Generator().manual_seed(17)
+    table, blocks = scattered(g, 2, 8)
+    pools, scales = make_cache(g, torch.int8, blocks, 2, 64, 64)
+    query, lengths = torch.randn(2, 4, 1, 64, generator=g).bfloat16().cuda(), torch.tensor([500, 100]).cuda()
+    cases = [lambda s=s: b200.b200_paged_decode_attention_8bit(query, *pools, *scales, table.cuda(), lengths, None, scale=0.125,
+                                                               split_tokens=s) for s in (0, 40, 512)]
+    for m, k, n in ((8, 256, 512), (8, 1024, 128), (300, 512, 512)):
+        values, weight = (torch.randint(-127, 128, (r, k), generator=g, dtype=torch.int8).cuda() for r in (m, n))
+        cases.append(lambda a=(values, torch.rand(m, generator=g).cuda(), weight, torch.rand(n, generator=g).cuda()):
+                     b200.b200_linear_int8(*a))
+    want = [case() for case in cases]
+    kernels.runtime().check_status()
+    library = _lib.load()
+    for case, right in zip(cases, want):
+        library.b200_debug_set_waits(2000, 1)
+        try:
+            case()
+            torch.cuda.synchronize()
+        finally:
+            library.b200_debug_set_waits(4000000, 0)
+        with pytest.raises(kernels.KernelStatusError, match="wait gave up"):
+            kernels.runtime().check_status()
+        assert torch.equal(case(), right)
+        kernels.runtime().check_status()
 
 
 def test_calls_without_rows_launch_nothing():
