@@ -47,6 +47,10 @@ quantized_store_kernel(const StoreParams p) {
     if (threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0) atomicOr(p.status, B200_STATUS_BAD_POSITION);
     return;
   }
+  if (position >= p.max_blocks * p.block_size) {
+    if (threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0) atomicOr(p.status, B200_STATUS_KV_OVERFLOW);
+    return;
+  }
   const int64_t column = position / p.block_size + blockIdx.x;
   const int64_t first = position > column * p.block_size ? position : column * p.block_size;
   const int64_t end = min(position + p.tokens, (column + 1) * p.block_size);

@@ -28,8 +28,8 @@ from typing import Dict, Optional
 
 import torch
 
-from . import kernels
-from .kv_state import ExecutionError, PagedKVCacheState, PreallocatedKVCacheState
+from . import kernels, quantized_kernels
+from .kv_state import ExecutionError, PagedKVCacheState, PreallocatedKVCacheState, QuantizedPagedKVCacheState
 from .qwen2 import Qwen2Config, inverse_frequency
 
 
@@ -148,11 +148,15 @@ class Qwen2Engine(ServingEngine):
     def __init__(self, config: Qwen2Config, weights: Dict[str, torch.Tensor], *, batch: int,
                  capacity: int, numerical_mode: str = "fast",
                  device: Optional[torch.device] = None, kv_layout: str = "contiguous",
-                 block_size: int = 128, num_blocks: Optional[int] = None) -> None:
+                 block_size: int = 128, num_blocks: Optional[int] = None,
+                 kv_dtype: Optional[torch.dtype] = None) -> None:
         """kv_layout "paged": K / V live in block pools of `num_blocks` blocks of `block_size`
         tokens per layer (default: as many as the contiguous layout would hold) behind one block
         table; `capacity` is then the longest context one sequence may reach. Blocks are handed
-        out on the host, ahead of the steps that need them."""
+        out on the host, ahead of the steps that need them.
+
+        kv_dtype torch.int8 or torch.float8_e4m3fn (paged layout, bf16 and fp16 weights): the cache in
+        8 bits with a scale for each block and KV head, half the bytes that a step reads of it."""
 
         if numerical_mode not in ("fast", "pytorch_compatible"):
             raise ValueError(f"unknown numerical mode {numerical_mode!r}")
@@ -183,15 +187,19 @@ class Qwen2Engine(ServingEngine):
 
         layers = config.num_layers
         self.paged = kv_layout == "paged"
+        self.quantized = kv_dtype is not None
+        if self.quantized and (not self.paged or self.dtype == torch.float32 or
+                               kv_dtype not in quantized_kernels.CACHE_CODES):
+            raise ValueError("a cache in 8 bits (int8 or float8_e4m3fn) needs the paged layout and 16-bit weights")
         # length arena rows: [0, L) per-slot lengths, L = positions, L + 1 = attention lengths
         if self.paged:
-            if self.dtype != torch.bfloat16:
+            if self.dtype != torch.bfloat16 and not self.quantized:
                 raise ValueError("the paged KV layout holds bf16")
             blocks = num_blocks if num_blocks is not None else batch * -(-capacity // block_size)
-            self.state = PagedKVCacheState.allocate_paged(
+            self.state = (QuantizedPagedKVCacheState if self.quantized else PagedKVCacheState).allocate_paged(
                 num_layers=layers, batch=batch, max_tokens=capacity, block_size=block_size,
                 num_blocks=blocks, kv_heads=config.num_kv_heads, head_dim=config.head_dim,
-                dtype=self.dtype, device=self.device, extra_length_rows=2)
+                dtype=kv_dtype or self.dtype, device=self.device, extra_length_rows=2)
             self.capacity = capacity = self.state.capacity  # whole blocks
         else:
             self.state = PreallocatedKVCacheState.allocate(
@@ -283,11 +291,14 @@ class Qwen2Engine(ServingEngine):
         # nothing to hide between launches of 100 us, and waiting CTAs of the next one cost them 1 %: 4 x 4096 tokens of
         # the 0.5B model, some 3000 of the 7B.)
         chained = self.programmatic_launch and batch * tokens * cfg.hidden_size <= 4 << 20
-        with kernels.launch_mode(programmatic=chained, constant_weights=chained, keep_variants=True):
-            x = kernels.b200_qwen2_prompt_layers(
-                x, self.layers, self.state.keys, self.state.values, cosine, sine, self.positions,  # all zero right now
-                q_heads=cfg.num_heads, scale=self.scale, epsilon=cfg.rms_norm_eps, numerical_mode=self.mode,
-                block_table=self.state.block_table if self.paged else None)
+        if self.quantized:
+            x = self._quantized_prompt_layers(x, cosine, sine)
+        else:
+            with kernels.launch_mode(programmatic=chained, constant_weights=chained, keep_variants=True):
+                x = kernels.b200_qwen2_prompt_layers(
+                    x, self.layers, self.state.keys, self.state.values, cosine, sine, self.positions,  # all zero right now
+                    q_heads=cfg.num_heads, scale=self.scale, epsilon=cfg.rms_norm_eps, numerical_mode=self.mode,
+                    block_table=self.state.block_table if self.paged else None)
         if all_logits:
             h = kernels.b200_rms_norm(x, self.final_norm, epsilon=cfg.rms_norm_eps,
                                       round_before_weight=True, numerical_mode=self.mode)
@@ -305,6 +316,29 @@ class Qwen2Engine(ServingEngine):
         kernels.b200_advance_lengths(self.attention_lengths, 1, self.capacity + 1)
         self.logits = last
         return logits
+
+    def _quantized_prompt_layers(self, x: torch.Tensor, cosine: torch.Tensor, sine: torch.Tensor) -> torch.Tensor:
+        """The prompt's layers with a cache in 8 bits: a prompt attends to its own keys and values in 16 bits, and they
+        are quantised on their way into the cache."""
+
+        cfg = self.config
+        batch, tokens, _ = x.shape
+        sizes = [cfg.q_size, cfg.kv_size, cfg.kv_size]
+        for index, layer in enumerate(self.layers):
+            h = kernels.b200_rms_norm(x, layer["input_norm"], epsilon=cfg.rms_norm_eps, round_before_weight=True,
+                                      numerical_mode=self.mode)
+            qkv = kernels.b200_linear(h, layer["qkv_w"], layer["qkv_b"])
+            q, k, v = (part.view(batch, tokens, -1, cfg.head_dim).transpose(1, 2) for part in qkv.split(sizes, dim=2))
+            q, k = kernels.b200_rope(q, k, cosine, sine)
+            self.state.store(index, k, v, self.positions)  # (all zero right now)
+            attn = kernels.b200_prefill_attention(q, k, v, None, scale=self.scale, causal=True, numerical_mode=self.mode)
+            x = kernels.b200_linear(attn.transpose(1, 2).reshape(batch, tokens, cfg.q_size), layer["o_w"], residual=x,
+                                    epilogue="residual")
+            h = kernels.b200_rms_norm(x, layer["post_norm"], epsilon=cfg.rms_norm_eps, round_before_weight=True,
+                                      numerical_mode=self.mode)
+            a = kernels.b200_linear(h, layer["gate_up_w"], epilogue="swiglu")
+            x = kernels.b200_linear(a, layer["down_w"], residual=x, epilogue="residual")
+        return x
 
     def load_context(self, lengths: torch.Tensor, *, next_ids: Optional[torch.Tensor] = None) -> None:
         """Benchmark entry: declares that the KV buffers already hold `lengths[b]` tokens per
@@ -363,7 +397,7 @@ class Qwen2Engine(ServingEngine):
         """Whether a decode step runs the launch chain (fast bf16, up to 128 sequences)."""
         # (the paged layout has the folded five-launch chain and the separate kernels)
         return self.dtype == torch.bfloat16 and self.mode == "fast" and self.batch <= 128 and \
-            (not self.paged or self.folded_norms)
+            (not self.paged or self.folded_norms) and not self.quantized
 
     @property
     def attention_is_fused(self) -> bool:
@@ -374,9 +408,9 @@ class Qwen2Engine(ServingEngine):
     def _decode_step(self) -> None:
         if self.chained:
             self._decode_step_chain()
-        elif self.dtype == torch.bfloat16:
+        elif self.dtype == torch.bfloat16 and not self.quantized:
             self._decode_step_separate()
-        else:  # (fp32, fp16: the norms, RoPE, attention and projections of few rows wait on the device)
+        else:  # (fp32, fp16, a cache in 8 bits: the norms, RoPE, attention and projections of few rows wait on the device)
             with kernels.launch_mode(programmatic=self.programmatic_launch, constant_weights=self.programmatic_launch,
                                      keep_variants=True):
                 self._decode_step_separate()
@@ -506,7 +540,14 @@ class Qwen2Engine(ServingEngine):
             q = qkv[:, :q_size].view(batch, cfg.num_heads, cfg.head_dim)
             k = qkv[:, q_size:q_size + kv_size].view(batch, cfg.num_kv_heads, cfg.head_dim)
             v = qkv[:, q_size + kv_size:].view(batch, cfg.num_kv_heads, cfg.head_dim)
-            if self.paged:
+            if self.quantized:
+                q, k = kernels.b200_rope(q.unsqueeze(2), k.unsqueeze(2), cosine, sine)
+                state = self.state
+                state.store(index, k, v.unsqueeze(2), self.positions)
+                attn = quantized_kernels.b200_paged_decode_attention_8bit(
+                    q, state.keys[index], state.values[index], state.key_scales[index], state.value_scales[index],
+                    state.block_table, self.attention_lengths, None, scale=self.scale, max_length_hint=self.max_length_hint)
+            elif self.paged:
                 q, k = kernels.b200_rope(q.unsqueeze(2), k.unsqueeze(2), cosine, sine)
                 kernels.b200_paged_kv_store(self.state.keys[index], self.state.values[index],
                                             self.state.block_table, k, v.unsqueeze(2), self.positions)

@@ -10,6 +10,8 @@ import torch
 import llm_compiler_b200 as b200
 import quantized_helpers as ref
 from llm_compiler_b200 import _lib, kernels
+from llm_compiler_b200 import qwen2 as q2
+from llm_compiler_b200.engine import Qwen2Engine
 from llm_compiler_b200.kv_state import ExecutionError, PagedKVCacheState, QuantizedPagedKVCacheState
 
 pytestmark = pytest.mark.gpu
@@ -124,7 +126,8 @@ def test_store_skips_what_has_no_place_and_says_so():
     (keys, values), (key_scales, value_scales) = make_cache(g, torch.int8, blocks, heads, size, dim)
     cached = ref.Cache(keys, key_scales)
     x = torch.randn(4, heads, 40, dim, generator=g).half()
-    for positions, match in (([0, 0, 0, 0], "negative KV position"), ([30, -1, 0, 30], "beyond capacity")):
+    for positions, match in (([0, 0, 0, 0], "negative KV position"), ([30, -1, 0, 30], "beyond capacity"),
+                             ([0, -1, 0, 2 ** 62], "beyond capacity"), ([0, -(2 ** 62), 0, 64], "beyond capacity")):
         positions = torch.tensor(positions)
         cached.store(table, x, positions)
         b200.b200_paged_kv_store_8bit(keys, values, key_scales, value_scales, table.cuda(), x.cuda(), x.cuda(), positions.cuda())
@@ -713,3 +716,45 @@ def test_a_layer_in_8_bits_step_by_step():
         x = project("down", *b200.b200_quantize_rows_int8(gated), residual=x, epilogue="residual")
         assert bool(x.isfinite().all())
     state.check()
+
+
+@pytest.mark.parametrize("weights_dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("cache", CACHES)
+def test_an_engine_serves_from_a_cache_in_8_bits(cache, weights_dtype):
+    """The prompt's cache is the definition's of the keys and values that the 16-bit engine caches; a captured step gives the
+    launched one's tokens; attention over the quantised prompt keeps the logits near the 16-bit engine's."""
+    config = q2.Qwen2Config(hidden_size=256, intermediate_size=512, num_layers=2, num_heads=4, num_kv_heads=2, rms_norm_eps=1e-6,
+                            rope_theta=1e6, vocab_size=512, tie_word_embeddings=True)
+    weights = {k: v.cuda() for k, v in q2.make_weights(config, seed=1, dtype=weights_dtype).items()}
+    prompt = q2.make_prompt_ids(config, 3, 77, seed=2)
+    make = lambda **options: Qwen2Engine(config, weights, batch=3, capacity=160, **options)
+    plain = make()
+    engine, other = (make(kv_layout="paged", block_size=32, kv_dtype=cache) for _ in range(2))
+    assert isinstance(engine.state, QuantizedPagedKVCacheState) and engine.state.keys[0].dtype == cache
+    empty = [ref.Cache(engine.state.keys[0], engine.state.key_scales[0]), ref.Cache(engine.state.values[0], engine.state.value_scales[0])]
+    wide, logits = plain.prefill(prompt), engine.prefill(prompt)
+    assert torch.equal(logits, wide)  # (a prompt attends in 16 bits)
+    # layer 0, whose inputs are the same whatever the launches: what the 16-bit engine caches, quantised
+    table = engine.state.block_table.cpu()
+    for cached, buffer, pool, scales in zip(empty, (plain.state.keys[0], plain.state.values[0]),
+                                            (engine.state.keys[0], engine.state.values[0]),
+                                            (engine.state.key_scales[0], engine.state.value_scales[0])):
+        cached.store(table, buffer[:, :77].transpose(1, 2), torch.zeros(3, dtype=torch.int64))
+        assert torch.equal(scales.cpu().double(), cached.scales) and same_codes(pool, cached)
+    tokens = engine.generate(prompt, 40)            # captured
+    assert torch.equal(other.generate(prompt, 40, use_graph=False), tokens)
+    for b in range(3):  # (the blocks themselves lie elsewhere: one engine has given its own back and taken new ones)
+        for mine, theirs in zip(engine.state.gather(1, b, 116), other.state.gather(1, b, 116)):
+            assert torch.equal(mine, theirs)
+    engine.state.check()
+    # one step behind the prompt: scores and values off by at most half a code each of their block's largest
+    engine.prefill(prompt)
+    plain.prefill(prompt)
+    plain.decode_step(feed_back=False)
+    engine.decode_step(feed_back=False)
+    off = (engine.logits.float() - plain.logits.float()).norm() / plain.logits.float().norm()
+    assert float(off) < (0.05 if cache == torch.int8 else 0.2)
+    with pytest.raises(ValueError, match="8 bits"):
+        make(kv_dtype=cache)
+    with pytest.raises(ValueError, match="8 bits"):
+        make(kv_layout="paged", kv_dtype=torch.int16)
