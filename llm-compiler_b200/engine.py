@@ -24,7 +24,7 @@ from __future__ import annotations
 
 import math
 import os
-from typing import Dict, Optional
+from typing import Callable, Dict, Optional
 
 import torch
 
@@ -149,14 +149,19 @@ class Qwen2Engine(ServingEngine):
                  capacity: int, numerical_mode: str = "fast",
                  device: Optional[torch.device] = None, kv_layout: str = "contiguous",
                  block_size: int = 128, num_blocks: Optional[int] = None,
-                 kv_dtype: Optional[torch.dtype] = None) -> None:
+                 kv_dtype: Optional[torch.dtype] = None,
+                 weight_dtype: Optional[torch.dtype] = None) -> None:
         """kv_layout "paged": K / V live in block pools of `num_blocks` blocks of `block_size`
         tokens per layer (default: as many as the contiguous layout would hold) behind one block
         table; `capacity` is then the longest context one sequence may reach. Blocks are handed
         out on the host, ahead of the steps that need them.
 
         kv_dtype torch.int8 or torch.float8_e4m3fn (paged layout, bf16 and fp16 weights): the cache in
-        8 bits with a scale for each block and KV head, half the bytes that a step reads of it."""
+        8 bits with a scale for each block and KV head, half the bytes that a step reads of it.
+
+        weight_dtype torch.int8 (bf16 and fp16 weights): the layers' projections in 8-bit integers, weights
+        with a scale per output column, rows of activations with a scale each; norms, attention, the
+        embedding and the LM head stay in 16 bits."""
 
         if numerical_mode not in ("fast", "pytorch_compatible"):
             raise ValueError(f"unknown numerical mode {numerical_mode!r}")
@@ -168,6 +173,10 @@ class Qwen2Engine(ServingEngine):
         self.mode = numerical_mode
         self.dtype = weights["embed_tokens.weight"].dtype
         self.scale = config.head_dim ** -0.5
+        self.int8_weights = weight_dtype is not None
+        if self.int8_weights and (weight_dtype != torch.int8 or self.dtype == torch.float32 or any(
+                size % 16 for size in (config.hidden_size, config.intermediate_size, config.q_size))):
+            raise ValueError("8-bit projections (int8) need 16-bit weights and sizes that are multiples of 16")
         # the five-launch decode layer (RMSNorm folded into q|k|v and gate|up, cluster split-K
         # o / down with the residual inside): bf16, fast mode, up to 128 rows while the layer's
         # largest matrix, gate|up, keeps its launch a chain of latencies, 64 rows for large models
@@ -175,7 +184,7 @@ class Qwen2Engine(ServingEngine):
         # the seven-launch layer with reduce consumers.
         gate_up_bytes = 2 * config.intermediate_size * config.hidden_size * 2
         chain_rows = int(os.environ.get("B200_CHAIN_ROWS", "0")) or kernels.decode_chain_rows(gate_up_bytes)
-        self.folded_norms = (self.dtype == torch.bfloat16 and numerical_mode == "fast" and
+        self.folded_norms = (self.dtype == torch.bfloat16 and numerical_mode == "fast" and not self.int8_weights and
                              batch <= chain_rows and
                              config.hidden_size % 8 == 0 and
                              os.environ.get("B200_DECODE_CHAIN", "folded") != "partials")
@@ -256,6 +265,9 @@ class Qwen2Engine(ServingEngine):
                 "gate_up_w": gate_up,
                 "down_w": weights[p + "mlp.down_proj.weight"],
             }
+            if self.int8_weights:  # codes and scales in the place of the 16-bit matrices
+                for name in ("qkv_w", "o_w", "gate_up_w", "down_w"):
+                    layer[name] = quantized_kernels.b200_quantize_rows_int8(layer[name])
             if self.folded_norms:
                 # the norm weights multiplied into the columns of the projections behind them
                 layer["qkv_w_folded"] = kernels.b200_scale_columns(qkv_w, layer["input_norm"])
@@ -291,8 +303,8 @@ class Qwen2Engine(ServingEngine):
         # nothing to hide between launches of 100 us, and waiting CTAs of the next one cost them 1 %: 4 x 4096 tokens of
         # the 0.5B model, some 3000 of the 7B.)
         chained = self.programmatic_launch and batch * tokens * cfg.hidden_size <= 4 << 20
-        if self.quantized:
-            x = self._quantized_prompt_layers(x, cosine, sine)
+        if self.quantized or self.int8_weights:
+            x = self._prompt_layers(x, cosine, sine)
         else:
             with kernels.launch_mode(programmatic=chained, constant_weights=chained, keep_variants=True):
                 x = kernels.b200_qwen2_prompt_layers(
@@ -317,28 +329,42 @@ class Qwen2Engine(ServingEngine):
         self.logits = last
         return logits
 
-    def _quantized_prompt_layers(self, x: torch.Tensor, cosine: torch.Tensor, sine: torch.Tensor) -> torch.Tensor:
-        """The prompt's layers with a cache in 8 bits: a prompt attends to its own keys and values in 16 bits, and they
-        are quantised on their way into the cache."""
+    def _prompt_layers(self, x: torch.Tensor, cosine: torch.Tensor, sine: torch.Tensor) -> torch.Tensor:
+        """The prompt's layers one operator at a time, for caches and projections in 8 bits: a prompt attends to its own
+        keys and values in 16 bits, a cache in 8 bits quantises them on their way in."""
 
         cfg = self.config
         batch, tokens, _ = x.shape
         sizes = [cfg.q_size, cfg.kv_size, cfg.kv_size]
+        norm = dict(epsilon=cfg.rms_norm_eps, round_before_weight=True, numerical_mode=self.mode)
         for index, layer in enumerate(self.layers):
-            h = kernels.b200_rms_norm(x, layer["input_norm"], epsilon=cfg.rms_norm_eps, round_before_weight=True,
-                                      numerical_mode=self.mode)
-            qkv = kernels.b200_linear(h, layer["qkv_w"], layer["qkv_b"])
-            q, k, v = (part.view(batch, tokens, -1, cfg.head_dim).transpose(1, 2) for part in qkv.split(sizes, dim=2))
-            q, k = kernels.b200_rope(q, k, cosine, sine)
-            self.state.store(index, k, v, self.positions)  # (all zero right now)
-            attn = kernels.b200_prefill_attention(q, k, v, None, scale=self.scale, causal=True, numerical_mode=self.mode)
-            x = kernels.b200_linear(attn.transpose(1, 2).reshape(batch, tokens, cfg.q_size), layer["o_w"], residual=x,
-                                    epilogue="residual")
-            h = kernels.b200_rms_norm(x, layer["post_norm"], epsilon=cfg.rms_norm_eps, round_before_weight=True,
-                                      numerical_mode=self.mode)
-            a = kernels.b200_linear(h, layer["gate_up_w"], epilogue="swiglu")
+            def attend(qkv: torch.Tensor) -> torch.Tensor:
+                q, k, v = (part.view(batch, tokens, -1, cfg.head_dim).transpose(1, 2) for part in qkv.split(sizes, dim=2))
+                q, k = kernels.b200_rope(q, k, cosine, sine)
+                self.state.store(index, k, v, self.positions)  # (all zero right now)
+                attn = kernels.b200_prefill_attention(q, k, v, None, scale=self.scale, causal=True, numerical_mode=self.mode)
+                return attn.transpose(1, 2).reshape(batch, tokens, cfg.q_size)
+
+            if self.int8_weights:
+                x = self._int8_layer(x, layer, attend)
+                continue
+            attn = attend(kernels.b200_linear(kernels.b200_rms_norm(x, layer["input_norm"], **norm), layer["qkv_w"], layer["qkv_b"]))
+            x = kernels.b200_linear(attn, layer["o_w"], residual=x, epilogue="residual")
+            a = kernels.b200_linear(kernels.b200_rms_norm(x, layer["post_norm"], **norm), layer["gate_up_w"], epilogue="swiglu")
             x = kernels.b200_linear(a, layer["down_w"], residual=x, epilogue="residual")
         return x
+
+    def _int8_layer(self, x: torch.Tensor, layer: dict, attend: Callable[[torch.Tensor], torch.Tensor]) -> torch.Tensor:
+        """A layer whose projections run in 8-bit integers, around `attend` (q|k|v in, attention out)."""
+
+        epsilon, out = self.config.rms_norm_eps, dict(out_dtype=self.dtype)
+        q8 = quantized_kernels
+        codes, scales, _ = q8.b200_rms_norm_int8(x, layer["input_norm"], epsilon=epsilon)
+        attn = attend(q8.b200_linear_int8(codes, scales, *layer["qkv_w"], layer["qkv_b"], **out))
+        x = q8.b200_linear_int8(*q8.b200_quantize_rows_int8(attn), *layer["o_w"], residual=x, epilogue="residual", **out)
+        codes, scales, _ = q8.b200_rms_norm_int8(x, layer["post_norm"], epsilon=epsilon)
+        a = q8.b200_linear_int8(codes, scales, *layer["gate_up_w"], epilogue="swiglu", **out)
+        return q8.b200_linear_int8(*q8.b200_quantize_rows_int8(a), *layer["down_w"], residual=x, epilogue="residual", **out)
 
     def load_context(self, lengths: torch.Tensor, *, next_ids: Optional[torch.Tensor] = None) -> None:
         """Benchmark entry: declares that the KV buffers already hold `lengths[b]` tokens per
@@ -397,7 +423,7 @@ class Qwen2Engine(ServingEngine):
         """Whether a decode step runs the launch chain (fast bf16, up to 128 sequences)."""
         # (the paged layout has the folded five-launch chain and the separate kernels)
         return self.dtype == torch.bfloat16 and self.mode == "fast" and self.batch <= 128 and \
-            (not self.paged or self.folded_norms) and not self.quantized
+            (not self.paged or self.folded_norms) and not self.quantized and not self.int8_weights
 
     @property
     def attention_is_fused(self) -> bool:
@@ -408,9 +434,9 @@ class Qwen2Engine(ServingEngine):
     def _decode_step(self) -> None:
         if self.chained:
             self._decode_step_chain()
-        elif self.dtype == torch.bfloat16 and not self.quantized:
+        elif self.dtype == torch.bfloat16 and not self.quantized and not self.int8_weights:
             self._decode_step_separate()
-        else:  # (fp32, fp16, a cache in 8 bits: the norms, RoPE, attention and projections of few rows wait on the device)
+        else:  # (fp32, fp16, 8 bits: the norms, RoPE, attention and projections of few rows wait on the device)
             with kernels.launch_mode(programmatic=self.programmatic_launch, constant_weights=self.programmatic_launch,
                                      keep_variants=True):
                 self._decode_step_separate()
@@ -512,6 +538,39 @@ class Qwen2Engine(ServingEngine):
         kernels.b200_advance_lengths(self.state._length_arena, 1, self.capacity + 1)
         self.kernels_per_step = kernels.launch_count(self.device) - before
 
+    def _attend_step(self, index: int, qkv: torch.Tensor, cosine: torch.Tensor, sine: torch.Tensor) -> torch.Tensor:
+        """RoPE, the store of the new token and attention of one layer, B x Hq x 1 x D."""
+
+        cfg, batch = self.config, self.batch
+        q_size, kv_size = cfg.q_size, cfg.kv_size
+        q = qkv[:, :q_size].view(batch, cfg.num_heads, cfg.head_dim)
+        k = qkv[:, q_size:q_size + kv_size].view(batch, cfg.num_kv_heads, cfg.head_dim)
+        v = qkv[:, q_size + kv_size:].view(batch, cfg.num_kv_heads, cfg.head_dim)
+        if self.quantized:
+            q, k = kernels.b200_rope(q.unsqueeze(2), k.unsqueeze(2), cosine, sine)
+            state = self.state
+            state.store(index, k, v.unsqueeze(2), self.positions)
+            attn = quantized_kernels.b200_paged_decode_attention_8bit(
+                q, state.keys[index], state.values[index], state.key_scales[index], state.value_scales[index],
+                state.block_table, self.attention_lengths, None, scale=self.scale, max_length_hint=self.max_length_hint)
+        elif self.paged:
+            q, k = kernels.b200_rope(q.unsqueeze(2), k.unsqueeze(2), cosine, sine)
+            kernels.b200_paged_kv_store(self.state.keys[index], self.state.values[index],
+                                        self.state.block_table, k, v.unsqueeze(2), self.positions)
+            attn = kernels.b200_paged_decode_attention(
+                q, self.state.keys[index], self.state.values[index], self.state.block_table,
+                self.attention_lengths, None, scale=self.scale, numerical_mode=self.mode,
+                split_tokens=self.split_tokens, max_length_hint=self.max_length_hint)
+        else:
+            q = kernels.b200_rope_kv_store(q, k, v, cosine, sine, self.state.keys[index],
+                                           self.state.values[index], self.positions)
+            attn = kernels.b200_decode_attention(
+                q, self.state.keys[index], self.state.values[index], self.attention_lengths,
+                None, scale=self.scale, numerical_mode=self.mode,
+                split_tokens=self.split_tokens, max_length_hint=self.max_length_hint,
+                sequence_order=self.sequence_order)
+        return attn
+
     def _decode_step_separate(self) -> None:
         cfg = self.config
         batch = self.batch
@@ -519,7 +578,7 @@ class Qwen2Engine(ServingEngine):
         x = kernels.b200_embedding(self.embed, self.input_ids)
         cosine, sine = kernels.b200_rope_table(self.positions.view(batch, 1), self.inv_freq,
                                                self.dtype)
-        q_size, kv_size = cfg.q_size, cfg.kv_size
+        q_size = cfg.q_size
 
         def normed_linear(x, norm_weight, weight, bias=None, epilogue="none"):
             """The norm and the projection behind it: one launch for a few fp32 rows where that pays, else two."""
@@ -536,33 +595,11 @@ class Qwen2Engine(ServingEngine):
             return y
 
         for index, layer in enumerate(self.layers):
+            if self.int8_weights:
+                x = self._int8_layer(x, layer, lambda qkv: self._attend_step(index, qkv, cosine, sine).view(batch, q_size))
+                continue
             qkv = normed_linear(x, layer["input_norm"], layer["qkv_w"], layer["qkv_b"])
-            q = qkv[:, :q_size].view(batch, cfg.num_heads, cfg.head_dim)
-            k = qkv[:, q_size:q_size + kv_size].view(batch, cfg.num_kv_heads, cfg.head_dim)
-            v = qkv[:, q_size + kv_size:].view(batch, cfg.num_kv_heads, cfg.head_dim)
-            if self.quantized:
-                q, k = kernels.b200_rope(q.unsqueeze(2), k.unsqueeze(2), cosine, sine)
-                state = self.state
-                state.store(index, k, v.unsqueeze(2), self.positions)
-                attn = quantized_kernels.b200_paged_decode_attention_8bit(
-                    q, state.keys[index], state.values[index], state.key_scales[index], state.value_scales[index],
-                    state.block_table, self.attention_lengths, None, scale=self.scale, max_length_hint=self.max_length_hint)
-            elif self.paged:
-                q, k = kernels.b200_rope(q.unsqueeze(2), k.unsqueeze(2), cosine, sine)
-                kernels.b200_paged_kv_store(self.state.keys[index], self.state.values[index],
-                                            self.state.block_table, k, v.unsqueeze(2), self.positions)
-                attn = kernels.b200_paged_decode_attention(
-                    q, self.state.keys[index], self.state.values[index], self.state.block_table,
-                    self.attention_lengths, None, scale=self.scale, numerical_mode=self.mode,
-                    split_tokens=self.split_tokens, max_length_hint=self.max_length_hint)
-            else:
-                q = kernels.b200_rope_kv_store(q, k, v, cosine, sine, self.state.keys[index],
-                                               self.state.values[index], self.positions)
-                attn = kernels.b200_decode_attention(
-                    q, self.state.keys[index], self.state.values[index], self.attention_lengths,
-                    None, scale=self.scale, numerical_mode=self.mode,
-                    split_tokens=self.split_tokens, max_length_hint=self.max_length_hint,
-                    sequence_order=self.sequence_order)
+            attn = self._attend_step(index, qkv, cosine, sine)
             # o and down have few N tiles: at up to 256 bf16 rows they run as cluster split-K
             # projections that add the residual themselves (same rounding points)
             splitk = self.dtype == torch.bfloat16 and batch <= 256 and cfg.hidden_size % 4 == 0

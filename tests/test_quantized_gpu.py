@@ -758,3 +758,28 @@ def test_an_engine_serves_from_a_cache_in_8_bits(cache, weights_dtype):
         make(kv_dtype=cache)
     with pytest.raises(ValueError, match="8 bits"):
         make(kv_layout="paged", kv_dtype=torch.int16)
+
+
+@pytest.mark.parametrize("layout", [{}, dict(kv_layout="paged", block_size=32), dict(kv_layout="paged", block_size=32, kv_dtype=torch.int8)])
+@pytest.mark.parametrize("weights_dtype", [torch.bfloat16, torch.float16])
+def test_an_engine_projects_in_8_bit_integers(layout, weights_dtype):
+    """It runs on every layout, captured as launched, and its logits stay near the 16-bit engine's: weights and rows are
+    each off by at most half a code of their row's largest, a few tenths of a percent of the sums."""
+    config = q2.Qwen2Config(hidden_size=256, intermediate_size=512, num_layers=2, num_heads=4, num_kv_heads=2, rms_norm_eps=1e-6,
+                            rope_theta=1e6, vocab_size=512, tie_word_embeddings=True)
+    if weights_dtype == torch.float16 and layout and "kv_dtype" not in layout:
+        pytest.skip("the 16-bit paged layout holds bf16")
+    weights = {k: v.cuda() for k, v in q2.make_weights(config, seed=1, dtype=weights_dtype).items()}
+    prompt = q2.make_prompt_ids(config, 3, 77, seed=2)
+    make = lambda **options: Qwen2Engine(config, weights, batch=3, capacity=160, **layout, **options)
+    plain, engine, other = make(), make(weight_dtype=torch.int8), make(weight_dtype=torch.int8)
+    assert engine.layers[0]["o_w"][0].dtype == torch.int8
+    assert torch.equal(engine.generate(prompt, 30), other.generate(prompt, 30, use_graph=False))
+    wide, logits = plain.prefill(prompt).float(), engine.prefill(prompt).float()
+    assert float((logits - wide).norm() / wide.norm()) < 0.1
+    plain.decode_step(feed_back=False)
+    engine.decode_step(feed_back=False)
+    assert float((engine.logits.float() - plain.logits.float()).norm() / plain.logits.float().norm()) < 0.1
+    engine.state.check()
+    with pytest.raises(ValueError, match="8-bit projections"):
+        make(weight_dtype=torch.int16)
