@@ -17,7 +17,7 @@ Plan plan_of(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim, int6
   plan.head_blocks = ceil_div(group, dim == 256 ? 8 : 16);
   plan.block_heads = ceil_div(group, plan.head_blocks);
   const int64_t items = batch * kv_heads * plan.head_blocks;
-  const int64_t slots = static_cast<int64_t>(kNumSMs) * (dim == 64 ? 4 : dim == 128 ? 3 : 1);
+  const int64_t slots = static_cast<int64_t>(kNumSMs) * (dim == 256 ? 1 : dim == 64 && plan.block_heads <= 8 ? 4 : 3);
   if (split_tokens > 0) {
     plan.splits = ceil_div(longest, split_tokens);
   } else {
