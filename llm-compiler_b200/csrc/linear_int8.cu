@@ -16,6 +16,7 @@
 //   (at 128 x 256 a CTA they are what limits it: 96 of 128 bytes a cycle in, as many out). Two accumulators alternate, so
 //   the epilogue of a tile runs under the products of the next.
 #include <algorithm>
+#include <type_traits>
 
 #include "quantized.cuh"
 #include "tcgen05.cuh"
@@ -212,6 +213,19 @@ linear_int8_stream_kernel(const Int8LinearParams p, const __grid_constant__ CUte
     int done = 0;
     for (int tile = tile_first; tile < tiles; tile += tile_step, ++done) {
       const int acc = done & 1;
+      // a thread owns a column; 16 rows at a time: all operands before all stores, which the compiler may not swap, and
+      // what comes from memory before the wait for the products or beside the rows in front
+      const int col = tile * 128 + warp * 32 + lane;
+      const bool there = col < p.n && p.slices == 1;
+      const float w_scale = there ? p.w_scales[col] : 0.0f;
+      const float bias = there && p.bias != nullptr ? Elem<T>::load(static_cast<const T*>(p.bias) + col) : 0.0f;
+      float other[16];
+      auto fetch = [&](int r0) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          other[r] = there && r0 + r < p.m ? Elem<T>::load(residual + (r0 + r) * out_cols + col) : 0.0f;
+      };
+      if (residual != nullptr) fetch(0);
       ok = __all_sync(0xffffffffu, mbarrier_wait_bounded(smem_u32(&acc_full[acc]), (done >> 1) & 1, p.wait_limit));
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -228,33 +242,21 @@ linear_int8_stream_kernel(const Int8LinearParams p, const __grid_constant__ CUte
         }
         break;
       }
-      // a thread owns a column; 16 rows at a time: all operands before all stores, which the compiler may not swap
-      const int col = tile * 128 + warp * 32 + lane;
-      const bool there = col < p.n;
-      const float w_scale = there ? p.w_scales[col] : 0.0f;
-      const float bias = there && p.bias != nullptr ? Elem<T>::load(static_cast<const T*>(p.bias) + col) : 0.0f;
       const bool writes = there && !(swiglu && (lane & 1) != 0);
       T* to = out + (swiglu ? col / 2 : col);
 #pragma unroll 1
       for (int r0 = 0; r0 < p.m; r0 += 16) {
         float v[16];
+        tmem_load_32x32(t_addr + r0, v);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) v[r] = static_cast<float>(__float_as_int(v[r])) * scales[r0 + r] * w_scale + bias;
         if (residual != nullptr) {
-          float other[16];
 #pragma unroll
-          for (int r = 0; r < 16; ++r)
-            other[r] = there && r0 + r < p.m ? Elem<T>::load(residual + (r0 + r) * out_cols + col) : 0.0f;
-          tmem_load_32x32(t_addr + r0, v);
+          for (int r = 0; r < 16; ++r) v[r] += other[r];
+          if (r0 + 16 < p.m) fetch(r0 + 16);
+        } else if (swiglu) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r)
-            v[r] = static_cast<float>(__float_as_int(v[r])) * scales[r0 + r] * w_scale + bias + other[r];
-        } else {
-          tmem_load_32x32(t_addr + r0, v);
-#pragma unroll
-          for (int r = 0; r < 16; ++r) v[r] = static_cast<float>(__float_as_int(v[r])) * scales[r0 + r] * w_scale + bias;
-          if (swiglu) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) v[r] = silu_times(v[r], __shfl_xor_sync(0xffffffffu, v[r], 1));
-          }
+          for (int r = 0; r < 16; ++r) v[r] = silu_times(v[r], __shfl_xor_sync(0xffffffffu, v[r], 1));
         }
         if (writes) {
           T* at = to + r0 * out_cols;
@@ -330,7 +332,8 @@ constexpr int pair_smem() {
   return pair_stages<T>() * kPairStageBytes + kPairWarps * (32 * 32 * static_cast<int>(sizeof(T)) + 4 * 32 * 8);
 }
 
-template <typename T>
+// Piece: what a lane moves of a row at a time, 16 bytes or, where rows of y do not start on multiples of that, 4 or 2.
+template <typename T, typename Piece>
 __global__ void __launch_bounds__(kPairThreads, 1)
 linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtensorMap x_map,
                         const __grid_constant__ CUtensorMap w_map) {
@@ -429,14 +432,14 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
   } else if (warp < kPairWarps) {
     // ---- epilogue: this CTA's 128 rows; lanes 32 (warp % 4) .., every other chunk of 32 columns ----
     // Everything that comes from memory (scales, bias, the first residual chunk) is asked for before the wait for the
-    // products. A chunk leaves through a staging tile, so that a store writes whole rows of it and a residual is read so.
+    // products. A chunk leaves through a staging tile, so that a store writes whole rows of it and a residual is read so, in
+    // pieces of 16 bytes where rows allow it and of 4 or 2 where their length does not (2008 x 512 x 3890: 110 us with a thread
+    // for each row).
     const bool swiglu = p.epilogue == B200_EPILOGUE_SWIGLU;
     const int out_cols = swiglu ? p.n / 2 : p.n;
     T* out = static_cast<T*>(p.out);
     const T* residual = static_cast<const T*>(p.residual);
     constexpr int kVec = 16 / static_cast<int>(sizeof(T)), kUnits = 32 / kVec;  // of 16 bytes: a row of a chunk
-    const bool staged = (out_cols * static_cast<int>(sizeof(T))) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0 &&
-                        (residual == nullptr || (reinterpret_cast<uintptr_t>(residual) & 15u) == 0);
     const int quarter = warp & 3, turn0 = warp >> 2;
     constexpr int kStageTile = 32 * 32 * static_cast<int>(sizeof(T));
     const uint32_t stage_tile = smem_base + kPairStages * kPairStageBytes + warp * kStageTile;
@@ -445,6 +448,16 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
     // 16-byte unit `unit` of row r of a chunk with `units` of them: 128 bytes of rows side by side never share a bank
     auto unit_at = [&](int r, int unit, int units) {
       return stage_tile + r * units * 16 + ((unit ^ ((r * units >> 3) & (units - 1))) << 4);
+    };
+    // use(i, address in the staging tile, row, element of the row) of this lane's i-th piece of a chunk: pieces side by side
+    // over the lanes, whole rows one after another
+    auto each_piece = [&](auto units_tag, auto&& use) {
+      constexpr int kBytes = sizeof(Piece), units = decltype(units_tag)::value, kEach = units * 16 / kBytes;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int at = i * 32 + lane, r = at / kEach, byte = at % kEach * kBytes;
+        use(i, unit_at(r, byte >> 4, units) + (byte & 15), r, byte / static_cast<int>(sizeof(T)));
+      }
     };
     bool ok = true;
     int done = 0;
@@ -461,16 +474,22 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
             col < n_end ? p.w_scales[col] : 0.0f,
             col < n_end && p.bias != nullptr ? Elem<T>::load(static_cast<const T*>(p.bias) + col) : 0.0f);
       }
-      uint4 ahead[kUnits];  // the next chunk's residual: rows side by side over the lanes
+      constexpr int kWords = sizeof(Piece) < 4 ? 1 : sizeof(Piece) / 4;
+      uint32_t ahead[kUnits * 16 / sizeof(Piece) * kWords];  // the next chunk's residual
       auto fetch = [&](int c0) {
-        if (residual == nullptr || !staged || tile_n * bn + c0 + 32 > n_end) return;
-#pragma unroll
-        for (int i = 0; i < kUnits; ++i) {
-          const int r = (i * 32 + lane) / kUnits, unit = (i * 32 + lane) % kUnits;
-          ahead[i] = row0 + r < p.m ? *reinterpret_cast<const uint4*>(residual + static_cast<int64_t>(row0 + r) * p.n +
-                                                                      tile_n * bn + c0 + unit * kVec)
-                                    : make_uint4(0u, 0u, 0u, 0u);
-        }
+        const int col0 = tile_n * bn + c0;
+        if (residual == nullptr || col0 >= n_end) return;
+        const T* from = residual + static_cast<int64_t>(row0) * p.n + col0;
+        each_piece(std::integral_constant<int, kUnits>{}, [&](int i, uint32_t, int r, int element) {
+          Piece value = {};
+          if (row0 + r < p.m && col0 + element < n_end)
+            value = *reinterpret_cast<const Piece*>(from + static_cast<int64_t>(r) * p.n + element);
+          if constexpr (sizeof(Piece) == 16) {
+            ahead[4 * i] = value.x; ahead[4 * i + 1] = value.y; ahead[4 * i + 2] = value.z; ahead[4 * i + 3] = value.w;
+          } else {
+            ahead[i] = value;
+          }
+        });
       };
       fetch(turn0 * 32);
       ok = ok && __all_sync(0xffffffffu, mbarrier_wait_bounded(smem_u32(&acc_full[acc]), (done >> 1) & 1, p.wait_limit));
@@ -495,22 +514,30 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
           v[2 * i] = fmaf(static_cast<float>(__float_as_int(v[2 * i])) * row_scale, t.x, t.y);
           v[2 * i + 1] = fmaf(static_cast<float>(__float_as_int(v[2 * i + 1])) * row_scale, t.z, t.w);
         }
-        if (!staged || col0 + 32 > n_end) {
-          if (row < p.m) {
-            const int64_t at = static_cast<int64_t>(row) * out_cols + (swiglu ? col0 / 2 : col0);
-            if (swiglu) {
-#pragma unroll
-              for (int i = 0; i < 16; ++i)
-                if (col0 + 2 * i < n_end) Elem<T>::store(out + at + i, silu_times(v[2 * i], v[2 * i + 1]));
-            } else {
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (col0 + i < n_end) Elem<T>::store(out + at + i, v[i] + (residual ? Elem<T>::load(residual + at + i) : 0.0f));
-            }
-          }
-          continue;
-        }
         __syncwarp();  // the chunk before has been read
+        // the staged rows to y: `width` columns of them exist
+        auto rows_out = [&](auto units_tag, T* to, int width) {
+          Piece values[decltype(units_tag)::value * 16 / sizeof(Piece)];
+          each_piece(units_tag, [&](int i, uint32_t from, int, int) {
+            Piece& value = values[i];
+            if constexpr (sizeof(Piece) == 16)
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(value.x), "=r"(value.y), "=r"(value.z), "=r"(value.w) : "r"(from));
+            else if constexpr (sizeof(Piece) == 4)
+              asm volatile("ld.shared.b32 %0, [%1];" : "=r"(value) : "r"(from));
+            else
+              asm volatile("ld.shared.u16 %0, [%1];" : "=h"(value) : "r"(from));
+          });
+          if (row0 + 32 <= p.m && col0 + 32 <= n_end) {  // (a chunk that lies in y needs no questions)
+            each_piece(units_tag, [&](int i, uint32_t, int r, int element) {
+              *reinterpret_cast<Piece*>(to + static_cast<int64_t>(r) * out_cols + element) = values[i];
+            });
+          } else {
+            each_piece(units_tag, [&](int i, uint32_t, int r, int element) {
+              if (row0 + r < p.m && element < width)
+                *reinterpret_cast<Piece*>(to + static_cast<int64_t>(r) * out_cols + element) = values[i];
+            });
+          }
+        };
         if (swiglu) {
           constexpr int kHalf = kUnits / 2;
 #pragma unroll
@@ -524,22 +551,19 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
                          "r"(packed.z), "r"(packed.w) : "memory");
           }
           __syncwarp();
-#pragma unroll
-          for (int i = 0; i < kHalf; ++i) {
-            const int r = (i * 32 + lane) / kHalf, unit = (i * 32 + lane) % kHalf;
-            uint4 value;
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(value.x), "=r"(value.y), "=r"(value.z), "=r"(value.w)
-                         : "r"(unit_at(r, unit, kHalf)));
-            if (row0 + r < p.m)
-              *reinterpret_cast<uint4*>(out + static_cast<int64_t>(row0 + r) * out_cols + col0 / 2 + unit * kVec) = value;
-          }
+          rows_out(std::integral_constant<int, kHalf>{}, out + static_cast<int64_t>(row0) * out_cols + col0 / 2, (n_end - col0) / 2);
           continue;
         }
         if (residual != nullptr) {
-#pragma unroll
-          for (int i = 0; i < kUnits; ++i)
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(unit_at((i * 32 + lane) / kUnits, (i * 32 + lane) % kUnits, kUnits)),
-                         "r"(ahead[i].x), "r"(ahead[i].y), "r"(ahead[i].z), "r"(ahead[i].w) : "memory");
+          each_piece(std::integral_constant<int, kUnits>{}, [&](int i, uint32_t to, int, int) {
+            if constexpr (sizeof(Piece) == 16)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(ahead[4 * i]), "r"(ahead[4 * i + 1]),
+                           "r"(ahead[4 * i + 2]), "r"(ahead[4 * i + 3]) : "memory");
+            else if constexpr (sizeof(Piece) == 4)
+              asm volatile("st.shared.b32 [%0], %1;" ::"r"(to), "r"(ahead[i]) : "memory");
+            else
+              asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"(static_cast<uint16_t>(ahead[i])) : "memory");
+          });
           if (c0 + 64 < bn) fetch(c0 + 64);
           __syncwarp();
         }
@@ -562,15 +586,7 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
                        "r"(packed.z), "r"(packed.w) : "memory");
         }
         __syncwarp();
-#pragma unroll
-        for (int i = 0; i < kUnits; ++i) {
-          const int r = (i * 32 + lane) / kUnits, unit = (i * 32 + lane) % kUnits;
-          uint4 value;
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(value.x), "=r"(value.y), "=r"(value.z), "=r"(value.w)
-                       : "r"(unit_at(r, unit, kUnits)));
-          if (row0 + r < p.m)
-            *reinterpret_cast<uint4*>(out + static_cast<int64_t>(row0 + r) * out_cols + col0 + unit * kVec) = value;
-        }
+        rows_out(std::integral_constant<int, kUnits>{}, out + static_cast<int64_t>(row0) * out_cols + col0, n_end - col0);
       }
       tmem_load_wait(raw);  // (of a chunk beyond n, if there is one)
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -638,12 +654,22 @@ int launch_pair(Int8LinearParams p, const void* x, const void* w, cudaStream_t s
   if (!make_code_map(&x_map, x, p.m, p.k, 128) || !make_code_map(&w_map, w, p.n, p.k, p.cols / 2)) return B200_ERR_UNSUPPORTED;
   const int64_t tiles = tiles_m * ceil_div(p.n, p.cols);
   const unsigned pairs = static_cast<unsigned>(std::min<int64_t>(kPairs, tiles));
-  auto kernel = linear_int8_pair_kernel<T>;
-  static_assert(tensor_memory_fits(512, pair_smem<T>()) && pair_smem<T>() + 1024 <= 227 * 1024, "tensor memory under programmatic launches");
-  static std::atomic<uint64_t> allowed{0};
-  if (!allow_shared_memory(kernel, pair_smem<T>(), allowed)) return B200_ERR_LAUNCH;
-  return launch_chained_cluster(kernel, dim3(2 * pairs), dim3(kPairThreads), pair_smem<T>(), stream, 2u, p, x_map, w_map) == cudaSuccess
-             ? launch_status() : B200_ERR_LAUNCH;
+  // what every row of y and of the residual starts on a multiple of
+  const uint64_t starts = static_cast<uint64_t>(p.epilogue == B200_EPILOGUE_SWIGLU ? p.n / 2 : p.n) * sizeof(T) |
+                          reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.residual);
+  const auto launch = [&](auto piece) {
+    auto kernel = linear_int8_pair_kernel<T, decltype(piece)>;
+    static_assert(tensor_memory_fits(512, pair_smem<T>()) && pair_smem<T>() + 1024 <= 227 * 1024, "tensor memory under programmatic launches");
+    static std::atomic<uint64_t> allowed{0};
+    if (!allow_shared_memory(kernel, pair_smem<T>(), allowed)) return B200_ERR_LAUNCH;
+    return launch_chained_cluster(kernel, dim3(2 * pairs), dim3(kPairThreads), pair_smem<T>(), stream, 2u, p, x_map, w_map) ==
+                   cudaSuccess ? launch_status() : B200_ERR_LAUNCH;
+  };
+  if (starts % 16 == 0) return launch(uint4{});
+  if constexpr (sizeof(T) == 2) {
+    if (starts % 4 != 0) return launch(uint16_t{});
+  }
+  return launch(uint32_t{});
 }
 
 }  // namespace
