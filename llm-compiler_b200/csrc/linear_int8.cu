@@ -8,7 +8,8 @@
 //
 // linear_int8_stream_kernel, up to 256 rows (decode, short prompts): bound by the read of the weight. The WEIGHT's columns
 //   lie along the product's M (128 of them a tile) and all rows of x along its N, so every weight byte is read once and no
-//   row of x is padded beyond the next multiple of 16. A CTA per SM takes whole tiles in turn; where there are fewer tiles
+//   row of x is padded beyond the next multiple of 16. (More rows against a narrow weight go in chunks of up to 256, where
+//   that keeps more SMs busy than the other kernel's tiles.) A CTA per SM takes whole tiles in turn; where there are fewer tiles
 //   than SMs, the K slices of a tile are the CTAs of a cluster, which add their sums through distributed shared memory
 //   (4.0 us less than integer additions in global memory at 64 x 384 x 512, where the slices then wait for one another there).
 // linear_int8_pair_kernel, beyond: bound by the tensor cores. Two SMs work on one tile of 256 rows x up to 256 columns
@@ -131,6 +132,7 @@ linear_int8_stream_kernel(const Int8LinearParams p, const __grid_constant__ CUte
   const int rank = p.slices > 1 ? cluster_cta_rank() : 0;
   const int kb_first = all_kb * rank / p.slices, nkb = all_kb * (rank + 1) / p.slices - kb_first;  // this slice: two at least
   const int tile_first = blockIdx.x / p.slices, tile_step = gridDim.x / p.slices;
+  const int row_first = blockIdx.y * p.cols, rows = min(p.cols, p.m - row_first);  // this CTA's chunk of x
 
   if (threadIdx.x == 0) {
     failed = 0;
@@ -158,8 +160,8 @@ linear_int8_stream_kernel(const Int8LinearParams p, const __grid_constant__ CUte
   grid_dependency_wait();
   const bool swiglu = p.epilogue == B200_EPILOGUE_SWIGLU;
   const int64_t out_cols = swiglu ? p.n / 2 : p.n;
-  T* out = static_cast<T*>(p.out);
-  const T* residual = static_cast<const T*>(p.residual);
+  T* out = static_cast<T*>(p.out) + row_first * out_cols;
+  const T* residual = p.residual ? static_cast<const T*>(p.residual) + row_first * out_cols : nullptr;
 
   if (warp == kEpilogueWarps && !p.drop_loads) {
     // ---- producer: the ring runs on across tile ends ----
@@ -177,7 +179,7 @@ linear_int8_stream_kernel(const Int8LinearParams p, const __grid_constant__ CUte
         const uint32_t bar = smem_u32(&full[s]), dst = smem_base + s * stage_bytes;
         mbarrier_arrive_expect_tx_if(leader, bar, stage_bytes);
         tma_load_2d_if(leader, dst, &w_map, bar, (kb_first + kb) * kBK, tile * 128);
-        tma_load_2d_if(leader, dst + 128 * 128, &x_map, bar, (kb_first + kb) * kBK, 0);
+        tma_load_2d_if(leader, dst + 128 * 128, &x_map, bar, (kb_first + kb) * kBK, row_first);
         if (++s == stages) { s = 0; ++turn; }
       }
   } else if (warp == kEpilogueWarps + 1) {
@@ -207,7 +209,7 @@ linear_int8_stream_kernel(const Int8LinearParams p, const __grid_constant__ CUte
     if (!ok) failed = 1;
   } else if (warp < kEpilogueWarps) {
     // ---- epilogue: lanes of the accumulator are columns of y, its columns are rows ----
-    for (int r = threadIdx.x; r < p.cols; r += kEpilogueWarps * 32) scales[r] = r < p.m ? p.x_scales[r] : 0.0f;
+    for (int r = threadIdx.x; r < p.cols; r += kEpilogueWarps * 32) scales[r] = r < rows ? p.x_scales[row_first + r] : 0.0f;
     asm volatile("bar.sync 1, 128;" ::: "memory");
     bool ok = true;
     int done = 0;
@@ -219,13 +221,20 @@ linear_int8_stream_kernel(const Int8LinearParams p, const __grid_constant__ CUte
       const bool there = col < p.n && p.slices == 1;
       const float w_scale = there ? p.w_scales[col] : 0.0f;
       const float bias = there && p.bias != nullptr ? Elem<T>::load(static_cast<const T*>(p.bias) + col) : 0.0f;
-      float other[16];
-      auto fetch = [&](int r0) {
+      float near[16], far[16];  // the residual of the next 16 rows and of those behind them
+      auto fetch = [&](int r0, float (&other)[16]) {
+        if (residual == nullptr || !there) return;
+        const T* from = residual + r0 * out_cols + col;
+        if (r0 + 16 <= rows) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          other[r] = there && r0 + r < p.m ? Elem<T>::load(residual + (r0 + r) * out_cols + col) : 0.0f;
+          for (int r = 0; r < 16; ++r) other[r] = Elem<T>::load(from + r * out_cols);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) other[r] = r0 + r < rows ? Elem<T>::load(from + r * out_cols) : 0.0f;
+        }
       };
-      if (residual != nullptr) fetch(0);
+      fetch(0, near);
+      fetch(16, far);
       ok = __all_sync(0xffffffffu, mbarrier_wait_bounded(smem_u32(&acc_full[acc]), (done >> 1) & 1, p.wait_limit));
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -233,7 +242,7 @@ linear_int8_stream_kernel(const Int8LinearParams p, const __grid_constant__ CUte
       if (p.slices > 1) {
         // (one tile a CTA: every stage has been read, the sums take the ring's place: [row][128])
 #pragma unroll 1
-        for (int r0 = 0; r0 < p.m; r0 += 16) {
+        for (int r0 = 0; r0 < rows; r0 += 16) {
           float v[16];
           tmem_load_32x32(t_addr + r0, v);
           const uint32_t to = smem_base + r0 * 512 + (warp * 32 + lane) * 4;
@@ -244,8 +253,7 @@ linear_int8_stream_kernel(const Int8LinearParams p, const __grid_constant__ CUte
       }
       const bool writes = there && !(swiglu && (lane & 1) != 0);
       T* to = out + (swiglu ? col / 2 : col);
-#pragma unroll 1
-      for (int r0 = 0; r0 < p.m; r0 += 16) {
+      auto sixteen = [&](int r0, float (&other)[16]) {
         float v[16];
         tmem_load_32x32(t_addr + r0, v);
 #pragma unroll
@@ -253,17 +261,27 @@ linear_int8_stream_kernel(const Int8LinearParams p, const __grid_constant__ CUte
         if (residual != nullptr) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) v[r] += other[r];
-          if (r0 + 16 < p.m) fetch(r0 + 16);
+          if (r0 + 32 < rows) fetch(r0 + 32, other);
         } else if (swiglu) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) v[r] = silu_times(v[r], __shfl_xor_sync(0xffffffffu, v[r], 1));
         }
         if (writes) {
           T* at = to + r0 * out_cols;
+          if (r0 + 16 <= rows) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (r0 + r < p.m) Elem<T>::store(at + r * out_cols, v[r]);
+            for (int r = 0; r < 16; ++r) Elem<T>::store(at + r * out_cols, v[r]);
+          } else {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (r0 + r < rows) Elem<T>::store(at + r * out_cols, v[r]);
+          }
         }
+      };
+#pragma unroll 1
+      for (int r0 = 0; r0 < rows; r0 += 32) {
+        sixteen(r0, near);
+        if (r0 + 16 < rows) sixteen(r0 + 16, far);
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
@@ -275,22 +293,28 @@ linear_int8_stream_kernel(const Int8LinearParams p, const __grid_constant__ CUte
   if (p.slices > 1) {
     // ---- the slices' sums: this CTA finishes rows rank, rank + slices, ...; a lane takes four columns ----
     cluster_sync();
-    const int col = tile_first * 128 + 4 * lane;
+    const int col = tile_first * 128 + 4 * lane, width = min(p.n - col, 4);
     float w_scale[4], bias[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      w_scale[c] = col + c < p.n ? p.w_scales[col + c] : 0.0f;
-      bias[c] = col + c < p.n && p.bias != nullptr ? Elem<T>::load(static_cast<const T*>(p.bias) + col + c) : 0.0f;
+      w_scale[c] = c < width ? p.w_scales[col + c] : 0.0f;
+      bias[c] = c < width && p.bias != nullptr ? Elem<T>::load(static_cast<const T*>(p.bias) + col + c) : 0.0f;
     }
-    for (int row = rank + warp * p.slices; row < p.m; row += kThreads / 32 * p.slices) {
+    for (int row = rank + warp * p.slices; row < rows; row += kThreads / 32 * p.slices) {
       int4 part[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         part[i] = i < p.slices ? load_cluster_i32x4(map_to_rank(smem_base + row * 512 + lane * 16, i)) : make_int4(0, 0, 0, 0);
-      float y[4];
+      float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (residual != nullptr) {
+        const T* from = residual + row * out_cols + col;
+        if (width == 4) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-        y[c] = residual != nullptr && col + c < p.n ? Elem<T>::load(residual + row * out_cols + col + c) : 0.0f;
+          for (int c = 0; c < 4; ++c) y[c] = Elem<T>::load(from + c);
+        } else {
+          for (int c = 0; c < width; ++c) y[c] = Elem<T>::load(from + c);
+        }
+      }
 #pragma unroll
       for (int i = 1; i < 8; ++i) {
         part[0].x += part[i].x; part[0].y += part[i].y; part[0].z += part[i].z; part[0].w += part[i].w;
@@ -300,13 +324,15 @@ linear_int8_stream_kernel(const Int8LinearParams p, const __grid_constant__ CUte
       y[1] += static_cast<float>(part[0].y) * scale * w_scale[1] + bias[1];
       y[2] += static_cast<float>(part[0].z) * scale * w_scale[2] + bias[2];
       y[3] += static_cast<float>(part[0].w) * scale * w_scale[3] + bias[3];
+      T* to = out + row * out_cols + (swiglu ? col / 2 : col);
       if (swiglu) {
-        if (col < p.n) Elem<T>::store(out + row * out_cols + col / 2, silu_times(y[0], y[1]));
-        if (col + 2 < p.n) Elem<T>::store(out + row * out_cols + col / 2 + 1, silu_times(y[2], y[3]));
-      } else {
+        if (width > 0) Elem<T>::store(to, silu_times(y[0], y[1]));
+        if (width > 2) Elem<T>::store(to + 1, silu_times(y[2], y[3]));
+      } else if (width == 4) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-          if (col + c < p.n) Elem<T>::store(out + row * out_cols + col + c, y[c]);
+        for (int c = 0; c < 4; ++c) Elem<T>::store(to + c, y[c]);
+      } else {
+        for (int c = 0; c < width; ++c) Elem<T>::store(to + c, y[c]);
       }
     }
     __syncwarp();
@@ -618,42 +644,68 @@ bool make_code_map(CUtensorMap* map, const void* base, int64_t rows, int64_t k, 
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int stream_rows(int64_t m) { return static_cast<int>(ceil_div(m, 16) * 16); }
+// What either kernel takes, to a few microseconds, from what was measured: a k-block of the stream kernel 0.2 us and 0.42
+// more at 256 rows, its epilogue 2.5 us at 256 rows (256 x 18944 x 3584: 27.9 us in 112 CTAs of 37 k-blocks; 256 x 512 x 18944:
+// 8.4 in 4); of the pair kernel 0.26 us at 128 columns and 0.35 at 256 (257 x 18944 x 3584: 41.8 us in one round of 148
+// k-blocks; 1407 x 3488 x 25: 10.6 in 28), an epilogue of 3.3 us a tile beside the products of the next.
+struct StreamPlan { int cols, chunks, slices; double us; };
+StreamPlan plan_stream(int64_t m, int64_t k, int64_t n) {
+  const int64_t tiles = ceil_div(n, 128), blocks = ceil_div(k, kBK);
+  StreamPlan best = {0, 0, 0, 1e30};
+  for (int64_t chunks = ceil_div(m, kRowsAtMost); chunks <= std::max<int64_t>(16, ceil_div(m, kRowsAtMost)); ++chunks) {
+    const int64_t cols = ceil_div(ceil_div(m, chunks), 16) * 16, units = tiles * ceil_div(m, cols);
+    // slices of K that fill the GPU where the tiles do not: clusters of 2, 4 or 8, two k-blocks a slice at least
+    int64_t slices = 1;
+    while (slices < 8 && units * slices * 2 <= kNumSMs && blocks >= slices * 4) slices *= 2;
+    const double share = cols / 256.0;
+    const double us = 4.0 + ceil_div(units * slices, kNumSMs) * (ceil_div(blocks, slices) * (0.2 + 0.42 * share) + 2.5 * share);
+    if (us < 0.9 * best.us) best = {static_cast<int>(cols), static_cast<int>(ceil_div(m, cols)), static_cast<int>(slices), us};
+  }
+  return best;
+}
+struct PairPlan { int cols; double us; };
+PairPlan plan_pair(int64_t m, int64_t k, int64_t n) {
+  // columns of a tile: the fewest column-steps over all rounds of the GPU's pairs
+  const int64_t tiles_m = ceil_div(m, 256), blocks = ceil_div(k, kBK);
+  int64_t best = INT64_MAX;
+  PairPlan plan = {0, 0.0};
+  for (int bn = 256; bn >= 128; bn -= 32) {
+    const int64_t rounds = ceil_div(tiles_m * ceil_div(n, bn), kNumSMs / 2);
+    if (rounds * bn >= best) continue;
+    best = rounds * bn;
+    const double tile = blocks * 0.26 * (256 + bn) / 384;
+    plan = {bn, 3.5 + std::max(tile, 2.0) + (rounds - 1) * std::max(tile, 3.3)};
+  }
+  return plan;
+}
 
 template <typename T>
-int launch_stream(Int8LinearParams p, const void* x, const void* w, cudaStream_t stream) {
-  p.cols = stream_rows(p.m);
+int launch_stream(Int8LinearParams p, const StreamPlan& plan, const void* x, const void* w, cudaStream_t stream) {
+  p.cols = plan.cols;
+  p.slices = plan.slices;
   p.stages = std::min(10, kRingBytes / ((128 + p.cols) * 128));
   CUtensorMap w_map, x_map;
   if (!make_code_map(&w_map, w, p.n, p.k, 128) || !make_code_map(&x_map, x, p.m, p.k, p.cols)) return B200_ERR_UNSUPPORTED;
-  // slices of K that fill the GPU where the tiles do not: clusters of 2, 4 or 8, two k-blocks a slice at least
-  const int64_t tiles = ceil_div(p.n, 128), blocks = ceil_div(p.k, kBK);
-  p.slices = 1;
-  while (p.slices < 8 && tiles * p.slices * 2 <= kNumSMs && blocks >= p.slices * 4) p.slices *= 2;
-  const unsigned ctas = static_cast<unsigned>(p.slices > 1 ? tiles * p.slices : std::min<int64_t>(kNumSMs, tiles));
+  const int64_t tiles = ceil_div(p.n, 128);
+  // (whole tiles in turn: chunks side by side share the SMs)
+  const int64_t across = std::max<int64_t>(1, kNumSMs / plan.chunks);
+  const dim3 grid(static_cast<unsigned>(p.slices > 1 ? tiles * p.slices : std::min(across, tiles)), static_cast<unsigned>(plan.chunks));
   auto kernel = linear_int8_stream_kernel<T>;
   static_assert(tensor_memory_fits(512, kRingBytes), "tensor memory under programmatic launches");
   static std::atomic<uint64_t> allowed{0};
   if (!allow_shared_memory(kernel, kRingBytes, allowed)) return B200_ERR_LAUNCH;
-  return launch_chained_cluster(kernel, dim3(ctas), dim3(kThreads), kRingBytes, stream, static_cast<unsigned>(p.slices), p,
+  return launch_chained_cluster(kernel, grid, dim3(kThreads), kRingBytes, stream, static_cast<unsigned>(p.slices), p,
                                 w_map, x_map) == cudaSuccess ? launch_status() : B200_ERR_LAUNCH;
 }
 
 template <typename T>
-int launch_pair(Int8LinearParams p, const void* x, const void* w, cudaStream_t stream) {
-  // columns of a tile: the fewest column-steps over all rounds of the GPU's pairs
-  const int64_t tiles_m = ceil_div(p.m, 256);
-  constexpr int kPairs = kNumSMs / 2;
-  int64_t best = INT64_MAX;
-  for (int bn = 256; bn >= 128; bn -= 32) {
-    const int64_t cost = ceil_div(tiles_m * ceil_div(p.n, bn), kPairs) * bn;
-    if (cost < best) { best = cost; p.cols = bn; }
-  }
+int launch_pair(Int8LinearParams p, const PairPlan& plan, const void* x, const void* w, cudaStream_t stream) {
+  p.cols = plan.cols;
   p.n_fastest = p.n <= p.m;
   CUtensorMap x_map, w_map;
   if (!make_code_map(&x_map, x, p.m, p.k, 128) || !make_code_map(&w_map, w, p.n, p.k, p.cols / 2)) return B200_ERR_UNSUPPORTED;
-  const int64_t tiles = tiles_m * ceil_div(p.n, p.cols);
-  const unsigned pairs = static_cast<unsigned>(std::min<int64_t>(kPairs, tiles));
+  const int64_t tiles = ceil_div(p.m, 256) * ceil_div(p.n, p.cols);
+  const unsigned pairs = static_cast<unsigned>(std::min<int64_t>(kNumSMs / 2, tiles));
   // what every row of y and of the residual starts on a multiple of
   const uint64_t starts = static_cast<uint64_t>(p.epilogue == B200_EPILOGUE_SWIGLU ? p.n / 2 : p.n) * sizeof(T) |
                           reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.residual);
@@ -695,11 +747,15 @@ extern "C" int b200_linear_int8(const b200_linear_int8_call* call, void* stream)
   p.bias = c.bias; p.residual = c.residual; p.out = c.output; p.status = c.status;
   p.m = static_cast<int>(m); p.k = static_cast<int>(k); p.n = static_cast<int>(n); p.epilogue = static_cast<int>(c.epilogue);
   p.wait_limit = wait_limit(); p.drop_loads = drop_loads();
+  const StreamPlan stream_plan = plan_stream(m, k, n);
+  const PairPlan pair_plan = plan_pair(m, k, n);
+  // (what the two take is known well enough to choose where they are far apart; up to 256 rows every weight is read once)
+  const bool streamed = m <= kRowsAtMost || (stream_plan.us < 0.85 * pair_plan.us && stream_plan.chunks <= 64);
   int code = B200_ERR_UNSUPPORTED;
   with_element_type(dtype, [&](auto tag) {
     using T = typename decltype(tag)::type;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    code = m <= kRowsAtMost ? launch_stream<T>(p, c.x, c.weight, s) : launch_pair<T>(p, c.x, c.weight, s);
+    code = streamed ? launch_stream<T>(p, stream_plan, c.x, c.weight, s) : launch_pair<T>(p, pair_plan, c.x, c.weight, s);
   });
   return code;
 }
