@@ -347,25 +347,41 @@ linear_int8_stream_kernel(const Int8LinearParams p, const __grid_constant__ CUte
 }
 
 // -------------------------------------------------------------------------------------------------------------- pair ----
-template <typename T>
-__host__ __device__ constexpr int pair_stages() { return sizeof(T) == 4 ? 5 : 6; }  // (staging tiles of fp32 take the sixth one's place)
 constexpr int kPairStageBytes = 2 * 128 * 128;  // half of 256 rows of x, half of up to 256 of the weight
 constexpr int kPairWarps = 8;      // of the epilogue: two for each quarter of the accumulator's lanes
 constexpr int kPairThreads = (kPairWarps + 2) * 32;
 
-template <typename T>
+// Staging tiles of 32 x 32 a warp of the epilogue has, and what that leaves of the ring.
+template <typename T, typename Piece>
+__host__ __device__ constexpr int pair_tiles() { return sizeof(Piece) < 16 ? 1 : sizeof(T) == 4 ? 2 : 3; }
+template <typename T, typename Piece>
+__host__ __device__ constexpr int pair_stages() { return (sizeof(Piece) < 16 ? 6 : 5) - (sizeof(T) == 4 ? 1 : 0); }
+template <typename T, typename Piece>
 constexpr int pair_smem() {
-  return pair_stages<T>() * kPairStageBytes + kPairWarps * (32 * 32 * static_cast<int>(sizeof(T)) + 4 * 32 * 8);
+  return pair_stages<T, Piece>() * kPairStageBytes +
+         kPairWarps * (pair_tiles<T, Piece>() * 32 * 32 * static_cast<int>(sizeof(T)) + 4 * 32 * 8);
 }
 
-// Piece: what a lane moves of a row at a time, 16 bytes or, where rows of y do not start on multiples of that, 4 or 2.
+__device__ __forceinline__ void tma_store_2d(const void* tensor_map, uint32_t from, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
+               ::"l"(reinterpret_cast<uint64_t>(tensor_map)), "r"(from), "r"(c0), "r"(c1) : "memory");
+}
+// All but the thread's last `kLeft` stores have read shared memory.
+template <int kLeft>
+__device__ __forceinline__ void stores_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kLeft) : "memory"); }
+
+// Piece: uint4 where rows of y start on multiples of 16 bytes: chunks of y leave, and those of a residual come, by TMA (with
+// the warps' own loads and stores of 16 bytes BEFORE). Else what a lane moves of a row at a time, 4 bytes or 2.
 template <typename T, typename Piece>
 __global__ void __launch_bounds__(kPairThreads, 1)
 linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtensorMap x_map,
-                        const __grid_constant__ CUtensorMap w_map) {
-  constexpr int kPairStages = pair_stages<T>();
+                        const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap y_map,
+                        const __grid_constant__ CUtensorMap residual_map) {
+  constexpr bool kBulk = sizeof(Piece) == 16;
+  constexpr int kPairStages = pair_stages<T, Piece>(), kTiles = pair_tiles<T, Piece>();
   extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ __align__(8) uint64_t full[kPairStages], empty[kPairStages], acc_full[2], acc_empty[2];
+  __shared__ __align__(8) uint64_t arrived[kPairWarps * kTiles];  // a residual's chunks
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
 
@@ -391,6 +407,8 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
       mbarrier_init(smem_u32(&acc_full[a]), 1);
       mbarrier_init(smem_u32(&acc_empty[a]), 2 * kPairWarps);  // (the first CTA's counts: both CTAs' warps)
     }
+    if constexpr (kBulk)
+      for (int i = 0; i < kPairWarps * kTiles; ++i) mbarrier_init(smem_u32(&arrived[i]), 1);
     fence_mbarrier_init();
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&x_map)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&w_map)) : "memory");
@@ -457,10 +475,9 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
     if (!ok) failed = 1;
   } else if (warp < kPairWarps) {
     // ---- epilogue: this CTA's 128 rows; lanes 32 (warp % 4) .., every other chunk of 32 columns ----
-    // Everything that comes from memory (scales, bias, the first residual chunk) is asked for before the wait for the
-    // products. A chunk leaves through a staging tile, so that a store writes whole rows of it and a residual is read so, in
-    // pieces of 16 bytes where rows allow it and of 4 or 2 where their length does not (2008 x 512 x 3890: 110 us with a thread
-    // for each row).
+    // What comes from memory is asked for ahead: scales and bias during the tile before, a residual one chunk or two. A
+    // chunk leaves through a staging tile, by TMA where rows allow it; where their length does not, the warp writes whole rows
+    // of it in pieces of 4 bytes or 2 (2008 x 512 x 3890: 110 us with a thread for each row).
     const bool swiglu = p.epilogue == B200_EPILOGUE_SWIGLU;
     const int out_cols = swiglu ? p.n / 2 : p.n;
     T* out = static_cast<T*>(p.out);
@@ -468,10 +485,12 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
     constexpr int kVec = 16 / static_cast<int>(sizeof(T)), kUnits = 32 / kVec;  // of 16 bytes: a row of a chunk
     const int quarter = warp & 3, turn0 = warp >> 2;
     constexpr int kStageTile = 32 * 32 * static_cast<int>(sizeof(T));
-    const uint32_t stage_tile = smem_base + kPairStages * kPairStageBytes + warp * kStageTile;
-    float2* column_terms = reinterpret_cast<float2*>(smem + kPairStages * kPairStageBytes + kPairWarps * kStageTile) + warp * 128;
+    const uint32_t stage_tiles = smem_base + kPairStages * kPairStageBytes + warp * kTiles * kStageTile;
+    float2* column_terms = reinterpret_cast<float2*>(smem + kPairStages * kPairStageBytes + kPairWarps * kTiles * kStageTile) + warp * 128;
     const uint32_t acc_empty_first = map_to_rank(smem_u32(&acc_empty[0]), 0);
-    // 16-byte unit `unit` of row r of a chunk with `units` of them: 128 bytes of rows side by side never share a bank
+    uint32_t stage_tile = stage_tiles;
+    // 16-byte unit `unit` of row r of a chunk with `units` of them: 128 bytes of rows side by side never share a bank (the
+    // swizzle of a tensor map whose boxes have rows of 32, 64 or 128 bytes)
     auto unit_at = [&](int r, int unit, int units) {
       return stage_tile + r * units * 16 + ((unit ^ ((r * units >> 3) & (units - 1))) << 4);
     };
@@ -485,54 +504,103 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
         use(i, unit_at(r, byte >> 4, units) + (byte & 15), r, byte / static_cast<int>(sizeof(T)));
       }
     };
+    auto first_row = [&](int tile_m) { return tile_m * 256 + rank * 128 + quarter * 32; };
+    // scales and bias of a tile's columns that this warp works on
+    float next_row_scale = 0.0f, next_scale[4], next_bias[4];
+    auto ask_terms = [&](int tile) {
+      if (tile >= tiles) return;
+      int tile_m, tile_n;
+      place(tile, tile_m, tile_n);
+      const int row = first_row(tile_m) + lane, n_end = min(p.n, (tile_n + 1) * bn);
+      next_row_scale = row < p.m ? p.x_scales[row] : 0.0f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int col = tile_n * bn + turn0 * 32 + q * 64 + lane;
+        next_scale[q] = col < n_end ? p.w_scales[col] : 0.0f;
+        next_bias[q] = col < n_end && p.bias != nullptr ? Elem<T>::load(static_cast<const T*>(p.bias) + col) : 0.0f;
+      }
+    };
+    // kBulk: the residual's chunks in the order in which they are used, each into the staging tile that it leaves through
+    int asked = 0, asked_tile = pair, asked_c0 = turn0 * 32;
+    const uint32_t arrivals = smem_u32(&arrived[kBulk ? warp * kTiles : 0]);
+    auto ask_residual = [&]() {
+      while (asked_tile < tiles) {
+        int tile_m, tile_n;
+        place(asked_tile, tile_m, tile_n);
+        const int col0 = tile_n * bn + asked_c0;
+        const bool there = asked_c0 < bn && col0 < p.n;
+        if (there) {
+          if (lane == 0) {
+            const uint32_t bar = arrivals + asked % kTiles * 8;
+            mbarrier_arrive_expect_tx_if(1u, bar, kStageTile);
+            tma_load_2d_if(1u, stage_tiles + asked % kTiles * kStageTile, &residual_map, bar, col0, first_row(tile_m));
+          }
+          ++asked;
+          asked_c0 += 64;
+          return;
+        }
+        asked_tile += pairs;
+        asked_c0 = turn0 * 32;
+      }
+    };
+    const bool bulk_residual = kBulk && residual != nullptr;
     bool ok = true;
-    int done = 0;
+    int done = 0, chunks = 0;
+    ask_terms(pair);
+    if (bulk_residual)
+      for (int i = 0; i + 1 < kTiles; ++i) ask_residual();
     for (int tile = pair; tile < tiles; tile += pairs, ++done) {
       int tile_m, tile_n;
       place(tile, tile_m, tile_n);
-      const int acc = done & 1, row0 = tile_m * 256 + rank * 128 + quarter * 32, row = row0 + lane;
+      const int acc = done & 1, row0 = first_row(tile_m);
       const int n_end = min(p.n, (tile_n + 1) * bn);
-      const float row_scale = row < p.m ? p.x_scales[row] : 0.0f;
+      const float row_scale = next_row_scale;
       __syncwarp();  // (the tile before is done with the terms)
-      for (int c0 = turn0 * 32, q = 0; c0 < bn; c0 += 64, ++q) {
-        const int col = tile_n * bn + c0 + lane;
-        column_terms[q * 32 + lane] = make_float2(
-            col < n_end ? p.w_scales[col] : 0.0f,
-            col < n_end && p.bias != nullptr ? Elem<T>::load(static_cast<const T*>(p.bias) + col) : 0.0f);
-      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) column_terms[q * 32 + lane] = make_float2(next_scale[q], next_bias[q]);
+      __syncwarp();
+      ask_terms(tile + pairs);
       constexpr int kWords = sizeof(Piece) < 4 ? 1 : sizeof(Piece) / 4;
-      uint32_t ahead[kUnits * 16 / sizeof(Piece) * kWords];  // the next chunk's residual
+      uint32_t ahead[kBulk ? 1 : kUnits * 16 / sizeof(Piece) * kWords];  // the next chunk's residual
       auto fetch = [&](int c0) {
-        const int col0 = tile_n * bn + c0;
-        if (residual == nullptr || col0 >= n_end) return;
-        const T* from = residual + static_cast<int64_t>(row0) * p.n + col0;
-        each_piece(std::integral_constant<int, kUnits>{}, [&](int i, uint32_t, int r, int element) {
-          Piece value = {};
-          if (row0 + r < p.m && col0 + element < n_end)
-            value = *reinterpret_cast<const Piece*>(from + static_cast<int64_t>(r) * p.n + element);
-          if constexpr (sizeof(Piece) == 16) {
-            ahead[4 * i] = value.x; ahead[4 * i + 1] = value.y; ahead[4 * i + 2] = value.z; ahead[4 * i + 3] = value.w;
-          } else {
+        if constexpr (!kBulk) {
+          const int col0 = tile_n * bn + c0;
+          if (residual == nullptr || col0 >= n_end) return;
+          const T* from = residual + static_cast<int64_t>(row0) * p.n + col0;
+          each_piece(std::integral_constant<int, kUnits>{}, [&](int i, uint32_t, int r, int element) {
+            Piece value = {};
+            if (row0 + r < p.m && col0 + element < n_end)
+              value = *reinterpret_cast<const Piece*>(from + static_cast<int64_t>(r) * p.n + element);
             ahead[i] = value;
-          }
-        });
+          });
+        }
       };
       fetch(turn0 * 32);
       ok = ok && __all_sync(0xffffffffu, mbarrier_wait_bounded(smem_u32(&acc_full[acc]), (done >> 1) & 1, p.wait_limit));
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t t_addr = tmem_base + acc * 256 + (static_cast<uint32_t>(quarter * 32) << 16);
+      // (relaxed: what has to be over are the reads of tensor memory, which the fence orders. A release would wait for the
+      // stores of the tile to reach L2, 1 us of it: 16384 x 896 x 9728 144 us with it)
+      auto sums_read = [&]() {
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0)
+          asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(acc_empty_first + acc * 8) : "memory");
+      };
       uint32_t raw[32];  // the next chunk's sums, on their way while a chunk is worked on
-      tmem_load_32x32_issue(t_addr + turn0 * 32, raw);
+      if (tile_n * bn + turn0 * 32 < n_end) tmem_load_32x32_issue(t_addr + turn0 * 32, raw);
+      else sums_read();
 #pragma unroll 1
-      for (int c0 = turn0 * 32, q = 0; c0 < bn; c0 += 64, ++q) {
+      for (int c0 = turn0 * 32, q = 0; c0 < bn; c0 += 64, ++q, ++chunks) {
         const int col0 = tile_n * bn + c0;
         if (col0 >= n_end) break;  // (warp-uniform)
         tmem_load_wait(raw);
         float v[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(raw[i]);
-        if (c0 + 64 < bn) tmem_load_32x32_issue(t_addr + c0 + 64, raw);
+        if (c0 + 64 < bn && col0 + 64 < n_end) tmem_load_32x32_issue(t_addr + c0 + 64, raw);
+        else sums_read();
         const float4* terms = reinterpret_cast<const float4*>(column_terms + q * 32);  // scale, bias of two columns
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -540,28 +608,48 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
           v[2 * i] = fmaf(static_cast<float>(__float_as_int(v[2 * i])) * row_scale, t.x, t.y);
           v[2 * i + 1] = fmaf(static_cast<float>(__float_as_int(v[2 * i + 1])) * row_scale, t.z, t.w);
         }
-        __syncwarp();  // the chunk before has been read
-        // the staged rows to y: `width` columns of them exist
-        auto rows_out = [&](auto units_tag, T* to, int width) {
-          Piece values[decltype(units_tag)::value * 16 / sizeof(Piece)];
-          each_piece(units_tag, [&](int i, uint32_t from, int, int) {
-            Piece& value = values[i];
-            if constexpr (sizeof(Piece) == 16)
-              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(value.x), "=r"(value.y), "=r"(value.z), "=r"(value.w) : "r"(from));
-            else if constexpr (sizeof(Piece) == 4)
-              asm volatile("ld.shared.b32 %0, [%1];" : "=r"(value) : "r"(from));
-            else
-              asm volatile("ld.shared.u16 %0, [%1];" : "=h"(value) : "r"(from));
-          });
-          if (row0 + 32 <= p.m && col0 + 32 <= n_end) {  // (a chunk that lies in y needs no questions)
-            each_piece(units_tag, [&](int i, uint32_t, int r, int element) {
-              *reinterpret_cast<Piece*>(to + static_cast<int64_t>(r) * out_cols + element) = values[i];
-            });
+        if constexpr (kBulk) {
+          stage_tile = stage_tiles + chunks % kTiles * kStageTile;
+          if (residual != nullptr) {
+            ok = __all_sync(0xffffffffu, mbarrier_wait_bounded(arrivals + chunks % kTiles * 8, chunks / kTiles & 1, p.wait_limit));
+            if (!ok) break;
           } else {
-            each_piece(units_tag, [&](int i, uint32_t, int r, int element) {
-              if (row0 + r < p.m && element < width)
-                *reinterpret_cast<Piece*>(to + static_cast<int64_t>(r) * out_cols + element) = values[i];
+            if (lane == 0) stores_read<kTiles - 1>();  // the tile's chunk before
+            __syncwarp();
+          }
+        } else {
+          __syncwarp();  // the chunk before has been read
+        }
+        // the staged rows to y: `width` columns of them exist
+        auto rows_out = [&](auto units_tag, int to_col, int width) {
+          if constexpr (kBulk) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+              if (row0 < p.m) tma_store_2d(&y_map, stage_tile, to_col, row0);
+              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            }
+          } else {
+            __syncwarp();
+            T* to = out + static_cast<int64_t>(row0) * out_cols + to_col;
+            Piece values[decltype(units_tag)::value * 16 / sizeof(Piece)];
+            each_piece(units_tag, [&](int i, uint32_t from, int, int) {
+              Piece& value = values[i];
+              if constexpr (sizeof(Piece) == 4)
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(value) : "r"(from));
+              else
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(value) : "r"(from));
             });
+            if (row0 + 32 <= p.m && col0 + 32 <= n_end) {  // (a chunk that lies in y needs no questions)
+              each_piece(units_tag, [&](int i, uint32_t, int r, int element) {
+                *reinterpret_cast<Piece*>(to + static_cast<int64_t>(r) * out_cols + element) = values[i];
+              });
+            } else {
+              each_piece(units_tag, [&](int i, uint32_t, int r, int element) {
+                if (row0 + r < p.m && element < width)
+                  *reinterpret_cast<Piece*>(to + static_cast<int64_t>(r) * out_cols + element) = values[i];
+              });
+            }
           }
         };
         if (swiglu) {
@@ -576,22 +664,20 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(unit_at(lane, unit, kHalf)), "r"(packed.x), "r"(packed.y),
                          "r"(packed.z), "r"(packed.w) : "memory");
           }
-          __syncwarp();
-          rows_out(std::integral_constant<int, kHalf>{}, out + static_cast<int64_t>(row0) * out_cols + col0 / 2, (n_end - col0) / 2);
+          rows_out(std::integral_constant<int, kHalf>{}, col0 / 2, (n_end - col0) / 2);
           continue;
         }
-        if (residual != nullptr) {
-          each_piece(std::integral_constant<int, kUnits>{}, [&](int i, uint32_t to, int, int) {
-            if constexpr (sizeof(Piece) == 16)
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(ahead[4 * i]), "r"(ahead[4 * i + 1]),
-                           "r"(ahead[4 * i + 2]), "r"(ahead[4 * i + 3]) : "memory");
-            else if constexpr (sizeof(Piece) == 4)
-              asm volatile("st.shared.b32 [%0], %1;" ::"r"(to), "r"(ahead[i]) : "memory");
-            else
-              asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"(static_cast<uint16_t>(ahead[i])) : "memory");
-          });
-          if (c0 + 64 < bn) fetch(c0 + 64);
-          __syncwarp();
+        if constexpr (!kBulk) {
+          if (residual != nullptr) {
+            each_piece(std::integral_constant<int, kUnits>{}, [&](int i, uint32_t to, int, int) {
+              if constexpr (sizeof(Piece) == 4)
+                asm volatile("st.shared.b32 [%0], %1;" ::"r"(to), "r"(ahead[i]) : "memory");
+              else
+                asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"(static_cast<uint16_t>(ahead[i])) : "memory");
+            });
+            if (c0 + 64 < bn) fetch(c0 + 64);
+            __syncwarp();
+          }
         }
 #pragma unroll
         for (int unit = 0; unit < kUnits; ++unit) {
@@ -611,16 +697,20 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(unit_at(lane, unit, kUnits)), "r"(packed.x), "r"(packed.y),
                        "r"(packed.z), "r"(packed.w) : "memory");
         }
-        __syncwarp();
-        rows_out(std::integral_constant<int, kUnits>{}, out + static_cast<int64_t>(row0) * out_cols + col0, n_end - col0);
+        rows_out(std::integral_constant<int, kUnits>{}, col0, n_end - col0);
+        if (bulk_residual) {
+          if (lane == 0) stores_read<1>();  // the chunk before this one has left its tile
+          __syncwarp();
+          ask_residual();
+        }
       }
-      tmem_load_wait(raw);  // (of a chunk beyond n, if there is one)
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      if (!ok) break;
+    }
+    if constexpr (kBulk) {
+      if (bulk_residual)  // (after a failure: copies still on their way)
+        for (; chunks < asked; ++chunks) mbarrier_wait_bounded(arrivals + chunks % kTiles * 8, chunks / kTiles & 1, p.wait_limit);
+      if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
       __syncwarp();
-      // (relaxed: what has to be over are the reads of tensor memory, which the fence orders. A release would wait for the
-      // stores of the tile to reach L2, 1 us of it: 16384 x 896 x 9728 144 us with it)
-      if (lane == 0)
-        asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(acc_empty_first + acc * 8) : "memory");
     }
     if (!ok) failed = 1;
   }
@@ -630,6 +720,21 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
   cluster_sync();  // neither CTA leaves while the other may still signal it
   if (warp == kPairWarps + 1)
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+}
+
+// y or a residual [m, cols] in boxes of 32 rows of `width` columns, 32, 64 or 128 bytes of them, swizzled as the warps write.
+template <typename T>
+bool make_chunk_map(CUtensorMap* map, const void* base, int64_t m, int64_t cols, int width) {
+  EncodeTiledFn encode = tensor_map_encoder();
+  if (encode == nullptr) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(m)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols) * sizeof(T)};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(width), 32}, element_strides[2] = {1, 1};
+  const int bytes = width * static_cast<int>(sizeof(T));
+  return encode(map, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(base), dims,
+                strides, box, element_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                bytes == 32 ? CU_TENSOR_MAP_SWIZZLE_32B : bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // [rows, K] codes in boxes of box_rows x 128 (128-byte rows, 128B swizzle); zeros beyond both.
@@ -648,8 +753,9 @@ bool make_code_map(CUtensorMap* map, const void* base, int64_t rows, int64_t k, 
 // more at 256 rows, its epilogue 2.5 us at 256 rows (256 x 18944 x 3584: 27.9 us in 112 CTAs of 37 k-blocks; 256 x 512 x 18944:
 // 8.4 in 4); of the pair kernel 0.26 us at 128 columns and 0.35 at 256 (257 x 18944 x 3584: 41.8 us in one round of 148
 // k-blocks; 1407 x 3488 x 25: 10.6 in 28), an epilogue of 3.3 us a tile beside the products of the next.
+constexpr double kStreamEpilogue[] = {4.5, 15.0, 7.0};  // none, residual, SwiGLU
 struct StreamPlan { int cols, chunks, slices; double us; };
-StreamPlan plan_stream(int64_t m, int64_t k, int64_t n) {
+StreamPlan plan_stream(int64_t m, int64_t k, int64_t n, int epilogue) {
   const int64_t tiles = ceil_div(n, 128), blocks = ceil_div(k, kBK);
   StreamPlan best = {0, 0, 0, 1e30};
   for (int64_t chunks = ceil_div(m, kRowsAtMost); chunks <= std::max<int64_t>(16, ceil_div(m, kRowsAtMost)); ++chunks) {
@@ -658,7 +764,9 @@ StreamPlan plan_stream(int64_t m, int64_t k, int64_t n) {
     int64_t slices = 1;
     while (slices < 8 && units * slices * 2 <= kNumSMs && blocks >= slices * 4) slices *= 2;
     const double share = cols / 256.0;
-    const double us = 4.0 + ceil_div(units * slices, kNumSMs) * (ceil_div(blocks, slices) * (0.2 + 0.42 * share) + 2.5 * share);
+    const int64_t across = std::max<int64_t>(1, kNumSMs / chunks), rounds = slices > 1 ? 1 : ceil_div(tiles, across);
+    const double products = ceil_div(blocks, slices) * (0.2 + 0.42 * share);
+    const double us = 4.0 + products + 2.5 * share + (rounds - 1) * std::max(products, kStreamEpilogue[epilogue] * share);
     if (us < 0.9 * best.us) best = {static_cast<int>(cols), static_cast<int>(ceil_div(m, cols)), static_cast<int>(slices), us};
   }
   return best;
@@ -702,7 +810,7 @@ template <typename T>
 int launch_pair(Int8LinearParams p, const PairPlan& plan, const void* x, const void* w, cudaStream_t stream) {
   p.cols = plan.cols;
   p.n_fastest = p.n <= p.m;
-  CUtensorMap x_map, w_map;
+  CUtensorMap x_map, w_map, y_map = {}, residual_map = {};
   if (!make_code_map(&x_map, x, p.m, p.k, 128) || !make_code_map(&w_map, w, p.n, p.k, p.cols / 2)) return B200_ERR_UNSUPPORTED;
   const int64_t tiles = ceil_div(p.m, 256) * ceil_div(p.n, p.cols);
   const unsigned pairs = static_cast<unsigned>(std::min<int64_t>(kNumSMs / 2, tiles));
@@ -710,14 +818,22 @@ int launch_pair(Int8LinearParams p, const PairPlan& plan, const void* x, const v
   const uint64_t starts = static_cast<uint64_t>(p.epilogue == B200_EPILOGUE_SWIGLU ? p.n / 2 : p.n) * sizeof(T) |
                           reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.residual);
   const auto launch = [&](auto piece) {
-    auto kernel = linear_int8_pair_kernel<T, decltype(piece)>;
-    static_assert(tensor_memory_fits(512, pair_smem<T>()) && pair_smem<T>() + 1024 <= 227 * 1024, "tensor memory under programmatic launches");
+    using Piece = decltype(piece);
+    auto kernel = linear_int8_pair_kernel<T, Piece>;
+    constexpr int kSmem = pair_smem<T, Piece>();
+    static_assert(tensor_memory_fits(512, kSmem) && kSmem + 1024 <= 227 * 1024, "tensor memory under programmatic launches");
     static std::atomic<uint64_t> allowed{0};
-    if (!allow_shared_memory(kernel, pair_smem<T>(), allowed)) return B200_ERR_LAUNCH;
-    return launch_chained_cluster(kernel, dim3(2 * pairs), dim3(kPairThreads), pair_smem<T>(), stream, 2u, p, x_map, w_map) ==
-                   cudaSuccess ? launch_status() : B200_ERR_LAUNCH;
+    if (!allow_shared_memory(kernel, kSmem, allowed)) return B200_ERR_LAUNCH;
+    return launch_chained_cluster(kernel, dim3(2 * pairs), dim3(kPairThreads), kSmem, stream, 2u, p, x_map, w_map, y_map,
+                                  residual_map) == cudaSuccess ? launch_status() : B200_ERR_LAUNCH;
   };
-  if (starts % 16 == 0) return launch(uint4{});
+  if (starts % 16 == 0) {
+    const bool swiglu = p.epilogue == B200_EPILOGUE_SWIGLU;
+    if (!make_chunk_map<T>(&y_map, p.out, p.m, swiglu ? p.n / 2 : p.n, swiglu ? 16 : 32) ||
+        (p.residual && !make_chunk_map<T>(&residual_map, p.residual, p.m, p.n, 32)))
+      return B200_ERR_UNSUPPORTED;
+    return launch(uint4{});
+  }
   if constexpr (sizeof(T) == 2) {
     if (starts % 4 != 0) return launch(uint16_t{});
   }
@@ -747,7 +863,7 @@ extern "C" int b200_linear_int8(const b200_linear_int8_call* call, void* stream)
   p.bias = c.bias; p.residual = c.residual; p.out = c.output; p.status = c.status;
   p.m = static_cast<int>(m); p.k = static_cast<int>(k); p.n = static_cast<int>(n); p.epilogue = static_cast<int>(c.epilogue);
   p.wait_limit = wait_limit(); p.drop_loads = drop_loads();
-  const StreamPlan stream_plan = plan_stream(m, k, n);
+  const StreamPlan stream_plan = plan_stream(m, k, n, p.epilogue);
   const PairPlan pair_plan = plan_pair(m, k, n);
   // (what the two take is known well enough to choose where they are far apart; up to 256 rows every weight is read once)
   const bool streamed = m <= kRowsAtMost || (stream_plan.us < 0.85 * pair_plan.us && stream_plan.chunks <= 64);
