@@ -102,6 +102,13 @@ __device__ __forceinline__ float silu_times(float gate, float up) {
   return gate * inverse * up;
 }
 
+// a = a row t.x + t.z and b = b row t.y + t.w, each product and sum of the two in one instruction
+__device__ __forceinline__ void scale_two(float& a, float& b, float row, const float4& t) {
+  asm("{\n\t.reg .b64 v, r, s, c;\n\tmov.b64 v, {%0, %1};\n\tmov.b64 r, {%2, %2};\n\tmov.b64 s, {%3, %4};\n\t"
+      "mov.b64 c, {%5, %6};\n\tmul.rn.f32x2 v, v, r;\n\tfma.rn.f32x2 v, v, s, c;\n\tmov.b64 {%0, %1}, v;\n\t}"
+      : "+f"(a), "+f"(b) : "f"(row), "f"(t.x), "f"(t.y), "f"(t.z), "f"(t.w));
+}
+
 // ------------------------------------------------------------------------------------------------------------ stream ----
 __device__ __forceinline__ int4 load_cluster_i32x4(uint32_t remote) {
   int4 v;
@@ -348,7 +355,8 @@ linear_int8_stream_kernel(const Int8LinearParams p, const __grid_constant__ CUte
 
 // -------------------------------------------------------------------------------------------------------------- pair ----
 constexpr int kPairStageBytes = 2 * 128 * 128;  // half of 256 rows of x, half of up to 256 of the weight
-constexpr int kPairWarps = 8;      // of the epilogue: two for each quarter of the accumulator's lanes
+constexpr int kPairWarps = 8;      // of the epilogue, for each quarter of the accumulator's lanes
+constexpr int kAcross = kPairWarps / 4, kStep = kAcross * 32, kChunksAtMost = (8 + kAcross - 1) / kAcross;  // a quarter's warps share the columns
 constexpr int kPairThreads = (kPairWarps + 2) * 32;
 
 // Staging tiles of 32 x 32 a warp of the epilogue has, and what that leaves of the ring.
@@ -359,12 +367,16 @@ __host__ __device__ constexpr int pair_stages() { return (sizeof(Piece) < 16 ? 6
 template <typename T, typename Piece>
 constexpr int pair_smem() {
   return pair_stages<T, Piece>() * kPairStageBytes +
-         kPairWarps * (pair_tiles<T, Piece>() * 32 * 32 * static_cast<int>(sizeof(T)) + 4 * 32 * 8);
+         kPairWarps * (pair_tiles<T, Piece>() * 32 * 32 * static_cast<int>(sizeof(T)) + kChunksAtMost * 32 * 8);
 }
 
-__device__ __forceinline__ void tma_store_2d(const void* tensor_map, uint32_t from, int c0, int c1) {
-  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
-               ::"l"(reinterpret_cast<uint64_t>(tensor_map)), "r"(from), "r"(c0), "r"(c1) : "memory");
+// A box of shared memory to memory, if `leader`; a group of its own (an empty one for the other lanes: no branch, which would
+// cost as much as the store).
+__device__ __forceinline__ void tma_store_2d_if(uint32_t leader, const void* tensor_map, uint32_t from, int c0, int c1) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %4, 0;\n\t"
+               "@q cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];\n\t}\n\t"
+               "cp.async.bulk.commit_group;"
+               ::"l"(reinterpret_cast<uint64_t>(tensor_map)), "r"(from), "r"(c0), "r"(c1), "r"(leader) : "memory");
 }
 // All but the thread's last `kLeft` stores have read shared memory.
 template <int kLeft>
@@ -392,10 +404,21 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
   const int nkb = (p.k + kBK - 1) / kBK;
   const int tiles_n = (p.n + bn - 1) / bn, tiles_m = (p.m + 255) / 256, tiles = tiles_n * tiles_m;
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  auto place = [&](int tile, int& tile_m, int& tile_n) {
-    if (p.n_fastest) { tile_m = tile / tiles_n; tile_n = tile - tile_m * tiles_n; }
-    else { tile_n = tile / tiles_m; tile_m = tile - tile_n * tiles_m; }
+  // a pair's tiles, one after another without a division each
+  struct Place {
+    int tile, slow, fast, step, step_slow, step_fast, along;
+    bool n_fastest;
+    __device__ Place(int first, int step_, int along_, bool n_fastest_)
+        : tile(first), slow(first / along_), fast(first % along_), step(step_), step_slow(step_ / along_), step_fast(step_ % along_),
+          along(along_), n_fastest(n_fastest_) {}
+    __device__ void next() {
+      tile += step; slow += step_slow; fast += step_fast;
+      if (fast >= along) { fast -= along; ++slow; }
+    }
+    __device__ int m() const { return n_fastest ? slow : fast; }
+    __device__ int n() const { return n_fastest ? fast : slow; }
   };
+  const Place start(pair, pairs, p.n_fastest ? tiles_n : tiles_m, p.n_fastest);
 
   if (threadIdx.x == 0) {
     failed = 0;
@@ -430,9 +453,8 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
     const uint32_t leader = elect_one();
     bool ok = true;
     int s = 0, turn = 0;
-    for (int tile = pair; ok && tile < tiles; tile += pairs) {
-      int tile_m, tile_n;
-      place(tile, tile_m, tile_n);
+    for (Place at = start; ok && at.tile < tiles; at.next()) {
+      const int tile_m = at.m(), tile_n = at.n();
       for (int kb = 0; kb < nkb; ++kb) {
         if (turn > 0 && !mbarrier_wait_warp(smem_u32(&empty[s]), (turn - 1) & 1, p.wait_limit)) {
           ok = false;
@@ -486,7 +508,7 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
     const int quarter = warp & 3, turn0 = warp >> 2;
     constexpr int kStageTile = 32 * 32 * static_cast<int>(sizeof(T));
     const uint32_t stage_tiles = smem_base + kPairStages * kPairStageBytes + warp * kTiles * kStageTile;
-    float2* column_terms = reinterpret_cast<float2*>(smem + kPairStages * kPairStageBytes + kPairWarps * kTiles * kStageTile) + warp * 128;
+    float* column_terms = reinterpret_cast<float*>(smem + kPairStages * kPairStageBytes + kPairWarps * kTiles * kStageTile) + warp * kChunksAtMost * 64;
     const uint32_t acc_empty_first = map_to_rank(smem_u32(&acc_empty[0]), 0);
     uint32_t stage_tile = stage_tiles;
     // 16-byte unit `unit` of row r of a chunk with `units` of them: 128 bytes of rows side by side never share a bank (the
@@ -506,60 +528,62 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
     };
     auto first_row = [&](int tile_m) { return tile_m * 256 + rank * 128 + quarter * 32; };
     // scales and bias of a tile's columns that this warp works on
-    float next_row_scale = 0.0f, next_scale[4], next_bias[4];
-    auto ask_terms = [&](int tile) {
-      if (tile >= tiles) return;
-      int tile_m, tile_n;
-      place(tile, tile_m, tile_n);
-      const int row = first_row(tile_m) + lane, n_end = min(p.n, (tile_n + 1) * bn);
+    float next_row_scale = 0.0f, next_scale[kChunksAtMost], next_bias[kChunksAtMost];
+    auto ask_terms = [&](const Place& at) {
+      if (at.tile >= tiles) return;
+      const int tile_n = at.n(), row = first_row(at.m()) + lane, n_end = min(p.n, (tile_n + 1) * bn);
       next_row_scale = row < p.m ? p.x_scales[row] : 0.0f;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int col = tile_n * bn + turn0 * 32 + q * 64 + lane;
+      for (int q = 0; q < kChunksAtMost; ++q) {
+        const int col = tile_n * bn + turn0 * 32 + q * kStep + lane;
         next_scale[q] = col < n_end ? p.w_scales[col] : 0.0f;
         next_bias[q] = col < n_end && p.bias != nullptr ? Elem<T>::load(static_cast<const T*>(p.bias) + col) : 0.0f;
       }
     };
     // kBulk: the residual's chunks in the order in which they are used, each into the staging tile that it leaves through
-    int asked = 0, asked_tile = pair, asked_c0 = turn0 * 32;
+    Place asked_at = start;
+    int asked = 0, asked_slot = 0, asked_c0 = turn0 * 32;
     const uint32_t arrivals = smem_u32(&arrived[kBulk ? warp * kTiles : 0]);
     auto ask_residual = [&]() {
-      while (asked_tile < tiles) {
-        int tile_m, tile_n;
-        place(asked_tile, tile_m, tile_n);
-        const int col0 = tile_n * bn + asked_c0;
+      while (asked_at.tile < tiles) {
+        const int col0 = asked_at.n() * bn + asked_c0;
         const bool there = asked_c0 < bn && col0 < p.n;
         if (there) {
-          if (lane == 0) {
-            const uint32_t bar = arrivals + asked % kTiles * 8;
-            mbarrier_arrive_expect_tx_if(1u, bar, kStageTile);
-            tma_load_2d_if(1u, stage_tiles + asked % kTiles * kStageTile, &residual_map, bar, col0, first_row(tile_m));
-          }
+          const uint32_t bar = arrivals + asked_slot * 8;
+          mbarrier_arrive_expect_tx_if(lane == 0, bar, kStageTile);
+          tma_load_2d_if(lane == 0, stage_tiles + asked_slot * kStageTile, &residual_map, bar, col0, first_row(asked_at.m()));
           ++asked;
-          asked_c0 += 64;
+          asked_slot = asked_slot + 1 == kTiles ? 0 : asked_slot + 1;
+          asked_c0 += kStep;
           return;
         }
-        asked_tile += pairs;
+        asked_at.next();
         asked_c0 = turn0 * 32;
       }
     };
     const bool bulk_residual = kBulk && residual != nullptr;
     bool ok = true;
-    int done = 0, chunks = 0;
-    ask_terms(pair);
+    int done = 0, chunks = 0, slot = 0;  // slot, phase: chunks % kTiles, chunks / kTiles & 1
+    uint32_t phase = 0;
+    if constexpr (kBulk) ask_terms(start);  // (else no registers are left for them)
     if (bulk_residual)
       for (int i = 0; i + 1 < kTiles; ++i) ask_residual();
-    for (int tile = pair; tile < tiles; tile += pairs, ++done) {
-      int tile_m, tile_n;
-      place(tile, tile_m, tile_n);
+    for (Place at = start; at.tile < tiles; ++done) {
+      const int tile_m = at.m(), tile_n = at.n();
+      if constexpr (!kBulk) ask_terms(at);
+      at.next();
       const int acc = done & 1, row0 = first_row(tile_m);
       const int n_end = min(p.n, (tile_n + 1) * bn);
       const float row_scale = next_row_scale;
       __syncwarp();  // (the tile before is done with the terms)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) column_terms[q * 32 + lane] = make_float2(next_scale[q], next_bias[q]);
+      for (int q = 0; q < kChunksAtMost; ++q) {
+        float* to = column_terms + q * 64 + (lane >> 1) * 4 + (lane & 1);
+        to[0] = next_scale[q];
+        to[2] = next_bias[q];
+      }
       __syncwarp();
-      ask_terms(tile + pairs);
+      if constexpr (kBulk) ask_terms(at);
       constexpr int kWords = sizeof(Piece) < 4 ? 1 : sizeof(Piece) / 4;
       uint32_t ahead[kBulk ? 1 : kUnits * 16 / sizeof(Piece) * kWords];  // the next chunk's residual
       auto fetch = [&](int c0) {
@@ -585,50 +609,49 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
       auto sums_read = [&]() {
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
-        if (lane == 0)
-          asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(acc_empty_first + acc * 8) : "memory");
+        asm volatile("{\n\t.reg .pred q;\n\tsetp.eq.s32 q, %1, 0;\n\t@q mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n\t}"
+                     ::"r"(acc_empty_first + acc * 8), "r"(lane) : "memory");
       };
-      uint32_t raw[32];  // the next chunk's sums, on their way while a chunk is worked on
-      if (tile_n * bn + turn0 * 32 < n_end) tmem_load_32x32_issue(t_addr + turn0 * 32, raw);
-      else sums_read();
+      uint32_t raw[32];  // kBulk: the next chunk's sums, on their way while a chunk is worked on
+      if (tile_n * bn + turn0 * 32 >= n_end) sums_read();
+      else if constexpr (kBulk) tmem_load_32x32_issue(t_addr + turn0 * 32, raw);
 #pragma unroll 1
-      for (int c0 = turn0 * 32, q = 0; c0 < bn; c0 += 64, ++q, ++chunks) {
+      for (int c0 = turn0 * 32, q = 0; c0 < bn; c0 += kStep, ++q, ++chunks) {
         const int col0 = tile_n * bn + c0;
         if (col0 >= n_end) break;  // (warp-uniform)
+        if constexpr (!kBulk) tmem_load_32x32_issue(t_addr + c0, raw);
         tmem_load_wait(raw);
         float v[32];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(raw[i]);
-        if (c0 + 64 < bn && col0 + 64 < n_end) tmem_load_32x32_issue(t_addr + c0 + 64, raw);
-        else sums_read();
-        const float4* terms = reinterpret_cast<const float4*>(column_terms + q * 32);  // scale, bias of two columns
+        for (int i = 0; i < 32; ++i) v[i] = static_cast<float>(static_cast<int>(raw[i]));
+        const bool more = c0 + kStep < bn && col0 + kStep < n_end;
+        if (!more) sums_read();
+        else if constexpr (kBulk) tmem_load_32x32_issue(t_addr + c0 + kStep, raw);
+        const float4* terms = reinterpret_cast<const float4*>(column_terms + q * 64);  // two columns' scales, their bias
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const float4 t = terms[i];
-          v[2 * i] = fmaf(static_cast<float>(__float_as_int(v[2 * i])) * row_scale, t.x, t.y);
-          v[2 * i + 1] = fmaf(static_cast<float>(__float_as_int(v[2 * i + 1])) * row_scale, t.z, t.w);
+          scale_two(v[2 * i], v[2 * i + 1], row_scale, t);
         }
         if constexpr (kBulk) {
-          stage_tile = stage_tiles + chunks % kTiles * kStageTile;
+          stage_tile = stage_tiles + slot * kStageTile;
           if (residual != nullptr) {
-            ok = __all_sync(0xffffffffu, mbarrier_wait_bounded(arrivals + chunks % kTiles * 8, chunks / kTiles & 1, p.wait_limit));
+            ok = __all_sync(0xffffffffu, mbarrier_wait_bounded(arrivals + slot * 8, phase, p.wait_limit));
             if (!ok) break;
           } else {
-            if (lane == 0) stores_read<kTiles - 1>();  // the tile's chunk before
+            stores_read<kTiles - 1>();  // the tile's chunk before
             __syncwarp();
           }
         } else {
           __syncwarp();  // the chunk before has been read
         }
+        if (++slot == kTiles) { slot = 0; phase ^= 1; }
         // the staged rows to y: `width` columns of them exist
         auto rows_out = [&](auto units_tag, int to_col, int width) {
           if constexpr (kBulk) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) {
-              if (row0 < p.m) tma_store_2d(&y_map, stage_tile, to_col, row0);
-              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-            }
+            tma_store_2d_if(lane == 0 && row0 < p.m, &y_map, stage_tile, to_col, row0);
           } else {
             __syncwarp();
             T* to = out + static_cast<int64_t>(row0) * out_cols + to_col;
@@ -675,7 +698,7 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
               else
                 asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"(static_cast<uint16_t>(ahead[i])) : "memory");
             });
-            if (c0 + 64 < bn) fetch(c0 + 64);
+            if (c0 + kStep < bn) fetch(c0 + kStep);
             __syncwarp();
           }
         }
@@ -699,7 +722,7 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
         }
         rows_out(std::integral_constant<int, kUnits>{}, col0, n_end - col0);
         if (bulk_residual) {
-          if (lane == 0) stores_read<1>();  // the chunk before this one has left its tile
+          stores_read<1>();  // the chunk before this one has left its tile
           __syncwarp();
           ask_residual();
         }
@@ -709,7 +732,7 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
     if constexpr (kBulk) {
       if (bulk_residual)  // (after a failure: copies still on their way)
         for (; chunks < asked; ++chunks) mbarrier_wait_bounded(arrivals + chunks % kTiles * 8, chunks / kTiles & 1, p.wait_limit);
-      if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+      asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
       __syncwarp();
     }
     if (!ok) failed = 1;
