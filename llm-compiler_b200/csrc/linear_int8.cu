@@ -518,13 +518,16 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
     };
     // use(i, address in the staging tile, row, element of the row) of this lane's i-th piece of a chunk: pieces side by side
     // over the lanes, whole rows one after another
-    auto each_piece = [&](auto units_tag, auto&& use) {
+    auto some_pieces = [&](auto units_tag, int first, auto many_tag, auto&& use) {
       constexpr int kBytes = sizeof(Piece), units = decltype(units_tag)::value, kEach = units * 16 / kBytes;
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) {
-        const int at = i * 32 + lane, r = at / kEach, byte = at % kEach * kBytes;
+      for (int i = 0; i < decltype(many_tag)::value; ++i) {
+        const int at = (first + i) * 32 + lane, r = at / kEach, byte = at % kEach * kBytes;
         use(i, unit_at(r, byte >> 4, units) + (byte & 15), r, byte / static_cast<int>(sizeof(T)));
       }
+    };
+    auto each_piece = [&](auto units_tag, auto&& use) {
+      some_pieces(units_tag, 0, std::integral_constant<int, decltype(units_tag)::value * 16 / static_cast<int>(sizeof(Piece))>{}, use);
     };
     auto first_row = [&](int tile_m) { return tile_m * 256 + rank * 128 + quarter * 32; };
     // scales and bias of a tile's columns that this warp works on
@@ -590,11 +593,12 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
         if constexpr (!kBulk) {
           const int col0 = tile_n * bn + c0;
           if (residual == nullptr || col0 >= n_end) return;
-          const T* from = residual + static_cast<int64_t>(row0) * p.n + col0;
+          constexpr int kRows = 32 / (kUnits * 16 / static_cast<int>(sizeof(Piece)));  // that the lanes cover at a time
+          const T* from = nullptr;
           each_piece(std::integral_constant<int, kUnits>{}, [&](int i, uint32_t, int r, int element) {
+            from = i == 0 ? residual + static_cast<int64_t>(row0 + r) * p.n + col0 + element : from + kRows * static_cast<int64_t>(p.n);
             Piece value = {};
-            if (row0 + r < p.m && col0 + element < n_end)
-              value = *reinterpret_cast<const Piece*>(from + static_cast<int64_t>(r) * p.n + element);
+            if (row0 + r < p.m && col0 + element < n_end) value = *reinterpret_cast<const Piece*>(from);
             ahead[i] = value;
           });
         }
@@ -654,24 +658,34 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
             tma_store_2d_if(lane == 0 && row0 < p.m, &y_map, stage_tile, to_col, row0);
           } else {
             __syncwarp();
-            T* to = out + static_cast<int64_t>(row0) * out_cols + to_col;
-            Piece values[decltype(units_tag)::value * 16 / sizeof(Piece)];
-            each_piece(units_tag, [&](int i, uint32_t from, int, int) {
-              Piece& value = values[i];
-              if constexpr (sizeof(Piece) == 4)
-                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(value) : "r"(from));
-              else
-                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(value) : "r"(from));
-            });
-            if (row0 + 32 <= p.m && col0 + 32 <= n_end) {  // (a chunk that lies in y needs no questions)
-              each_piece(units_tag, [&](int i, uint32_t, int r, int element) {
-                *reinterpret_cast<Piece*>(to + static_cast<int64_t>(r) * out_cols + element) = values[i];
+            T* to = nullptr;
+            constexpr int kRows = 32 / (decltype(units_tag)::value * 16 / static_cast<int>(sizeof(Piece)));
+            auto next_row = [&](int piece, int r, int element) {
+              to = piece == 0 ? out + static_cast<int64_t>(row0 + r) * out_cols + to_col + element : to + kRows * static_cast<int64_t>(out_cols);
+            };
+            const bool whole = row0 + 32 <= p.m && col0 + 32 <= n_end;  // (a chunk that lies in y needs no questions)
+            constexpr int kEach = decltype(units_tag)::value * 16 / static_cast<int>(sizeof(Piece));
+            std::integral_constant<int, (kEach < 8 ? kEach : 8)> many;
+#pragma unroll
+            for (int first = 0; first < kEach; first += 8) {
+              Piece values[8];
+              some_pieces(units_tag, first, many, [&](int i, uint32_t from, int, int) {
+                if constexpr (sizeof(Piece) == 4)
+                  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(values[i]) : "r"(from));
+                else
+                  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(values[i]) : "r"(from));
               });
-            } else {
-              each_piece(units_tag, [&](int i, uint32_t, int r, int element) {
-                if (row0 + r < p.m && element < width)
-                  *reinterpret_cast<Piece*>(to + static_cast<int64_t>(r) * out_cols + element) = values[i];
-              });
+              if (whole) {
+                some_pieces(units_tag, first, many, [&](int i, uint32_t, int r, int element) {
+                  next_row(first + i, r, element);
+                  *reinterpret_cast<Piece*>(to) = values[i];
+                });
+              } else {
+                some_pieces(units_tag, first, many, [&](int i, uint32_t, int r, int element) {
+                  next_row(first + i, r, element);
+                  if (row0 + r < p.m && element < width) *reinterpret_cast<Piece*>(to) = values[i];
+                });
+              }
             }
           }
         };
@@ -775,7 +789,7 @@ bool make_code_map(CUtensorMap* map, const void* base, int64_t rows, int64_t k, 
 // What either kernel takes, to a few microseconds, from what was measured: a k-block of the stream kernel 0.2 us and 0.42
 // more at 256 rows, its epilogue 2.5 us at 256 rows (256 x 18944 x 3584: 27.9 us in 112 CTAs of 37 k-blocks; 256 x 512 x 18944:
 // 8.4 in 4); of the pair kernel 0.26 us at 128 columns and 0.35 at 256 (257 x 18944 x 3584: 41.8 us in one round of 148
-// k-blocks; 1407 x 3488 x 25: 10.6 in 28), an epilogue of 3.3 us a tile beside the products of the next.
+// k-blocks; 1407 x 3488 x 25: 10.6 in 28), an epilogue of 2.8 us a tile beside the products of the next.
 constexpr double kStreamEpilogue[] = {4.5, 15.0, 7.0};  // none, residual, SwiGLU
 struct StreamPlan { int cols, chunks, slices; double us; };
 StreamPlan plan_stream(int64_t m, int64_t k, int64_t n, int epilogue) {
@@ -805,7 +819,7 @@ PairPlan plan_pair(int64_t m, int64_t k, int64_t n) {
     if (rounds * bn >= best) continue;
     best = rounds * bn;
     const double tile = blocks * 0.26 * (256 + bn) / 384;
-    plan = {bn, 3.5 + std::max(tile, 2.0) + (rounds - 1) * std::max(tile, 3.3)};
+    plan = {bn, 3.5 + std::max(tile, 2.0) + (rounds - 1) * std::max(tile, 2.8)};
   }
   return plan;
 }
