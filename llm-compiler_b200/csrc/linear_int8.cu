@@ -354,7 +354,9 @@ linear_int8_stream_kernel(const Int8LinearParams p, const __grid_constant__ CUte
 }
 
 // -------------------------------------------------------------------------------------------------------------- pair ----
-constexpr int kPairStageBytes = 2 * 128 * 128;  // half of 256 rows of x, half of up to 256 of the weight
+// A stage: half of 256 rows of x, half of a tile's columns of the weight.
+__host__ __device__ constexpr int pair_stage_bytes(int bn) { return (128 + bn / 2) * 128; }
+constexpr int kPairStagesAtMost = 8;
 constexpr int kPairWarps = 8;      // of the epilogue, for each quarter of the accumulator's lanes
 constexpr int kAcross = kPairWarps / 4, kStep = kAcross * 32, kChunksAtMost = (8 + kAcross - 1) / kAcross;  // a quarter's warps share the columns
 constexpr int kPairThreads = (kPairWarps + 2) * 32;
@@ -363,10 +365,10 @@ constexpr int kPairThreads = (kPairWarps + 2) * 32;
 template <typename T, typename Piece>
 __host__ __device__ constexpr int pair_tiles() { return sizeof(Piece) < 16 ? 1 : sizeof(T) == 4 ? 2 : 3; }
 template <typename T, typename Piece>
-__host__ __device__ constexpr int pair_stages() { return (sizeof(Piece) < 16 ? 6 : 5) - (sizeof(T) == 4 ? 1 : 0); }
+__host__ __device__ constexpr int pair_ring() { return ((sizeof(Piece) < 16 ? 6 : 5) - (sizeof(T) == 4 ? 1 : 0)) * pair_stage_bytes(256); }
 template <typename T, typename Piece>
 constexpr int pair_smem() {
-  return pair_stages<T, Piece>() * kPairStageBytes +
+  return pair_ring<T, Piece>() +
          kPairWarps * (pair_tiles<T, Piece>() * 32 * 32 * static_cast<int>(sizeof(T)) + kChunksAtMost * 32 * 8);
 }
 
@@ -390,16 +392,16 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
                         const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap y_map,
                         const __grid_constant__ CUtensorMap residual_map) {
   constexpr bool kBulk = sizeof(Piece) == 16;
-  constexpr int kPairStages = pair_stages<T, Piece>(), kTiles = pair_tiles<T, Piece>();
+  constexpr int kRing = pair_ring<T, Piece>(), kTiles = pair_tiles<T, Piece>();
   extern __shared__ __align__(1024) unsigned char smem[];
-  __shared__ __align__(8) uint64_t full[kPairStages], empty[kPairStages], acc_full[2], acc_empty[2];
+  __shared__ __align__(8) uint64_t full[kPairStagesAtMost], empty[kPairStagesAtMost], acc_full[2], acc_empty[2];
   __shared__ __align__(8) uint64_t arrived[kPairWarps * kTiles];  // a residual's chunks
   __shared__ uint32_t tmem_slot;
   __shared__ int failed;
 
   grid_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = cluster_cta_rank();
-  const int bn = p.cols, half = bn / 2;
+  const int bn = p.cols, half = bn / 2, stage_bytes = pair_stage_bytes(bn), stages = min(kRing / stage_bytes, kPairStagesAtMost);
   const uint32_t smem_base = smem_u32(smem);
   const int nkb = (p.k + kBK - 1) / kBK;
   const int tiles_n = (p.n + bn - 1) / bn, tiles_m = (p.m + 255) / 256, tiles = tiles_n * tiles_m;
@@ -422,7 +424,7 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
 
   if (threadIdx.x == 0) {
     failed = 0;
-    for (int s = 0; s < kPairStages; ++s) {
+    for (int s = 0; s < stages; ++s) {
       mbarrier_init(smem_u32(&full[s]), 1);
       mbarrier_init(smem_u32(&empty[s]), 1);
     }
@@ -458,15 +460,15 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
       for (int kb = 0; kb < nkb; ++kb) {
         if (turn > 0 && !mbarrier_wait_warp(smem_u32(&empty[s]), (turn - 1) & 1, p.wait_limit)) {
           ok = false;
-          if (rank == 0) wait_for_copies(full, kPairStages, s, turn, p.wait_limit);
+          if (rank == 0) wait_for_copies(full, stages, s, turn, p.wait_limit);
           break;
         }
-        const uint32_t dst = smem_base + s * kPairStageBytes;
+        const uint32_t dst = smem_base + s * stage_bytes;
         if (rank == 0) mbarrier_arrive_expect_tx_if(leader, smem_u32(&full[s]), 2 * (128 + half) * 128);
         const uint32_t bar = map_to_rank(smem_u32(&full[s]), 0);
         tma_load_pair_if(leader, dst, &x_map, bar, kb * kBK, tile_m * 256 + rank * 128);
         tma_load_pair_if(leader, dst + 128 * 128, &w_map, bar, kb * kBK, tile_n * bn + rank * half);
-        if (++s == kPairStages) { s = 0; ++turn; }
+        if (++s == stages) { s = 0; ++turn; }
       }
     }
     if (!ok) failed = 1;
@@ -484,13 +486,13 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
       for (int kb = 0; kb < nkb; ++kb) {
         if (!mbarrier_wait_warp(smem_u32(&full[s]), turn & 1, p.wait_limit)) { ok = false; break; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint64_t a_desc = smem_descriptor(smem_base + s * kPairStageBytes), b_desc = descriptor_advance(a_desc, 128 * 128);
+        const uint64_t a_desc = smem_descriptor(smem_base + s * stage_bytes), b_desc = descriptor_advance(a_desc, 128 * 128);
 #pragma unroll
         for (int q = 0; q < kBK / 32; ++q)
           umma_i8_if<2>(leader, d, descriptor_advance(a_desc, q * 32), descriptor_advance(b_desc, q * 32), idesc,
                         (kb > 0 || q > 0) ? 1u : 0u);
         umma_commit_pair_if(leader, smem_u32(&empty[s]));
-        if (++s == kPairStages) { s = 0; ++turn; }
+        if (++s == stages) { s = 0; ++turn; }
       }
       if (ok) umma_commit_pair_if(leader, smem_u32(&acc_full[acc]));
     }
@@ -507,8 +509,8 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
     constexpr int kVec = 16 / static_cast<int>(sizeof(T)), kUnits = 32 / kVec;  // of 16 bytes: a row of a chunk
     const int quarter = warp & 3, turn0 = warp >> 2;
     constexpr int kStageTile = 32 * 32 * static_cast<int>(sizeof(T));
-    const uint32_t stage_tiles = smem_base + kPairStages * kPairStageBytes + warp * kTiles * kStageTile;
-    float* column_terms = reinterpret_cast<float*>(smem + kPairStages * kPairStageBytes + kPairWarps * kTiles * kStageTile) + warp * kChunksAtMost * 64;
+    const uint32_t stage_tiles = smem_base + kRing + warp * kTiles * kStageTile;
+    float* column_terms = reinterpret_cast<float*>(smem + kRing + kPairWarps * kTiles * kStageTile) + warp * kChunksAtMost * 64;
     const uint32_t acc_empty_first = map_to_rank(smem_u32(&acc_empty[0]), 0);
     uint32_t stage_tile = stage_tiles;
     // 16-byte unit `unit` of row r of a chunk with `units` of them: 128 bytes of rows side by side never share a bank (the
@@ -788,7 +790,7 @@ bool make_code_map(CUtensorMap* map, const void* base, int64_t rows, int64_t k, 
 
 // What either kernel takes, to a few microseconds, from what was measured: a k-block of the stream kernel 0.2 us and 0.42
 // more at 256 rows, its epilogue 2.5 us at 256 rows (256 x 18944 x 3584: 27.9 us in 112 CTAs of 37 k-blocks; 256 x 512 x 18944:
-// 8.4 in 4); of the pair kernel 0.26 us at 128 columns and 0.35 at 256 (257 x 18944 x 3584: 41.8 us in one round of 148
+// 8.4 in 4); of the pair kernel 0.25 us at 128 columns and 0.345 at 256 (257 x 18944 x 3584: 41.8 us in one round of 148
 // k-blocks; 1407 x 3488 x 25: 10.6 in 28), an epilogue of 2.8 us a tile beside the products of the next.
 constexpr double kStreamEpilogue[] = {4.5, 15.0, 7.0};  // none, residual, SwiGLU
 struct StreamPlan { int cols, chunks, slices; double us; };
@@ -810,18 +812,15 @@ StreamPlan plan_stream(int64_t m, int64_t k, int64_t n, int epilogue) {
 }
 struct PairPlan { int cols; double us; };
 PairPlan plan_pair(int64_t m, int64_t k, int64_t n) {
-  // columns of a tile: the fewest column-steps over all rounds of the GPU's pairs
   const int64_t tiles_m = ceil_div(m, 256), blocks = ceil_div(k, kBK);
-  int64_t best = INT64_MAX;
-  PairPlan plan = {0, 0.0};
+  PairPlan best = {0, 1e30};
   for (int bn = 256; bn >= 128; bn -= 32) {
     const int64_t rounds = ceil_div(tiles_m * ceil_div(n, bn), kNumSMs / 2);
-    if (rounds * bn >= best) continue;
-    best = rounds * bn;
-    const double tile = blocks * 0.26 * (256 + bn) / 384;
-    plan = {bn, 3.5 + std::max(tile, 2.0) + (rounds - 1) * std::max(tile, 2.8)};
+    const double share = bn / 256.0, products = blocks * (0.155 + 0.19 * share);
+    const double us = 3.5 + std::max(products, 2.0) + (rounds - 1) * std::max(products, 2.8 * share);
+    if (us < 0.99 * best.us) best = {bn, us};
   }
-  return plan;
+  return best;
 }
 
 template <typename T>
