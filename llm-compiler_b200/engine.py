@@ -394,6 +394,23 @@ class Qwen2Engine(ServingEngine):
         self._block_slack = min(min(-(-(n + size) // size) * size, self.capacity) - n
                                 for n in self._host_lengths)
 
+    def fork(self, source: int, target: int) -> None:
+        """Paged layout: sequence `target` gives back what it holds and continues as a second branch of `source`, between
+        steps: whole blocks are shared, a last one that is partly full is copied, and the next input token is the same (set
+        `input_ids[target]` to branch)."""
+
+        if not self.paged:
+            raise ExecutionError("fork needs the paged KV layout")
+        if not (0 <= source < self.batch and 0 <= target < self.batch) or source == target:
+            raise ExecutionError("fork needs two different sequences of this engine")
+        self.state.release(target)
+        self._host_lengths[target] = 0
+        self.state.fork(source, target, tokens=self._host_lengths[source])
+        self.input_ids[target] = self.input_ids[source]
+        self._host_lengths[target] = self._host_lengths[source]
+        self._block_slack = 0
+        self._reserve_blocks()
+
     def sync_host_lengths(self) -> None:
         """Re-reads the context lengths from the device (one synchronising copy): for callers
         that set the length vectors themselves."""
@@ -414,6 +431,8 @@ class Qwen2Engine(ServingEngine):
 
         saved_lengths = self.state._length_arena.clone()
         saved_ids = self.input_ids.clone()
+        if self.quantized:
+            self.positions.fill_(-1)  # (nothing is stored: a row leaves its mark on the scale of its block)
         self._decode_step()
         self.state._length_arena.copy_(saved_lengths)
         self.input_ids.copy_(saved_ids)

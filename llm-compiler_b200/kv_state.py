@@ -322,7 +322,8 @@ class PagedKVCacheState(PreallocatedKVCacheState):
         """Makes the empty sequence `target` a continuation of the first `tokens` cached tokens of `source` (default: all
         of its lengths, read from the device, which synchronises). Whole blocks are shared; a last block that is only partly
         full is copied in every layer, one launch, so that either sequence may append to its own. Host-side, between
-        steps; every layer slot's length of `target` becomes `tokens`."""
+        steps; every layer slot's length of `target` becomes `tokens`, and its extra length rows stand as far from that as
+        the source's from its own length."""
 
         sequences = len(self._host_table)
         if not (0 <= source < sequences and 0 <= target < sequences) or source == target:
@@ -338,14 +339,15 @@ class PagedKVCacheState(PreallocatedKVCacheState):
         if partial and not self._free:
             raise ExecutionError("the KV block pool is exhausted")
         row = held[:whole]
+        if partial:
+            quantized_kernels.b200_copy_kv_blocks(self._pools, [held[whole]], [self._free[-1]])
         for block in row:
             self._sharers[block] = self._sharers.get(block, 1) + 1
-        if partial:
-            row = row + [self._free.pop()]
-            quantized_kernels.b200_copy_kv_blocks(self._pools, [held[whole]], [row[-1]])
-        self._host_table[target] = row
+        self._host_table[target] = row + ([self._free.pop()] if partial else [])
         self._write_table()
-        self._length_arena[:len(self.keys), target] = tokens
+        arena, layers = self._length_arena, len(self.keys)
+        arena[layers:, target] = arena[layers:, source] + (tokens - arena[0, source])
+        arena[:layers, target] = tokens
 
     def compact(self) -> int:
         """Moves blocks so that those in use are the lowest of the pool, one launch, and returns their number: what is

@@ -130,6 +130,30 @@ def test_fork_shares_whole_blocks_and_copies_a_partial_one(copies):
     assert state._host_table[0] == [] and state.blocks_in_use() == 2
 
 
+def test_fork_keeps_the_distances_of_the_extra_length_rows(copies):
+    """(an engine's positions and attention lengths stand behind the layers' rows)"""
+    state = PagedKVCacheState.allocate_paged(num_layers=2, batch=3, max_tokens=160, block_size=32, num_blocks=12, kv_heads=2,
+                                             head_dim=64, dtype=torch.bfloat16, device="cpu", extra_length_rows=2)
+    state.reserve([70, 33, 0])
+    state._length_arena.copy_(torch.tensor([[70, 33, 0], [70, 33, 0], [70, 33, 0], [71, 34, 1]]))
+    state.fork(0, 2)
+    assert state._length_arena[:, 2].tolist() == [70, 70, 70, 71] and state._length_arena[:, 0].tolist() == [70, 70, 70, 71]
+    state.release(2)
+    state.fork(0, 2, tokens=40)
+    assert state._length_arena[:, 2].tolist() == [40, 40, 40, 41]
+
+
+def test_a_fork_whose_copy_fails_changes_nothing(monkeypatch):
+    state = make_state()
+    state.reserve([70, 0, 0, 0])
+    def fails(*arguments):
+        raise RuntimeError("launch")
+    monkeypatch.setattr(quantized_kernels, "b200_copy_kv_blocks", fails)
+    with pytest.raises(RuntimeError):
+        state.fork(0, 1, tokens=70)
+    assert state._host_table == [[0, 1, 2], [], [], []] and state._sharers == {} and len(state._free) == 9
+
+
 def test_fork_refusals_change_nothing(copies):
     state = make_state(num_blocks=5)
     state.reserve([70, 33, 0, 0])

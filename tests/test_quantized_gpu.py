@@ -397,10 +397,12 @@ def test_waits_that_run_out_set_the_status_and_leave_the_next_calls_right():
     query, lengths = torch.randn(2, 4, 1, 64, generator=g).bfloat16().cuda(), torch.tensor([500, 100]).cuda()
     cases = [lambda s=s: b200.b200_paged_decode_attention_8bit(query, *pools, *scales, table.cuda(), lengths, None, scale=0.125,
                                                                split_tokens=s) for s in (0, 40, 512)]
-    for m, k, n in ((8, 256, 512), (8, 1024, 128), (300, 512, 512)):
+    for m, k, n in ((8, 256, 512), (8, 1024, 128), (300, 512, 512), (300, 2048, 200), (1024, 512, 2048), (1024, 512, 2050)):
         values, weight = (torch.randint(-127, 128, (r, k), generator=g, dtype=torch.int8).cuda() for r in (m, n))
-        cases.append(lambda a=(values, torch.rand(m, generator=g).cuda(), weight, torch.rand(n, generator=g).cuda()):
-                     b200.b200_linear_int8(*a))
+        a = (values, torch.rand(m, generator=g).cuda(), weight, torch.rand(n, generator=g).cuda())
+        cases.append(lambda a=a: b200.b200_linear_int8(*a))
+        residual = torch.randn(m, n, generator=g).bfloat16().cuda()
+        cases.append(lambda a=a, r=residual: b200.b200_linear_int8(*a, residual=r, epilogue="residual"))
     want = [case() for case in cases]
     kernels.runtime().check_status()
     library = _lib.load()
@@ -430,7 +432,7 @@ def test_calls_without_rows_launch_nothing():
 
 
 # ----------------------------------------------------------------------------------------------------------------- copy ----
-@pytest.mark.parametrize("shape", [(128, 64), (32, 256), (96, 24), (7, 3)])
+@pytest.mark.parametrize("shape", [(128, 64), (32, 256), (96, 24), (37, 31), (7, 3)])
 def test_copied_blocks_hold_what_their_sources_hold_and_the_others_keep_theirs(shape):
     g = torch.Generator().manual_seed(shape[0])
     layers, blocks, heads = 3, 40, 2
@@ -569,6 +571,42 @@ def test_linear_sums_are_exact_up_to_the_largest(m):
 @pytest.mark.parametrize("epilogue", ["none", "residual", "swiglu"])
 def test_linear_of_prompts(m, k, n, epilogue):
     check_linear(torch.Generator().manual_seed(m), m, k, n, epilogue, bias=epilogue != "residual")
+
+
+@pytest.mark.parametrize("m,k,n", [(300, 2048, 200), (900, 4096, 37), (1025, 3584, 520), (3068, 1424, 106), (258, 18944, 130)])
+@pytest.mark.parametrize("epilogue", ["none", "residual", "swiglu"])
+def test_linear_of_many_rows_against_a_narrow_weight(m, k, n, epilogue):
+    """(rows in chunks, K slices of a chunk where that fills the GPU)"""
+    n -= n % 2 if epilogue == "swiglu" else 0
+    check_linear(torch.Generator().manual_seed(m + n), m, k, n, epilogue, bias=True, dtype=torch.float16 if n % 4 else torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("epilogue", ["none", "residual", "swiglu"])
+@pytest.mark.parametrize("m,k,n", [(260, 256, 20000), (260, 256, 20008), (260, 80, 20004), (260, 80, 20006), (260, 80, 20003),
+                                   (2600, 144, 7976), (2600, 144, 7970)])
+def test_linear_whose_pairs_take_several_tiles(m, k, n, epilogue, dtype):
+    """Rows of y on multiples of 16, 8, 4 and 2 bytes, each pair of SMs with a few tiles, rows and columns that end inside one."""
+    n -= n % 2 if epilogue == "swiglu" else 0
+    check_linear(torch.Generator().manual_seed(m + n), m, k, n, epilogue, bias=epilogue != "none", dtype=dtype)
+
+
+def test_linear_of_a_prompt_sums_exactly_up_to_the_largest():
+    check_linear(torch.Generator().manual_seed(0), 300, 131056, 1040, dtype=torch.float32, extreme=True)
+
+
+@pytest.mark.parametrize("rows", [8, 600])
+@pytest.mark.parametrize("offset", [1, 2, 4, 8])
+def test_linear_residual_that_starts_anywhere(rows, offset):
+    """A residual that is a slice of a longer vector: the result does not depend on where it starts."""
+    g = torch.Generator().manual_seed(offset)
+    values, weight = (torch.randint(-127, 128, (r, 256), generator=g, dtype=torch.int8).cuda() for r in (rows, 1024))
+    scales = [torch.rand(r, generator=g).cuda() for r in (rows, 1024)]
+    whole = torch.randn(rows * 1024 + 16, generator=g).bfloat16().cuda()
+    part = whole[offset:offset + rows * 1024].view(rows, 1024)
+    one, other = (b200.b200_linear_int8(values, scales[0], weight, scales[1], residual=residual, epilogue="residual")
+                  for residual in (part, part.clone()))
+    assert torch.equal(one, other)
 
 
 def test_linear_keeps_leading_dimensions_and_passes_nan_scales_on():
@@ -758,6 +796,48 @@ def test_an_engine_serves_from_a_cache_in_8_bits(cache, weights_dtype):
         make(kv_dtype=cache)
     with pytest.raises(ValueError, match="8 bits"):
         make(kv_layout="paged", kv_dtype=torch.int16)
+
+
+@pytest.mark.parametrize("cache", [None, torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("tokens", [64, 77])
+def test_an_engine_forks_a_sequence(cache, tokens):
+    """A branch gives the tokens of the sequence it comes from while its input does, another input moves it alone; capturing
+    a step stores nothing in an 8-bit cache."""
+    config = q2.Qwen2Config(hidden_size=256, intermediate_size=512, num_layers=2, num_heads=4, num_kv_heads=2, rms_norm_eps=1e-6,
+                            rope_theta=1e6, vocab_size=512, tie_word_embeddings=True)
+    weights = {k: v.cuda() for k, v in q2.make_weights(config, seed=1, dtype=torch.bfloat16).items()}
+    prompt = q2.make_prompt_ids(config, 3, tokens, seed=2)
+    make = lambda: Qwen2Engine(config, weights, batch=3, capacity=160, kv_layout="paged", block_size=32, kv_dtype=cache)
+    engine, apart = make(), make()
+    expected = apart.generate(prompt, 24)
+    engine.prefill(prompt)
+    if cache is not None:
+        pools = [pool.clone() for pool in engine.state._pools]
+        engine.capture()
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(pools, engine.state._pools))
+    else:
+        engine.capture()
+    rows = [engine.input_ids.clone()]  # (next_ids holds the warm-up's)
+    for step in range(24):
+        if step == 5:
+            engine.fork(0, 2)
+        rows.append(engine.decode_step().clone())
+    rows = torch.stack(rows, dim=1)
+    assert torch.equal(rows[:2], expected[:2])                                  # the others go on as they would have
+    assert torch.equal(rows[2, :6], expected[2, :6]) and torch.equal(rows[2, 6:], expected[0, 6:])
+    assert engine.state.blocks_in_use() < sum(len(row) for row in engine.state._host_table)
+    engine.prefill(prompt)                                                      # shared blocks are given back
+    assert engine.state._sharers == {}
+    engine.fork(1, 0)
+    engine.input_ids[0] = (engine.input_ids[1] + 1) % 512
+    rows = torch.stack([engine.decode_step().clone() for _ in range(8)], dim=1)
+    assert torch.equal(rows[1], expected[1, 1:9])
+    engine.state.check()
+    for arguments in ((1, 1), (0, 9), (0, -1)):
+        with pytest.raises(ExecutionError):
+            engine.fork(*arguments)
+    with pytest.raises(ExecutionError, match="paged"):
+        Qwen2Engine(config, weights, batch=2, capacity=64).fork(0, 1)
 
 
 @pytest.mark.parametrize("layout", [{}, dict(kv_layout="paged", block_size=32), dict(kv_layout="paged", block_size=32, kv_dtype=torch.int8)])
