@@ -69,7 +69,7 @@ extern "C" {
  * partial-sum, folded-norm and cluster split-K forms, projections of a few rows, fp32 projections that stream their
  * weight, with or without the norm, grouped projections and the routing of experts, the two reduce_* consumers, decode,
  * prompt and latent attention, per-head products, RMS norms, RoPE with the KV store, the choice of tokens, the hybrid
- * layers' steps; every other kernel, advance_lengths /
+ * layers' steps, all kernels for serving in 8 bits; every other kernel, advance_lengths /
  * embedding / rope table among them, is always
  * launched fully serialised, which is what makes lengths[] stable before the attention's wait).
  * Thread-local: two engines driven from two threads do not see each other's promises; launches
@@ -764,7 +764,7 @@ int b200_advance_slots(int64_t* lengths, const int32_t* slots, const int32_t* st
  *   y = input                                                 norm_weight NULL (weights, or rows without a norm);
  *   y = r * rsqrt(mean(r^2) + epsilon) * norm_weight          r = input, or round(input + residual), written to `sum`
  * (which may be input or residual itself). A row whose y is not finite gets scale NaN and codes 0. dtype of input,
- * residual, sum and norm_weight: any.
+ * residual, sum and norm_weight: any; rows of up to 2^30 elements.
  *
  * b200_linear_int8: y[m, n] = (sum_k x[m, k] weight[n, k]) x_scales[m] weight_scales[n] + bias[n], sums in 32-bit integers
  * (exact), then the epilogue in fp32 and one rounding to dtype: B200_EPILOGUE_RESIDUAL adds residual[m, n];

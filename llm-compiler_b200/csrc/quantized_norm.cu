@@ -199,7 +199,6 @@ cudaError_t quantize_typed(const QuantParams& p, cudaStream_t stream) {
                       (!p.weight || aligned16(p.weight)) &&
                       (!p.residual || (aligned16(p.residual) && p.residual_stride % per == 0 && aligned16(p.sum)));
   const int64_t items = vector ? p.hidden / per : p.hidden;
-  if (items > INT32_MAX / 2) return cudaErrorInvalidValue;
   // A thread keeps four loads (of 16 bytes, or eight elements); with few rows there are threads to spare, and one each is
   // over sooner.
   const int64_t each = p.rows > 2 * kNumSMs ? (vector ? 4 : 8) : 1;
@@ -227,7 +226,7 @@ extern "C" int b200_quantize_rows_int8(const b200_quantize_rows_call* call, void
   if (!c.input || !c.codes || !c.scales || c.rows < 0 || c.hidden <= 0 || c.input_row_stride < c.hidden ||
       (c.residual && (!c.sum || c.residual_row_stride < c.hidden)) || c.dtype != dtype || !known_dtype(dtype))
     return B200_ERR_BAD_ARGUMENT;
-  if (c.rows > 0x7fffffff) return B200_ERR_TOO_LARGE;
+  if (c.rows > 0x7fffffff || c.hidden > (1 << 30)) return B200_ERR_TOO_LARGE;
   if (c.rows == 0) return B200_OK;
   QuantParams p = {};
   p.x = c.input; p.residual = c.residual; p.weight = c.norm_weight; p.sum = c.residual ? c.sum : nullptr;

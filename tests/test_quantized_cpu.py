@@ -74,6 +74,7 @@ def test_quantised_rows_and_linear_refusals():
 
     assert rows(x=None) == rows(residual=FAKE) == rows(hidden=0) == rows(stride=63) == rows(dtype=_lib.I8) == \
         _lib.ERR_BAD_ARGUMENT
+    assert rows(n=1 << 31) == rows(hidden=1 << 31, stride=1 << 31) == _lib.ERR_TOO_LARGE
     assert rows(n=0) == 0
 
     def linear(x=FAKE, weight=FAKE, residual=None, m=4, k=64, n=8, dtype=_lib.BF16, epilogue=0):
