@@ -25,7 +25,8 @@ struct QuantParams {
 
 // One row per CTA. kVector: rows in 16-byte loads, kKept of them a thread in registers; what is longer is read again.
 // What bounds it is memory: a thread asks for all it keeps of x, the residual and the weight before it uses any (four loads
-// of each at 512 bytes a warp; 16384 x 3584 bf16 with a residual: 168 us with one each). A code is the low byte of
+// of each at 512 bytes a warp; 16384 x 3584 bf16 with a residual: 168 us with one each, 61 with four, 6.7 TB/s; without one
+// 37 us, 4.8 TB/s: too few bytes between a row's reduction and the next row's loads). A code is the low byte of
 // y * inverse + 1.5 * 2^23, which rounds to the nearest integer, ties to even: one operation instead of clamps and a
 // conversion (|y * inverse| <= 127 (1 + 2^-22) by construction).
 __device__ __forceinline__ float max_or_nan(float a, float b) {  // (NaN if either is)
@@ -74,7 +75,15 @@ __global__ void __launch_bounds__(512) quantize_rows_kernel(const QuantParams p)
   };
   // r (stored where there is a residual) times the weight; its squares and its largest magnitude on the way
   float squares = 0.0f, most = 0.0f;
-  auto work = [&](int i, const Item& in, const Item& other, const Item& w, float (&y)[per]) {
+  auto weighted = [&](const Item& w, float (&y)[per]) {
+    if constexpr (kNorm) {
+      float f[per];
+      values(w, f);
+#pragma unroll
+      for (int e = 0; e < per; ++e) y[e] *= f[e];
+    }
+  };
+  auto work = [&](int i, Item& in, const Item& other, const Item& w, float (&y)[per]) {
     values(in, y);
     if constexpr (kResidual) {
       float r[per];
@@ -85,25 +94,28 @@ __global__ void __launch_bounds__(512) quantize_rows_kernel(const QuantParams p)
         Vec16<T> t;
 #pragma unroll
         for (int e = 0; e < per; ++e) t.v[e] = y[e];
-        t.store(sum + i * per);
+        t.store(in.v);
+        *reinterpret_cast<uint4*>(sum + i * per) = *reinterpret_cast<const uint4*>(&in);
       } else {
-        Elem<T>::store(sum + i, y[0]);
+        Elem<T>::store(in.v, y[0]);
+        sum[i] = in.v[0];
       }
     }
 #pragma unroll
-    for (int e = 0; e < per; ++e) squares = fmaf(y[e], y[e], squares);
-    if constexpr (kNorm) {
-      float f[per];
-      values(w, f);
-#pragma unroll
-      for (int e = 0; e < per; ++e) y[e] *= f[e];
-    }
+    for (int e = 0; e < per; ++e)
+      if constexpr (kNorm) squares = fmaf(y[e], y[e], squares);
+    weighted(w, y);
 #pragma unroll
     for (int e = 0; e < per; ++e) most = max_or_nan(most, fabsf(y[e]));
   };
-  float kept[kKept][per];
+  // What a thread keeps. With a residual r, as narrow as it came (y is one product away): registers for more CTAs, which
+  // wait for three operands (16384 x 3584: 67 us with y kept, 61 with r). Without one y: there the instructions count
+  // (37 us with y kept, 40 with r, 47 with two floats an instruction).
+  constexpr bool kNarrow = kResidual && per == 8;
+  Item in[kKept];
+  float kept[kNarrow ? 1 : kKept][per];
   {
-    Item in[kKept], other[kKept], w[kKept];
+    Item other[kKept], w[kKept];
 #pragma unroll
     for (int j = 0; j < kKept; ++j) {
       const int i = threadIdx.x + j * threads;
@@ -126,16 +138,16 @@ __global__ void __launch_bounds__(512) quantize_rows_kernel(const QuantParams p)
 #pragma unroll
     for (int j = 0; j < kKept; ++j) {
       const int i = threadIdx.x + j * threads;
-      if (i < items) work(i, in[j], other[j], w[j], kept[j]);
+      if (i < items) work(i, in[j], other[j], w[j], kept[kNarrow ? 0 : j]);
     }
   }
   for (int i = threadIdx.x + kKept * threads; i < items; i += threads) {
-    Item in, other, w;
-    float y[per];
-    load(x, i, in);
+    Item more, other, w;
+    load(x, i, more);
     if constexpr (kResidual) load(residual, i, other);
     if constexpr (kNorm) load(weight, i, w);
-    work(i, in, other, w, y);
+    float y[per];
+    work(i, more, other, w, y);
   }
   squares = warp_sum(squares);
 #pragma unroll
@@ -171,24 +183,26 @@ __global__ void __launch_bounds__(512) quantize_rows_kernel(const QuantParams p)
       codes[i] = fine ? static_cast<int8_t>(code_of(y[0], inverse)) : int8_t(0);
     }
   };
+  auto put_again = [&](const Item& r, int i) {
+    float y[per];
+    Item w;
+    values(r, y);
+    if constexpr (kNorm) load(weight, i, w);
+    weighted(w, y);
+    put(y, i);
+  };
 #pragma unroll
   for (int j = 0; j < kKept; ++j) {
     const int i = threadIdx.x + j * threads;
-    if (i < items) put(kept[j], i);
+    if (i < items) {
+      if constexpr (kNarrow) put_again(in[j], i);
+      else put(kept[j], i);
+    }
   }
   for (int i = threadIdx.x + kKept * threads; i < items; i += threads) {
-    Item in, w;
-    float y[per];
-    load(kResidual ? sum : x, i, in);  // (this thread's own store)
-    values(in, y);
-    if constexpr (kNorm) {
-      float f[per];
-      load(weight, i, w);
-      values(w, f);
-#pragma unroll
-      for (int e = 0; e < per; ++e) y[e] *= f[e];
-    }
-    put(y, i);
+    Item r;
+    load(kResidual ? sum : x, i, r);  // (this thread's own store)
+    put_again(r, i);
   }
 }
 
