@@ -12,10 +12,13 @@
 //   that keeps more SMs busy than the other kernel's tiles.) A CTA per SM takes whole tiles in turn; where there are fewer tiles
 //   than SMs, the K slices of a tile are the CTAs of a cluster, which add their sums through distributed shared memory
 //   (4.0 us less than integer additions in global memory at 64 x 384 x 512, where the slices then wait for one another there).
+//   48 x 3584 x 37888 SwiGLU: 25 us, 5.5 TB/s, 0.85 of a copy's rate; a call of a few tiles takes 4 to 5 us whatever its size.
 // linear_int8_pair_kernel, beyond: bound by the tensor cores. Two SMs work on one tile of 256 rows x up to 256 columns
 //   (cta_group::2): each holds half of both operands, which halves the bytes that shared memory and L2 deliver per product
 //   (at 128 x 256 a CTA they are what limits it: 96 of 128 bytes a cycle in, as many out). Two accumulators alternate, so
-//   the epilogue of a tile runs under the products of the next.
+//   the epilogue of a tile runs under the products of the next. 4096 x 3584 x 37888 SwiGLU: 324 us, 3.4 POP/s, the tensor
+//   pipe busy 97 % of the time; below K of some 1000 the epilogue (2.8 us a tile) is what is seen: 16384 x 896 x 9728 SwiGLU
+//   124 us where the products alone take 79.
 #include <algorithm>
 #include <type_traits>
 
@@ -385,7 +388,7 @@ template <int kLeft>
 __device__ __forceinline__ void stores_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kLeft) : "memory"); }
 
 // Piece: uint4 where rows of y start on multiples of 16 bytes: chunks of y leave, and those of a residual come, by TMA (with
-// the warps' own loads and stores of 16 bytes BEFORE). Else what a lane moves of a row at a time, 4 bytes or 2.
+// the warps' own loads and stores of 16 bytes 16384 x 128 x 9728 with a residual takes 204 us, so 139). Else what a lane moves of a row at a time, 4 bytes or 2.
 template <typename T, typename Piece>
 __global__ void __launch_bounds__(kPairThreads, 1)
 linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtensorMap x_map,
@@ -790,8 +793,11 @@ bool make_code_map(CUtensorMap* map, const void* base, int64_t rows, int64_t k, 
 
 // What either kernel takes, to a few microseconds, from what was measured: a k-block of the stream kernel 0.2 us and 0.42
 // more at 256 rows, its epilogue 2.5 us at 256 rows (256 x 18944 x 3584: 27.9 us in 112 CTAs of 37 k-blocks; 256 x 512 x 18944:
-// 8.4 in 4); of the pair kernel 0.25 us at 128 columns and 0.345 at 256 (257 x 18944 x 3584: 41.8 us in one round of 148
-// k-blocks; 1407 x 3488 x 25: 10.6 in 28), an epilogue of 2.8 us a tile beside the products of the next.
+// 8.4 in 4); of the pair kernel 0.25 us at 128 columns and 0.345 at 256 (257 x 18944 x 3584: 37.8 us in one round of 148
+// k-blocks; 1407 x 3488 x 25: 10.6 in 28), an epilogue of 2.8 us a tile beside the products
+// of the next; the stream kernel's runs behind them, and where a CTA has several tiles it takes 4.5 us each, 7 with SwiGLU,
+// 15 with a residual (6065 x 128 x 15736: 323 us there, 110 in pairs). Wide tiles need fewer bytes for a product and narrow ones
+// fewer rounds: 5632 x 1280 x 18432 97 us at 256 columns, 127 at 128; 4096 x 18944 x 3584 194 at 256, 217 at 160.
 constexpr double kStreamEpilogue[] = {4.5, 15.0, 7.0};  // none, residual, SwiGLU
 struct StreamPlan { int cols, chunks, slices; double us; };
 StreamPlan plan_stream(int64_t m, int64_t k, int64_t n, int epilogue) {

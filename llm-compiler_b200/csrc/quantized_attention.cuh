@@ -28,6 +28,11 @@
 // of 32), is contiguous in the pool, and is one box for K and one for V. Warps merge through shared memory. Up to eight
 // splits are a cluster, whose CTAs merge through distributed shared memory; more leave partials in the workspace, which the
 // CTA that arrives last adds in split order. Either way results do not depend on timing.
+//
+// Measured: 64 x 4096 tokens, 2 heads of 64 (67 MB): 16.7 us, 4.0 TB/s; 64 ragged to 8192, 4 heads of 128 (270 MB): 52 us,
+// 5.2 TB/s; 3 x 30001, 8 heads of 128 with a mask (185 MB): 36 us, 5.1 TB/s; 1 x 1000: 5.3 us. A CTA streams nothing for some
+// 5 us at its start and end (length, table row, first copies; merge, exchange in the cluster, stores), which is what is left
+// beside the rate: in between the SMs' rings keep 96 KB and more in flight.
 #pragma once
 
 #include <algorithm>
