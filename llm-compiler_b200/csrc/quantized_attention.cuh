@@ -30,7 +30,7 @@
 // CTA that arrives last adds in split order. Either way results do not depend on timing.
 //
 // Measured: 64 x 4096 tokens, 2 heads of 64 (67 MB): 16.7 us, 4.0 TB/s; 64 ragged to 8192, 4 heads of 128 (270 MB): 52 us,
-// 5.2 TB/s; 3 x 30001, 8 heads of 128 with a mask (185 MB): 36 us, 5.1 TB/s; 1 x 1000: 5.3 us. A CTA streams nothing for some
+// 5.2 TB/s; 3 x 30001, 8 heads of 128 with a mask (185 MB): 36 us, 5.1 TB/s; 1 x 1000: 5.0 us. A CTA streams nothing for some
 // 5 us at its start and end (length, table row, first copies; merge, exchange in the cluster, stores), which is what is left
 // beside the rate: in between the SMs' rings keep 96 KB and more in flight.
 #pragma once
@@ -69,6 +69,7 @@ struct Params {
   int cluster;     // the splits are a cluster
   int sorted;      // CTAs take the sequences from the longest to the shortest
   int q_vector;    // rows of q may be read 16 bytes at a time
+  uint64_t block_magic;  // 2^40 / tiles of a block, rounded up: tile * it >> 40 is the tile's block (tiles below 2^25, blocks of up to 2^15)
   float scale;
   uint32_t wait_limit;
   int drop_loads;
@@ -132,6 +133,19 @@ __device__ __forceinline__ float load_mask(const Params& p, int64_t i) {
   return __half2float(static_cast<const __half*>(p.mask)[i]);
 }
 
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void store_cluster_f32x4(uint32_t local_smem_addr, int rank, const float4& v) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local_smem_addr), "r"(rank));
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(remote), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+__device__ __forceinline__ void store_cluster_f32x2(uint32_t local_smem_addr, int rank, const float2& v) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local_smem_addr), "r"(rank));
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(remote), "f"(v.x), "f"(v.y) : "memory");
+}
+
 template <int D>
 struct Shape {
   static constexpr int kTile = 32;                             // tokens of a tile (D 128: 16 and a fourth CTA, 37 -> 41 us at 3 x 30001)
@@ -142,6 +156,14 @@ struct Shape {
   static constexpr int kStages = D == 128 ? 2 : 3;  // (shorter rings, more CTAs: 61 us where 96 KB of rings take 72, ragged to 8192)
   static constexpr int kResident(int n_tiles) { return D == 256 ? 1 : D == 64 && n_tiles == 1 ? 4 : 3; }  // CTAs of an SM
   static constexpr int kRingBytes = kWarps * kStages * 2 * kTileBytes;
+  // What the CTAs of a cluster give this one: beside the ring where it fits without costing a CTA, else in it
+  __host__ __device__ static constexpr int kGivenBytes(int n_tiles) { return n_tiles * 8 * D * 4 + 128; }
+  __host__ __device__ static constexpr bool kBeside(int n_tiles) { return !(D == 128 && n_tiles == 2); }
+  __host__ __device__ static constexpr int kPartBytes(int n_tiles) { return kWarps * n_tiles * 8 * D * 4; }
+  __host__ __device__ static constexpr int kGivenAt(int n_tiles) { return kBeside(n_tiles) ? kRingBytes : kPartBytes(n_tiles); }
+  static constexpr int kBytes(int n_tiles) {
+    return kBeside(n_tiles) ? kRingBytes + kGivenBytes(n_tiles) : std::max(kRingBytes, kPartBytes(n_tiles) + kGivenBytes(n_tiles));
+  }
   // byte offset of 16-byte chunk `chunk` of row `row` in a tile
   __device__ static uint32_t at(int row, int chunk) {
     if (D == 64) return row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
@@ -162,7 +184,7 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
   extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ __align__(8) uint64_t full[kWarps * kStages];
   __shared__ float merge_m[kWarps][kHeads], merge_l[kWarps][kHeads];
-  __shared__ float joined[kHeads][2];  // this CTA's maximum and sum
+  __shared__ __align__(8) float2 joined[8][kHeads];  // of the cluster's CTAs: their maximum and sum
   __shared__ int last_flag;
   __shared__ __align__(16) int row_cache[kTableCache];
 
@@ -172,8 +194,8 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
   int64_t b = blockIdx.z;
   const int head0 = kv * p.group + hb * p.block_heads;
   const int heads = min(p.block_heads, p.group - hb * p.block_heads);
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < kWarps * kStages; ++s) mbarrier_init(smem_u32(&full[s]), 1);
+  if (lane == 0) {
+    for (int s = 0; s < kStages; ++s) mbarrier_init(smem_u32(&full[warp * kStages + s]), 1);
     fence_mbarrier_init();
   }
   const int tiles_per_block = p.block_size / kTile, my_first = split * kWarps + warp;
@@ -220,6 +242,8 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
   const int length = static_cast<int>(length64), tiles = (length + kTile - 1) / kTile;
   const int active = max(min((tiles + kWarps - 1) / kWarps, p.num_splits), 1);  // splits with a tile for each warp
   if (split >= active) return;  // (a cluster's barriers do not wait for CTAs that have left)
+  const bool alone = active == 1;
+  if (S::kBeside(NT) && p.cluster && !alone) cluster_arrive();  // this CTA's memory is there
   const int stride = kWarps * active;
   const int mine = tiles > my_first ? (tiles - my_first + stride - 1) / stride : 0;
 
@@ -229,7 +253,7 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
   auto look_up = [&](int it) {
     Window w = {-1, 0, 0.0f, 0.0f};
     if (it >= mine) return w;
-    const int tile = my_first + it * stride, column = tile / tiles_per_block;
+    const int tile = my_first + it * stride, column = static_cast<int>(tile * p.block_magic >> 40);
     const int block = column < kTableCache ? row_cache[column] : table[column];
     if (block < 0 || block >= p.num_blocks) {
       bad = true;
@@ -529,6 +553,7 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
       }
     }
   __syncthreads();  // every ring is done with
+  if (!S::kBeside(NT) && p.cluster && !alone) cluster_arrive();
   float* parts = reinterpret_cast<float*>(smem);  // [warp][head][D]
 #pragma unroll
   for (int t = 0; t < NT; ++t)
@@ -555,7 +580,14 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
     value.z = fmaf(weight, part.z, value.z); value.w = fmaf(weight, part.w, value.w);
   };
   auto weight_of = [&](float one, float top) { return one == -INFINITY ? 0.0f : exp2_fast((one - top) * kToLog2); };
-  const bool alone = active == 1;
+  // In a cluster each CTA finishes every `active`-th run of four, and is given the others' parts of those: stores to another
+  // SM are over sooner than loads from it, and nobody reads from a CTA that would like to leave (1 x 1000: 5.3 us with loads).
+  float4* given = reinterpret_cast<float4*>(smem + S::kGivenAt(NT));  // [CTA][runs of this one]
+  const int runs = heads * (D / 4), own_runs = (runs + active - 1) / active;
+  if (p.cluster && !alone) {
+    __syncwarp();
+    cluster_wait();  // the others' memory is there
+  }
   for (int e = threadIdx.x; e < heads * (D / 4); e += kThreads) {
     const int head = e / (D / 4), d = e % (D / 4) * 4;
     float top = -INFINITY, sum = 0.0f;
@@ -568,12 +600,11 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
                *reinterpret_cast<const float4*>(parts + (w * kHeads + head) * D + d), sum, value);
     if (alone) {
       if (split == 0) put_out(head, d, value, sum);
-    } else if (p.cluster) {  // (each place of the first warp's part is read by the thread that writes it)
-      *reinterpret_cast<float4*>(parts + head * D + d) = value;
-      if (d == 0) {
-        joined[head][0] = top;
-        joined[head][1] = sum;
-      }
+    } else if (p.cluster) {
+      const int local = e / active;
+      store_cluster_f32x4(smem_u32(given + split * own_runs + local), e - local * active, value);
+      if (d == 0)
+        for (int i = 0; i < active; ++i) store_cluster_f32x2(smem_u32(&joined[split][head]), i, make_float2(top, sum));
     } else {
       const int64_t part = (item * p.num_splits + split) * p.block_heads + head;
       *reinterpret_cast<float4*>(p.ws_o + part * D + d) = value;
@@ -587,34 +618,17 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
     if (alone) return;
     __syncwarp();
     cluster_sync();
-    for (int e = threadIdx.x * active + split; e < heads * (D / 4); e += kThreads * active) {
-      const int head = e / (D / 4), d = e % (D / 4) * 4;
-      float2 ml[8];
-      float4 part[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (i >= active) break;
-        const float4 both = load_cluster_f32x4(smem_u32(parts + head * D + d), i);
-        part[i] = both;
-        ml[i].x = load_cluster_f32(smem_u32(&joined[head][0]), i);
-        ml[i].y = load_cluster_f32(smem_u32(&joined[head][1]), i);
-      }
+    for (int local = threadIdx.x; local * active + split < runs; local += kThreads) {
+      const int e = local * active + split, head = e / (D / 4), d = e % (D / 4) * 4;
       float top = -INFINITY, sum = 0.0f;
       float4 value = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (i >= active) break;
-        top = fmaxf(top, ml[i].x);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (i >= active) break;
-        add_part(weight_of(ml[i].x, top), ml[i].y, part[i], sum, value);
+      for (int i = 0; i < active; ++i) top = fmaxf(top, joined[i][head].x);
+      for (int i = 0; i < active; ++i) {
+        const float2 ml = joined[i][head];
+        add_part(weight_of(ml.x, top), ml.y, given[i * own_runs + local], sum, value);
       }
       put_out(head, d, value, sum);
     }
-    __syncwarp();
-    cluster_sync();  // (the others may still read this CTA's part)
     return;
   }
   if (alone) return;
@@ -675,7 +689,7 @@ int launch_shape(const Params& p, const void* keys, const void* values, int64_t 
   if (!make_pool_map<D>(&key_map, keys, p.num_blocks * p.kv_heads, p.block_size) ||
       !make_pool_map<D>(&value_map, values, p.num_blocks * p.kv_heads, p.block_size))
     return B200_ERR_UNSUPPORTED;
-  constexpr int smem = std::max(Shape<D>::kRingBytes, kWarps * 8 * NT * D * 4);
+  constexpr int smem = std::max(Shape<D>::kBytes(NT), Shape<D>::kPartBytes(NT));
   auto kernel = cache_attention_kernel<T, Code, D, NT, kMask>;
   static std::atomic<uint64_t> allowed{0};
   if (!allow_shared_memory(kernel, smem, allowed)) return B200_ERR_LAUNCH;
