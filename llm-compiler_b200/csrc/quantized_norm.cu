@@ -25,8 +25,9 @@ struct QuantParams {
 
 // One row per CTA. kVector: rows in 16-byte loads, kKept of them a thread in registers; what is longer is read again.
 // What bounds it is memory: a thread asks for all it keeps of x, the residual and the weight before it uses any (four loads
-// of each at 512 bytes a warp; 16384 x 3584 bf16 with a residual: 168 us with one each, 61 with four, 6.7 TB/s; without one
-// 37 us, 4.8 TB/s: too few bytes between a row's reduction and the next row's loads). A code is the low byte of
+// of each at 512 bytes a warp; 16384 x 3584 bf16 with a residual: 168 us with one each, 61 with four, 6.7 TB/s). Without
+// a residual a CTA takes rows in turn and asks for the next one before it reduces this one (16384 x 3584: 36.8 -> 35.6 us, 4.9
+// TB/s; 2048 x 16384 fp16 30.3 -> 21.4; what is left are the registers that hold a row twice). A code is the low byte of
 // y * inverse + 1.5 * 2^23, which rounds to the nearest integer, ties to even: one operation instead of clamps and a
 // conversion (|y * inverse| <= 127 (1 + 2^-22) by construction).
 __device__ __forceinline__ float max_or_nan(float a, float b) {  // (NaN if either is)
@@ -47,9 +48,10 @@ template <typename T, bool kVector, bool kResidual, bool kNorm, int kKept>
 __global__ void __launch_bounds__(512) quantize_rows_kernel(const QuantParams p) {
   constexpr int per = kVector ? Elem<T>::kPerVec : 1;
   grid_launch_dependents();
-  __shared__ float parts[2][16];
+  constexpr bool kLoop = kVector && !kResidual;
+  __shared__ float parts[2][2][16];
   const int threads = blockDim.x, warps = threads >> 5;
-  const int64_t row = blockIdx.x;
+  int64_t row = blockIdx.x;
   const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
   const T* residual = p.residual ? static_cast<const T*>(p.residual) + row * p.residual_stride : nullptr;
   const T* weight = static_cast<const T*>(p.weight);
@@ -74,7 +76,7 @@ __global__ void __launch_bounds__(512) quantize_rows_kernel(const QuantParams p)
     }
   };
   // r (stored where there is a residual) times the weight; its squares and its largest magnitude on the way
-  float squares = 0.0f, most = 0.0f;
+  float squares, most;
   auto weighted = [&](const Item& w, float (&y)[per]) {
     if constexpr (kNorm) {
       float f[per];
@@ -112,97 +114,94 @@ __global__ void __launch_bounds__(512) quantize_rows_kernel(const QuantParams p)
   // wait for three operands (16384 x 3584: 67 us with y kept, 61 with r). Without one y: there the instructions count
   // (37 us with y kept, 40 with r, 47 with two floats an instruction).
   constexpr bool kNarrow = kResidual && per == 8;
-  Item in[kKept];
-  float kept[kNarrow ? 1 : kKept][per];
-  {
-    Item other[kKept], w[kKept];
+  Item in[kKept], other[kKept], weights[kKept];
+  auto load_kept = [&](const T* from, Item (&items_of)[kKept]) {
 #pragma unroll
     for (int j = 0; j < kKept; ++j) {
       const int i = threadIdx.x + j * threads;
-      if (i < items) load(x, i, in[j]);
+      if (i < items) load(from, i, items_of[j]);
     }
-    if constexpr (kResidual) {
-#pragma unroll
-      for (int j = 0; j < kKept; ++j) {
-        const int i = threadIdx.x + j * threads;
-        if (i < items) load(residual, i, other[j]);
-      }
-    }
-    if constexpr (kNorm) {
-#pragma unroll
-      for (int j = 0; j < kKept; ++j) {
-        const int i = threadIdx.x + j * threads;
-        if (i < items) load(weight, i, w[j]);
-      }
-    }
+  };
+  load_kept(x, in);
+  if constexpr (kResidual) load_kept(residual, other);
+  if constexpr (kNorm) load_kept(weight, weights);
+  for (int turn = 0;; turn ^= 1) {
+    squares = most = 0.0f;
+    float kept[kNarrow ? 1 : kKept][per];
 #pragma unroll
     for (int j = 0; j < kKept; ++j) {
       const int i = threadIdx.x + j * threads;
-      if (i < items) work(i, in[j], other[j], w[j], kept[kNarrow ? 0 : j]);
+      if (i < items) work(i, in[j], other[j], weights[j], kept[kNarrow ? 0 : j]);
     }
-  }
-  for (int i = threadIdx.x + kKept * threads; i < items; i += threads) {
-    Item more, other, w;
-    load(x, i, more);
-    if constexpr (kResidual) load(residual, i, other);
-    if constexpr (kNorm) load(weight, i, w);
-    float y[per];
-    work(i, more, other, w, y);
-  }
-  squares = warp_sum(squares);
+    if constexpr (kLoop)
+      if (row + gridDim.x < p.rows) load_kept(x + gridDim.x * p.x_stride, in);
+    for (int i = threadIdx.x + kKept * threads; i < items; i += threads) {
+      Item more, other, w;
+      load(x, i, more);
+      if constexpr (kResidual) load(residual, i, other);
+      if constexpr (kNorm) load(weight, i, w);
+      float y[per];
+      work(i, more, other, w, y);
+    }
+    squares = warp_sum(squares);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) most = max_or_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
-  if (warps > 1) {
-    if ((threadIdx.x & 31) == 0) {
-      parts[0][threadIdx.x >> 5] = squares;
-      parts[1][threadIdx.x >> 5] = most;
+    for (int o = 16; o > 0; o >>= 1) most = max_or_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (warps > 1) {
+      if ((threadIdx.x & 31) == 0) {
+        parts[turn][0][threadIdx.x >> 5] = squares;
+        parts[turn][1][threadIdx.x >> 5] = most;
+      }
+      __syncthreads();
+      squares = 0.0f;
+      for (int w = 0; w < warps; ++w) {
+        squares += parts[turn][0][w];
+        most = max_or_nan(most, parts[turn][1][w]);
+      }
     }
-    __syncthreads();
-    squares = 0.0f;
-    for (int w = 0; w < warps; ++w) {
-      squares += parts[0][w];
-      most = max_or_nan(most, parts[1][w]);
+    const bool fine = most < INFINITY;
+    const float inverse = fine && most > 0.0f ? fminf(__fdiv_rn(127.0f, most), 3.0e38f) : 0.0f;
+    if (threadIdx.x == 0) {
+      float scale = most * (1.0f / 127.0f);
+      if (kNorm && most > 0.0f) scale *= rsqrtf(squares / static_cast<float>(p.hidden) + p.epsilon);
+      p.scales[row] = fine ? scale : NAN;
     }
-  }
-  const bool fine = most < INFINITY;
-  const float inverse = fine && most > 0.0f ? fminf(__fdiv_rn(127.0f, most), 3.0e38f) : 0.0f;
-  if (threadIdx.x == 0) {
-    float scale = most * (1.0f / 127.0f);
-    if (kNorm && most > 0.0f) scale *= rsqrtf(squares / static_cast<float>(p.hidden) + p.epsilon);
-    p.scales[row] = fine ? scale : NAN;
-  }
-  auto put = [&](const float (&y)[per], int i) {
-    if constexpr (kVector) {
-      uint32_t packed[per / 4];
+    auto put = [&](const float (&y)[per], int i) {
+      if constexpr (kVector) {
+        uint32_t packed[per / 4];
 #pragma unroll
-      for (int q = 0; q < per / 4; ++q)
-        packed[q] = fine ? four_codes(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3], inverse) : 0u;
-      if constexpr (per == 8) *reinterpret_cast<uint2*>(codes + i * 8) = make_uint2(packed[0], packed[1]);
-      else *reinterpret_cast<uint32_t*>(codes + i * 4) = packed[0];
-    } else {
-      codes[i] = fine ? static_cast<int8_t>(code_of(y[0], inverse)) : int8_t(0);
-    }
-  };
-  auto put_again = [&](const Item& r, int i) {
-    float y[per];
-    Item w;
-    values(r, y);
-    if constexpr (kNorm) load(weight, i, w);
-    weighted(w, y);
-    put(y, i);
-  };
+        for (int q = 0; q < per / 4; ++q)
+          packed[q] = fine ? four_codes(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3], inverse) : 0u;
+        if constexpr (per == 8) *reinterpret_cast<uint2*>(codes + i * 8) = make_uint2(packed[0], packed[1]);
+        else *reinterpret_cast<uint32_t*>(codes + i * 4) = packed[0];
+      } else {
+        codes[i] = fine ? static_cast<int8_t>(code_of(y[0], inverse)) : int8_t(0);
+      }
+    };
+    auto put_again = [&](const Item& r, int i) {
+      float y[per];
+      Item w;
+      values(r, y);
+      if constexpr (kNorm) load(weight, i, w);
+      weighted(w, y);
+      put(y, i);
+    };
 #pragma unroll
-  for (int j = 0; j < kKept; ++j) {
-    const int i = threadIdx.x + j * threads;
-    if (i < items) {
-      if constexpr (kNarrow) put_again(in[j], i);
-      else put(kept[j], i);
+    for (int j = 0; j < kKept; ++j) {
+      const int i = threadIdx.x + j * threads;
+      if (i < items) {
+        if constexpr (kNarrow) put_again(in[j], i);
+        else put(kept[j], i);
+      }
     }
-  }
-  for (int i = threadIdx.x + kKept * threads; i < items; i += threads) {
-    Item r;
-    load(kResidual ? sum : x, i, r);  // (this thread's own store)
-    put_again(r, i);
+    for (int i = threadIdx.x + kKept * threads; i < items; i += threads) {
+      Item r;
+      load(kResidual ? sum : x, i, r);  // (this thread's own store)
+      put_again(r, i);
+    }
+    row += gridDim.x;
+    if (!kLoop || row >= p.rows) return;
+    x += gridDim.x * p.x_stride;
+    codes += gridDim.x * p.hidden;
   }
 }
 
@@ -217,11 +216,19 @@ cudaError_t quantize_typed(const QuantParams& p, cudaStream_t stream) {
   // over sooner.
   const int64_t each = p.rows > 2 * kNumSMs ? (vector ? 4 : 8) : 1;
   const int threads = static_cast<int>(std::min<int64_t>(512, ceil_div(ceil_div(items, each), 32) * 32));
-  const dim3 grid(static_cast<unsigned>(p.rows)), block(static_cast<unsigned>(threads));
+  const dim3 block(static_cast<unsigned>(threads));
   const auto launch = [&](auto with_residual, auto with_norm) {
     constexpr bool kResidual = decltype(with_residual)::value, kNorm = decltype(with_norm)::value;
-    return vector ? launch_chained(quantize_rows_kernel<T, true, kResidual, kNorm, 4>, grid, block, 0, stream, p)
-                  : launch_chained(quantize_rows_kernel<T, false, kResidual, kNorm, 8>, grid, block, 0, stream, p);
+    dim3 grid(static_cast<unsigned>(p.rows));
+    if (!vector) return launch_chained(quantize_rows_kernel<T, false, kResidual, kNorm, 8>, grid, block, 0, stream, p);
+    auto kernel = quantize_rows_kernel<T, true, kResidual, kNorm, 4>;
+    if (!kResidual && p.rows > 2 * kNumSMs) {  // CTAs that take rows in turn: as many as there is room for
+      int resident = 0;
+      const cudaError_t error = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, threads, 0);
+      if (error != cudaSuccess) return error;
+      grid.x = static_cast<unsigned>(std::min<int64_t>(p.rows, static_cast<int64_t>(kNumSMs) * std::max(resident, 1)));
+    }
+    return launch_chained(kernel, grid, block, 0, stream, p);
   };
   if (p.residual != nullptr)
     return p.weight != nullptr ? launch(std::true_type{}, std::true_type{}) : launch(std::true_type{}, std::false_type{});

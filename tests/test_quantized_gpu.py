@@ -511,6 +511,29 @@ def test_norm_of_strided_higher_rank_and_unaligned_inputs():
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,hidden,stride", [(5200, 1024, 1024), (1500, 3584, 3600), (450, 20000, 20000)])
+def test_rows_that_a_cta_takes_in_turn(dtype, rows, hidden, stride):
+    """More rows than CTAs: each row is its own, whatever was in front of it; rows of zeros and of NaN among them."""
+    g = torch.Generator().manual_seed(hidden)
+    x = torch.randn(rows, stride, generator=g)[:, :hidden] * torch.exp2(torch.arange(rows) % 13 - 6.0)[:, None]
+    x[7::100] = 0
+    x = x.to(dtype)
+    weight = (1 + 0.2 * torch.randn(hidden, generator=g)).to(dtype)
+    bad = list(range(11, rows, 150))
+    whole = torch.zeros(rows, stride, dtype=dtype, device="cuda")
+    whole[:, :hidden] = x.cuda()
+    on = whole[:, :hidden]
+    on[bad, 3] = math.nan
+    good = torch.ones(rows, dtype=torch.bool)
+    good[bad] = False
+    _, y = ref.norm(x, None, weight, 1e-6)
+    for (codes, scales), want, slack in ((b200.b200_rms_norm_int8(on, weight.cuda(), epsilon=1e-6)[:2], y, hidden / 2 + 8),
+                                         (b200.b200_quantize_rows_int8(on), x.double(), 2)):
+        assert bool(scales[bad].isnan().all()) and not bool(codes[bad].any())
+        check_rows(codes.cpu()[good], scales.cpu()[good], want[good], slack * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 def test_rows_without_a_norm_and_rows_that_are_not_finite(dtype):
     g = torch.Generator().manual_seed(2)
     x = (torch.randn(9, 272, generator=g) * torch.exp2(torch.arange(9.0) * 2 - 8)[:, None]).to(dtype)
