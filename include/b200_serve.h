@@ -79,7 +79,7 @@ extern "C" {
  * B200_LAUNCH_PROGRAMMATIC: each of those kernels may become resident before its predecessor
  * in the stream has finished and waits on the device (griddepcontrol.wait) before touching
  * any tensor; results are unchanged. B200_LAUNCH_CONSTANT_WEIGHTS additionally lets the
- * linear kernels, the per-head products (b200_head_linear), the experts' router and b200_reduce_residual_rms_norm fetch
+ * linear kernels (of up to 128 rows in 8-bit integers), the per-head products (b200_head_linear), the experts' router and b200_reduce_residual_rms_norm fetch
  * their weight operands before that wait: only valid while no kernel that writes a weight tensor is in flight on the
  * device. B200_LAUNCH_STABLE_KV_PREFIX lets decode attention
  * read lengths[] and request the KV rows below lengths[b] - 1 before the wait: valid when the

@@ -48,6 +48,7 @@ struct Int8LinearParams {
   int stages;   // stream
   int slices;   // stream: of K, the CTAs of a cluster
   int n_fastest;  // pair: order of the tiles
+  int ahead;      // stream: the weight may be read while what is in front of the kernel still runs
   uint32_t wait_limit;
   int drop_loads;
 };
@@ -167,6 +168,18 @@ linear_int8_stream_kernel(const Int8LinearParams p, const __grid_constant__ CUte
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_base = tmem_slot;
+  // Where the weight may be read ahead (a step's projections, launched while the kernel in front still runs), the ring's
+  // stages are asked for before the wait, all but their rows of x.
+  int ahead = 0;
+  if (p.ahead && warp == kEpilogueWarps && !p.drop_loads) {
+    const uint32_t leader = elect_one();
+    ahead = min(stages, nkb * ((tiles - tile_first + tile_step - 1) / tile_step));
+    for (int s = 0, tile = tile_first, kb = 0; s < ahead; ++s) {
+      mbarrier_arrive_expect_tx_if(leader, smem_u32(&full[s]), stage_bytes);
+      tma_load_2d_if(leader, smem_base + s * stage_bytes, &w_map, smem_u32(&full[s]), (kb_first + kb) * kBK, tile * 128);
+      if (++kb == nkb) { kb = 0; tile += tile_step; }
+    }
+  }
   grid_dependency_wait();
   const bool swiglu = p.epilogue == B200_EPILOGUE_SWIGLU;
   const int64_t out_cols = swiglu ? p.n / 2 : p.n;
@@ -187,8 +200,12 @@ linear_int8_stream_kernel(const Int8LinearParams p, const __grid_constant__ CUte
           break;
         }
         const uint32_t bar = smem_u32(&full[s]), dst = smem_base + s * stage_bytes;
-        mbarrier_arrive_expect_tx_if(leader, bar, stage_bytes);
-        tma_load_2d_if(leader, dst, &w_map, bar, (kb_first + kb) * kBK, tile * 128);
+        if (ahead > 0) {
+          --ahead;
+        } else {
+          mbarrier_arrive_expect_tx_if(leader, bar, stage_bytes);
+          tma_load_2d_if(leader, dst, &w_map, bar, (kb_first + kb) * kBK, tile * 128);
+        }
         tma_load_2d_if(leader, dst + 128 * 128, &x_map, bar, (kb_first + kb) * kBK, row_first);
         if (++s == stages) { s = 0; ++turn; }
       }
@@ -834,6 +851,9 @@ int launch_stream(Int8LinearParams p, const StreamPlan& plan, const void* x, con
   p.cols = plan.cols;
   p.slices = plan.slices;
   p.stages = std::min(10, kRingBytes / ((128 + p.cols) * 128));
+  // (a decode step of 6 layers of 896, 64 rows: 315 -> 304 us; 4 layers of 3584: 8 rows 393 -> 378, 64 494 -> 484, 256 868 -> 871)
+  constexpr int kAhead = B200_LAUNCH_PROGRAMMATIC | B200_LAUNCH_CONSTANT_WEIGHTS;
+  p.ahead = (launch_mode() & kAhead) == kAhead && p.cols <= 128;
   CUtensorMap w_map, x_map;
   if (!make_code_map(&w_map, w, p.n, p.k, 128) || !make_code_map(&x_map, x, p.m, p.k, p.cols)) return B200_ERR_UNSUPPORTED;
   const int64_t tiles = ceil_div(p.n, 128);

@@ -440,15 +440,15 @@ class Qwen2Engine(ServingEngine):
     @property
     def chained(self) -> bool:
         """Whether a decode step runs the launch chain (fast bf16, up to 128 sequences)."""
-        # (the paged layout has the folded five-launch chain and the separate kernels)
+        # (the paged layout has the folded chain, five launches, seven with a cache in 8 bits, and the separate kernels)
         return self.dtype == torch.bfloat16 and self.mode == "fast" and self.batch <= 128 and \
-            (not self.paged or self.folded_norms) and not self.quantized and not self.int8_weights
+            (not self.paged or self.folded_norms) and not self.int8_weights
 
     @property
     def attention_is_fused(self) -> bool:
         """Whether the step's attention launches are the fused form (q|k|v reduction, RoPE and
         KV store inside), which serves a CTA's tokens with 16 warps at head_dim 64."""
-        return self.chained and self.fused_qkv_attention
+        return self.chained and self.fused_qkv_attention and not self.quantized
 
     def _decode_step(self) -> None:
         if self.chained:
@@ -478,7 +478,8 @@ class Qwen2Engine(ServingEngine):
         """Five launches per layer: q|k|v partials of the un-normalised x against the
         norm-folded weight -> attention (reduces q|k|v, applies the row's RMS factor, bias, RoPE,
         KV store) -> o projection (cluster split-K, + residual) -> gate|up + SwiGLU on the
-        un-normalised x with the folded weight -> down projection (cluster split-K, + residual)."""
+        un-normalised x with the folded weight -> down projection (cluster split-K, + residual).
+        With a cache in 8 bits a projection of its own, RoPE, store and attention are the first two."""
 
         cfg = self.config
         batch = self.batch
@@ -487,29 +488,36 @@ class Qwen2Engine(ServingEngine):
         x = kernels.b200_embedding(self.embed, self.input_ids)
         cosine, sine = kernels.b200_rope_table(self.positions.view(batch, 1), self.inv_freq,
                                                self.dtype)
+        x_squares = None
         for index, layer in enumerate(self.layers):
-            partials, squares = kernels.b200_linear_partial(x, layer["qkv_w_folded"],
-                                                            row_squares=True)
-            common = dict(q_heads=cfg.num_heads, scale=self.scale, split_tokens=self.split_tokens,
-                          max_length_hint=self.max_length_hint, norm_row_squares=squares,
-                          norm_hidden=cfg.hidden_size, norm_epsilon=eps,
-                          sequence_order=self.sequence_order)
-            if self.paged:
-                attn = kernels.b200_paged_qkv_decode_attention(
-                    partials, layer["qkv_b"], cosine, sine, self.state.keys[index],
-                    self.state.values[index], self.state.block_table, self.attention_lengths, **common)
+            if self.quantized:
+                qkv = kernels.b200_linear_rms_input(x, layer["qkv_w_folded"], layer["qkv_b"], epsilon=eps,
+                                                    row_squares=x_squares)
+                attn = self._attend_step(index, qkv, cosine, sine)
             else:
-                attn = kernels.b200_qkv_decode_attention(
-                    partials, layer["qkv_b"], cosine, sine, self.state.keys[index],
-                    self.state.values[index], self.attention_lengths, **common)
+                partials, squares = kernels.b200_linear_partial(x, layer["qkv_w_folded"],
+                                                                row_squares=True)
+                common = dict(q_heads=cfg.num_heads, scale=self.scale, split_tokens=self.split_tokens,
+                              max_length_hint=self.max_length_hint, norm_row_squares=squares,
+                              norm_hidden=cfg.hidden_size, norm_epsilon=eps,
+                              sequence_order=self.sequence_order)
+                if self.paged:
+                    attn = kernels.b200_paged_qkv_decode_attention(
+                        partials, layer["qkv_b"], cosine, sine, self.state.keys[index],
+                        self.state.values[index], self.state.block_table, self.attention_lengths, **common)
+                else:
+                    attn = kernels.b200_qkv_decode_attention(
+                        partials, layer["qkv_b"], cosine, sine, self.state.keys[index],
+                        self.state.values[index], self.attention_lengths, **common)
             x = kernels.b200_linear_splitk_residual(attn.view(batch, cfg.q_size), layer["o_w"], x,
                                                     row_squares=self.producer_squares)
             x, x_squares = x if self.producer_squares else (x, None)
             a = kernels.b200_linear_rms_input(x, layer["gate_up_w_folded"], epsilon=eps,
                                               epilogue="swiglu", row_squares=x_squares)
-            last = self.producer_squares and index + 1 == len(self.layers)
-            x = kernels.b200_linear_splitk_residual(a, layer["down_w"], x, row_squares=last)
-            x, x_squares = x if last else (x, None)  # (only the LM head's norm takes them)
+            # (only the LM head's norm takes them, and the q|k|v projection in front of a cache in 8 bits)
+            squares_of_down = self.producer_squares and (self.quantized or index + 1 == len(self.layers))
+            x = kernels.b200_linear_splitk_residual(a, layer["down_w"], x, row_squares=squares_of_down)
+            x, x_squares = x if squares_of_down else (x, None)
         self.logits = kernels.b200_linear_rms_input(x, self.lm_head_folded, epsilon=eps,
                                                     row_squares=x_squares)
         kernels.b200_argmax(self.logits, self.next_ids)

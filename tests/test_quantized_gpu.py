@@ -618,6 +618,29 @@ def test_linear_of_a_prompt_sums_exactly_up_to_the_largest():
     check_linear(torch.Generator().manual_seed(0), 300, 131056, 1040, dtype=torch.float32, extreme=True)
 
 
+@pytest.mark.parametrize("m,k,n,epilogue", [(64, 896, 9728, "swiglu"), (16, 4864, 896, "residual"), (8, 256, 40000, "none"),
+                                            (48, 3584, 37888, "swiglu"), (1, 64, 64, "none"), (256, 1024, 3584, "residual")])
+def test_linear_whose_weight_is_read_ahead(m, k, n, epilogue):
+    """Chained launches that may read the weight while the kernel in front, which writes the rows, still runs: the results
+    of launches one after another, whatever the rows were before."""
+    g = torch.Generator().manual_seed(m + n)
+    weight, scales = b200.b200_quantize_rows_int8(torch.randn(n, k, generator=g).bfloat16().cuda())
+    norm = torch.ones(k, dtype=torch.bfloat16, device="cuda")
+    rows = [torch.randn(m, k, generator=g).bfloat16().cuda() for _ in range(6)]
+    residual = torch.randn(m, n, generator=g).bfloat16().cuda() if epilogue == "residual" else None
+    def run(x):
+        codes, row_scales, _ = b200.b200_rms_norm_int8(x, norm, epsilon=1e-6)
+        return b200.b200_linear_int8(codes, row_scales, weight, scales, residual=residual, epilogue=epilogue)
+    want = [run(x) for x in rows]
+    torch.cuda.synchronize()
+    with kernels.launch_mode(programmatic=True, constant_weights=True, keep_variants=True):
+        got = [run(x) for x in rows]
+        codes, row_scales, _ = b200.b200_rms_norm_int8(rows[0], norm, epsilon=1e-6)
+        again = [b200.b200_linear_int8(codes, row_scales, weight, scales, residual=residual, epilogue=epilogue) for _ in range(3)]
+    assert all(torch.equal(a, b) for a, b in zip(got + again, want + 3 * want[:1]))
+    kernels.runtime().check_status()
+
+
 @pytest.mark.parametrize("rows", [8, 600])
 @pytest.mark.parametrize("offset", [1, 2, 4, 8])
 def test_linear_residual_that_starts_anywhere(rows, offset):
