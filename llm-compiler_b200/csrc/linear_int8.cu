@@ -6,19 +6,20 @@
 // anywhere along K. Both operands are K-major; a stage of the rings holds 128 codes of K, one 128-byte swizzled row each,
 // copied by TMA with zeros beyond M, N and K. Two kernels:
 //
-// linear_int8_stream_kernel, up to 256 rows (decode, short prompts): bound by the read of the weight. The WEIGHT's columns
+// linear_int8_stream_kernel, few rows (decode, short prompts): bound by the read of the weight. The WEIGHT's columns
 //   lie along the product's M (128 of them a tile) and all rows of x along its N, so every weight byte is read once and no
 //   row of x is padded beyond the next multiple of 16. (More rows against a narrow weight go in chunks of up to 256, where
 //   that keeps more SMs busy than the other kernel's tiles.) A CTA per SM takes whole tiles in turn; where there are fewer tiles
 //   than SMs, the K slices of a tile are the CTAs of a cluster, which add their sums through distributed shared memory
 //   (4.0 us less than integer additions in global memory at 64 x 384 x 512, where the slices then wait for one another there).
 //   48 x 3584 x 37888 SwiGLU: 25 us, 5.5 TB/s, 0.85 of a copy's rate; a call of a few tiles takes 4 to 5 us whatever its size.
-// linear_int8_pair_kernel, beyond: bound by the tensor cores. Two SMs work on one tile of 256 rows x up to 256 columns
+// linear_int8_pair_kernel, more rows: bound by the tensor cores. Two SMs work on one tile of 256 rows x up to 256 columns
 //   (cta_group::2): each holds half of both operands, which halves the bytes that shared memory and L2 deliver per product
 //   (at 128 x 256 a CTA they are what limits it: 96 of 128 bytes a cycle in, as many out). Two accumulators alternate, so
-//   the epilogue of a tile runs under the products of the next. 4096 x 3584 x 37888 SwiGLU: 324 us, 3.4 POP/s, the tensor
-//   pipe busy 97 % of the time; below K of some 1000 the epilogue (2.8 us a tile) is what is seen: 16384 x 896 x 9728 SwiGLU
-//   124 us where the products alone take 79.
+//   the epilogue of a tile runs under the products of the next; where there are few tiles and K is long, two to four pairs of a
+//   cluster take slices of K and add their sums through distributed shared memory (512 x 4864 x 896: 8.9 us, 10.9 without).
+//   4096 x 3584 x 37888 SwiGLU: 324 us, 3.4 POP/s, the tensor pipe busy 97 % of the time; below K of some 1000 the epilogue
+//   (2.8 us a tile) is what is seen: 16384 x 896 x 9728 SwiGLU 124 us where the products alone take 79.
 #include <algorithm>
 #include <type_traits>
 
@@ -69,11 +70,11 @@ __device__ __forceinline__ void umma_i8_if(uint32_t leader, uint32_t tmem_d, uin
                  "@q tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
                  ::"r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(leader) : "memory");
 }
-// The products so far arrive on the barrier at this offset in both CTAs of the pair.
-__device__ __forceinline__ void umma_commit_pair_if(uint32_t leader, uint32_t bar) {
-  asm volatile("{\n\t.reg .pred q;\n\t.reg .b16 both;\n\tsetp.ne.b32 q, %1, 0;\n\tmov.b16 both, 3;\n\t"
-               "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], both;\n\t}"
-               ::"r"(bar), "r"(leader) : "memory");
+// The products so far arrive on the barrier at this offset in both CTAs of the pair, whose first has rank `first`.
+__device__ __forceinline__ void umma_commit_pair_if(uint32_t leader, uint32_t bar, int first) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+               "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %2;\n\t}"
+               ::"r"(bar), "r"(leader), "h"(static_cast<uint16_t>(3 << first)) : "memory");
 }
 // A box into this CTA's memory whose bytes count on a barrier of the pair's first CTA.
 __device__ __forceinline__ void tma_load_pair_if(uint32_t leader, uint32_t dst, const void* tensor_map, uint32_t bar, int c0, int c1) {
@@ -113,7 +114,6 @@ __device__ __forceinline__ void scale_two(float& a, float& b, float row, const f
       : "+f"(a), "+f"(b) : "f"(row), "f"(t.x), "f"(t.y), "f"(t.z), "f"(t.w));
 }
 
-// ------------------------------------------------------------------------------------------------------------ stream ----
 __device__ __forceinline__ int4 load_cluster_i32x4(uint32_t remote) {
   int4 v;
   asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(remote)
@@ -121,6 +121,57 @@ __device__ __forceinline__ int4 load_cluster_i32x4(uint32_t remote) {
   return v;
 }
 
+// Four columns of a row whose sums are in shared memory of the cluster's CTAs at `addr`, CTAs `step` apart from `first`: the
+// epilogue, behind the slices of K.
+template <typename T>
+struct FourColumns {
+  int col, width;  // the first, and how many of the four there are
+  float w_scale[4], bias[4];
+  __device__ FourColumns(const Int8LinearParams& p, int col_) : col(col_), width(min(p.n - col_, 4)) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      w_scale[c] = c < width ? p.w_scales[col + c] : 0.0f;
+      bias[c] = c < width && p.bias != nullptr ? Elem<T>::load(static_cast<const T*>(p.bias) + col + c) : 0.0f;
+    }
+  }
+  template <int kSlices>
+  __device__ void finish(uint32_t addr, int first, int step, int slices, float scale, const T* residual, T* out, bool swiglu) const {
+    int4 part[kSlices];
+#pragma unroll
+    for (int i = 0; i < kSlices; ++i)
+      part[i] = i < slices ? load_cluster_i32x4(map_to_rank(addr, first + i * step)) : make_int4(0, 0, 0, 0);
+    float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (residual != nullptr) {
+      const T* from = residual + col;
+      if (width == 4) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) y[c] = Elem<T>::load(from + c);
+      } else {
+        for (int c = 0; c < width; ++c) y[c] = Elem<T>::load(from + c);
+      }
+    }
+#pragma unroll
+    for (int i = 1; i < kSlices; ++i) {
+      part[0].x += part[i].x; part[0].y += part[i].y; part[0].z += part[i].z; part[0].w += part[i].w;
+    }
+    y[0] += static_cast<float>(part[0].x) * scale * w_scale[0] + bias[0];
+    y[1] += static_cast<float>(part[0].y) * scale * w_scale[1] + bias[1];
+    y[2] += static_cast<float>(part[0].z) * scale * w_scale[2] + bias[2];
+    y[3] += static_cast<float>(part[0].w) * scale * w_scale[3] + bias[3];
+    T* to = out + (swiglu ? col / 2 : col);
+    if (swiglu) {
+      if (width > 0) Elem<T>::store(to, silu_times(y[0], y[1]));
+      if (width > 2) Elem<T>::store(to + 1, silu_times(y[2], y[3]));
+    } else if (width == 4) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) Elem<T>::store(to + c, y[c]);
+    } else {
+      for (int c = 0; c < width; ++c) Elem<T>::store(to + c, y[c]);
+    }
+  }
+};
+
+// ------------------------------------------------------------------------------------------------------------ stream ----
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 1)
 linear_int8_stream_kernel(const Int8LinearParams p, const __grid_constant__ CUtensorMap w_map,
@@ -320,48 +371,10 @@ linear_int8_stream_kernel(const Int8LinearParams p, const __grid_constant__ CUte
   if (p.slices > 1) {
     // ---- the slices' sums: this CTA finishes rows rank, rank + slices, ...; a lane takes four columns ----
     cluster_sync();
-    const int col = tile_first * 128 + 4 * lane, width = min(p.n - col, 4);
-    float w_scale[4], bias[4];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      w_scale[c] = c < width ? p.w_scales[col + c] : 0.0f;
-      bias[c] = c < width && p.bias != nullptr ? Elem<T>::load(static_cast<const T*>(p.bias) + col + c) : 0.0f;
-    }
-    for (int row = rank + warp * p.slices; row < rows; row += kThreads / 32 * p.slices) {
-      int4 part[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        part[i] = i < p.slices ? load_cluster_i32x4(map_to_rank(smem_base + row * 512 + lane * 16, i)) : make_int4(0, 0, 0, 0);
-      float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (residual != nullptr) {
-        const T* from = residual + row * out_cols + col;
-        if (width == 4) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) y[c] = Elem<T>::load(from + c);
-        } else {
-          for (int c = 0; c < width; ++c) y[c] = Elem<T>::load(from + c);
-        }
-      }
-#pragma unroll
-      for (int i = 1; i < 8; ++i) {
-        part[0].x += part[i].x; part[0].y += part[i].y; part[0].z += part[i].z; part[0].w += part[i].w;
-      }
-      const float scale = scales[row];
-      y[0] += static_cast<float>(part[0].x) * scale * w_scale[0] + bias[0];
-      y[1] += static_cast<float>(part[0].y) * scale * w_scale[1] + bias[1];
-      y[2] += static_cast<float>(part[0].z) * scale * w_scale[2] + bias[2];
-      y[3] += static_cast<float>(part[0].w) * scale * w_scale[3] + bias[3];
-      T* to = out + row * out_cols + (swiglu ? col / 2 : col);
-      if (swiglu) {
-        if (width > 0) Elem<T>::store(to, silu_times(y[0], y[1]));
-        if (width > 2) Elem<T>::store(to + 1, silu_times(y[2], y[3]));
-      } else if (width == 4) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) Elem<T>::store(to + c, y[c]);
-      } else {
-        for (int c = 0; c < width; ++c) Elem<T>::store(to + c, y[c]);
-      }
-    }
+    const FourColumns<T> four(p, tile_first * 128 + 4 * lane);
+    for (int row = rank + warp * p.slices; row < rows; row += kThreads / 32 * p.slices)
+      four.template finish<8>(smem_base + row * 512 + lane * 16, 0, 1, p.slices, scales[row],
+                              residual != nullptr ? residual + row * out_cols : nullptr, out + row * out_cols, swiglu);
     __syncwarp();
     cluster_sync();  // (the others may still read this CTA's sums)
   }
@@ -406,7 +419,8 @@ __device__ __forceinline__ void stores_read() { asm volatile("cp.async.bulk.wait
 
 // Piece: uint4 where rows of y start on multiples of 16 bytes: chunks of y leave, and those of a residual come, by TMA (with
 // the warps' own loads and stores of 16 bytes 16384 x 128 x 9728 with a residual takes 204 us, so 139). Else what a lane moves of a row at a time, 4 bytes or 2.
-template <typename T, typename Piece>
+// kSplit: K in slices, pairs of one cluster; they add their sums through distributed shared memory (a tile a cluster).
+template <typename T, typename Piece, bool kSplit>
 __global__ void __launch_bounds__(kPairThreads, 1)
 linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtensorMap x_map,
                         const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap y_map,
@@ -420,12 +434,14 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
   __shared__ int failed;
 
   grid_launch_dependents();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = cluster_cta_rank();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int place_in_cluster = cluster_cta_rank(), rank = place_in_cluster & 1, first_rank = kSplit ? place_in_cluster & ~1 : 0;
   const int bn = p.cols, half = bn / 2, stage_bytes = pair_stage_bytes(bn), stages = min(kRing / stage_bytes, kPairStagesAtMost);
   const uint32_t smem_base = smem_u32(smem);
-  const int nkb = (p.k + kBK - 1) / kBK;
+  const int slices = kSplit ? p.slices : 1, slice = first_rank >> 1, all_kb = (p.k + kBK - 1) / kBK;
+  const int kb_first = kSplit ? all_kb * slice / slices : 0, nkb = kSplit ? all_kb * (slice + 1) / slices - kb_first : all_kb;
   const int tiles_n = (p.n + bn - 1) / bn, tiles_m = (p.m + 255) / 256, tiles = tiles_n * tiles_m;
-  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int pair = blockIdx.x / (2 * slices), pairs = gridDim.x / (2 * slices);  // (kSplit: as many as tiles)
   // a pair's tiles, one after another without a division each
   struct Place {
     int tile, slow, fast, step, step_slow, step_fast, along;
@@ -485,9 +501,9 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
         }
         const uint32_t dst = smem_base + s * stage_bytes;
         if (rank == 0) mbarrier_arrive_expect_tx_if(leader, smem_u32(&full[s]), 2 * (128 + half) * 128);
-        const uint32_t bar = map_to_rank(smem_u32(&full[s]), 0);
-        tma_load_pair_if(leader, dst, &x_map, bar, kb * kBK, tile_m * 256 + rank * 128);
-        tma_load_pair_if(leader, dst + 128 * 128, &w_map, bar, kb * kBK, tile_n * bn + rank * half);
+        const uint32_t bar = map_to_rank(smem_u32(&full[s]), first_rank);
+        tma_load_pair_if(leader, dst, &x_map, bar, (kb_first + kb) * kBK, tile_m * 256 + rank * 128);
+        tma_load_pair_if(leader, dst + 128 * 128, &w_map, bar, (kb_first + kb) * kBK, tile_n * bn + rank * half);
         if (++s == stages) { s = 0; ++turn; }
       }
     }
@@ -511,13 +527,31 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
         for (int q = 0; q < kBK / 32; ++q)
           umma_i8_if<2>(leader, d, descriptor_advance(a_desc, q * 32), descriptor_advance(b_desc, q * 32), idesc,
                         (kb > 0 || q > 0) ? 1u : 0u);
-        umma_commit_pair_if(leader, smem_u32(&empty[s]));
+        umma_commit_pair_if(leader, smem_u32(&empty[s]), first_rank);
         if (++s == stages) { s = 0; ++turn; }
       }
-      if (ok) umma_commit_pair_if(leader, smem_u32(&acc_full[acc]));
+      if (ok) umma_commit_pair_if(leader, smem_u32(&acc_full[acc]), first_rank);
     }
     if (!ok) failed = 1;
-  } else if (warp < kPairWarps) {
+  } else if (kSplit && warp < kPairWarps) {
+    // ---- this slice's sums, in the place of the ring, whose stages have all been read: [row][bn], the 16-byte units of
+    // eight rows in different banks ----
+    const bool ok = __all_sync(0xffffffffu, mbarrier_wait_bounded(smem_u32(&acc_full[0]), 0, p.wait_limit));
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const int quarter = warp & 3, row = quarter * 32 + lane;
+    if (!ok) failed = 1;
+#pragma unroll 1
+    for (int c0 = (warp >> 2) * 32; ok && c0 < bn; c0 += kStep) {
+      float v[32];
+      tmem_load_32x32(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + c0, v);
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};"
+                     ::"r"(smem_base + row * bn * 4 + (((c0 / 4 + u) ^ (row & 7)) << 4)), "f"(v[4 * u]), "f"(v[4 * u + 1]),
+                       "f"(v[4 * u + 2]), "f"(v[4 * u + 3]) : "memory");
+    }
+    __syncwarp();
+  } else if (!kSplit && warp < kPairWarps) {
     // ---- epilogue: this CTA's 128 rows; lanes 32 (warp % 4) .., every other chunk of 32 columns ----
     // What comes from memory is asked for ahead: scales and bias during the tile before, a residual one chunk or two. A
     // chunk leaves through a staging tile, by TMA where rows allow it; where their length does not, the warp writes whole rows
@@ -774,6 +808,24 @@ linear_int8_pair_kernel(const Int8LinearParams p, const __grid_constant__ CUtens
     if (!ok) failed = 1;
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  if constexpr (kSplit) {
+    // ---- the slices' sums: this CTA finishes rows slice, slice + slices, ... of its half; a lane takes four columns ----
+    __syncwarp();
+    cluster_sync();
+    const bool swiglu = p.epilogue == B200_EPILOGUE_SWIGLU;
+    const int64_t out_cols = swiglu ? p.n / 2 : p.n;
+    const int tile_m = start.m(), tile_n = start.n(), row0 = tile_m * 256 + rank * 128, rows = min(128, p.m - row0);
+    const T* residual = static_cast<const T*>(p.residual);
+    for (int unit = lane; unit < bn / 4; unit += 32) {
+      const FourColumns<T> four(p, tile_n * bn + 4 * unit);
+      if (four.width <= 0) break;
+      for (int row = slice + warp * slices; row < rows; row += kPairThreads / 32 * slices)
+        four.template finish<4>(smem_base + row * bn * 4 + ((unit ^ (row & 7)) << 4), rank, 2, slices, p.x_scales[row0 + row],
+                                residual != nullptr ? residual + (row0 + row) * out_cols : nullptr,
+                                static_cast<T*>(p.out) + (row0 + row) * out_cols, swiglu);
+    }
+    __syncwarp();
+  }
   __syncthreads();
   if (threadIdx.x == 0 && failed) atomicOr(p.status, B200_STATUS_WAIT_TIMEOUT);
   cluster_sync();  // neither CTA leaves while the other may still signal it
@@ -808,13 +860,18 @@ bool make_code_map(CUtensorMap* map, const void* base, int64_t rows, int64_t k, 
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// What either kernel takes, to a few microseconds, from what was measured: a k-block of the stream kernel 0.2 us and 0.42
-// more at 256 rows, its epilogue 2.5 us at 256 rows (256 x 18944 x 3584: 27.9 us in 112 CTAs of 37 k-blocks; 256 x 512 x 18944:
-// 8.4 in 4); of the pair kernel 0.25 us at 128 columns and 0.345 at 256 (257 x 18944 x 3584: 37.8 us in one round of 148
-// k-blocks; 1407 x 3488 x 25: 10.6 in 28), an epilogue of 2.8 us a tile beside the products
-// of the next; the stream kernel's runs behind them, and where a CTA has several tiles it takes 4.5 us each, 7 with SwiGLU,
-// 15 with a residual (6065 x 128 x 15736: 323 us there, 110 in pairs). Wide tiles need fewer bytes for a product and narrow ones
-// fewer rounds: 5632 x 1280 x 18432 97 us at 256 columns, 127 at 128; 4096 x 18944 x 3584 194 at 256, 217 at 160.
+// What either kernel takes, to a few microseconds, from what was measured. Stream: a k-block 0.2 us and 0.42 more at 256 rows,
+// the epilogue 2.5 us at 256 rows (256 x 18944 x 3584: 27.9 us in 112 CTAs of 37 k-blocks; 256 x 512 x 18944: 8.4 in 4) behind
+// the products, and where a CTA has several tiles 4.5 us each, 7 with SwiGLU, 15 with a residual (6065 x 128 x 15736: 323 us
+// there, 110 in pairs). Pair: a k-block 0.25 us at 128 columns and 0.345 at 256 (1407 x 3488 x 25: 10.6 in 28), the epilogue
+// 2.8 us a tile beside the products of the next; 4 where rows of y do not start on multiples of 16 bytes, and 2.5 for the last
+// tile (910 x 288 x 577 fp32: 9.6 us, 4.5 in the stream kernel); slices of K 6 us at 256 columns (256 x 18944 x 3584 22 us in four,
+// 512 x 18944 x 3584 36 in two, 40 in one). Wide tiles need fewer bytes for a product and narrow ones fewer rounds: 5632 x 1280 x
+// 18432 97 us at 256 columns, 127 at 128; 4096 x 18944 x 3584 194 at 256, 217 at 160.
+// Clusters of `ctas` CTAs, one an SM, that the GPU holds at once (a B200 whose GPCs have lost other SMs may hold one less: of 8
+// CTAs 15 measured, 22 of 6, 33 of 4; beyond it a tile waits for a second round: 256 x 18944 x 3584 in 16 clusters of 8 37 us, in 14 22; 64 x 3584 x 4608 in 36 of 4 11.7, in 36
+// of 2 7.2).
+constexpr int64_t clusters_at_once(int64_t ctas) { return ctas > 6 ? 14 : ctas > 4 ? 21 : ctas > 2 ? 32 : ctas > 1 ? kNumSMs / 2 : kNumSMs; }
 constexpr double kStreamEpilogue[] = {4.5, 15.0, 7.0};  // none, residual, SwiGLU
 struct StreamPlan { int cols, chunks, slices; double us; };
 StreamPlan plan_stream(int64_t m, int64_t k, int64_t n, int epilogue) {
@@ -824,7 +881,7 @@ StreamPlan plan_stream(int64_t m, int64_t k, int64_t n, int epilogue) {
     const int64_t cols = ceil_div(ceil_div(m, chunks), 16) * 16, units = tiles * ceil_div(m, cols);
     // slices of K that fill the GPU where the tiles do not: clusters of 2, 4 or 8, two k-blocks a slice at least
     int64_t slices = 1;
-    while (slices < 8 && units * slices * 2 <= kNumSMs && blocks >= slices * 4) slices *= 2;
+    while (slices < 8 && units <= clusters_at_once(2 * slices) && blocks >= slices * 4) slices *= 2;
     const double share = cols / 256.0;
     const int64_t across = std::max<int64_t>(1, kNumSMs / chunks), rounds = slices > 1 ? 1 : ceil_div(tiles, across);
     const double products = ceil_div(blocks, slices) * (0.2 + 0.42 * share);
@@ -833,15 +890,21 @@ StreamPlan plan_stream(int64_t m, int64_t k, int64_t n, int epilogue) {
   }
   return best;
 }
-struct PairPlan { int cols; double us; };
-PairPlan plan_pair(int64_t m, int64_t k, int64_t n) {
+struct PairPlan { int cols, slices; double us; };  // whole_rows: rows of y start on multiples of 16 bytes
+PairPlan plan_pair(int64_t m, int64_t k, int64_t n, bool whole_rows) {
   const int64_t tiles_m = ceil_div(m, 256), blocks = ceil_div(k, kBK);
-  PairPlan best = {0, 1e30};
+  PairPlan best = {0, 0, 1e30};
   for (int bn = 256; bn >= 128; bn -= 32) {
-    const int64_t rounds = ceil_div(tiles_m * ceil_div(n, bn), kNumSMs / 2);
-    const double share = bn / 256.0, products = blocks * (0.155 + 0.19 * share);
-    const double us = 3.5 + std::max(products, 2.0) + (rounds - 1) * std::max(products, 2.8 * share);
-    if (us < 0.99 * best.us) best = {bn, us};
+    const int64_t tiles = tiles_m * ceil_div(n, bn);
+    const double share = bn / 256.0, block = 0.155 + 0.19 * share;
+    // slices of K where the tiles leave pairs idle: clusters of 4, 6 or 8 CTAs
+    for (int64_t slices = 1; slices <= 4 && (slices == 1 || (tiles <= clusters_at_once(2 * slices) && blocks >= 4 * slices)); ++slices) {
+      const int64_t rounds = slices > 1 ? 1 : ceil_div(tiles, kNumSMs / 2);
+      const double products = ceil_div(blocks, slices) * block;
+      const double us = 3.5 + std::max(products, 2.0) + (rounds - 1) * std::max(products, (whole_rows ? 2.8 : 4.0) * share) +
+                        (slices > 1 ? 1.5 + 4.5 * share : whole_rows ? 0.0 : 2.5 * std::min<int64_t>(n, bn) / 256.0);
+      if (us < 0.99 * best.us) best = {bn, static_cast<int>(slices), us};
+    }
   }
   return best;
 }
@@ -871,35 +934,37 @@ int launch_stream(Int8LinearParams p, const StreamPlan& plan, const void* x, con
 template <typename T>
 int launch_pair(Int8LinearParams p, const PairPlan& plan, const void* x, const void* w, cudaStream_t stream) {
   p.cols = plan.cols;
+  p.slices = plan.slices;
   p.n_fastest = p.n <= p.m;
   CUtensorMap x_map, w_map, y_map = {}, residual_map = {};
   if (!make_code_map(&x_map, x, p.m, p.k, 128) || !make_code_map(&w_map, w, p.n, p.k, p.cols / 2)) return B200_ERR_UNSUPPORTED;
   const int64_t tiles = ceil_div(p.m, 256) * ceil_div(p.n, p.cols);
-  const unsigned pairs = static_cast<unsigned>(std::min<int64_t>(kNumSMs / 2, tiles));
+  const unsigned pairs = static_cast<unsigned>(plan.slices > 1 ? tiles * plan.slices : std::min<int64_t>(kNumSMs / 2, tiles));
   // what every row of y and of the residual starts on a multiple of
   const uint64_t starts = static_cast<uint64_t>(p.epilogue == B200_EPILOGUE_SWIGLU ? p.n / 2 : p.n) * sizeof(T) |
                           reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.residual);
-  const auto launch = [&](auto piece) {
+  const auto launch = [&](auto piece, auto split) {
     using Piece = decltype(piece);
-    auto kernel = linear_int8_pair_kernel<T, Piece>;
+    auto kernel = linear_int8_pair_kernel<T, Piece, decltype(split)::value>;
     constexpr int kSmem = pair_smem<T, Piece>();
     static_assert(tensor_memory_fits(512, kSmem) && kSmem + 1024 <= 227 * 1024, "tensor memory under programmatic launches");
     static std::atomic<uint64_t> allowed{0};
     if (!allow_shared_memory(kernel, kSmem, allowed)) return B200_ERR_LAUNCH;
-    return launch_chained_cluster(kernel, dim3(2 * pairs), dim3(kPairThreads), kSmem, stream, 2u, p, x_map, w_map, y_map,
-                                  residual_map) == cudaSuccess ? launch_status() : B200_ERR_LAUNCH;
+    return launch_chained_cluster(kernel, dim3(2 * pairs), dim3(kPairThreads), kSmem, stream, 2u * static_cast<unsigned>(plan.slices), p,
+                                  x_map, w_map, y_map, residual_map) == cudaSuccess ? launch_status() : B200_ERR_LAUNCH;
   };
+  if (plan.slices > 1) return launch(uint32_t{}, std::true_type{});  // (rows of any alignment)
   if (starts % 16 == 0) {
     const bool swiglu = p.epilogue == B200_EPILOGUE_SWIGLU;
     if (!make_chunk_map<T>(&y_map, p.out, p.m, swiglu ? p.n / 2 : p.n, swiglu ? 16 : 32) ||
         (p.residual && !make_chunk_map<T>(&residual_map, p.residual, p.m, p.n, 32)))
       return B200_ERR_UNSUPPORTED;
-    return launch(uint4{});
+    return launch(uint4{}, std::false_type{});
   }
   if constexpr (sizeof(T) == 2) {
-    if (starts % 4 != 0) return launch(uint16_t{});
+    if (starts % 4 != 0) return launch(uint16_t{}, std::false_type{});
   }
-  return launch(uint32_t{});
+  return launch(uint32_t{}, std::false_type{});
 }
 
 }  // namespace
@@ -926,9 +991,10 @@ extern "C" int b200_linear_int8(const b200_linear_int8_call* call, void* stream)
   p.m = static_cast<int>(m); p.k = static_cast<int>(k); p.n = static_cast<int>(n); p.epilogue = static_cast<int>(c.epilogue);
   p.wait_limit = wait_limit(); p.drop_loads = drop_loads();
   const StreamPlan stream_plan = plan_stream(m, k, n, p.epilogue);
-  const PairPlan pair_plan = plan_pair(m, k, n);
-  // (what the two take is known well enough to choose where they are far apart; up to 256 rows every weight is read once)
-  const bool streamed = m <= kRowsAtMost || (stream_plan.us < 0.85 * pair_plan.us && stream_plan.chunks <= 64);
+  const int64_t row_bytes = (p.epilogue == B200_EPILOGUE_SWIGLU ? n / 2 : n) * (dtype == B200_F32 ? 4 : 2);
+  const PairPlan pair_plan = plan_pair(m, k, n, row_bytes % 16 == 0);
+  // (beyond 256 rows the stream kernel reads the weight more than once, which other work on the GPU would feel)
+  const bool streamed = m <= kRowsAtMost / 2 || (stream_plan.us < (m <= kRowsAtMost ? 1.0 : 0.95) * pair_plan.us && stream_plan.chunks <= 64);
   int code = B200_ERR_UNSUPPORTED;
   with_element_type(dtype, [&](auto tag) {
     using T = typename decltype(tag)::type;

@@ -397,7 +397,7 @@ def test_waits_that_run_out_set_the_status_and_leave_the_next_calls_right():
     query, lengths = torch.randn(2, 4, 1, 64, generator=g).bfloat16().cuda(), torch.tensor([500, 100]).cuda()
     cases = [lambda s=s: b200.b200_paged_decode_attention_8bit(query, *pools, *scales, table.cuda(), lengths, None, scale=0.125,
                                                                split_tokens=s) for s in (0, 40, 512)]
-    for m, k, n in ((8, 256, 512), (8, 1024, 128), (300, 512, 512), (300, 2048, 200), (1024, 512, 2048), (1024, 512, 2050)):
+    for m, k, n in ((8, 256, 512), (8, 1024, 128), (300, 512, 512), (300, 2048, 200), (1024, 512, 2048), (1024, 512, 2050), (250, 12000, 2500)):
         values, weight = (torch.randint(-127, 128, (r, k), generator=g, dtype=torch.int8).cuda() for r in (m, n))
         a = (values, torch.rand(m, generator=g).cuda(), weight, torch.rand(n, generator=g).cuda())
         cases.append(lambda a=a: b200.b200_linear_int8(*a))
@@ -612,6 +612,19 @@ def test_linear_whose_pairs_take_several_tiles(m, k, n, epilogue, dtype):
     """Rows of y on multiples of 16, 8, 4 and 2 bytes, each pair of SMs with a few tiles, rows and columns that end inside one."""
     n -= n % 2 if epilogue == "swiglu" else 0
     check_linear(torch.Generator().manual_seed(m + n), m, k, n, epilogue, bias=epilogue != "none", dtype=dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("epilogue", ["none", "residual", "swiglu"])
+@pytest.mark.parametrize("m,k,n", [(512, 4864, 896), (458, 9136, 1213), (520, 9136, 1800), (600, 9136, 1500), (250, 12000, 2500)])
+def test_linear_whose_k_is_cut_between_pairs(m, k, n, epilogue, dtype):
+    """Few tiles and a long K: two, three or four pairs of a cluster share a tile's products."""
+    n -= n % 2 if epilogue == "swiglu" else 0
+    check_linear(torch.Generator().manual_seed(m + n), m, k, n, epilogue, bias=epilogue != "none", dtype=dtype)
+
+
+def test_linear_cut_between_pairs_sums_exactly_up_to_the_largest():
+    check_linear(torch.Generator().manual_seed(0), 200, 131056, 1500, dtype=torch.float32, extreme=True)
 
 
 def test_linear_of_a_prompt_sums_exactly_up_to_the_largest():
