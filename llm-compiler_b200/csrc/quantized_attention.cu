@@ -11,34 +11,40 @@ struct Plan {
     return splits > 1 && !cluster ? batch * kv_heads * head_blocks * splits * block_heads : 0;
   }
 };
+// Clusters of `size` CTAs that the GPU holds at once, with 4, 3 or 1 CTAs an SM: fewer than its CTAs divided by `size`, for a
+// cluster stays within a GPC. (As counted on a B200; where one holds fewer, the last few wait for a second round.)
+int64_t clusters_at_once(int64_t resident, int64_t size) {
+  constexpr int kOfFour[] = {592, 296, 187, 142, 112, 93, 78, 71}, kOfThree[] = {444, 222, 142, 104, 82, 71, 56, 48},
+                kOfOne[] = {148, 74, 45, 33, 26, 22, 15, 15};
+  return (resident == 4 ? kOfFour : resident == 3 ? kOfThree : kOfOne)[size - 1];
+}
 Plan plan_of(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t longest, int64_t split_tokens) {
   Plan plan;
   const int64_t group = q_heads / kv_heads;
   plan.head_blocks = ceil_div(group, dim == 256 ? 8 : 16);
   plan.block_heads = ceil_div(group, plan.head_blocks);
   const int64_t items = batch * kv_heads * plan.head_blocks;
-  const int64_t slots = static_cast<int64_t>(kNumSMs) * (dim == 256 ? 1 : dim == 64 && plan.block_heads <= 8 ? 4 : 3);
+  const int64_t resident = dim == 256 ? 1 : dim == 64 && plan.block_heads <= 8 ? 4 : 3, slots = kNumSMs * resident;
   if (split_tokens > 0) {
     plan.splits = ceil_div(longest, split_tokens);
   } else {
-    // One round of the CTAs that the GPU holds at once, if a power of two of splits fits: a CTA streams nothing for some 5 us
-    // at its start and end, and a second round waits for that (32 x 4096 tokens, 4 heads of 128: 28 us in 256 CTAs, 39 in
-    // 512; 64 x 4096, 2 heads of 64: 18 in 512, 24 in 1024). Beyond a cluster's eight only 1024 tokens and more a CTA (16 x
-    // 4096, 2 heads of 64: 9.5 in 8 splits, 11 in 16; 1 x 32768, 4 heads of 128: 36 in 8, 20 in 32, 22 in 64). Where one
-    // round cannot split at all, several of short CTAs even out lengths that differ (64 ragged to 8192, 4 heads of 128: 79
-    // in one split, 63 in two, 59 in four; 64 x 4096 of one length 47, 64 and 62).
-    const int64_t rounds = slots / items;
-    plan.splits = 1;
-    while (plan.splits * 2 <= rounds && (plan.splits < 8 || plan.splits * 2 * 1024 <= longest)) plan.splits *= 2;
-    if (rounds == 1) plan.splits = 2;
+    // One round of the clusters that the GPU holds at once: a CTA streams nothing for some 5 us at its start and end, and a
+    // second round waits for that (32 x 4096 tokens, 4 heads of 128: 28 us in 256 CTAs, 39 in 512; 25 x 4096, 2 of 128: 15.5 in
+    // 50 clusters of 7, 16.2 of 4, 22 of 8, two of which wait; 18 x 8192, one of 256: 23 in 6, 28 in 4, 35 in 8). Beyond a
+    // cluster's eight only 1024 tokens and more a CTA (16 x 4096, 2 heads of 64: 9.5 in 8 splits, 11 in 16; 1 x 32768, 4 heads of
+    // 128: 36 in 8, 20 in 32, 22 in 64). Where one round cannot split at all, several of short CTAs even out lengths that
+    // differ (64 ragged to 8192, 4 heads of 128: 79 in one split, 63 in two, 59 in four; 64 x 4096 of one length 47, 64 and 62).
+    plan.splits = 8;
+    while (plan.splits > 1 && items > clusters_at_once(resident, plan.splits)) --plan.splits;
+    if (plan.splits == 8)
+      while (items * plan.splits * 2 <= slots && plan.splits * 2 * 1024 <= longest) plan.splits *= 2;
+    if (plan.splits == 1 && items <= slots) plan.splits = 2;
   }
   // (a CTA has a tile for each of its warps)
   plan.splits = std::max<int64_t>(1, std::min(plan.splits, ceil_div(longest, 32 * kWarps)));
   if (items > kMaxCounters) plan.splits = std::min<int64_t>(plan.splits, 8);
   plan.cluster = plan.splits > 1 && plan.splits <= 8;
-  if (plan.cluster)  // clusters of a power of two fit every GPC
-    while ((plan.splits & (plan.splits - 1)) != 0) ++plan.splits;
-  plan.rounds = ceil_div(items * plan.splits, slots);
+  plan.rounds = plan.cluster ? ceil_div(items, clusters_at_once(resident, plan.splits)) : ceil_div(items * plan.splits, slots);
   return plan;
 }
 }  // namespace
