@@ -868,10 +868,8 @@ bool make_code_map(CUtensorMap* map, const void* base, int64_t rows, int64_t k, 
 // tile (910 x 288 x 577 fp32: 9.6 us, 4.5 in the stream kernel); slices of K 6 us at 256 columns (256 x 18944 x 3584 22 us in four,
 // 512 x 18944 x 3584 36 in two, 40 in one). Wide tiles need fewer bytes for a product and narrow ones fewer rounds: 5632 x 1280 x
 // 18432 97 us at 256 columns, 127 at 128; 4096 x 18944 x 3584 194 at 256, 217 at 160.
-// Clusters of `ctas` CTAs, one an SM, that the GPU holds at once (a B200 whose GPCs have lost other SMs may hold one less: of 8
-// CTAs 15 measured, 22 of 6, 33 of 4; beyond it a tile waits for a second round: 256 x 18944 x 3584 in 16 clusters of 8 37 us, in 14 22; 64 x 3584 x 4608 in 36 of 4 11.7, in 36
-// of 2 7.2).
-constexpr int64_t clusters_at_once(int64_t ctas) { return ctas > 6 ? 14 : ctas > 4 ? 21 : ctas > 2 ? 32 : ctas > 1 ? kNumSMs / 2 : kNumSMs; }
+// Slices of K are clusters, and more of them than the GPU holds at once cost a second round: 256 x 18944 x 3584 in 16 clusters of
+// 8 37 us, in 14 22; 8 x 3584 x 4608 in 36 of 4 9.8, in 36 of 2 6.3, in 36 of 3 5.6.
 constexpr double kStreamEpilogue[] = {4.5, 15.0, 7.0};  // none, residual, SwiGLU
 struct StreamPlan { int cols, chunks, slices; double us; };
 StreamPlan plan_stream(int64_t m, int64_t k, int64_t n, int epilogue) {
@@ -879,9 +877,9 @@ StreamPlan plan_stream(int64_t m, int64_t k, int64_t n, int epilogue) {
   StreamPlan best = {0, 0, 0, 1e30};
   for (int64_t chunks = ceil_div(m, kRowsAtMost); chunks <= std::max<int64_t>(16, ceil_div(m, kRowsAtMost)); ++chunks) {
     const int64_t cols = ceil_div(ceil_div(m, chunks), 16) * 16, units = tiles * ceil_div(m, cols);
-    // slices of K that fill the GPU where the tiles do not: clusters of 2, 4 or 8, two k-blocks a slice at least
-    int64_t slices = 1;
-    while (slices < 8 && units <= clusters_at_once(2 * slices) && blocks >= slices * 4) slices *= 2;
+    // slices of K that fill the GPU where the tiles do not, two k-blocks a slice at least
+    int64_t slices = 8;
+    while (slices > 1 && (units > clusters_at_once(1, slices) || blocks < 2 * slices)) --slices;
     const double share = cols / 256.0;
     const int64_t across = std::max<int64_t>(1, kNumSMs / chunks), rounds = slices > 1 ? 1 : ceil_div(tiles, across);
     const double products = ceil_div(blocks, slices) * (0.2 + 0.42 * share);
@@ -898,7 +896,7 @@ PairPlan plan_pair(int64_t m, int64_t k, int64_t n, bool whole_rows) {
     const int64_t tiles = tiles_m * ceil_div(n, bn);
     const double share = bn / 256.0, block = 0.155 + 0.19 * share;
     // slices of K where the tiles leave pairs idle: clusters of 4, 6 or 8 CTAs
-    for (int64_t slices = 1; slices <= 4 && (slices == 1 || (tiles <= clusters_at_once(2 * slices) && blocks >= 4 * slices)); ++slices) {
+    for (int64_t slices = 1; slices <= 4 && (slices == 1 || (tiles <= clusters_at_once(1, 2 * slices) && blocks >= 4 * slices)); ++slices) {
       const int64_t rounds = slices > 1 ? 1 : ceil_div(tiles, kNumSMs / 2);
       const double products = ceil_div(blocks, slices) * block;
       const double us = 3.5 + std::max(products, 2.0) + (rounds - 1) * std::max(products, (whole_rows ? 2.8 : 4.0) * share) +

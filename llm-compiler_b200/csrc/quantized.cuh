@@ -41,6 +41,14 @@ constexpr float kSmallestScale = 1.17549435e-38f;  // the smallest normal number
 
 __device__ __forceinline__ bool is_finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
 
+// Clusters of `size` CTAs that the GPU holds at once, with 4, 3 or 1 CTAs an SM: fewer than its CTAs divided by `size`, for a
+// cluster stays within a GPC. (As counted on a B200; where one holds fewer, the last few wait for a second round.)
+inline int64_t clusters_at_once(int64_t resident, int64_t size) {
+  constexpr int kOfFour[] = {592, 296, 187, 142, 112, 93, 78, 71}, kOfThree[] = {444, 222, 142, 104, 82, 71, 56, 48},
+                kOfOne[] = {148, 74, 45, 33, 26, 22, 15, 15};
+  return (resident == 4 ? kOfFour : resident == 3 ? kOfThree : kOfOne)[size - 1];
+}
+
 // Opt-in to `bytes` of dynamic shared memory of a kernel, asked of the runtime once per device (a third of a microsecond a
 // call otherwise). `done`: a bit per device, of this kernel and size.
 template <typename Kernel>

@@ -11,13 +11,6 @@ struct Plan {
     return splits > 1 && !cluster ? batch * kv_heads * head_blocks * splits * block_heads : 0;
   }
 };
-// Clusters of `size` CTAs that the GPU holds at once, with 4, 3 or 1 CTAs an SM: fewer than its CTAs divided by `size`, for a
-// cluster stays within a GPC. (As counted on a B200; where one holds fewer, the last few wait for a second round.)
-int64_t clusters_at_once(int64_t resident, int64_t size) {
-  constexpr int kOfFour[] = {592, 296, 187, 142, 112, 93, 78, 71}, kOfThree[] = {444, 222, 142, 104, 82, 71, 56, 48},
-                kOfOne[] = {148, 74, 45, 33, 26, 22, 15, 15};
-  return (resident == 4 ? kOfFour : resident == 3 ? kOfThree : kOfOne)[size - 1];
-}
 Plan plan_of(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t longest, int64_t split_tokens) {
   Plan plan;
   const int64_t group = q_heads / kv_heads;
