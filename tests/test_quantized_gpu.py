@@ -214,6 +214,22 @@ def test_attention_of_blocks_and_splits(cache, size, lengths):
     check_attention(g, cache, torch.bfloat16, lengths, 8, 2, 64, size, hint=10, split_tokens=64)  # a hint bounds nothing
 
 
+@pytest.mark.parametrize("dim,heads", [(64, 7), (64, 16), (128, 8), (128, 13), (256, 4)])
+@pytest.mark.parametrize("splits", [2, 3, 5, 6, 7, 8, 9])
+def test_attention_of_any_number_of_splits(dim, heads, splits):
+    """Clusters of any size, all of whose CTAs have tiles or only some, and more splits than a cluster holds."""
+    g = torch.Generator().manual_seed(dim + splits)
+    for cache, dtype in ((torch.int8, torch.bfloat16), (torch.float8_e4m3fn, torch.float16)):
+        check_attention(g, cache, dtype, [1500, 700, 0, 129, 1], heads, 1, dim, 32, split_tokens=-(-1504 // splits))
+
+
+@pytest.mark.parametrize("batch,dim", [(25, 128), (30, 128), (36, 128), (50, 128), (60, 128), (90, 128), (45, 64), (13, 256), (40, 256)])
+def test_attention_of_batches_between_the_sizes_of_clusters(batch, dim):
+    g = torch.Generator().manual_seed(batch)
+    lengths = torch.randint(0, 1100, (batch,), generator=g).tolist()
+    check_attention(g, torch.int8, torch.bfloat16, lengths, 4, 2, dim, 64, capacity=1100)
+
+
 @pytest.mark.parametrize("cache", CACHES)
 @pytest.mark.parametrize("kind", ["padded", "lowest", "soft", "empty-row", "half", "positive-infinity"])
 def test_attention_masks(cache, kind):
