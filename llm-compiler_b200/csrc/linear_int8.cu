@@ -418,7 +418,8 @@ template <int kLeft>
 __device__ __forceinline__ void stores_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kLeft) : "memory"); }
 
 // Piece: uint4 where rows of y start on multiples of 16 bytes: chunks of y leave, and those of a residual come, by TMA (with
-// the warps' own loads and stores of 16 bytes 16384 x 128 x 9728 with a residual takes 204 us, so 139). Else what a lane moves of a row at a time, 4 bytes or 2.
+// the warps' own loads and stores of 16 bytes 16384 x 128 x 9728 with a residual takes 204 us, so 139). Else what a lane moves
+// of a row at a time, 4 bytes or 2.
 // kSplit: K in slices, pairs of one cluster; they add their sums through distributed shared memory (a tile a cluster).
 template <typename T, typename Piece, bool kSplit>
 __global__ void __launch_bounds__(kPairThreads, 1)
@@ -885,6 +886,7 @@ StreamPlan plan_stream(int64_t m, int64_t k, int64_t n, int epilogue) {
     const double products = ceil_div(blocks, slices) * (0.2 + 0.42 * share);
     const double us = 4.0 + products + 2.5 * share + (rounds - 1) * std::max(products, kStreamEpilogue[epilogue] * share);
     if (us < 0.9 * best.us) best = {static_cast<int>(cols), static_cast<int>(ceil_div(m, cols)), static_cast<int>(slices), us};
+    if (cols == 16) break;  // (no chunk is smaller)
   }
   return best;
 }
@@ -990,9 +992,9 @@ extern "C" int b200_linear_int8(const b200_linear_int8_call* call, void* stream)
   p.wait_limit = wait_limit(); p.drop_loads = drop_loads();
   const StreamPlan stream_plan = plan_stream(m, k, n, p.epilogue);
   const int64_t row_bytes = (p.epilogue == B200_EPILOGUE_SWIGLU ? n / 2 : n) * (dtype == B200_F32 ? 4 : 2);
-  const PairPlan pair_plan = plan_pair(m, k, n, row_bytes % 16 == 0);
+  const PairPlan pair_plan = m > kRowsAtMost / 2 ? plan_pair(m, k, n, row_bytes % 16 == 0) : PairPlan{0, 0, 1e30};
   // (beyond 256 rows the stream kernel reads the weight more than once, which other work on the GPU would feel)
-  const bool streamed = m <= kRowsAtMost / 2 || (stream_plan.us < (m <= kRowsAtMost ? 1.0 : 0.95) * pair_plan.us && stream_plan.chunks <= 64);
+  const bool streamed = stream_plan.us < (m <= kRowsAtMost ? 1.0 : 0.95) * pair_plan.us && stream_plan.chunks <= 64;
   int code = B200_ERR_UNSUPPORTED;
   with_element_type(dtype, [&](auto tag) {
     using T = typename decltype(tag)::type;
