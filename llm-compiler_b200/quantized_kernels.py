@@ -18,6 +18,9 @@ from . import _lib
 from .kernels import (_DTYPE_CODES, _EPILOGUES, _RUNTIMES, DeviceRuntime, _check, _code, _dense, _guard_current_device,
                       _stream, runtime)
 
+# (looked up at every call otherwise)
+_BFLOAT16, _FLOAT16, _FLOAT32, _INT32, _INT64 = torch.bfloat16, torch.float16, torch.float32, torch.int32, torch.int64
+
 # The formats of a cache in 8 bits: the code of the C ABI.
 CACHE_CODES = {torch.int8: _lib.I8, torch.float8_e4m3fn: _lib.E4M3}
 MAX_K = 131056  # (a sum of that many products of two 8-bit integers stays below 2^31)
@@ -55,21 +58,21 @@ def _cache_code(dtype: torch.dtype) -> int:
 
 
 def _check_cache(key_pool: torch.Tensor, value_pool: torch.Tensor, key_scales: torch.Tensor, value_scales: torch.Tensor,
-                 block_table: torch.Tensor, batch: int) -> Tuple[int, int, int, int]:
-    """(blocks, kv heads, block size, head dim) of a cache whose parts fit together."""
+                 block_table: torch.Tensor, batch: int) -> Tuple[int, int, int, int, int]:
+    """(blocks, kv heads, block size, head dim, columns of the table) of a cache whose parts fit together."""
 
     shape = key_pool.shape
     if len(shape) != 4 or value_pool.shape != shape or not key_pool.is_contiguous() or not value_pool.is_contiguous() or \
-            key_pool.dtype != value_pool.dtype:
+            key_pool.dtype is not value_pool.dtype:
         raise ValueError("KV pools must be contiguous blocks x H x block_size x D tensors of one shape and dtype")
-    per_block = shape[:2]
-    for scales in (key_scales, value_scales):
-        if scales.shape != per_block or scales.dtype != torch.float32 or not scales.is_contiguous():
-            raise ValueError("scales must be contiguous float32 blocks x H tensors")
-    if block_table.dtype != torch.int32 or block_table.ndim != 2 or block_table.shape[0] != batch or \
-            not block_table.is_contiguous():
+    per_block = key_scales.shape
+    if per_block != shape[:2] or value_scales.shape != per_block or key_scales.dtype is not _FLOAT32 or \
+            value_scales.dtype is not _FLOAT32 or not key_scales.is_contiguous() or not value_scales.is_contiguous():
+        raise ValueError("scales must be contiguous float32 blocks x H tensors")
+    table_shape = block_table.shape
+    if block_table.dtype is not _INT32 or len(table_shape) != 2 or table_shape[0] != batch or not block_table.is_contiguous():
         raise ValueError("block_table must be a contiguous int32 B x max_blocks tensor")
-    return shape
+    return (*shape, table_shape[1])
 
 
 def b200_paged_kv_store_8bit(key_pool: torch.Tensor, value_pool: torch.Tensor, key_scales: torch.Tensor,
@@ -87,14 +90,16 @@ def b200_paged_kv_store_8bit(key_pool: torch.Tensor, value_pool: torch.Tensor, k
     if key.ndim != 4 or key.shape != value.shape or key.dtype != value.dtype:
         raise ValueError("key/value must be B x H x T x D tensors of one shape and dtype")
     batch, heads, tokens, dim = key.shape
-    blocks, pool_heads, block_size, pool_dim = _check_cache(key_pool, value_pool, key_scales, value_scales, block_table, batch)
+    blocks, pool_heads, block_size, pool_dim, columns = _check_cache(key_pool, value_pool, key_scales, value_scales,
+                                                                     block_table, batch)
     if heads != pool_heads or dim != pool_dim:
         raise ValueError("key/value heads or head_dim do not match the pools")
-    if key.dtype not in (torch.bfloat16, torch.float16):
+    dtype = key.dtype
+    if dtype is not _BFLOAT16 and dtype is not _FLOAT16:
         raise ValueError(f"key/value must be bfloat16 or float16, not {key.dtype}")
     if dim % 16:
         raise ValueError("head_dim must be a multiple of 16")
-    if positions.shape != (batch,) or positions.dtype != torch.int64 or not positions.is_contiguous():
+    if positions.shape != (batch,) or positions.dtype is not _INT64 or not positions.is_contiguous():
         raise ValueError("positions must be a contiguous int64 batch vector")
     cache = _cache_code(key_pool.dtype)
     if batch == 0 or tokens == 0:
@@ -102,7 +107,7 @@ def b200_paged_kv_store_8bit(key_pool: torch.Tensor, value_pool: torch.Tensor, k
     code = _lib.load().b200_paged_kv_store_8bit(_STORE_CALL(
         key_pool.data_ptr(), value_pool.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(), block_table.data_ptr(),
         key.data_ptr(), value.data_ptr(), positions.data_ptr(), rt.status.data_ptr(), batch, heads, tokens, dim, blocks,
-        block_size, block_table.shape[1], *key.stride(), *value.stride(), _DTYPE_CODES[key.dtype], cache), _stream())
+        block_size, columns, *key.stride(), *value.stride(), _DTYPE_CODES[dtype], cache), _stream())
     if code:
         _check(code, "b200_paged_kv_store_8bit")
     rt.launches += 1
@@ -124,25 +129,26 @@ def b200_paged_decode_attention_8bit(query: torch.Tensor, key_pool: torch.Tensor
     split of the work and bounds nothing."""
 
     rt = _runtime_of(query, key_pool, value_pool, key_scales, value_scales, block_table, lengths, attention_mask)
-    if query.ndim != 4 or query.shape[2] != 1:
+    shape, dtype = query.shape, query.dtype
+    if len(shape) != 4 or shape[2] != 1:
         raise ValueError("query must be B x H x 1 x D")
-    batch, q_heads, _, dim = query.shape
-    blocks, kv_heads, block_size, pool_dim = _check_cache(key_pool, value_pool, key_scales, value_scales, block_table, batch)
+    batch, q_heads, _, dim = shape
+    blocks, kv_heads, block_size, pool_dim, max_blocks = _check_cache(key_pool, value_pool, key_scales, value_scales,
+                                                                      block_table, batch)
     if pool_dim != dim or kv_heads <= 0 or q_heads % kv_heads:
         raise ValueError("query does not match the pools")
-    if query.dtype not in (torch.bfloat16, torch.float16):
+    if dtype is not _BFLOAT16 and dtype is not _FLOAT16:
         raise ValueError(f"query must be bfloat16 or float16, not {query.dtype}")
     if dim not in (64, 128, 256):
         raise ValueError("head_dim must be 64, 128 or 256")
     if block_size % 32:
         raise ValueError("the block size must be a multiple of 32 tokens")
-    if lengths.shape != (batch,) or lengths.dtype != torch.int64 or not lengths.is_contiguous():
+    if lengths.shape != (batch,) or lengths.dtype is not _INT64 or not lengths.is_contiguous():
         raise ValueError("lengths must be a contiguous int64 batch vector")
     q_batch_stride, q_head_stride, _, q_stride = query.stride()
     if q_stride != 1:
         query = _dense(query)
         q_batch_stride, q_head_stride = q_heads * dim, dim
-    max_blocks = block_table.shape[1]
     mask_pointer, mask_len, mask_stride, mask_code = 0, max_blocks * block_size, 0, _lib.F32
     if attention_mask is not None:
         if attention_mask.ndim != 4 or attention_mask.shape[:3] != (batch, 1, 1):
@@ -164,7 +170,7 @@ def b200_paged_decode_attention_8bit(query: torch.Tensor, key_pool: torch.Tensor
         query.data_ptr(), key_pool.data_ptr(), value_pool.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr(),
         block_table.data_ptr(), lengths.data_ptr(), mask_pointer, output.data_ptr(), workspace, rt.status.data_ptr(), batch,
         q_heads, kv_heads, dim, blocks, block_size, max_blocks, mask_len, q_batch_stride, q_head_stride, mask_stride, mask_code,
-        _DTYPE_CODES[query.dtype], cache, split_tokens, max_length_hint, need, scale), _stream())
+        _DTYPE_CODES[dtype], cache, split_tokens, max_length_hint, need, scale), _stream())
     if code:
         _check(code, "b200_paged_decode_attention_8bit")
     rt.launches += 1
@@ -234,28 +240,31 @@ def _quantize(tensor: torch.Tensor, residual: Optional[torch.Tensor], weight: Op
     shape, dtype = tensor.shape, tensor.dtype
     if not shape or shape[-1] <= 0:
         raise ValueError("the input must have rows of at least one element")
-    hidden, code_dtype = shape[-1], _code(dtype)
+    hidden = shape[-1]
+    code_dtype = _DTYPE_CODES.get(dtype)
+    if code_dtype is None:
+        _code(dtype)  # (raises)
     weight_pointer = residual_pointer = total_pointer = 0
     if weight is not None:
-        if weight.shape != (hidden,) or weight.dtype != dtype or not weight.is_contiguous():
+        if weight.shape != (hidden,) or weight.dtype is not dtype or not weight.is_contiguous():
             raise ValueError("weight must be a contiguous vector of the row length in the input dtype")
         weight_pointer = weight.data_ptr()
-    stride = _row_stride(tensor)
+    stride = hidden if tensor.is_contiguous() else _row_stride(tensor)
     if stride is None:
         tensor, stride = _dense(tensor), hidden
     like = tensor if stride == hidden else None  # (contiguous: outputs may be made like it)
     residual_stride, total = hidden, None
     if residual is not None:
-        if residual.shape != shape or residual.dtype != dtype:
+        if residual.shape != shape or residual.dtype is not dtype:
             raise ValueError("residual must match the input's shape and dtype")
-        residual_stride = _row_stride(residual)
+        residual_stride = hidden if residual.is_contiguous() else _row_stride(residual)
         if residual_stride is None:
             residual, residual_stride = _dense(residual), hidden
         total = torch.empty_like(tensor) if like is not None else tensor.new_empty(shape)
         residual_pointer, total_pointer = residual.data_ptr(), total.data_ptr()
     codes = torch.empty_like(tensor, dtype=torch.int8) if like is not None else tensor.new_empty(shape, dtype=torch.int8)
     # (one size in place of a shape: 1 us less)
-    scales = tensor.new_empty(shape[0] if len(shape) == 2 else shape[:-1], dtype=torch.float32)
+    scales = tensor.new_empty(shape[0] if len(shape) == 2 else shape[:-1], dtype=_FLOAT32)
     rows = scales.numel()
     if rows == 0:
         return codes, scales, total
