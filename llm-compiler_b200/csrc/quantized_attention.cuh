@@ -14,14 +14,17 @@
 //  - V comes through ldmatrix.trans in units of two bytes: a lane gets d and d + 1 of two tokens, and splits them into the
 //    two tokens' even and odd element, which are rows of two halves of an A operand;
 //  - P^T is transposed 8 x 8 by movmatrix.
-// q is brought to [1, 2) per head by a power of two (exact; fp16 alone would overflow), which goes back into the scores.
+// q is brought to [1, 2) per head by a power of two, which goes back into the scores: exact but for elements below 2^-14 of the
+// head's largest, which are off by at most 2^-25 of it (fp16 alone would overflow).
 //
 // Scales. ks multiplies the scores. vs is folded into the probabilities relative to a running reference `vref`, which the
-// accumulators are carried in; it follows vs (accumulators rescaled) only when they are more than 16 apart, so P stays well
-// inside fp16. The running maximum moves only when a score passes it by more than 5: the softmax is the same, and most tiles
-// need no reduction across lanes. P is rounded to fp16, half a step of which is 2^-11 of it, its sum stays fp32: an eighth of
-// the rounding of a bf16 result. An fp16 result's own rounding is no larger than P's, so there P is two fp16 numbers, what the
-// first leaves in the second (2^-22): one more product per V fragment.
+// accumulators are carried in; it follows vs (accumulators rescaled) only when vs is more than twice it or less than a quarter
+// of it. The running maximum moves only when a score passes it by more than 3 (in units of log 2): the softmax is the same, and
+// most tiles need no reduction across lanes. So P, at most 2^3 * 2, is carried 2^11 higher, which fills fp16: P is rounded by
+// 2^-11 of it, an eighth of the rounding of a bf16 result, down to 2^-23 of the largest probability and by 2^-34 of the largest
+// below (carried at 1 with wider limits, a token that got e^14 of the others' weight left them 1 % off and e^18 nothing); its sum stays
+// fp32. An fp16 result's own rounding is no larger than P's, so there P is two fp16 numbers, what the first leaves in the
+// second (2^-22, and 2^-34 of the largest probability as before): one more product per V fragment.
 //
 // Work. The tiles (32 tokens) of one (sequence, KV head, up to 8 NT heads) are dealt to `splits` CTAs of four warps, a tile
 // to a warp in turn. Each warp has a ring of its own that TMA fills: a tile never spans two blocks (block sizes are multiples
@@ -47,7 +50,8 @@ namespace cache_attention {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kSlack = 5.0f;  // how far a score may pass the running maximum before it moves
+constexpr float kSlack = 3.0f;      // how far a score may pass the running maximum before it moves, in units of log 2
+constexpr float kLift = 2048.0f;    // what the probabilities are carried times: 2^kSlack * 2 (block scales) * kLift = 2^15
 constexpr int64_t kCounterBytes = 65536;
 constexpr int64_t kMaxCounters = kCounterBytes / 4;
 constexpr int kTableCache = 512;  // entries of a sequence's row of the block table that wait in shared memory
@@ -448,7 +452,7 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        over = over || highest(t, h) > m[t][h] + kSlack;
+        over = over || highest(t, h) > m[t][h] + kSlack / kToLog2;
     if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
       for (int t = 0; t < NT; ++t)
@@ -469,7 +473,7 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
           }
         }
     }
-    if (vs > 0.0f && !(vs <= 16.0f * vref && vref <= 16.0f * vs)) {
+    if (vs > 0.0f && !(vs <= 2.0f * vref && vref <= 4.0f * vs)) {
       // (2^60: far enough that nothing of the smaller side is seen in the larger one)
       const float unit = vref > 0.0f ? fminf(fmaxf(vs, vref * 0x1p-60f), vref * 0x1p60f) : vs;
       const float keep = vref > 0.0f ? vref / unit : 1.0f;
@@ -483,7 +487,8 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
         }
     }
     float weight = vs * inverse_vref;
-    if (weight > 16.0f) weight = 16.0f;  // (a NaN stays)
+    if (weight > 2.0f) weight = 2.0f;  // (a NaN stays)
+    weight *= kLift;
 
     // ---- probabilities, transposed into B operands ----
     uint32_t pb[NT][kParts][2], rest[NT][kParts][2];
@@ -563,7 +568,7 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
       for (int h = 0; h < 2; ++h) {
         const int head = 8 * t + 2 * j + h;
         *reinterpret_cast<float2*>(parts + (warp * kHeads + head) * D + 16 * i + 2 * g) =
-            make_float2(o[t][i][h] * vref, o[t][i][2 + h] * vref);
+            make_float2(o[t][i][h] * (1.0f / kLift) * vref, o[t][i][2 + h] * (1.0f / kLift) * vref);
       }
   __syncthreads();
   const int64_t item = b * gridDim.y + item_head;

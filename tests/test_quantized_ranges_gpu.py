@@ -1,0 +1,91 @@
+"""Operators in 8 bits over the whole range of what they may be given: tails of small probabilities behind a token that
+dominates."""
+
+import pytest
+import torch
+
+import llm_compiler_b200 as b200
+import quantized_helpers as ref
+from llm_compiler_b200 import kernels
+
+pytestmark = pytest.mark.gpu
+CACHES = [torch.int8, torch.float8_e4m3fn]
+
+
+def attention(query, keys, values, table, length, mask, scale):
+    """(result, bound on the kernel's distance from it) of one sequence, 1 x Hq x 1 x D, in 64 bits.
+
+    With A = sum p|v|, an element of the result is off by
+     - its own rounding;
+     - a probability's rounding to fp16: 2^-11 of it (fp16 results, two numbers: 2^-22), or, where that is less, half of
+       fp16's smallest step, which is 2^-34 of the largest probability (2^-25 on numbers that are carried 2^11 higher, a block's
+       scale at least a quarter of its reference), and never more than the probability itself;
+     - the scores: products of D terms in 32 bits, (D + 4) u of the sum of magnitudes, 2^-25 of the query's largest times the
+       keys' sum, a mask's addition; twice, for the normalisation;
+     - exponentials good to 2^-21 of arguments (in units of log 2) of up to 64, rounded to u: 2^-18;
+     - sums in 32 bits: a warp of four adds a product of 16 tokens at a time, four roundings each, and its lanes' sums of
+       probabilities one of 8 tokens at a time; merges and rescalings 64 u."""
+    u = 2.0 ** -24
+    half = ref.HALF_STEP[query.dtype]
+    probability = 2.0 ** -11 if query.dtype == torch.bfloat16 else 2.0 ** -22
+    smallest = 2.0 ** -25 if query.dtype == torch.float16 else 2.0 ** -133
+    q = query.double()
+    _, heads, _, dim = q.shape
+    out, bound = torch.empty_like(q), torch.empty_like(q)
+    k, v = keys.rows(table[0], length), values.rows(table[0], length)
+    group = heads // k.shape[0]
+    for h in range(heads):
+        kk, vv, one = k[h // group], v[h // group], q[0, h, 0]
+        scores = kk @ one * scale
+        slack = ((dim + 4) * u * (kk.abs() @ one.abs()) + 2.0 ** -25 * one.abs().max() * kk.abs().sum(1)) * scale
+        if mask is not None:
+            scores = scores + mask[0, 0, 0, :length].double()
+            slack = slack + u * scores.abs().nan_to_num(0.0, 0.0, 0.0)
+        p = torch.softmax(scores, 0)
+        out[0, h, 0] = p @ vv
+        a = p @ vv.abs()
+        rounding = torch.maximum(probability * p, torch.minimum(p, 2.0 ** -34 * p.max())) @ vv.abs()
+        off = 2 * float(torch.where(p > 0, slack, 0.0).max())
+        sums = u * (length / 64 * 4 + length / 32 + 64)
+        bound[0, h, 0] = half * out[0, h, 0].abs() + rounding + a * (off + 2.0 ** -18 + sums) + smallest
+    return out, bound
+
+
+def check(query, pools, scales, table, length, mask, scale, **options):
+    want, bound = attention(query, ref.Cache(pools[0], scales[0]), ref.Cache(pools[1], scales[1]), table, length, mask, scale)
+    got = b200.b200_paged_decode_attention_8bit(query.cuda(), *pools, *scales, table.cuda(), torch.tensor([length]).cuda(),
+                                                None if mask is None else mask.cuda(), scale=scale, **options)
+    got = got.cpu().double()
+    assert bool(want.isfinite().all()) and bool(got.isfinite().all())
+    worst = float(((got - want).abs() / bound).max())
+    assert worst <= 1.0, f"{worst:.3g} of the bound"
+    kernels.runtime().check_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("above", [8, 14, 18])
+@pytest.mark.parametrize("ratio", [1.0, 3.9, 12.0, 0.1])
+@pytest.mark.parametrize("masked", [False, True])
+def test_attention_of_a_long_tail_behind_a_token_that_dominates(dtype, cache, above, ratio, masked):
+    """One token `above` the others' scores whose value is zero, in a block of `ratio` times the others' value scale: the
+    result is the tail's alone, each probability of it some e^-above of the largest."""
+    g = torch.Generator().manual_seed(above)
+    length, size, dim, heads = 30100, 128, 64, 4
+    blocks = -(-length // size)
+    top = ref.TOP[cache]
+    keys = torch.zeros(blocks, 1, size, dim)
+    values = 40 + (top - 40) * torch.rand(blocks, 1, size, dim, generator=g)  # of one sign
+    at = 1000
+    keys[at // size, 0, at % size, 0] = 100.0
+    values[at // size, 0, at % size] = 0.0
+    pools = [(x.round() if cache == torch.int8 else x).to(cache).cuda() for x in (keys, values)]
+    scales = [torch.full((blocks, 1), 0.01).cuda(), torch.full((blocks, 1), 1.0 / top).cuda()]
+    scales[1][at // size] *= ratio
+    query = torch.zeros(1, heads, 1, dim)
+    query[..., 0] = above / 0.125
+    query[:, :, :, 1:] = torch.randn(1, heads, 1, dim - 1, generator=g)
+    table = torch.arange(blocks, dtype=torch.int32).view(1, blocks)
+    mask = torch.zeros(1, 1, 1, length) if masked else None
+    check(query.to(dtype), pools, scales, table, length, mask, 0.125)
+    check(query.to(dtype), pools, scales, table, length, mask, 0.125, split_tokens=length)
