@@ -18,8 +18,9 @@
 // head's largest, which are off by at most 2^-25 of it (fp16 alone would overflow).
 //
 // Scales. ks multiplies the scores. vs is folded into the probabilities relative to a running reference `vref`, which the
-// accumulators are carried in; it follows vs (accumulators rescaled) only when vs is more than twice it or less than a quarter
-// of it. The running maximum moves only when a score passes it by more than 3 (in units of log 2): the softmax is the same, and
+// accumulators are carried in: a power of two that follows vs (accumulators rescaled, exactly) only when vs is more than twice it
+// or less than a quarter of it. It follows any distance up, where what is in the accumulators may underflow, and down as far as
+// they stay within fp32's range, where it is the tile that may; a tile that no head gives any weight does not move it. The running maximum moves only when a score passes it by more than 3 (in units of log 2): the softmax is the same, and
 // most tiles need no reduction across lanes. So P, at most 2^3 * 2, is carried 2^11 higher, which fills fp16: P is rounded by
 // 2^-11 of it, an eighth of the rounding of a bf16 result, down to 2^-23 of the largest probability and by 2^-34 of the largest
 // below (carried at 1 with wider limits, a token that got e^14 of the others' weight left them 1 % off and e^18 nothing); its sum stays
@@ -32,11 +33,13 @@
 // splits are a cluster, whose CTAs merge through distributed shared memory; more leave partials in the workspace, which the
 // CTA that arrives last adds in split order. Either way results do not depend on timing.
 //
-// Measured: 64 x 4096 tokens, 2 heads of 64 (67 MB): 16.7 us, 4.0 TB/s; 64 ragged to 8192, 4 heads of 128 (270 MB): 52 us,
-// 5.2 TB/s; 3 x 30001, 8 heads of 128 with a mask (185 MB): 36 us, 5.1 TB/s; 1 x 1000: 5.0 us. A CTA streams nothing for some
+// Measured: 64 x 4096 tokens, 2 heads of 64 (67 MB): 16.7 us, 4.0 TB/s; 64 ragged to 8192, 4 heads of 128 (270 MB): 51 us,
+// 5.2 TB/s; 3 x 30001, 8 heads of 128 with a mask (185 MB): 37 us, 5.0 TB/s; 1 x 1000: 4.8 us. A CTA streams nothing for some
 // 5 us at its start and end (length, table row, first copies; merge, exchange in the cluster, stores), which is what is left
 // beside the rate: in between the SMs' rings keep 96 KB and more in flight.
 #pragma once
+
+#include <float.h>
 
 #include <algorithm>
 #include <type_traits>
@@ -51,6 +54,7 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 3.0f;      // how far a score may pass the running maximum before it moves, in units of log 2
+constexpr float kUnseen = 36.0f;    // a probability that far below the running maximum is 0 in fp16
 constexpr float kLift = 2048.0f;    // what the probabilities are carried times: 2^kSlack * 2 (block scales) * kLift = 2^15
 constexpr int64_t kCounterBytes = 65536;
 constexpr int64_t kMaxCounters = kCounterBytes / 4;
@@ -355,7 +359,8 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.0f;
   }
-  float vref = 0.0f, inverse_vref = 1.0f;
+  int vref_exponent = 0;  // biased; 0: none so far
+  float inverse_vref = 0.0f;
   bool timed_out = false;
   const int my_token = S::token(g);
   float mask_next[kEach];
@@ -473,21 +478,44 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
           }
         }
     }
-    if (vs > 0.0f && !(vs <= 2.0f * vref && vref <= 4.0f * vs)) {
-      // (2^60: far enough that nothing of the smaller side is seen in the larger one)
-      const float unit = vref > 0.0f ? fminf(fmaxf(vs, vref * 0x1p-60f), vref * 0x1p60f) : vs;
-      const float keep = vref > 0.0f ? vref / unit : 1.0f;
-      vref = unit;
-      inverse_vref = 1.0f / unit;
+    float weight = vs * inverse_vref;
+    if (vs != 0.0f && fabsf(vs) <= FLT_MAX && !(fabsf(weight) >= 0.25f && fabsf(weight) <= 2.0f)) {
+      // (only heads that are there count: a column without one weighs every token)
+      bool seen = false;
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-          o[t][i][0] *= keep; o[t][i][1] *= keep; o[t][i][2] *= keep; o[t][i][3] *= keep;
+        for (int h = 0; h < 2; ++h) seen = seen || (8 * t + 2 * j + h < heads && highest(t, h) > m[t][h] - kUnseen / kToLog2);
+      if (__any_sync(0xffffffffu, seen)) {
+        int to = min(max(static_cast<int>((__float_as_uint(vs) >> 23) & 255u), 1), 253);
+        if (to < vref_exponent) {
+          // O grows by as much as leaves its largest element below 2^96, and never by more than one factor can
+          float most = 0.0f;
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if (8 * t + 2 * j + h < heads)
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i) most = fmaxf(most, fmaxf(fabsf(o[t][i][h]), fabsf(o[t][i][2 + h])));
+#pragma unroll
+          for (int x = 1; x < 32; x *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, x));
+          if (most > 0.0f) to = max(to, vref_exponent - max(min(223 - static_cast<int>(__float_as_uint(most) >> 23), 127), 0));
         }
+        const int turn = 127 + vref_exponent - to;  // 2^(old - new); beyond one factor's range O is 0, or nothing of it is seen
+        const float keep = vref_exponent == 0 || turn > 254 ? 1.0f : turn < 1 ? 0.0f : __uint_as_float(static_cast<uint32_t>(turn) << 23);
+        vref_exponent = to;
+        inverse_vref = __uint_as_float(static_cast<uint32_t>(254 - to) << 23);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int i = 0; i < kSteps; ++i) {
+            o[t][i][0] *= keep; o[t][i][1] *= keep; o[t][i][2] *= keep; o[t][i][3] *= keep;
+          }
+      }
+      weight = vs * inverse_vref;
+      if (fabsf(weight) >= 4.0f) weight = 0.0f;  // (unseen)
     }
-    float weight = vs * inverse_vref;
-    if (weight > 2.0f) weight = 2.0f;  // (a NaN stays)
     weight *= kLift;
 
     // ---- probabilities, transposed into B operands ----
@@ -560,6 +588,7 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
   __syncthreads();  // every ring is done with
   if (!S::kBeside(NT) && p.cluster && !alone) cluster_arrive();
   float* parts = reinterpret_cast<float*>(smem);  // [warp][head][D]
+  const float vref = __uint_as_float(static_cast<uint32_t>(vref_exponent) << 23);
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll

@@ -1,5 +1,7 @@
-"""Operators in 8 bits over the whole range of what they may be given: tails of small probabilities behind a token that
-dominates."""
+"""Operators in 8 bits over the whole range of what they may be given: value blocks any distance apart, tails of small
+probabilities behind a token that dominates."""
+
+import math
 
 import pytest
 import torch
@@ -60,6 +62,66 @@ def check(query, pools, scales, table, length, mask, scale, **options):
     worst = float(((got - want).abs() / bound).max())
     assert worst <= 1.0, f"{worst:.3g} of the bound"
     kernels.runtime().check_status()
+
+
+def random_codes(g, cache, blocks, heads, size, dim):
+    top = ref.TOP[cache]
+    codes = (torch.randn(blocks, heads, size, dim, generator=g) * top / 3).clamp(-top, top)
+    return (codes.round() if cache == torch.int8 else codes).to(cache).cuda()
+
+
+# what the blocks' value scales are, 2^x, four blocks (a tile for each warp) at a time
+PATTERNS = {
+    "tiny-first": [-73, -6], "tinier-first": [-100, -6], "tiny-last": [-6, -100], "zero-like": [-126, -5, -126, -6],
+    "70-up": [-40, 30], "70-down": [30, -40], "120-up": [-90, 30], "120-down": [30, -90],
+    "down-and-down": [0, -58, -116], "down-down-up": [0, -59, -118, 20, -20], "up-and-up": [-118, -59, 0],
+    "sawtooth": [-10, 60, -30, 90, -110, 5],
+}
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("dtype,dim,heads", [(torch.bfloat16, 64, 4), (torch.bfloat16, 128, 12), (torch.bfloat16, 256, 3)])
+@pytest.mark.parametrize("pattern", PATTERNS)
+@pytest.mark.parametrize("visible", ["all", "smallest", "largest"])
+def test_attention_of_value_blocks_any_distance_apart(cache, dtype, dim, heads, pattern, visible):
+    """All blocks weigh alike, or those of the smallest (largest) scale alone: the others are masked out, in front and behind.
+    (bf16 values, whose scales lie between 2^-126 and 2^121.)"""
+    g = torch.Generator().manual_seed(dim)
+    exponents = [e for e in PATTERNS[pattern] for _ in range(4)]
+    blocks, size = len(exponents), 32
+    pools = [random_codes(g, cache, blocks, 1, size, dim) for _ in range(2)]
+    top = ref.TOP[cache]
+    scales = [torch.full((blocks, 1), 3.0 / top), (1 + torch.rand(blocks, 1, generator=g)) * torch.tensor(
+        [[2.0 ** e] for e in exponents])]
+    table = torch.randperm(blocks, generator=g).to(torch.int32).view(1, blocks)
+    scales[1][table[0].long()] = scales[1].clone()  # (block i of the sequence has the i-th scale)
+    scales = [s.cuda() for s in scales]
+    length = blocks * size - 5
+    mask = None
+    if visible != "all":
+        keep = min(exponents) if visible == "smallest" else max(exponents)
+        mask = torch.full((1, 1, 1, length), -math.inf)
+        for i, e in enumerate(exponents):
+            if e == keep:
+                mask[..., i * size:(i + 1) * size] = 0.0
+    query = torch.randn(1, heads, 1, dim, generator=g).to(dtype)
+    for split_tokens in (0, blocks * size):  # a tile a warp, and all of them in turn
+        check(query, pools, scales, table, length, mask, dim ** -0.5, split_tokens=split_tokens)
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("seed", range(6))
+def test_attention_of_value_blocks_at_random_distances_and_probabilities(cache, seed):
+    """Scales anywhere in bf16's range, scores from a few units to a hundred apart."""
+    g = torch.Generator().manual_seed(seed)
+    blocks, size, dim, heads = 40, 32, 64, 6
+    pools = [random_codes(g, cache, blocks, 2, size, dim) for _ in range(2)]
+    scales = [torch.full((blocks, 2), 3.0 / ref.TOP[cache]).cuda(),
+              torch.exp2(-126 + 226 * torch.rand(blocks, 2, generator=g)).cuda()]
+    table = torch.randperm(blocks, generator=g).to(torch.int32).view(1, blocks)
+    query = (torch.randn(1, heads, 1, dim, generator=g) * [0.1, 1.0, 10.0][seed % 3]).bfloat16()
+    for split_tokens in (0, 320, blocks * size):
+        check(query, pools, scales, table, blocks * size - 3, None, 0.125, split_tokens=split_tokens)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
