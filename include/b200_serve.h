@@ -760,7 +760,7 @@ int b200_advance_slots(int64_t* lengths, const int32_t* slots, const int32_t* st
  * outside [0, num_blocks) is skipped and sets B200_STATUS_BAD_POSITION.
  *
  * b200_quantize_rows_int8: codes [rows, hidden] and one fp32 scale per row, code = round(y / scale), scale = amax|y| / 127
- * (0 for a row of zeros, whose codes are 0), with
+ * (0 for a row of zeros, whose codes are 0; at least 2^-126, times the norm's factor where there is one), with
  *   y = input                                                 norm_weight NULL (weights, or rows without a norm);
  *   y = r * rsqrt(mean(r^2) + epsilon) * norm_weight          r = input, or round(input + residual), written to `sum`
  * (which may be input or residual itself). A row whose y is not finite gets scale NaN and codes 0. dtype of input,

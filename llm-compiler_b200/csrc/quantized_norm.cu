@@ -3,6 +3,8 @@
 //     r = round(x + residual),  y_i = r_i w_i / sqrt(mean(r^2) + eps),  scale = max|y| / 127,  code_i = round(y_i / scale).
 // The row factor 1 / sqrt(..) is common to max|y| and to every y_i, so code_i = round(r_i w_i * (127 / max|r w|)) does not
 // need it: the sum of squares and the maximum come out of ONE pass and one reduction, and only the scale carries the factor.
+// max|r w| / 127 is at least the smallest normal number (as in a cache's store): below it neither it nor its inverse would
+// keep their bits, and such a row's codes stay below 127 instead.
 // A row is read once, held in registers, and written as codes (and as r where there is a residual).
 #include <algorithm>
 #include <type_traits>
@@ -159,9 +161,9 @@ __global__ void __launch_bounds__(512) quantize_rows_kernel(const QuantParams p)
       }
     }
     const bool fine = most < INFINITY;
-    const float inverse = fine && most > 0.0f ? fminf(__fdiv_rn(127.0f, most), 3.0e38f) : 0.0f;
+    const float inverse = fine && most > 0.0f ? fminf(__fdiv_rn(127.0f, most), 1.0f / kSmallestScale) : 0.0f;
     if (threadIdx.x == 0) {
-      float scale = most * (1.0f / 127.0f);
+      float scale = most > 0.0f ? fmaxf(most * (1.0f / 127.0f), kSmallestScale) : 0.0f;
       if (kNorm && most > 0.0f) scale *= rsqrtf(squares / static_cast<float>(p.hidden) + p.epsilon);
       p.scales[row] = fine ? scale : NAN;
     }

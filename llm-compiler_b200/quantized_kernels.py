@@ -282,7 +282,8 @@ def b200_rms_norm_int8(tensor: torch.Tensor, weight: torch.Tensor, *, epsilon: f
                        ) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
     """serve.rms_norm with the residual's addition in front and its output in 8-bit integers, one launch: (codes int8,
     scales float32 per row, sum). sum = round(tensor + residual) in the input dtype (None without a residual: the rows
-    themselves are normalised); codes * scales stand for the normalised rows, the largest of each row being 127."""
+    themselves are normalised); codes * scales stand for the normalised rows, the largest of each row being 127 (less where
+    the row's largest, before the norm's factor, is below 127 * 2^-126: a scale that small would lose its bits)."""
 
     if weight is None:
         raise ValueError("a norm has a weight")
@@ -291,7 +292,7 @@ def b200_rms_norm_int8(tensor: torch.Tensor, weight: torch.Tensor, *, epsilon: f
 
 def b200_quantize_rows_int8(tensor: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """(codes int8, scales float32 per row): rows of activations in front of a projection, or a weight's rows, which are its
-    output columns."""
+    output columns. The largest code of a row is 127, or less where its largest magnitude is below 127 * 2^-126."""
 
     codes, scales, _ = _quantize(tensor, None, None, 0.0, "b200_quantize_rows_int8")
     return codes, scales

@@ -1,5 +1,5 @@
 """Operators in 8 bits over the whole range of what they may be given: value blocks any distance apart, tails of small
-probabilities behind a token that dominates."""
+probabilities behind a token that dominates, rows of tiny numbers."""
 
 import math
 
@@ -151,3 +151,33 @@ def test_attention_of_a_long_tail_behind_a_token_that_dominates(dtype, cache, ab
     mask = torch.zeros(1, 1, 1, length) if masked else None
     check(query.to(dtype), pools, scales, table, length, mask, 0.125)
     check(query.to(dtype), pools, scales, table, length, mask, 0.125, split_tokens=length)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,hidden", [(12, 136), (12, 1001), (900, 2048)])
+def test_rows_of_tiny_numbers(dtype, rows, hidden):
+    """Rows whose largest magnitude is 2^-112 .. 2^-149, fp32's end, without a norm and behind one: codes * scales stand for
+    the row to half a step of its scale, which is the largest magnitude / 127 and no less than the smallest normal number
+    (behind a norm: times the row's factor)."""
+    g = torch.Generator().manual_seed(hidden)
+    lowest = -149 if dtype == torch.float32 else -133
+    x = 2 * torch.rand(rows, hidden, generator=g, dtype=torch.float64) - 1
+    x = (x * torch.exp2(torch.linspace(-112, lowest, rows, dtype=torch.float64))[:, None]).to(dtype)
+    weight = (1 + 0.2 * torch.randn(hidden, generator=g)).to(dtype)
+    zeros = torch.zeros_like(x)
+    r = x.double()
+    weighted = r * weight.double()
+    factor = 1.0 / torch.sqrt((r * r).mean(-1) + 1e-6)
+    plain = b200.b200_quantize_rows_int8(x.cuda())
+    normed = b200.b200_rms_norm_int8(x.cuda(), weight.cuda(), epsilon=1e-6)[:2]
+    behind = b200.b200_rms_norm_int8(zeros.cuda(), weight.cuda(), epsilon=1e-6, residual=x.cuda())[:2]
+    for (codes, scales), y, by in ((plain, r, torch.ones(rows, dtype=torch.float64)), (normed, weighted, factor), (behind, weighted, factor)):
+        codes, scales = codes.cpu().double(), scales.cpu().double()
+        most = y.abs().amax(-1)
+        step = torch.where(most > 0, (most / 127).clamp_min(ref.SMALLEST), 0.0)
+        # a product with a weight is rounded to 2^-149 here, half of that off; 1 / 127, the product with it, the sum of squares,
+        # its root and the last product: 8 u
+        assert bool(((scales - step * by).abs() <= by * (8 * 2.0 ** -24 * step + 2.0 ** -150)).all())
+        off = (codes - y / step.clamp_min(1e-300)[:, None]).abs()
+        assert float(torch.where(most[:, None] > 0, off, 0.0).max()) <= 0.5 + 127 * 5 * 2.0 ** -24 + 2.0 ** -150 / ref.SMALLEST
+        assert not bool(codes[most == 0].any())
