@@ -22,7 +22,7 @@ from . import kernels
 from .contracts import SymbolError, bind_symbols
 from .dispatch_plan import resolve_dispatch_plan, split_tokens_of
 from .kernel_ir import decode_attribute, require_full_lowering, value_dtype, value_rank
-from .kv_state import ExecutionError, PagedKVCacheState, PreallocatedKVCacheState
+from .kv_state import ExecutionError, PagedKVCacheState, PreallocatedKVCacheState, QuantizedPagedKVCacheState
 
 _DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16,
            "i64": torch.int64, "i32": torch.int32, "i1": torch.bool}
@@ -438,17 +438,18 @@ class B200Executor:
     def _qkv_decode_attention_paged(self, state, slot, tensor, norm_weight, weight, folded, bias, cosine,
                                     sine, mask, q_heads, kv_heads, dim, epsilon, scale, offset, attributes):
         """The fused decode-layer op on a paged state: up to CHAIN_ROWS bf16 rows the same two
-        launches as on the contiguous layout, through the block table; beyond, the same ops one
-        kernel each through the state's own store / attention methods."""
+        launches as on the contiguous layout, through the block table; beyond, and on a cache in 8 bits,
+        the same ops one kernel each through the state's own store / attention methods."""
 
         rows = tensor.numel() // tensor.shape[-1]
+        fused = rows <= self._chain_rows(weight) and tensor.dtype == torch.bfloat16 and \
+            not isinstance(state, QuantizedPagedKVCacheState)
         bound = mask.shape[-1] if mask is not None else state.capacity
         if bound > state.capacity:
             raise ExecutionError("decode attention mask is longer than the KV capacity")
         self.lowering_trace.append({"backend": "b200", "op": "qkv_decode_attention", "rows": rows,
-                                    "fused": rows <= self._chain_rows(weight), "length_offset": offset,
-                                    "layout": "paged"})
-        if rows <= self._chain_rows(weight) and tensor.dtype == torch.bfloat16:
+                                    "fused": fused, "length_offset": offset, "layout": "paged"})
+        if fused:
             flat = tensor.reshape(rows, tensor.shape[-1])
             partials, squares = kernels.b200_linear_partial(flat, folded, row_squares=True)
             pool_key, pool_value, lengths = state._slot(slot)

@@ -475,8 +475,11 @@ class QuantizedPagedKVCacheState(PagedKVCacheState):
         return self
 
     def decode_attention(self, slot: int, query: torch.Tensor, attention_mask: torch.Tensor, *,
-                         groups: int, scale: float, runner: Optional[Callable] = None,
+                         groups: int, scale: float, runner: Optional[Callable] = None, numerical_mode: str = "fast",
                          **options) -> torch.Tensor:
+        """(both numerical modes take the one kernel, whose scores, statistics and sums are fp32)"""
+
+        kernels._mode(numerical_mode)
         pool_key, pool_value, lengths = self._slot(slot)
         if query.ndim != 4 or query.shape[2] != 1:
             raise ExecutionError("decode attention query must be B x H x 1 x D")
