@@ -276,23 +276,22 @@ class PagedKVCacheState(PreallocatedKVCacheState):
     def reserve(self, tokens_per_sequence: Sequence[int], *, order: Optional[Sequence[int]] = None) -> None:
         """Makes sure sequence b owns blocks for tokens_per_sequence[b] tokens (host-side, between
         steps). `order`: the pool blocks to hand out first (tests use a shuffled order to prove
-        that nothing assumes contiguity)."""
+        that nothing assumes contiguity). One that cannot be met takes no block."""
 
         if order is not None:
             taken = {block for row in self._host_table for block in row}
             self._free[:] = [block for block in reversed(list(order)) if block not in taken]
-        changed = False
-        for b, tokens in enumerate(tokens_per_sequence):
-            need = -(-int(tokens) // self.block_size)
+        needs = [-(-int(tokens) // self.block_size) for tokens in tokens_per_sequence]
+        for b, need in enumerate(needs):
             if need > self.block_table.shape[1]:
-                raise ExecutionError(f"sequence {b} needs {tokens} tokens, beyond the paged capacity "
+                raise ExecutionError(f"sequence {b} needs {tokens_per_sequence[b]} tokens, beyond the paged capacity "
                                      f"{self.capacity}")
-            while len(self._host_table[b]) < need:
-                if not self._free:
-                    raise ExecutionError("the KV block pool is exhausted")
-                self._host_table[b].append(self._free.pop())
-                changed = True
-        if changed:
+        missing = [max(need - len(self._host_table[b]), 0) for b, need in enumerate(needs)]
+        if sum(missing) > len(self._free):
+            raise ExecutionError("the KV block pool is exhausted")
+        for row, count in zip(self._host_table, missing):
+            row.extend(self._free.pop() for _ in range(count))
+        if any(missing):
             self._write_table()
 
     def _write_table(self) -> None:
