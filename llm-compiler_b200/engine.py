@@ -24,7 +24,7 @@ from __future__ import annotations
 
 import math
 import os
-from typing import Callable, Dict, Optional
+from typing import Callable, Dict, List, Optional, Sequence
 
 import torch
 
@@ -390,24 +390,27 @@ class Qwen2Engine(ServingEngine):
         if not self.paged or self._block_slack > 0:
             return
         size = self.state.block_size
-        self.state.reserve([min(n + size, self.capacity) for n in self._host_lengths])
+        self.state.reserve(self._tokens_ahead(self._host_lengths))
         self._block_slack = min(min(-(-(n + size) // size) * size, self.capacity) - n
                                 for n in self._host_lengths)
+
+    def _tokens_ahead(self, lengths: Sequence[int]) -> List[int]:
+        return [min(n + self.state.block_size, self.capacity) for n in lengths]
 
     def fork(self, source: int, target: int) -> None:
         """Paged layout: sequence `target` gives back what it holds and continues as a second branch of `source`, between
         steps: whole blocks are shared, a last one that is partly full is copied, and the next input token is the same (set
-        `input_ids[target]` to branch)."""
+        `input_ids[target]` to branch). A fork that fails (a pool without room for the copy and the next step) changes nothing."""
 
         if not self.paged:
             raise ExecutionError("fork needs the paged KV layout")
         if not (0 <= source < self.batch and 0 <= target < self.batch) or source == target:
             raise ExecutionError("fork needs two different sequences of this engine")
-        self.state.release(target)
-        self._host_lengths[target] = 0
-        self.state.fork(source, target, tokens=self._host_lengths[source])
+        lengths = list(self._host_lengths)
+        lengths[target] = lengths[source]
+        self.state._fork(source, target, lengths[source], replace=True, ahead=self._tokens_ahead(lengths))
         self.input_ids[target] = self.input_ids[source]
-        self._host_lengths[target] = self._host_lengths[source]
+        self._host_lengths = lengths
         self._block_slack = 0
         self._reserve_blocks()
 

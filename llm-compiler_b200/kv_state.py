@@ -322,12 +322,19 @@ class PagedKVCacheState(PreallocatedKVCacheState):
         of its lengths, read from the device, which synchronises). Whole blocks are shared; a last block that is only partly
         full is copied in every layer, one launch, so that either sequence may append to its own. Host-side, between
         steps; every layer slot's length of `target` becomes `tokens`, and its extra length rows stand as far from that as
-        the source's from its own length."""
+        the source's from its own length. A fork that fails changes nothing."""
+
+        self._fork(source, target, tokens)
+
+    def _fork(self, source: int, target: int, tokens: Optional[int], *, replace: bool = False, ahead: Optional[Sequence[int]] = None
+              ) -> None:
+        """fork; `replace`: the target gives back what it holds, `ahead`: tokens of each sequence that are reserved behind it.
+        What may fail is done before anything changes."""
 
         sequences = len(self._host_table)
         if not (0 <= source < sequences and 0 <= target < sequences) or source == target:
             raise ExecutionError("fork needs two different sequences of this state")
-        if self._host_table[target]:
+        if self._host_table[target] and not replace:
             raise ExecutionError(f"sequence {target} still holds blocks: release it first")
         if tokens is None:
             tokens = int(self.lengths[0][source].item())
@@ -335,11 +342,17 @@ class PagedKVCacheState(PreallocatedKVCacheState):
         if tokens < 0 or tokens > len(held) * self.block_size:
             raise ExecutionError(f"sequence {source} does not hold {tokens} tokens")
         whole, partial = divmod(tokens, self.block_size)
-        if partial and not self._free:
+        free = self._free + [block for block in reversed(self._host_table[target]) if self._sharers.get(block, 1) == 1]
+        rows = [len(row) for row in self._host_table]
+        rows[target] = whole + (partial > 0)
+        needed = (partial > 0) + sum(max(-(-int(count) // self.block_size) - rows[b], 0) for b, count in enumerate(ahead or ()))
+        if needed > len(free):
             raise ExecutionError("the KV block pool is exhausted")
         row = held[:whole]
         if partial:
-            quantized_kernels.b200_copy_kv_blocks(self._pools, [held[whole]], [self._free[-1]])
+            quantized_kernels.b200_copy_kv_blocks(self._pools, [held[whole]], [free[-1]])
+        if self._host_table[target]:
+            self.release(target)  # (free[-1] is the last of the free blocks then)
         for block in row:
             self._sharers[block] = self._sharers.get(block, 1) + 1
         self._host_table[target] = row + ([self._free.pop()] if partial else [])
