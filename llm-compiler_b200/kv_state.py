@@ -276,23 +276,27 @@ class PagedKVCacheState(PreallocatedKVCacheState):
     def reserve(self, tokens_per_sequence: Sequence[int], *, order: Optional[Sequence[int]] = None) -> None:
         """Makes sure sequence b owns blocks for tokens_per_sequence[b] tokens (host-side, between
         steps). `order`: the pool blocks to hand out first (tests use a shuffled order to prove
-        that nothing assumes contiguity). One that cannot be met takes no block."""
+        that nothing assumes contiguity). Where the pool runs out, the sequences keep what they were given until
+        then, and the device's table says so."""
 
         if order is not None:
             taken = {block for row in self._host_table for block in row}
             self._free[:] = [block for block in reversed(list(order)) if block not in taken]
-        needs = [-(-int(tokens) // self.block_size) for tokens in tokens_per_sequence]
-        for b, need in enumerate(needs):
-            if need > self.block_table.shape[1]:
-                raise ExecutionError(f"sequence {b} needs {tokens_per_sequence[b]} tokens, beyond the paged capacity "
-                                     f"{self.capacity}")
-        missing = [max(need - len(self._host_table[b]), 0) for b, need in enumerate(needs)]
-        if sum(missing) > len(self._free):
-            raise ExecutionError("the KV block pool is exhausted")
-        for row, count in zip(self._host_table, missing):
-            row.extend(self._free.pop() for _ in range(count))
-        if any(missing):
-            self._write_table()
+        changed = False
+        try:
+            for b, tokens in enumerate(tokens_per_sequence):
+                need = -(-int(tokens) // self.block_size)
+                if need > self.block_table.shape[1]:
+                    raise ExecutionError(f"sequence {b} needs {tokens} tokens, beyond the paged capacity "
+                                         f"{self.capacity}")
+                while len(self._host_table[b]) < need:
+                    if not self._free:
+                        raise ExecutionError("the KV block pool is exhausted")
+                    self._host_table[b].append(self._free.pop())
+                    changed = True
+        finally:
+            if changed:
+                self._write_table()
 
     def _write_table(self) -> None:
         host = torch.full(tuple(self.block_table.shape), -1, dtype=torch.int32)

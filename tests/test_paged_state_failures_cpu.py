@@ -1,4 +1,5 @@
-"""Steps of a paged KV state and of an engine's fork that fail change nothing: neither blocks, table, lengths nor sharers."""
+"""Steps of a paged KV state and of an engine that fail: a fork changes neither blocks, table, lengths nor sharers, a reservation
+leaves host and device with one table."""
 
 import pytest
 import torch
@@ -18,17 +19,17 @@ def bookkeeping(state):
             state._length_arena.tolist())
 
 
-@pytest.mark.parametrize("tokens", [[64, 96, 200], [64, 160, 96]])
-def test_a_reservation_that_cannot_be_met_takes_no_block(tokens):
-    """(a sequence beyond the capacity, a pool too small: the sequences in front of it had room)"""
+@pytest.mark.parametrize("tokens,held", [([64, 96, 200], [2, 3, 1]), ([64, 160, 96], [2, 3, 1]), ([96, 200, 64], [3, 1, 1])])
+def test_a_reservation_that_cannot_be_met_leaves_the_table_as_the_host_has_it(tokens, held):
+    """A sequence beyond the capacity, a pool too small: the sequences in front keep what they were given, on both sides."""
     state = make_state(num_blocks=6)
     state.reserve([32, 32, 32])
-    before = bookkeeping(state)
     with pytest.raises(ExecutionError):
         state.reserve(tokens)
-    assert bookkeeping(state) == before
-    state.reserve([64, 32, 32])
-    assert state.block_table[0, :2].tolist() == state._host_table[0] and len(state._host_table[0]) == 2
+    assert [len(row) for row in state._host_table] == held
+    for b, row in enumerate(state._host_table):
+        assert state.block_table[b].tolist() == row + [-1] * (5 - len(row))
+    assert sorted(state._free + [block for row in state._host_table for block in row]) == list(range(6))
 
 
 def make_engine(num_blocks, lengths, kind=QuantizedPagedKVCacheState, dtype=torch.int8):
