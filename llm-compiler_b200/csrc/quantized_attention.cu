@@ -96,7 +96,7 @@ extern "C" int b200_paged_decode_attention_8bit(const b200_cache_attention_call*
   p.head_blocks = static_cast<int>(plan.head_blocks); p.block_heads = static_cast<int>(plan.block_heads);
   p.block_size = static_cast<int>(c.block_size); p.mask_dtype = static_cast<int>(c.mask_dtype);
   const uint64_t block_tiles = static_cast<uint64_t>(c.block_size / 32);
-  p.block_magic = ((uint64_t(1) << 40) + block_tiles - 1) / block_tiles;
+  p.block_magic = ((uint64_t(1) << 63) + block_tiles - 1) / block_tiles;
   p.q_vector = aligned16(c.query) && c.q_batch_stride % 8 == 0 && c.q_head_stride % 8 == 0;
   p.scale = static_cast<float>(c.scale); p.wait_limit = wait_limit(); p.drop_loads = drop_loads();
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -77,7 +77,8 @@ struct Params {
   int cluster;     // the splits are a cluster
   int sorted;      // CTAs take the sequences from the longest to the shortest
   int q_vector;    // rows of q may be read 16 bytes at a time
-  uint64_t block_magic;  // 2^40 / tiles of a block, rounded up: tile * it >> 40 is the tile's block (tiles below 2^25, blocks of up to 2^15)
+  uint64_t block_magic;  // 2^63 / tiles of a block, rounded up: tile * it >> 63 is the tile's block (it is off by less than the
+                         // divisor, at most 2^15, and a tile is below 2^25: their product stays below 2^63)
   float scale;
   uint32_t wait_limit;
   int drop_loads;
@@ -261,7 +262,7 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
   auto look_up = [&](int it) {
     Window w = {-1, 0, 0.0f, 0.0f};
     if (it >= mine) return w;
-    const int tile = my_first + it * stride, column = static_cast<int>(tile * p.block_magic >> 40);
+    const int tile = my_first + it * stride, column = static_cast<int>(__umul64hi(2 * static_cast<uint64_t>(tile), p.block_magic));
     const int block = column < kTableCache ? row_cache[column] : table[column];
     if (block < 0 || block >= p.num_blocks) {
       bad = true;

@@ -1,5 +1,5 @@
 """Operators in 8 bits over the whole range of what they may be given: value blocks any distance apart, tails of small
-probabilities behind a token that dominates, rows of tiny numbers."""
+probabilities behind a token that dominates, tables of more than 2^24 tiles, rows of tiny numbers."""
 
 import math
 
@@ -151,6 +151,31 @@ def test_attention_of_a_long_tail_behind_a_token_that_dominates(dtype, cache, ab
     mask = torch.zeros(1, 1, 1, length) if masked else None
     check(query.to(dtype), pools, scales, table, length, mask, 0.125)
     check(query.to(dtype), pools, scales, table, length, mask, 0.125, split_tokens=length)
+
+
+@pytest.mark.parametrize("size,columns", [(32, (1 << 24) + 2), (96, 5592406 + 3)])
+def test_attention_behind_the_first_half_billion_tokens(size, columns):
+    """A table of more than 2^24 tiles whose entries share a block, all but the last two: their tokens' scores are 40 above the
+    others', so that the e^20 of those weigh e^-20 of them, and the result is those two blocks' mean."""
+    g = torch.Generator().manual_seed(0)
+    dim = 64
+    keys = torch.zeros(3, 1, size, dim, dtype=torch.int8)
+    keys[1:, :, :, 0] = 100
+    pools = [keys.cuda(), torch.randint(-127, 128, (3, 1, size, dim), generator=g, dtype=torch.int8).cuda()]
+    scales = [torch.full((3, 1), 0.01).cuda(), torch.full((3, 1), 1 / 127).cuda()]
+    table = torch.zeros(1, columns, dtype=torch.int32, device="cuda")
+    table[0, -2:] = torch.tensor([1, 2], dtype=torch.int32)
+    query = torch.zeros(1, 2, 1, dim, dtype=torch.bfloat16, device="cuda")
+    query[..., 0] = 320.0
+    got = b200.b200_paged_decode_attention_8bit(query, *pools, *scales, table, torch.tensor([columns * size - 7]).cuda(), None,
+                                                scale=0.125).cpu().double()
+    values = torch.cat([pools[1][1, 0], pools[1][2, 0, :-7]]).cpu().double() / 127
+    want = values.mean(0)
+    # the result's rounding, a probability's, and the others' weight: e^-40 each of some 2^29 tokens, against 57 and more
+    others = columns * size * math.exp(-40) / values.shape[0]
+    bound = 2.0 ** -8 * want.abs() + 2.0 ** -10 * values.abs().mean(0) + 2 * others + 2.0 ** -18
+    assert bool(((got - want).abs() <= bound).all())
+    kernels.runtime().check_status()
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
