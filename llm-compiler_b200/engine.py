@@ -157,7 +157,7 @@ class Qwen2Engine(ServingEngine):
         out on the host, ahead of the steps that need them.
 
         kv_dtype torch.int8 or torch.float8_e4m3fn (paged layout, bf16 and fp16 weights): the cache in
-        8 bits with a scale for each block and KV head, half the bytes that a step reads of it.
+        8 bits with a scale for each block and KV head, half the bytes that a step reads of it; heads of 64, 128 or 256.
 
         weight_dtype torch.int8 (bf16 and fp16 weights): the layers' projections in 8-bit integers, weights
         with a scale per output column, rows of activations with a scale each; norms, attention, the
@@ -167,6 +167,8 @@ class Qwen2Engine(ServingEngine):
             raise ValueError(f"unknown numerical mode {numerical_mode!r}")
         if kv_layout not in ("contiguous", "paged"):
             raise ValueError(f"unknown KV layout {kv_layout!r}")
+        if kv_dtype is not None and config.head_dim not in quantized_kernels.ATTENTION_HEAD_DIMS:
+            raise ValueError(f"a cache in 8 bits serves head sizes of {quantized_kernels.ATTENTION_HEAD_DIMS}, not {config.head_dim}")
         self.config = config
         self._init_step(batch, device or torch.device("cuda", torch.cuda.current_device()))
         self.capacity = capacity

@@ -23,6 +23,7 @@ _BFLOAT16, _FLOAT16, _FLOAT32, _INT32, _INT64 = torch.bfloat16, torch.float16, t
 
 # The formats of a cache in 8 bits: the code of the C ABI.
 CACHE_CODES = {torch.int8: _lib.I8, torch.float8_e4m3fn: _lib.E4M3}
+ATTENTION_HEAD_DIMS = (64, 128, 256)
 MAX_K = 131056  # (a sum of that many products of two 8-bit integers stays below 2^31)
 
 # The ABI's structs: pointers, 64-bit integers, doubles.
@@ -139,7 +140,7 @@ def b200_paged_decode_attention_8bit(query: torch.Tensor, key_pool: torch.Tensor
         raise ValueError("query does not match the pools")
     if dtype is not _BFLOAT16 and dtype is not _FLOAT16:
         raise ValueError(f"query must be bfloat16 or float16, not {query.dtype}")
-    if dim not in (64, 128, 256):
+    if dim not in ATTENTION_HEAD_DIMS:
         raise ValueError("head_dim must be 64, 128 or 256")
     if block_size % 32:
         raise ValueError("the block size must be a multiple of 32 tokens")

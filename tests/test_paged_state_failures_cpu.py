@@ -1,10 +1,11 @@
 """Steps of a paged KV state and of an engine that fail: a fork changes neither blocks, table, lengths nor sharers, a reservation
-leaves host and device with one table."""
+leaves host and device with one table, an engine is refused when it is built."""
 
 import pytest
 import torch
 
 from llm_compiler_b200 import quantized_kernels
+from llm_compiler_b200 import qwen2 as q2
 from llm_compiler_b200.engine import Qwen2Engine
 from llm_compiler_b200.kv_state import ExecutionError, PagedKVCacheState, QuantizedPagedKVCacheState
 
@@ -120,3 +121,13 @@ def test_a_fork_whose_copy_cannot_be_launched_changes_nothing(monkeypatch):
     with pytest.raises(RuntimeError):
         engine.fork(0, 1)
     assert everything(engine) == before
+
+
+def test_an_engine_refuses_head_sizes_that_a_cache_in_8_bits_has_no_attention_for():
+    """When it is built, not at its first step."""
+    config = q2.Qwen2Config(hidden_size=128, intermediate_size=256, num_layers=1, num_heads=4, num_kv_heads=2, rms_norm_eps=1e-6,
+                            rope_theta=1e6, vocab_size=64, tie_word_embeddings=True)
+    weights = q2.make_weights(config, seed=0, dtype=torch.bfloat16)
+    assert config.head_dim == 32
+    with pytest.raises(ValueError, match="head sizes"):
+        Qwen2Engine(config, weights, batch=2, capacity=64, kv_layout="paged", block_size=32, kv_dtype=torch.int8)
