@@ -127,6 +127,12 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// 1 / x of a sum of probabilities, good to 2^-23; 0 where there are none (a sum is 0, or from 1 to 2^44)
+__device__ __forceinline__ float inverse_of(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return x != 0.0f ? y : 0.0f;
+}
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
   const __half2 v = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&v);
@@ -572,7 +578,9 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
     if (lane == 0) atomicOr(p.status, B200_STATUS_WAIT_TIMEOUT);
   }
 
-  // ---- the four warps' parts: O in units of 1, through the ring's memory ----
+  // ---- the four warps' parts, through the ring's memory: means, since the sum of a long sequence's values may leave fp32
+  // where they do not ----
+  float share[NT][2];
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -585,6 +593,7 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
         merge_m[warp][8 * t + 2 * j + h] = m[t][h];
         merge_l[warp][8 * t + 2 * j + h] = sum;
       }
+      share[t][h] = inverse_of(kLift * sum);
     }
   __syncthreads();  // every ring is done with
   if (!S::kBeside(NT) && p.cluster && !alone) cluster_arrive();
@@ -598,21 +607,19 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
       for (int h = 0; h < 2; ++h) {
         const int head = 8 * t + 2 * j + h;
         *reinterpret_cast<float2*>(parts + (warp * kHeads + head) * D + 16 * i + 2 * g) =
-            make_float2(o[t][i][h] * (1.0f / kLift) * vref, o[t][i][2 + h] * (1.0f / kLift) * vref);
+            make_float2(o[t][i][h] * share[t][h] * vref, o[t][i][2 + h] * share[t][h] * vref);
       }
   __syncthreads();
   const int64_t item = b * gridDim.y + item_head;
   // merged by a thread for a whole row of four; NaN in a part stays (a weight of zero does not silence it)
-  auto put_out = [&](int head, int d, float4 value, float sum) {  // (0 / 0 = NaN for a sequence without tokens)
+  auto put_out = [&](int head, int d, float4 value, float sum) {
     const int64_t at = (b * p.q_heads + head0 + head) * D + d;
-    const float scale = 1.0f / sum;
-    value.x *= scale; value.y *= scale; value.z *= scale; value.w *= scale;
+    if (sum == 0.0f) value = make_float4(NAN, NAN, NAN, NAN);  // (a sequence without tokens, or with none left by its mask)
     *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at) = make_uint2(Elem<T>::pack(value.x, value.y), Elem<T>::pack(value.z, value.w));
   };
-  auto add_part = [](float weight, float l, const float4& part, float& sum, float4& value) {
-    sum = fmaf(weight, l, sum);
-    value.x = fmaf(weight, part.x, value.x); value.y = fmaf(weight, part.y, value.y);
-    value.z = fmaf(weight, part.z, value.z); value.w = fmaf(weight, part.w, value.w);
+  auto add_part = [](float share, const float4& part, float4& value) {
+    value.x = fmaf(share, part.x, value.x); value.y = fmaf(share, part.y, value.y);
+    value.z = fmaf(share, part.z, value.z); value.w = fmaf(share, part.w, value.w);
   };
   auto weight_of = [&](float one, float top) { return one == -INFINITY ? 0.0f : exp2_fast((one - top) * kToLog2); };
   // In a cluster each CTA finishes every `active`-th run of four, and is given the others' parts of those: stores to another
@@ -625,14 +632,19 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
   }
   for (int e = threadIdx.x; e < heads * (D / 4); e += kThreads) {
     const int head = e / (D / 4), d = e % (D / 4) * 4;
-    float top = -INFINITY, sum = 0.0f;
+    float top = -INFINITY, sum = 0.0f, part_l[kWarps];
     float4 value = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) top = fmaxf(top, merge_m[w][head]);
 #pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      part_l[w] = weight_of(merge_m[w][head], top) * merge_l[w][head];
+      sum += part_l[w];
+    }
+    const float inverse = inverse_of(sum);
+#pragma unroll
     for (int w = 0; w < kWarps; ++w)
-      add_part(weight_of(merge_m[w][head], top), merge_l[w][head],
-               *reinterpret_cast<const float4*>(parts + (w * kHeads + head) * D + d), sum, value);
+      add_part(part_l[w] * inverse, *reinterpret_cast<const float4*>(parts + (w * kHeads + head) * D + d), value);
     if (alone) {
       if (split == 0) put_out(head, d, value, sum);
     } else if (p.cluster) {
@@ -657,11 +669,21 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
       const int e = local * active + split, head = e / (D / 4), d = e % (D / 4) * 4;
       float top = -INFINITY, sum = 0.0f;
       float4 value = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      for (int i = 0; i < active; ++i) top = fmaxf(top, joined[i][head].x);
-      for (int i = 0; i < active; ++i) {
-        const float2 ml = joined[i][head];
-        add_part(weight_of(ml.x, top), ml.y, given[i * own_runs + local], sum, value);
+      float2 ml[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        ml[i] = i < active ? joined[i][head] : make_float2(-INFINITY, 0.0f);
+        top = fmaxf(top, ml[i].x);
       }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        ml[i].y *= weight_of(ml[i].x, top);
+        sum += ml[i].y;
+      }
+      const float inverse = inverse_of(sum);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < active) add_part(ml[i].y * inverse, given[i * own_runs + local], value);
       put_out(head, d, value, sum);
     }
     return;
@@ -692,13 +714,20 @@ cache_attention_kernel(const Params p, const __grid_constant__ CUtensorMap key_m
       float over_all = top;
 #pragma unroll
       for (int i = 0; i < 16; ++i) over_all = fmaxf(over_all, ml[i].x);  // (the last one again does no harm)
-      const float keep = weight_of(top, over_all);
+      const float before = sum * weight_of(top, over_all);
       top = over_all;
-      sum *= keep;
+      sum = before;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (s0 + i < active) {
+          ml[i].y *= weight_of(ml[i].x, top);
+          sum += ml[i].y;
+        }
+      const float inverse = inverse_of(sum), keep = before * inverse;
       value.x *= keep; value.y *= keep; value.z *= keep; value.w *= keep;
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        if (s0 + i < active) add_part(weight_of(ml[i].x, top), ml[i].y, part[i], sum, value);
+        if (s0 + i < active) add_part(ml[i].y * inverse, part[i], value);
     }
     put_out(head, d, value, sum);
   }

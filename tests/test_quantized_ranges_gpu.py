@@ -1,4 +1,4 @@
-"""Operators in 8 bits over the whole range of what they may be given: value blocks any distance apart, tails of small
+"""Operators in 8 bits over the whole range of what they may be given: values of any size, value blocks any distance apart, tails of small
 probabilities behind a token that dominates, tables of more than 2^24 tiles, rows of tiny numbers."""
 
 import math
@@ -151,6 +151,25 @@ def test_attention_of_a_long_tail_behind_a_token_that_dominates(dtype, cache, ab
     mask = torch.zeros(1, 1, 1, length) if masked else None
     check(query.to(dtype), pools, scales, table, length, mask, 0.125)
     check(query.to(dtype), pools, scales, table, length, mask, 0.125, split_tokens=length)
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("dtype,dim,heads", [(torch.bfloat16, 64, 4), (torch.bfloat16, 128, 12), (torch.bfloat16, 256, 3)])
+@pytest.mark.parametrize("largest", [2.0 ** 127, 2.0 ** -120])
+def test_attention_of_values_at_the_ends_of_their_range(cache, dtype, dim, heads, largest):
+    """Values up to half of fp32's largest number, thousands of them of one sign and of one weight, and down to its smallest: the
+    result lies among them, though their sum does not."""
+    g = torch.Generator().manual_seed(dim)
+    length, size = 5000, 32
+    blocks = -(-length // size)
+    top = ref.TOP[cache]
+    pools = [random_codes(g, cache, blocks, 1, size, dim) for _ in range(2)]
+    pools[1] = pools[1].float().abs().to(cache)
+    scales = [torch.full((blocks, 1), 1.0 / top).cuda(), (largest / top * (0.5 + 0.5 * torch.rand(blocks, 1, generator=g))).cuda()]
+    table = torch.randperm(blocks, generator=g).to(torch.int32).view(1, blocks)
+    query = torch.randn(1, heads, 1, dim, generator=g).to(dtype)
+    for split_tokens in (0, length, 800, 256):  # the library's choice, one CTA, a cluster, partials in the workspace
+        check(query, pools, scales, table, length, None, dim ** -0.5, split_tokens=split_tokens)
 
 
 @pytest.mark.parametrize("size,columns", [(32, (1 << 24) + 2), (96, 5592406 + 3)])
