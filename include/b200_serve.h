@@ -747,7 +747,8 @@ int b200_advance_slots(int64_t* lengths, const int32_t* slots, const int32_t* st
  *
  * b200_paged_decode_attention_8bit: one query token per sequence, B x Hq x 1 x D in B200_BF16 or B200_F16 (last dim
  * contiguous), over the first lengths[b] entries: softmax(scale * q . K + mask) V with fp32 scores, statistics and sums.
- * The mask is additive, B x 1 x 1 x mask_len, or NULL. head_dim 64, 128 or 256, block_size a multiple of 32. A length
+ * Probabilities are rounded to 11 bits (22 for B200_F16) down to 2^-23 of the largest one, and by at most 2^-34 of that below;
+ * scales and values may be of any size. The mask is additive, B x 1 x 1 x mask_len, or NULL. head_dim 64, 128 or 256, block_size a multiple of 32. A length
  * above mask_len is clamped and sets B200_STATUS_LENGTH_OVER_MASK; tokens of a block outside [0, num_blocks) are left out
  * and set B200_STATUS_BAD_POSITION. A sequence without tokens, or with every token masked by -inf, gives NaN as
  * b200_decode_attention does. split_tokens: tokens a CTA serves (0: the library's choice); max_length_hint: the longest

@@ -20,12 +20,14 @@
 // Scales. ks multiplies the scores. vs is folded into the probabilities relative to a running reference `vref`, which the
 // accumulators are carried in: a power of two that follows vs (accumulators rescaled, exactly) only when vs is more than twice it
 // or less than a quarter of it. It follows any distance up, where what is in the accumulators may underflow, and down as far as
-// they stay within fp32's range, where it is the tile that may; a tile that no head gives any weight does not move it. The running maximum moves only when a score passes it by more than 3 (in units of log 2): the softmax is the same, and
-// most tiles need no reduction across lanes. So P, at most 2^3 * 2, is carried 2^11 higher, which fills fp16: P is rounded by
-// 2^-11 of it, an eighth of the rounding of a bf16 result, down to 2^-23 of the largest probability and by 2^-34 of the largest
-// below (carried at 1 with wider limits, a token that got e^14 of the others' weight left them 1 % off and e^18 nothing); its sum stays
-// fp32. An fp16 result's own rounding is no larger than P's, so there P is two fp16 numbers, what the first leaves in the
-// second (2^-22, and 2^-34 of the largest probability as before): one more product per V fragment.
+// they stay within fp32's range, where it is the tile that may; a tile that no head gives any weight does not move it.
+//
+// Probabilities. The running maximum moves only when a score passes it by more than 3 (in units of log 2): the softmax is the
+// same, and most tiles need no reduction across lanes. So P, at most 2^3 * 2, is carried 2^11 higher, which fills fp16: P is
+// rounded by 2^-11 of it, an eighth of the rounding of a bf16 result, down to 2^-23 of the largest probability, and by 2^-34 of
+// the largest below (carried at 1 and with wider limits, the tail behind a token e^14 above it came out 1 % off, and behind one
+// e^18 above it as nothing); its sum stays fp32. An fp16 result's own rounding is no larger than P's, so there P is two fp16
+// numbers, what the first leaves in the second (2^-22, and 2^-34 of the largest as before): one more product per V fragment.
 //
 // Work. The tiles (32 tokens) of one (sequence, KV head, up to 8 NT heads) are dealt to `splits` CTAs of four warps, a tile
 // to a warp in turn. Each warp has a ring of its own that TMA fills: a tile never spans two blocks (block sizes are multiples
@@ -33,7 +35,7 @@
 // splits are a cluster, whose CTAs merge through distributed shared memory; more leave partials in the workspace, which the
 // CTA that arrives last adds in split order. Either way results do not depend on timing.
 //
-// Measured: 64 x 4096 tokens, 2 heads of 64 (67 MB): 16.7 us, 4.0 TB/s; 64 ragged to 8192, 4 heads of 128 (270 MB): 51 us,
+// Measured: 64 x 4096 tokens, 2 heads of 64 (67 MB): 16.7 us, 4.0 TB/s; 64 ragged to 8192, 4 heads of 128 (270 MB): 52 us,
 // 5.2 TB/s; 3 x 30001, 8 heads of 128 with a mask (185 MB): 37 us, 5.0 TB/s; 1 x 1000: 4.8 us. A CTA streams nothing for some
 // 5 us at its start and end (length, table row, first copies; merge, exchange in the cluster, stores), which is what is left
 // beside the rate: in between the SMs' rings keep 96 KB and more in flight.
